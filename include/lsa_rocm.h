@@ -435,6 +435,75 @@ int lsa_decode_flat_noalloc(const void* q, const void* k, const void* v, int dty
                             int32_t reset_counters, int32_t* lists, int32_t* lengths, void* out, int32_t* status,
                             void* stream);
 
+/* Attention of a batch over prefixes that its rows share, and over each row's own read list:
+ * one softmax over both. No counterpart in the reference, whose rows each hold their whole
+ * cache. q [B, Tq, Hq, D]. The prefixes are k_prefix / v_prefix [P, Tp, Hkv, D] (element
+ * strides; prefix_cache_rows >= Tp rows a batch entry) or, with prefix_slots [P, Tp] (rows
+ * prefix_slot_stride apart), the cache rows it names of one pool of prefix_cache_rows rows
+ * (prefix_batch_stride unused; a slot outside the pool is skipped). Of prefix p the first
+ * prefix_lengths[p] keys count (NULL: Tp); batch row b reads prefix prefix_rows[b] (NULL: 0;
+ * none where it is outside [0, P)). The own part as lsa_read (W == 0: none; k, v, ids and
+ * lengths may be NULL then). A row without any key gives zeros. lse (NULL: not wanted) [B, Tq,
+ * Hq] fp32: the natural logarithm of the softmax's sum, -inf for a row without keys.
+ * scratch: lsa_prefix_read_scratch_bytes(), 16-byte aligned, no initialisation; nothing of it
+ * is needed after the call's kernels. */
+size_t lsa_prefix_read_scratch_bytes(int dtype, int64_t B, int64_t Tq, int64_t P, int64_t Tp, int32_t Hq, int32_t Hkv,
+                                     int32_t D, int32_t W);
+int lsa_prefix_read(const void* q, const void* k_prefix, const void* v_prefix, int dtype, int64_t B, int64_t Tq,
+                    int64_t P, int64_t Tp, int64_t prefix_cache_rows, int32_t Hq, int32_t Hkv, int32_t D,
+                    int64_t prefix_batch_stride, int64_t prefix_token_stride, int64_t prefix_head_stride,
+                    const int32_t* prefix_rows, const int32_t* prefix_lengths, const int32_t* prefix_slots,
+                    int64_t prefix_slot_stride, const void* k, const void* v, int64_t Tk, int64_t kv_batch_stride,
+                    int64_t kv_token_stride, int64_t kv_head_stride, const int32_t* ids, const int32_t* lengths,
+                    int32_t W, int ids_per_head, float scale, void* scratch, size_t scratch_bytes, void* out,
+                    float* lse, void* stream);
+
+/* Adds to mass [caches, Hkv, Tk] (fp32, element strides, keys contiguous) the softmax weight
+ * that each listed key receives from batch row b's query rows, summed over them and over the
+ * query heads of its kv-head. q [B, Tq, Hq, D], K as lsa_read's, `caches` = B caches or one
+ * pool for every row; lists as lsa_read's (a key listed twice counts twice). The weights are
+ * those of the softmax over the row's own list, or exp(score - lse) with lse [B, Tq, Hq] (a
+ * wider softmax's, as lsa_prefix_read gives it; -inf and NaN: no weight). A softmax whose sum
+ * is not a number gives none. The result does not depend on the order in which workgroups run.
+ * zero_first != 0: mass (dense) begins at zero. No counterpart in the reference. scratch:
+ * lsa_key_mass_scratch_bytes(), 16-byte aligned, no initialisation. */
+size_t lsa_key_mass_scratch_bytes(int dtype, int64_t B, int64_t Tq, int64_t caches, int64_t Tk, int32_t Hq, int32_t Hkv,
+                                  int32_t D, int32_t W);
+int lsa_key_mass(const void* q, const void* k, int dtype, int64_t B, int64_t Tq, int64_t caches, int64_t Tk,
+                 int32_t Hq, int32_t Hkv, int32_t D, int64_t k_batch_stride, int64_t k_token_stride,
+                 int64_t k_head_stride, const int32_t* ids, const int32_t* lengths, int32_t W, int ids_per_head,
+                 float scale, const float* lse, int zero_first, void* scratch, size_t scratch_bytes, float* mass,
+                 int64_t mass_batch_stride, int64_t mass_head_stride, void* stream);
+
+/* Which positions of a cache to keep. mass [B, Hkv, T] fp32 (element strides, positions
+ * contiguous). Of row b's lengths[b] positions (NULL: T) the first `sink` and the last `window`
+ * stay and, of the others, those of largest mass up to `budget` in all (sink + window <= budget
+ * <= T), ties to the lower position, a NaN below every number; a row of at most `budget` keeps
+ * all. kept [B, Hkv, budget] int32: the positions, ascending, -1 behind them; new_lengths [B].
+ * shared != 0: one selection a row, kept [B, budget], by the masses summed over the kv-heads
+ * (in fp64, head by head, rounded to fp32). With a slot table [B, T] (shared; rows table_stride
+ * apart) mass is a pool's, [Hkv, pool_rows], and new_table [B, T] receives each table row with
+ * its kept entries first, then the others of its length, then what was behind it (entries
+ * outside the pool weigh least). scratch: lsa_evict_scratch_bytes(B, T, shared). No counterpart
+ * in the reference. */
+size_t lsa_evict_scratch_bytes(int64_t B, int64_t T, int summed);
+int lsa_evict_keep(const float* mass, int64_t B, int32_t Hkv, int64_t T, int64_t mass_batch_stride,
+                   int64_t mass_head_stride, const int32_t* lengths, int32_t budget, int32_t window, int32_t sink,
+                   int shared, const int32_t* table, int64_t table_stride, int64_t pool_rows, void* scratch,
+                   size_t scratch_bytes, int32_t* kept, int32_t* new_lengths, int32_t* new_table,
+                   int64_t new_table_stride, void* stream);
+
+/* Moves the kept rows (lsa_evict_keep's `kept`, shared or per kv-head) of K, V and mass to the
+ * front of another cache: k_out / v_out rows [0, budget) and mass_out [.., 0, budget), which must
+ * not overlap the inputs. Rows past the kept ones are zeroed (zero_tail != 0) or left as they
+ * were. K/V rows 16-byte aligned, of a multiple of 16 bytes. */
+int lsa_evict_rows(const void* k, const void* v, const float* mass, int dtype, int64_t B, int64_t T, int32_t Hkv,
+                   int32_t D, int64_t kv_batch_stride, int64_t kv_token_stride, int64_t kv_head_stride,
+                   int64_t mass_batch_stride, int64_t mass_head_stride, const int32_t* kept, int shared,
+                   int32_t budget, void* k_out, void* v_out, int64_t out_batch_stride, int64_t out_token_stride,
+                   int64_t out_head_stride, float* mass_out, int64_t mass_out_batch_stride,
+                   int64_t mass_out_head_stride, int zero_tail, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,426 @@
+// The attention weight that each listed key received, added up over query rows, for gfx950.
+//
+//   mass[b, g, key] += sum over batch row b's query rows and the group's heads of
+//                      2^(s - m) / l,   s = q . k scale log2(e),
+// with m and l the row's own (the softmax over its list) or, from a given lse, a wider
+// softmax's. K alone is read.
+//
+//   mass_scores_kernel  gathers the listed K rows and leaves their scores and each span's
+//                       (maximum, sum) a head;
+//   mass_add_kernel     turns the scores into weights and adds them.
+//
+// A key that a list names twice counts twice; several query rows of one cache add to the same
+// keys. Sums must not depend on the order in which workgroups arrive. With one query row a cache, all
+// additions to a key come from one list and are the same number, so fp32 atomics will do.
+// With more, the weights go to 64-bit integers of 2^-44 first (integer sums have no order;
+// 2^-45 of rounding a weight, against 2^-24 of the fp32 sum), and mass_fold_kernel adds those to
+// the fp32 weights.
+#include <math.h>
+
+#include <algorithm>
+
+#include "lsa_abi_common.h"
+#include "lsa_read_dev.h"
+
+using namespace lsa;
+
+namespace {
+
+constexpr float kFix = 17592186044416.0f;  // 2^44: weights up to 2^19 in all
+constexpr float kMaxWeight = 65536.0f;     // a given lse may be off; a weight is at most this
+
+struct MassArgs {
+  const void* q;
+  const void* k;
+  const int32_t* ids;
+  const int32_t* lengths;
+  const float* lse;       // [rows, Hq] or nullptr
+  int64_t Tq, Tk;
+  int64_t k_sb, k_st, k_sh;
+  int Hq, Hkv, W, per_head;
+  float scale_log2;
+  int span;               // list slots of a workgroup of mass_scores_kernel
+  int n_span;
+  float* scores;          // [units, W, GQ], log2 domain
+  float* stats;           // [units, n_span, GQ, 2]
+  float* mass;
+  int64_t m_sb, m_sh;     // batch stride 0: one pool for every batch row
+  int64_t m_n;            // caches * Hkv * Tk (zero: fresh weights are written whole)
+  int caches;
+  int zero;               // the weights begin at zero
+  uint64_t* fixed;        // [caches, Hkv, Tk] or nullptr
+  int whole;              // fixed is cleared and folded whole, not by the lists
+};
+
+struct MassList {
+  const int32_t* ids;
+  int n;
+};
+
+__device__ __forceinline__ MassList mass_list(const MassArgs& a, int64_t row, int g) {
+  const int64_t li = a.per_head ? row * a.Hkv + g : row;
+  int n = a.lengths[li];
+  n = n < 0 ? 0 : (n > a.W ? a.W : n);
+  return {a.ids + li * a.W, n};
+}
+
+// (maximum, sum of 2^(x - maximum)) joined with another's
+__device__ __forceinline__ void join(float& m, float& l, float mo, float lo) {
+  const float mn = fmaxf(m, mo);
+  l = l * fast_exp2(m - mn) + lo * fast_exp2(mo - mn);
+  m = mn;
+}
+
+template <typename T, int D>
+struct MassShape {
+  static constexpr bool MM = sizeof(T) == 2;             // scores on the matrix cores
+  static constexpr int VEC = Row16<T>::N;
+  static constexpr int LPT = MM ? 4 : D / VEC;           // lanes a token
+  static constexpr int TPW = LSA_WAVE / LPT;             // tokens of a wave's step
+  static constexpr int LD = MM ? D / 32 : 1;             // 16-byte loads a lane a token
+  static constexpr int U = 16 / LD;                      // steps in flight: 16 loads a lane
+  static constexpr int NT = LSA_WAVES * TPW * U;
+};
+
+// grid (row * Hkv, span). Matrix-core form: 16 tokens a wave's step, Q as the A operand (heads
+// past the group are zero rows), K as the B operand: lane (row, col) loads dims 32 i + 8 row ..
+// + 8 of token col and receives the scores of heads 4 row .. + 3 against it.
+template <typename T, int D, int GQ>
+__global__ __launch_bounds__(LSA_BLOCK) void mass_scores_kernel(MassArgs a) {
+  using S = MassShape<T, D>;
+  constexpr int U = S::U, TPW = S::TPW, NT = S::NT;
+  constexpr int HL = S::MM ? (GQ < 4 ? GQ : 4) : GQ;  // heads of a lane
+  __shared__ float sm[LSA_WAVES][GQ], sl[LSA_WAVES][GQ];
+  const int tid = threadIdx.x, lane = tid & (LSA_WAVE - 1), w = tid / LSA_WAVE;
+  const int64_t unit = blockIdx.x;
+  const int sp = blockIdx.y;
+  const int64_t row = unit / a.Hkv;
+  const int g = (int)(unit % a.Hkv);
+  if (a.zero || a.whole) {  // this workgroup's share of the weights, and of the integers
+    const int64_t grid = (int64_t)gridDim.x * gridDim.y * LSA_BLOCK;
+    const int64_t at = ((int64_t)sp * gridDim.x + unit) * LSA_BLOCK + tid;
+    if (a.zero) {
+      for (int64_t i = at; i < a.m_n; i += grid) a.mass[i] = 0.0f;
+    }
+    if (a.whole) {
+      for (int64_t i = at; i < a.m_n; i += grid) a.fixed[i] = 0;
+    }
+  }
+  const MassList list = mass_list(a, row, g);
+  const int lo = sp * a.span, hi = min(lo + a.span, list.n);
+  if (lo >= hi) return;
+  const int64_t b = row / a.Tq;
+  const int64_t c = a.caches > 1 ? b : 0;
+  const T* kb = (const T*)a.k + b * a.k_sb + g * a.k_sh;
+  const T* qrow = (const T*)a.q + (row * a.Hq + (int64_t)g * GQ) * D;
+  float* scores = a.scores + unit * (int64_t)a.W * GQ;
+  uint64_t* fixed = a.fixed && !a.whole ? a.fixed + (c * a.Hkv + g) * a.Tk : nullptr;
+
+  float m[HL], l[HL];
+#pragma unroll
+  for (int h = 0; h < HL; ++h) {
+    m[h] = kNegBig;
+    l[h] = 0.0f;
+  }
+  const int rowq = lane >> 4, col = lane & 15;                   // matrix-core form
+  const int tg = S::MM ? col : lane / S::LPT, lp = S::MM ? rowq : lane % S::LPT;
+  uint4 qm[S::LD];
+  float qf[S::MM ? 1 : GQ][S::VEC];
+  if constexpr (S::MM) {
+#pragma unroll
+    for (int i = 0; i < S::LD; ++i) {
+      const uint4 x = *(const uint4*)(qrow + (int64_t)(col < GQ ? col : 0) * D + 32 * i + 8 * rowq);
+      qm[i] = col < GQ ? x : make_uint4(0u, 0u, 0u, 0u);
+    }
+  } else {
+#pragma unroll
+    for (int h = 0; h < GQ; ++h) Row16<T>::cvt(*(const uint4*)(qrow + (int64_t)h * D + lp * S::VEC), qf[h]);
+  }
+  for (int base = lo; base < hi; base += NT) {
+    bool ok[U];
+    uint4 kr[U][S::LD];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = base + (u * LSA_WAVES + w) * TPW + tg;
+      const int32_t id = list.ids[j < hi ? j : hi - 1];
+      ok[u] = j < hi && id >= 0 && id < a.Tk;
+      const T* src = kb + (int64_t)(ok[u] ? id : 0) * a.k_st + (S::MM ? 8 : S::VEC) * lp;
+#pragma unroll
+      for (int i = 0; i < S::LD; ++i) kr[u][i] = *(const uint4*)(src + 32 * i);
+      if (fixed && ok[u] && lp == 0) fixed[id] = 0;
+    }
+    float s[U][HL];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if constexpr (S::MM) {
+        f32x4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < S::LD; ++i) x = Mfma16<T>::run(qm[i], kr[u][i], x);
+#pragma unroll
+        for (int h = 0; h < HL; ++h) s[u][h] = ok[u] ? x[h] * a.scale_log2 : -INFINITY;
+      } else {
+        float kf[S::VEC];
+        Row16<T>::cvt(kr[u][0], kf);
+#pragma unroll
+        for (int h = 0; h < HL; ++h) {
+          float p = 0.0f;
+#pragma unroll
+          for (int e = 0; e < S::VEC; ++e) p = fmaf(qf[h][e], kf[e], p);
+          p = group_sum<S::LPT>(p);
+          s[u][h] = ok[u] ? p * a.scale_log2 : -INFINITY;
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < HL; ++h) {
+      float mt = m[h];
+#pragma unroll
+      for (int u = 0; u < U; ++u) mt = fmaxf(mt, s[u][h]);
+      float sum = l[h] * fast_exp2(m[h] - mt);
+#pragma unroll
+      for (int u = 0; u < U; ++u) sum += fast_exp2(s[u][h] - mt);
+      m[h] = mt;
+      l[h] = sum;
+    }
+    if (S::MM ? HL * rowq < GQ : lp == 0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = base + (u * LSA_WAVES + w) * TPW + tg;
+        if (j < hi) {
+          float* to = scores + (int64_t)j * GQ + (S::MM ? HL * rowq : 0);
+#pragma unroll
+          for (int h = 0; h < HL; ++h) to[h] = s[u][h];
+        }
+      }
+    }
+  }
+  // the wave's tokens, then the four waves
+  constexpr int FIRST = S::MM ? 1 : S::LPT, LAST = S::MM ? 16 : LSA_WAVE;
+#pragma unroll
+  for (int x = FIRST; x < LAST; x <<= 1) {
+#pragma unroll
+    for (int h = 0; h < HL; ++h) join(m[h], l[h], lane_xor(m[h], x), lane_xor(l[h], x));
+  }
+  if (S::MM ? (col == 0 && HL * rowq < GQ) : lane == 0) {
+#pragma unroll
+    for (int h = 0; h < HL; ++h) {
+      sm[w][(S::MM ? HL * rowq : 0) + h] = m[h];
+      sl[w][(S::MM ? HL * rowq : 0) + h] = l[h];
+    }
+  }
+  __syncthreads();
+  if (tid < GQ) {
+    float mm = sm[0][tid], ll = sl[0][tid];
+#pragma unroll
+    for (int x = 1; x < LSA_WAVES; ++x) join(mm, ll, sm[x][tid], sl[x][tid]);
+    float* st = a.stats + ((unit * a.n_span + sp) * GQ + tid) * 2;
+    st[0] = mm;
+    st[1] = ll;
+  }
+}
+
+// grid (row * Hkv, slots / 256).
+template <int GQ>
+__global__ __launch_bounds__(LSA_BLOCK) void mass_add_kernel(MassArgs a) {
+  __shared__ float sm[GQ], sinv[GQ];
+  const int tid = threadIdx.x;
+  const int64_t unit = blockIdx.x;
+  const int64_t row = unit / a.Hkv;
+  const int g = (int)(unit % a.Hkv);
+  const MassList list = mass_list(a, row, g);
+  const int j = blockIdx.y * LSA_BLOCK + tid;
+  if (blockIdx.y * LSA_BLOCK >= list.n) return;
+  if (tid < GQ) {
+    float m = kNegBig, l = 0.0f;
+    if (a.lse) {
+      m = a.lse[row * a.Hq + g * GQ + tid] * kLog2e;
+      l = m > -INFINITY ? 1.0f : 0.0f;  // no keys at all, or not a number: no weight
+    } else {
+      const int n_act = (list.n + a.span - 1) / a.span;
+      for (int s = 0; s < n_act; ++s) {
+        const float* st = a.stats + ((unit * a.n_span + s) * GQ + tid) * 2;
+        join(m, l, st[0], st[1]);
+      }
+    }
+    sm[tid] = m;
+    sinv[tid] = l > 0.0f ? 1.0f / l : 0.0f;  // a sum that is not a number counts as none, as in the read
+  }
+  __syncthreads();
+  if (j >= list.n) return;
+  const int32_t id = list.ids[j];
+  if (id < 0 || id >= a.Tk) return;
+  const float* s = a.scores + (unit * (int64_t)a.W + j) * GQ;
+  float sum = 0.0f;
+#pragma unroll
+  for (int h = 0; h < GQ; ++h) {
+    const float x = fast_exp2(s[h] - sm[h]) * sinv[h];
+    sum += sinv[h] > 0.0f && x > 0.0f ? fminf(x, kMaxWeight) : 0.0f;
+  }
+  if (!(sum > 0.0f)) return;
+  const int64_t b = row / a.Tq;
+  const int64_t c = a.caches > 1 ? b : 0;
+  if (a.fixed) {
+    atomicAdd((unsigned long long*)a.fixed + (c * a.Hkv + g) * a.Tk + id,
+              (unsigned long long)__float2ull_rn(sum * kFix));
+  } else {
+    atomicAdd(a.mass + c * a.m_sb + g * a.m_sh + id, sum);
+  }
+}
+
+// The integers into the weights: whole (grid-stride over the caches), or by the lists, where the first
+// to take a key's integer (leaving zero) adds it.
+__global__ __launch_bounds__(LSA_BLOCK) void mass_fold_kernel(MassArgs a) {
+  if (a.whole) {
+    const int64_t grid = (int64_t)gridDim.x * LSA_BLOCK;
+    for (int64_t i = (int64_t)blockIdx.x * LSA_BLOCK + threadIdx.x; i < a.m_n; i += grid) {
+      const uint64_t x = a.fixed[i];
+      if (x == 0) continue;
+      const int64_t cg = i / a.Tk;
+      float* m = a.mass + (cg / a.Hkv) * a.m_sb + (cg % a.Hkv) * a.m_sh + i % a.Tk;
+      *m += (float)((double)x / (double)kFix);
+    }
+    return;
+  }
+  const int64_t unit = blockIdx.x;
+  const int64_t row = unit / a.Hkv;
+  const int g = (int)(unit % a.Hkv);
+  const MassList list = mass_list(a, row, g);
+  const int j = blockIdx.y * LSA_BLOCK + threadIdx.x;
+  if (j >= list.n) return;
+  const int32_t id = list.ids[j];
+  if (id < 0 || id >= a.Tk) return;
+  const int64_t c = a.caches > 1 ? row / a.Tq : 0;
+  const uint64_t x = atomicExch((unsigned long long*)a.fixed + (c * a.Hkv + g) * a.Tk + id, 0ull);
+  if (x) a.mass[c * a.m_sb + g * a.m_sh + id] += (float)((double)x / (double)kFix);
+}
+
+int mass_span(int dtype, int D, int64_t units, int W) {
+  const int loads = dtype == LSA_F32 ? 1 : D / 32;
+  const int tokens = dtype == LSA_F32 ? LSA_WAVE / (D / 4) : 16;
+  const int nt = LSA_WAVES * tokens * (16 / loads);
+  const int64_t want = std::max<int64_t>(1, 1024 / std::max<int64_t>(units, 1));  // workgroups a list
+  const int tiles = (W + nt - 1) / nt;
+  const int per = (int)((tiles + want - 1) / want);
+  return (per > 0 ? per : 1) * nt;
+}
+
+struct MassPlan {
+  int span, n_span;
+  bool fixed, whole;
+  size_t scores, stats, fix, total;
+};
+
+MassPlan mass_plan(int dtype, int64_t B, int64_t Tq, int64_t caches, int64_t Tk, int32_t Hq, int32_t Hkv, int32_t D,
+                   int32_t W) {
+  MassPlan p;
+  const int64_t units = B * Tq * Hkv, gq = Hq / Hkv;
+  p.span = mass_span(dtype, D, units, W);
+  p.n_span = std::max(1, (W + p.span - 1) / p.span);
+  p.fixed = B * Tq > caches;
+  const int64_t cells = caches * Hkv * Tk;
+  p.whole = p.fixed && cells <= 4 * units * (int64_t)W;
+  auto up = [](size_t x) { return (x + 15) / 16 * 16; };
+  p.scores = up((size_t)units * W * gq * 4);
+  p.stats = up((size_t)units * p.n_span * gq * 8);
+  p.fix = p.fixed ? (size_t)cells * 8 : 0;
+  p.total = p.scores + p.stats + p.fix;
+  return p;
+}
+
+template <typename T, int D>
+void launch_scores(const MassArgs& a, int gq, dim3 grid, hipStream_t s) {
+  switch (gq) {
+    case 1: mass_scores_kernel<T, D, 1><<<grid, LSA_BLOCK, 0, s>>>(a); break;
+    case 2: mass_scores_kernel<T, D, 2><<<grid, LSA_BLOCK, 0, s>>>(a); break;
+    case 4: mass_scores_kernel<T, D, 4><<<grid, LSA_BLOCK, 0, s>>>(a); break;
+    default: mass_scores_kernel<T, D, 8><<<grid, LSA_BLOCK, 0, s>>>(a); break;
+  }
+}
+
+template <typename T>
+void launch_scores_d(const MassArgs& a, int D, int gq, dim3 grid, hipStream_t s) {
+  switch (D) {
+    case 32: launch_scores<T, 32>(a, gq, grid, s); break;
+    case 64: launch_scores<T, 64>(a, gq, grid, s); break;
+    case 128: launch_scores<T, 128>(a, gq, grid, s); break;
+    default: launch_scores<T, 256>(a, gq, grid, s); break;
+  }
+}
+
+bool mass_shape_ok(int dtype, int64_t B, int64_t Tq, int64_t caches, int64_t Tk, int32_t Hq, int32_t Hkv, int32_t D,
+                   int32_t W) {
+  if (!(dtype == LSA_F32 || dtype == LSA_BF16 || dtype == LSA_F16)) return false;
+  if (!(D == 32 || D == 64 || D == 128 || D == 256) || Hq < 1 || Hkv < 1 || Hq % Hkv) return false;
+  const int gq = Hq / Hkv;
+  if (!(gq == 1 || gq == 2 || gq == 4 || gq == 8)) return false;
+  return B >= 0 && Tq >= 0 && Tk >= 0 && Tk <= 0x7FFFFFFF && W >= 0 && (caches == B || caches == 1) &&
+         B * Tq <= 0x7FFFFFFF / Hkv;
+}
+
+}  // namespace
+
+extern "C" size_t lsa_key_mass_scratch_bytes(int dtype, int64_t B, int64_t Tq, int64_t caches, int64_t Tk, int32_t Hq,
+                                             int32_t Hkv, int32_t D, int32_t W) {
+  if (!mass_shape_ok(dtype, B, Tq, caches, Tk, Hq, Hkv, D, W) || B * Tq == 0 || W == 0 || Tk == 0) return 0;
+  return mass_plan(dtype, B, Tq, caches, Tk, Hq, Hkv, D, W).total;
+}
+
+extern "C" int lsa_key_mass(const void* q, const void* k, int dtype, int64_t B, int64_t Tq, int64_t caches, int64_t Tk,
+                            int32_t Hq, int32_t Hkv, int32_t D, int64_t k_batch_stride, int64_t k_token_stride,
+                            int64_t k_head_stride, const int32_t* ids, const int32_t* lengths, int32_t W,
+                            int ids_per_head, float scale, const float* lse, int zero_first, void* scratch,
+                            size_t scratch_bytes, float* mass, int64_t mass_batch_stride, int64_t mass_head_stride,
+                            void* stream) {
+  LSA_REQUIRE(q && k && ids && lengths && mass, LSA_ERR_NULL, "lsa_key_mass: NULL pointer");
+  LSA_TRY(check_dtype(dtype));
+  LSA_REQUIRE(mass_shape_ok(dtype, B, Tq, caches, Tk, Hq, Hkv, D, W), LSA_ERR_SHAPE,
+              "lsa_key_mass: B %lld Tq %lld caches %lld Tk %lld Hq %d Hkv %d D %d W %d (D in {32,64,128,256}, groups of "
+              "1/2/4/8, B caches or 1)", (long long)B, (long long)Tq, (long long)caches, (long long)Tk, Hq, Hkv, D, W);
+  const int64_t e = dtype == LSA_F32 ? 4 : 2;
+  LSA_REQUIRE(k_batch_stride >= 0 && k_token_stride >= D && k_head_stride >= D && mass_batch_stride >= 0 &&
+                  mass_head_stride >= 0, LSA_ERR_SHAPE, "lsa_key_mass: strides must leave rows apart");
+  LSA_REQUIRE((((uintptr_t)q | (uintptr_t)k) & 15) == 0 &&
+                  ((k_batch_stride | k_token_stride | k_head_stride) * e) % 16 == 0, LSA_ERR_ALIGN,
+              "lsa_key_mass: q and K rows must be 16-byte aligned");
+  LSA_REQUIRE(!zero_first || (mass_head_stride == Tk && mass_batch_stride == Hkv * Tk), LSA_ERR_SHAPE,
+              "lsa_key_mass: weights that begin at zero must be dense");
+  if (B * Tq == 0 || W == 0 || Tk == 0) return LSA_OK;
+  const MassPlan p = mass_plan(dtype, B, Tq, caches, Tk, Hq, Hkv, D, W);
+  LSA_REQUIRE(scratch && scratch_bytes >= p.total && ((uintptr_t)scratch & 15) == 0, LSA_ERR_WORKSPACE,
+              "lsa_key_mass: scratch missing, not 16-byte aligned or %zu < %zu bytes", scratch_bytes, p.total);
+  const int64_t units = B * Tq * Hkv;
+  const int64_t chunks = ((int64_t)W + LSA_BLOCK - 1) / LSA_BLOCK;
+  LSA_REQUIRE(p.n_span <= 65535 && chunks <= 65535, LSA_ERR_SHAPE, "lsa_key_mass: lists of %d slots are too wide", W);
+  MassArgs a = {};
+  a.q = q; a.k = k; a.ids = ids; a.lengths = lengths; a.lse = lse; a.Tq = Tq; a.Tk = Tk;
+  a.k_sb = caches > 1 ? k_batch_stride : 0; a.k_st = k_token_stride; a.k_sh = k_head_stride;
+  a.Hq = Hq; a.Hkv = Hkv; a.W = W; a.per_head = ids_per_head ? 1 : 0; a.scale_log2 = scale * kLog2e;
+  a.span = p.span; a.n_span = p.n_span;
+  a.scores = (float*)scratch;
+  a.stats = (float*)((char*)scratch + p.scores);
+  a.fixed = p.fixed ? (uint64_t*)((char*)scratch + p.scores + p.stats) : nullptr;
+  a.whole = p.whole ? 1 : 0;
+  a.mass = mass; a.m_sb = caches > 1 ? mass_batch_stride : 0; a.m_sh = mass_head_stride;
+  a.m_n = caches * Hkv * Tk; a.caches = (int)caches; a.zero = zero_first ? 1 : 0;
+  hipStream_t s = (hipStream_t)stream;
+  const int gq = Hq / Hkv;
+  const dim3 grid((unsigned)units, (unsigned)p.n_span);
+  if (dtype == LSA_BF16) launch_scores_d<bf16_t>(a, D, gq, grid, s);
+  else if (dtype == LSA_F16) launch_scores_d<_Float16>(a, D, gq, grid, s);
+  else launch_scores_d<float>(a, D, gq, grid, s);
+  LSA_LAUNCHED("lsa_key_mass");
+  const dim3 add((unsigned)units, (unsigned)chunks);
+  switch (gq) {
+    case 1: mass_add_kernel<1><<<add, LSA_BLOCK, 0, s>>>(a); break;
+    case 2: mass_add_kernel<2><<<add, LSA_BLOCK, 0, s>>>(a); break;
+    case 4: mass_add_kernel<4><<<add, LSA_BLOCK, 0, s>>>(a); break;
+    default: mass_add_kernel<8><<<add, LSA_BLOCK, 0, s>>>(a); break;
+  }
+  LSA_LAUNCHED("lsa_key_mass");
+  if (p.fixed) {
+    const dim3 fold = p.whole ? dim3((unsigned)std::min<int64_t>((a.m_n + LSA_BLOCK - 1) / LSA_BLOCK, 4096)) : add;
+    mass_fold_kernel<<<fold, LSA_BLOCK, 0, s>>>(a);
+    LSA_LAUNCHED("lsa_key_mass");
+  }
+  return LSA_OK;
+}

@@ -219,15 +219,16 @@ struct AttnState {
 // the loads it does not feed (memory counters retire in order, so a wait for an id must
 // not also wait for the rows in flight). The V side's ids come from the K side's by lane
 // permutes. Slots past the span read -1 (a partial last tile): those rows load token 0
-// (cache hits) and weigh nothing.
-template <typename T, int D, int GQ>
+// (cache hits) and weigh nothing. With ZERO their V rows count as zeros, so that token 0 may hold
+// anything; without, a token 0 that is not finite makes the sum so.
+template <typename T, int D, int GQ, bool ZERO = false>
 struct MfmaTile {
   static constexpr int NM = D / 32;
   uint4 k[NM], v[4];
-  bool ok[4];
+  bool ok[4], okv[ZERO ? 4 : 1];
 };
 
-template <typename T, int D, int GQ, bool PIPE, typename IdOf>
+template <typename T, int D, int GQ, bool PIPE, bool ZERO, typename IdOf>
 __device__ __forceinline__ void attend_tiles_mfma(const QueryRegs<T, D, GQ>& q, const T* kb, const T* vb,
                                                   int64_t tstride, int64_t Tk, int lo, int hi, IdOf id_of,
                                                   float scale_log2, AttnState<T, D, GQ>& st) {
@@ -245,7 +246,7 @@ __device__ __forceinline__ void attend_tiles_mfma(const QueryRegs<T, D, GQ>& q, 
     lrun = col == h ? st.l[h] : lrun;
   }
 
-  auto issue = [&](int32_t idk, MfmaTile<T, D, GQ>& t) {
+  auto issue = [&](int32_t idk, MfmaTile<T, D, GQ, ZERO>& t) {
     const bool okk = idk >= 0 && idk < Tk;
     const uint64_t koff = (uint64_t)(uint32_t)(okk ? idk : 0) * (uint32_t)tstride;
 #pragma unroll
@@ -255,10 +256,11 @@ __device__ __forceinline__ void attend_tiles_mfma(const QueryRegs<T, D, GQ>& q, 
       const int32_t idv = __shfl(idk, 4 * row + u, LSA_WAVE);  // token 4 row + u's id
       const bool okv = idv >= 0 && idv < Tk;
       t.ok[u] = okv && col < GQ;
+      if constexpr (ZERO) t.okv[u] = okv;
       t.v[u] = *(const uint4*)(vb + (uint64_t)(uint32_t)(okv ? idv : 0) * (uint32_t)tstride);
     }
   };
-  auto compute = [&](const MfmaTile<T, D, GQ>& t) {
+  auto compute = [&](const MfmaTile<T, D, GQ, ZERO>& t) {
     f32x4_t c = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < NM; ++i) c = Mfma16<T>::run(t.k[i], q.qm[i], c);
@@ -299,7 +301,8 @@ __device__ __forceinline__ void attend_tiles_mfma(const QueryRegs<T, D, GQ>& q, 
 #pragma unroll
       for (int h = 0; h < GQ; ++h) ph[h] = pw[w][4 * row + u][h];
       float vf[VEC];
-      Row16<T>::cvt(t.v[u], vf);
+      if constexpr (ZERO) Row16<T>::cvt(t.okv[u] ? t.v[u] : make_uint4(0u, 0u, 0u, 0u), vf);
+      else Row16<T>::cvt(t.v[u], vf);
 #pragma unroll
       for (int h = 0; h < GQ; ++h) {
 #pragma unroll
@@ -317,7 +320,7 @@ __device__ __forceinline__ void attend_tiles_mfma(const QueryRegs<T, D, GQ>& q, 
     // next tile's rows land in the other buffer while this one is computed. A copy from
     // a "next" buffer into a "current" one would wait for the rows in flight, which
     // leaves one tile's gather exposed every iteration.
-    MfmaTile<T, D, GQ> ta, tb;
+    MfmaTile<T, D, GQ, ZERO> ta, tb;
     // One exit, at the loop's head: a loop with exits in its middle is folded into one exit
     // behind a flow block that re-enters the head with rows still in flight, and the head
     // then waits for all of them.
@@ -342,7 +345,7 @@ __device__ __forceinline__ void attend_tiles_mfma(const QueryRegs<T, D, GQ>& q, 
       compute(ta);
     }
   } else {
-    MfmaTile<T, D, GQ> cur;
+    MfmaTile<T, D, GQ, ZERO> cur;
     int32_t id1 = id_of(lo + s0);
     for (int base = lo; base < hi; base += NT) {
       issue(id1, cur);
@@ -361,12 +364,13 @@ __device__ __forceinline__ void attend_tiles_mfma(const QueryRegs<T, D, GQ>& q, 
 // slot j, or -1 (skipped); it must be cheap and unconditional (a clamped load or an LDS
 // read). kb / vb point at the kv-head's row 0 plus this lane's VEC-element offset. fresh:
 // the state is empty, so the first tile needs no rescale.
-template <typename T, int D, int GQ, bool PIPE = false, typename IdOf>
+// ZERO: skipped slots' V rows count as zeros (see MfmaTile).
+template <typename T, int D, int GQ, bool PIPE = false, bool ZERO = false, typename IdOf>
 __device__ __forceinline__ void attend_tiles(const QueryRegs<T, D, GQ>& q, const T* kb, const T* vb, int64_t tstride,
                                              int64_t Tk, int lo, int hi, IdOf id_of, float scale_log2, bool fresh,
                                              AttnState<T, D, GQ>& st) {
   if constexpr (ReadMfma<T, D, GQ>::ON) {
-    attend_tiles_mfma<T, D, GQ, PIPE>(q, kb, vb, tstride, Tk, lo, hi, id_of, scale_log2, st);
+    attend_tiles_mfma<T, D, GQ, PIPE, ZERO>(q, kb, vb, tstride, Tk, lo, hi, id_of, scale_log2, st);
     return;
   }
   using S = ReadShape<T, D, GQ>;
@@ -434,7 +438,8 @@ __device__ __forceinline__ void attend_tiles(const QueryRegs<T, D, GQ>& q, const
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float vf[VEC];
-      Row16<T>::cvt(vr[u], vf);
+      if constexpr (ZERO) Row16<T>::cvt(ok[u] ? vr[u] : make_uint4(0u, 0u, 0u, 0u), vf);
+      else Row16<T>::cvt(vr[u], vf);
 #pragma unroll
       for (int h = 0; h < GQ; ++h) {
         st.l[h] += sc[h][u];
@@ -472,13 +477,13 @@ __device__ __forceinline__ void merge_token_groups(AttnState<T, D, GQ>& st) {
 
 // Attention of the GQ query heads of one kv-head over list slots [lo, hi) from an empty
 // state, token groups merged (qrow: the GQ contiguous query rows).
-template <typename T, int D, int GQ, typename IdOf>
+template <typename T, int D, int GQ, bool ZERO = false, typename IdOf>
 __device__ __forceinline__ void attend_span(const T* qrow, const T* kb, const T* vb, int64_t tstride, int64_t Tk,
                                             int lo, int hi, IdOf id_of, float scale_log2, AttnState<T, D, GQ>& st) {
   QueryRegs<T, D, GQ> q;
   q.load(qrow, scale_log2);
   st.clear();
-  attend_tiles<T, D, GQ, true>(q, kb, vb, tstride, Tk, lo, hi, id_of, scale_log2, true, st);
+  attend_tiles<T, D, GQ, true, ZERO>(q, kb, vb, tstride, Tk, lo, hi, id_of, scale_log2, true, st);
   merge_token_groups<T, D, GQ>(st);
 }
 

@@ -1,0 +1,283 @@
+// Attention of a batch over prefixes that its rows share, and over each row's own read list,
+// for gfx950.
+//
+// The softmax over both parts is one: each part leaves partials (running maximum m, sum l and
+// weighted value row, in fp32, log2 domain), and the usual rescaling joins them.
+//
+//   prefix_gather_kernel  a prefix's partials row by row (any type and head dim);
+//   prefix_join_kernel    a row's own list (the gather read's span loop) and the join.
+//
+// A prefix of n keys is cut into pieces of whole 64-key tiles, a workgroup a piece, the same for
+// both kernels (prefix_pieces). Partials of (row, kv-head) unit i: piece s of n_p at
+// [i][splits - n_p + s], the own list's spans behind them, so the join finds them in a line.
+#include <math.h>
+
+#include <algorithm>
+
+#include "lsa_abi_common.h"
+#include "lsa_read_dev.h"
+
+using namespace lsa;
+
+namespace {
+
+constexpr int kPieceTile = 64;  // keys; a piece is a multiple of it
+constexpr int kMaxPieces = 128;
+constexpr int kMaxOwn = 64;
+
+struct PrefixArgs {
+  const void* q;
+  const void* kp;
+  const void* vp;
+  const int32_t* prefix_rows;     // [B] or nullptr: 0
+  const int32_t* prefix_lengths;  // [P] or nullptr: Tp
+  const int32_t* slots;           // [P, Tp] cache rows of a pool, or nullptr
+  int64_t slot_stride, pool;      // rows the prefix cache holds a batch entry
+  int64_t p_sb, p_st, p_sh;
+  const void* k;
+  const void* v;
+  int64_t kv_sb, kv_st, kv_sh, Tk;
+  const int32_t* ids;
+  const int32_t* lengths;
+  int W, per_head;
+  int64_t B, Tq, Tp;
+  int P, Hq, Hkv;
+  float scale_log2;
+  int splits;      // pieces of a prefix at most
+  int own_splits;  // spans of an own list at most
+  int own_span;    // list slots of a span
+  int* counters;   // [units]: cleared by the prefix kernel, arrivals of the own spans
+  float* parts;    // [units][splits + own_splits][GQ (D + 2)]
+  void* out;
+  float* lse;      // [B, Tq, Hq] or nullptr
+};
+
+struct Pieces {
+  int n;      // keys
+  int count;  // pieces with keys in them
+  int keys;   // of a piece
+};
+
+__device__ __forceinline__ Pieces prefix_pieces(const PrefixArgs& a, int p) {
+  Pieces x{0, 0, kPieceTile};
+  if (p < 0 || p >= a.P) return x;  // no prefix
+  const int64_t n = a.prefix_lengths ? (int64_t)a.prefix_lengths[p] : a.Tp;
+  x.n = (int)(n < 0 ? 0 : (n > a.Tp ? a.Tp : n));
+  const int tiles = (x.n + kPieceTile - 1) / kPieceTile;
+  const int per = (tiles + a.splits - 1) / a.splits;
+  x.keys = (per > 0 ? per : 1) * kPieceTile;
+  x.count = (x.n + x.keys - 1) / x.keys;
+  return x;
+}
+__device__ __forceinline__ int prefix_of(const PrefixArgs& a, int64_t b) {
+  return a.prefix_rows ? a.prefix_rows[b] : 0;
+}
+
+// grid (row * Hkv, piece).
+template <typename T, int D, int GQ>
+__global__ __launch_bounds__(LSA_BLOCK) void prefix_gather_kernel(PrefixArgs a) {
+  __shared__ ReadLds<D, GQ, kMaxPieces + kMaxOwn> sh;
+  constexpr int PSTRIDE = GQ * (D + 2);
+  const int64_t i = blockIdx.x, row = i / a.Hkv;
+  const int g = (int)(i % a.Hkv), s = blockIdx.y;
+  if (s == 0 && threadIdx.x == 0) a.counters[i] = 0;
+  const int p = prefix_of(a, row / a.Tq);
+  const Pieces pc = prefix_pieces(a, p);
+  if (s >= pc.count) return;
+  const int lo = s * pc.keys, hi = min(lo + pc.keys, pc.n);
+  const int lp = (threadIdx.x & (LSA_WAVE - 1)) % ReadShape<T, D, GQ>::LPT;
+  const int64_t at = (a.slots ? 0 : p * a.p_sb) + g * a.p_sh + lp * ReadShape<T, D, GQ>::VEC;
+  const int32_t* slots = a.slots ? a.slots + p * a.slot_stride : nullptr;
+  AttnState<T, D, GQ> st;
+  attend_span<T, D, GQ, true>((const T*)a.q + (row * a.Hq + (int64_t)g * GQ) * D, (const T*)a.kp + at, (const T*)a.vp + at,
+                        a.p_st, a.pool, lo, hi,
+                        [&](int j) {
+                          const int jc = j < hi ? j : hi - 1;
+                          const int32_t id = slots ? slots[jc] : jc;
+                          return j < hi ? id : -1;
+                        },
+                        a.scale_log2, st);
+  float* part = a.parts + (i * (a.splits + a.own_splits) + a.splits - pc.count + s) * (int64_t)PSTRIDE;
+  finish_span<T, D, GQ, kMaxPieces + kMaxOwn, true>(sh, st, false, (T*)nullptr, part, 0);
+}
+
+// grid (row * Hkv, own span). The last span of a unit to arrive joins the unit's partials.
+template <typename T, int D, int GQ>
+__global__ __launch_bounds__(LSA_BLOCK) void prefix_join_kernel(PrefixArgs a) {
+  __shared__ ReadLds<D, GQ, kMaxPieces + kMaxOwn> sh;
+  constexpr int PSTRIDE = GQ * (D + 2);
+  const int64_t i = blockIdx.x, row = i / a.Hkv;
+  const int g = (int)(i % a.Hkv), s = blockIdx.y;
+  const int64_t b = row / a.Tq;
+  int n = 0;
+  const int32_t* list = nullptr;
+  if (a.W > 0) {
+    const int64_t li = a.per_head ? row * a.Hkv + g : row;
+    n = a.lengths[li];
+    n = (n < 0 || a.Tk <= 0) ? 0 : (n > a.W ? a.W : n);
+    list = a.ids + li * a.W;
+  }
+  const int n_own = (n + a.own_span - 1) / a.own_span;
+  if (s >= max(n_own, 1)) return;
+  const Pieces pc = prefix_pieces(a, prefix_of(a, b));
+  float* parts = a.parts + (i * (a.splits + a.own_splits) + a.splits - pc.count) * (int64_t)PSTRIDE;
+  if (n > 0) {
+    const int lo = s * a.own_span, hi = min(lo + a.own_span, n);
+    const int lp = (threadIdx.x & (LSA_WAVE - 1)) % ReadShape<T, D, GQ>::LPT;
+    const int64_t at = b * a.kv_sb + g * a.kv_sh + lp * ReadShape<T, D, GQ>::VEC;
+    AttnState<T, D, GQ> st;
+    attend_span<T, D, GQ, true>((const T*)a.q + (row * a.Hq + (int64_t)g * GQ) * D, (const T*)a.k + at, (const T*)a.v + at,
+                          a.kv_st, a.Tk, lo, hi,
+                          [&](int j) {
+                            const int32_t id = list[j < hi ? j : hi - 1];
+                            return j < hi ? id : -1;
+                          },
+                          a.scale_log2, st);
+    finish_span<T, D, GQ, kMaxPieces + kMaxOwn, true>(sh, st, false, (T*)nullptr,
+                                                      parts + (int64_t)(pc.count + s) * PSTRIDE, 0);
+    // the partials complete before they are read back, by this workgroup or the last one
+    if (!arrive_last(&a.counters[i], n_own, &sh.flag)) return;
+  }
+  const int total = pc.count + n_own;
+  T* outp = (T*)a.out + (row * a.Hq + (int64_t)g * GQ) * D;
+  if (total == 0) {
+    for (int j = threadIdx.x; j < GQ * D; j += LSA_BLOCK) store_out<T>(outp + j, 0.0f);
+  } else {
+    combine_partials<T, D, GQ>(sh, parts, total, outp, 0);
+  }
+  if (a.lse) {
+    const int lane = threadIdx.x & (LSA_WAVE - 1);
+    for (int h = threadIdx.x / LSA_WAVE; h < GQ; h += LSA_WAVES) {
+      float M = kNegBig;
+      for (int x = lane; x < total; x += LSA_WAVE) M = fmaxf(M, coherent_load(parts + (int64_t)x * PSTRIDE + h));
+      M = wave_max(M);
+      if (lane == 0) {
+        const float L = total ? sh.ltot[h] : 0.0f;
+        // no keys, or a sum that is not a number, which counts as none
+        a.lse[row * a.Hq + g * GQ + h] = L > 0.0f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+      }
+    }
+  }
+}
+
+struct PrefixPlan {
+  int splits, own_splits, own_span;
+  size_t parts, total;
+};
+
+// Pieces and own spans by size. About 512 workgroups of pieces; own spans of at least 256 slots,
+// as many as make 512 workgroups.
+PrefixPlan prefix_plan(int dtype, int64_t B, int64_t Tq, int64_t Tp, int32_t Hq, int32_t Hkv, int32_t D, int32_t W) {
+  PrefixPlan p;
+  const int64_t units = B * Tq * Hkv;
+  const int64_t tiles = (Tp + kPieceTile - 1) / kPieceTile;
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({tiles, kMaxPieces, 512 / std::max<int64_t>(units, 1)}));
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kMaxOwn, 512 / std::max<int64_t>(units, 1)));
+  const int64_t per = std::max<int64_t>((W + want - 1) / want, 256);
+  p.own_span = (int)((per + 63) / 64 * 64);
+  p.own_splits = std::max(1, (W + p.own_span - 1) / p.own_span);
+  const int64_t gq = Hq / Hkv;
+  p.parts = (size_t)units * (p.splits + p.own_splits) * (size_t)(gq * (D + 2)) * sizeof(float);
+  p.total = p.parts + (size_t)units * sizeof(int);
+  return p;
+}
+
+bool prefix_shape_ok(int dtype, int64_t B, int64_t Tq, int64_t P, int64_t Tp, int32_t Hq, int32_t Hkv, int32_t D,
+                     int32_t W) {
+  if (!(dtype == LSA_F32 || dtype == LSA_BF16 || dtype == LSA_F16)) return false;
+  if (!(D == 32 || D == 64 || D == 128 || D == 256) || Hq < 1 || Hkv < 1 || Hq % Hkv) return false;
+  const int gq = Hq / Hkv;
+  if (!(gq == 1 || gq == 2 || gq == 4 || gq == 8)) return false;
+  return B >= 0 && Tq >= 0 && B <= 0x7FFFFFFF && Tq <= 0x7FFFFFFF && B * Tq <= 0x7FFFFFFF / Hq && P >= 1 && P <= 65535 &&
+         Tp >= 0 && Tp <= 0x7FFFFFC0 && W >= 0 && W <= 0x7FFFFFC0;
+}
+
+template <typename T, int D>
+void launch_prefix_gq(const PrefixArgs& a, int gq, int64_t units, hipStream_t s) {
+  const dim3 gp((unsigned)units, (unsigned)a.splits), go((unsigned)units, (unsigned)a.own_splits);
+#define LSA_PREFIX(GQ)                                         \
+  prefix_gather_kernel<T, D, GQ><<<gp, LSA_BLOCK, 0, s>>>(a);  \
+  prefix_join_kernel<T, D, GQ><<<go, LSA_BLOCK, 0, s>>>(a)
+  switch (gq) {
+    case 1: LSA_PREFIX(1); break;
+    case 2: LSA_PREFIX(2); break;
+    case 4: LSA_PREFIX(4); break;
+    default: LSA_PREFIX(8); break;
+  }
+#undef LSA_PREFIX
+}
+
+template <typename T>
+void launch_prefix(const PrefixArgs& a, int D, int gq, int64_t units, hipStream_t s) {
+  switch (D) {
+    case 32: launch_prefix_gq<T, 32>(a, gq, units, s); break;
+    case 64: launch_prefix_gq<T, 64>(a, gq, units, s); break;
+    case 128: launch_prefix_gq<T, 128>(a, gq, units, s); break;
+    default: launch_prefix_gq<T, 256>(a, gq, units, s); break;
+  }
+}
+
+}  // namespace
+
+extern "C" size_t lsa_prefix_read_scratch_bytes(int dtype, int64_t B, int64_t Tq, int64_t P, int64_t Tp, int32_t Hq,
+                                                int32_t Hkv, int32_t D, int32_t W) {
+  if (!prefix_shape_ok(dtype, B, Tq, P, Tp, Hq, Hkv, D, W) || B * Tq == 0) return 0;
+  return prefix_plan(dtype, B, Tq, Tp, Hq, Hkv, D, W).total;
+}
+
+extern "C" int lsa_prefix_read(const void* q, const void* k_prefix, const void* v_prefix, int dtype, int64_t B,
+                               int64_t Tq, int64_t P, int64_t Tp, int64_t prefix_cache_rows, int32_t Hq, int32_t Hkv,
+                               int32_t D, int64_t prefix_batch_stride, int64_t prefix_token_stride,
+                               int64_t prefix_head_stride, const int32_t* prefix_rows, const int32_t* prefix_lengths,
+                               const int32_t* prefix_slots, int64_t prefix_slot_stride, const void* k, const void* v,
+                               int64_t Tk, int64_t kv_batch_stride, int64_t kv_token_stride, int64_t kv_head_stride,
+                               const int32_t* ids, const int32_t* lengths, int32_t W, int ids_per_head, float scale,
+                               void* scratch, size_t scratch_bytes, void* out, float* lse, void* stream) {
+  LSA_REQUIRE(q && out && (Tp == 0 || (k_prefix && v_prefix)), LSA_ERR_NULL, "lsa_prefix_read: NULL pointer");
+  LSA_TRY(check_dtype(dtype));
+  LSA_REQUIRE(prefix_shape_ok(dtype, B, Tq, P, Tp, Hq, Hkv, D, W), LSA_ERR_SHAPE,
+              "lsa_prefix_read: B %lld Tq %lld P %lld Tp %lld Hq %d Hkv %d D %d W %d (D in {32,64,128,256}, groups of "
+              "1/2/4/8, 1..65535 prefixes)", (long long)B, (long long)Tq, (long long)P, (long long)Tp, Hq, Hkv, D, W);
+  LSA_REQUIRE(W == 0 || (k && v && ids && lengths && Tk >= 0 && Tk <= 0x7FFFFFFF), LSA_ERR_NULL,
+              "lsa_prefix_read: own lists need K, V, ids and lengths");
+  LSA_REQUIRE(prefix_cache_rows >= 0 && prefix_cache_rows <= 0x7FFFFFFF && (prefix_slots || prefix_cache_rows >= Tp),
+              LSA_ERR_SHAPE, "lsa_prefix_read: a prefix cache of %lld rows for prefixes of %lld",
+              (long long)prefix_cache_rows, (long long)Tp);
+  LSA_REQUIRE(!prefix_slots || (prefix_slot_stride >= Tp && prefix_cache_rows >= 1), LSA_ERR_SHAPE,
+              "lsa_prefix_read: slot rows of stride %lld for %lld positions", (long long)prefix_slot_stride, (long long)Tp);
+  const int64_t e = dtype == LSA_F32 ? 4 : 2;
+  const bool own = W > 0;
+  LSA_REQUIRE(prefix_batch_stride >= 0 && prefix_token_stride >= D && prefix_head_stride >= D &&
+                  (!own || (kv_batch_stride >= 0 && kv_token_stride >= D && kv_head_stride >= D)),
+              LSA_ERR_SHAPE, "lsa_prefix_read: K/V strides must leave rows of %d elements apart", D);
+  LSA_REQUIRE((((uintptr_t)q | (uintptr_t)k_prefix | (uintptr_t)v_prefix | (own ? (uintptr_t)k | (uintptr_t)v : 0)) & 15) == 0 &&
+                  ((prefix_batch_stride | prefix_token_stride | prefix_head_stride |
+                    (own ? kv_batch_stride | kv_token_stride | kv_head_stride : 0)) * e) % 16 == 0,
+              LSA_ERR_ALIGN, "lsa_prefix_read: q and K/V rows must be 16-byte aligned");
+  // the span loop multiplies a 32-bit row by a 32-bit stride
+  LSA_REQUIRE(prefix_token_stride <= 0x7FFFFFFF && (!own || kv_token_stride <= 0x7FFFFFFF), LSA_ERR_SHAPE,
+              "lsa_prefix_read: token strides past 2^31 elements");
+  if (B * Tq == 0) return LSA_OK;
+  const PrefixPlan p = prefix_plan(dtype, B, Tq, Tp, Hq, Hkv, D, W);
+  LSA_REQUIRE(scratch && scratch_bytes >= p.total && ((uintptr_t)scratch & 15) == 0, LSA_ERR_WORKSPACE,
+              "lsa_prefix_read: scratch missing, not 16-byte aligned or %zu < %zu bytes", scratch_bytes, p.total);
+  PrefixArgs a = {};
+  a.q = q; a.kp = k_prefix; a.vp = v_prefix; a.prefix_rows = prefix_rows; a.prefix_lengths = prefix_lengths;
+  a.slots = prefix_slots; a.slot_stride = prefix_slot_stride; a.pool = prefix_slots ? prefix_cache_rows : Tp;
+  a.p_sb = prefix_batch_stride; a.p_st = prefix_token_stride; a.p_sh = prefix_head_stride;
+  a.k = k; a.v = v; a.kv_sb = kv_batch_stride; a.kv_st = kv_token_stride; a.kv_sh = kv_head_stride; a.Tk = Tk;
+  a.ids = ids; a.lengths = lengths; a.W = W; a.per_head = ids_per_head ? 1 : 0;
+  a.B = B; a.Tq = Tq; a.Tp = Tp; a.P = (int)P; a.Hq = Hq; a.Hkv = Hkv; a.scale_log2 = scale * kLog2e;
+  a.splits = p.splits; a.own_splits = p.own_splits; a.own_span = p.own_span;
+  a.parts = (float*)scratch;
+  a.counters = (int*)((char*)scratch + p.parts);
+  a.out = out; a.lse = lse;
+  hipStream_t s = (hipStream_t)stream;
+  const int64_t units = B * Tq * Hkv;
+  const int gq = Hq / Hkv;
+  if (dtype == LSA_BF16) launch_prefix<bf16_t>(a, D, gq, units, s);
+  else if (dtype == LSA_F16) launch_prefix<_Float16>(a, D, gq, units, s);
+  else launch_prefix<float>(a, D, gq, units, s);
+  LSA_LAUNCHED("lsa_prefix_read");
+  return LSA_OK;
+}

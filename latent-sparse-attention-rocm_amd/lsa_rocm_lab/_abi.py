@@ -105,6 +105,18 @@ SIGNATURES = {
     "lsa_decode_flat_noalloc": (_int, [_p, _p, _p, _int, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _i64, _p, _p, _p,
                                        _i32, _i32, _i32, _i64, _i64, _int, _p, _i32, _i32, _i32, _i32, _i32, _i32,
                                        _f32, _i32, _i32, _i32, _p, _p, _p, _p, _p]),
+    "lsa_prefix_read_scratch_bytes": (_sz, [_int, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32]),
+    "lsa_prefix_read": (_int, [_p, _p, _p, _int, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _i64, _p,
+                               _p, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _i32, _int, _f32, _p, _sz, _p, _p,
+                               _p]),
+    "lsa_key_mass_scratch_bytes": (_sz, [_int, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32]),
+    "lsa_key_mass": (_int, [_p, _p, _int, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _i64, _p, _p, _i32,
+                            _int, _f32, _p, _int, _p, _sz, _p, _i64, _i64, _p]),
+    "lsa_evict_scratch_bytes": (_sz, [_i64, _i64, _int]),
+    "lsa_evict_keep": (_int, [_p, _i64, _i32, _i64, _i64, _i64, _p, _i32, _i32, _i32, _int, _p, _i64, _i64, _p, _sz, _p,
+                              _p, _p, _i64, _p]),
+    "lsa_evict_rows": (_int, [_p, _p, _p, _int, _i64, _i64, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _p, _int, _i32,
+                              _p, _p, _i64, _i64, _i64, _p, _i64, _i64, _int, _p]),
 }
 
 
@@ -244,6 +256,15 @@ class Workspace:
             buf = torch.empty(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
             cls._buffers[key] = buf
         return buf
+
+
+def scratch(device: torch.device, purpose: str, nbytes: int) -> torch.Tensor | None:
+    """Scratch of one call whose kernels need nothing of it afterwards: ``Workspace``'s, or,
+    while a HIP graph is captured, memory of that graph's own pool, so that graphs captured on
+    one stream may be replayed on several at once."""
+    if nbytes > 0 and torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return Workspace.get(device, purpose, nbytes)
 
 
 class Counters:

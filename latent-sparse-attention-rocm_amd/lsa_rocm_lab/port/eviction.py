@@ -1,0 +1,236 @@
+"""A cache that is cut down to the keys that carry attention weight.
+
+``key_mass`` adds up the softmax weight each listed key received (from decode steps as they run,
+or from a prompt's last rows); ``evict`` keeps the heaviest keys of a dense cache, beside its
+first and last ones, and ``evict_slots`` does so for a paged cache by reordering its slot table.
+The kept keys stay in their order, so bucket tables are built over the smaller cache as over any
+other (``pipeline.segment_buckets``, ``build_buckets``). No counterpart in the reference.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from lsa_rocm_lab import _abi
+from lsa_rocm_lab.port.shared_prefix import aligned, cache_pair, cache_strides, int32_on, launch_device, lists_of, one_device
+
+_SLAB_BYTES = 256 << 20  # scores of query rows held at once (more rows go through in slabs)
+
+
+def key_mass(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    read_lists: torch.Tensor,
+    lengths: torch.Tensor,
+    scale: float | None = None,
+    lse: torch.Tensor | None = None,
+    mass: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """The attention weight that each listed key receives, summed over the query rows of its
+    cache and the query heads of its kv-head.
+
+    q [B, Tq, Hq, D], k [B, Tk, Hkv, D] (or one pool [1, Tk, Hkv, D] for every row),
+    ``read_lists`` / ``lengths`` as ``lsa_read`` takes them (``[B, Tq, W]`` or ``[B, Tq, Hkv, W]``;
+    ids outside the cache are skipped, a key listed twice counts twice). The weights are of the
+    softmax over the row's list, or, with ``lse`` [B, Tq, Hq] (``prefix_read(return_lse=True)``'s),
+    of the wider softmax it belongs to. A row whose sum is not a number gives none, as it reads
+    as no keys in ``lsa_read``. Returns [B or 1, Hkv, Tk] fp32: new, or ``mass`` with the weights
+    added in place. The bits do not depend on the order in which rows and workgroups run.
+    """
+    device = one_device("key_mass", q, k, lse, mass)
+    if q.dim() != 4 or k.dim() != 4 or k.shape[0] not in (q.shape[0], 1) or k.shape[3] != q.shape[3]:
+        raise ValueError(f"key_mass: q [B, Tq, Hq, D] and k [B or 1, Tk, Hkv, D], got {tuple(q.shape)} and "
+                         f"{tuple(k.shape)}")
+    if q.dtype != k.dtype:
+        raise ValueError(f"key_mass: q/k dtypes differ: {q.dtype} {k.dtype}")
+    dt = _abi.dtype_code(q.dtype)
+    B, Tq, Hq, D = q.shape
+    caches, Tk, Hkv = k.shape[:3]
+    if Hkv < 1 or Hq % Hkv:
+        raise ValueError(f"key_mass: {Hq} query heads do not group onto {Hkv} kv-heads")
+    ids, lens, W, per_head = lists_of(read_lists, lengths, B * Tq, Hkv, device)
+    if lse is not None and (tuple(lse.shape) != (B, Tq, Hq) or lse.dtype != torch.float32):
+        raise ValueError(f"key_mass: lse must be fp32 [{B}, {Tq}, {Hq}], got {lse.dtype} {tuple(lse.shape)}")
+    fresh = mass is None
+    if fresh:
+        mass = torch.empty(caches, Hkv, Tk, dtype=torch.float32, device=device)
+    elif (tuple(mass.shape) != (caches, Hkv, Tk) or mass.dtype != torch.float32 or (Tk > 1 and mass.stride(2) != 1)
+          or (Hkv > 1 and mass.stride(1) < Tk) or (caches > 1 and mass.stride(0) < Tk)):
+        raise ValueError(f"key_mass: mass must be fp32 [{caches}, {Hkv}, {Tk}] with contiguous keys, got {mass.dtype} "
+                         f"{tuple(mass.shape)} at strides {mass.stride()}")
+    if B * Tq == 0 or W == 0 or Tk == 0:
+        return mass.zero_() if fresh else mass
+    q = aligned(q)
+    if k.stride(-1) != 1 or k.data_ptr() % 16:
+        k = aligned(k)
+    sb, st, sh = cache_strides(k)
+    lse = None if lse is None else lse.contiguous()
+    scale = float(D ** -0.5 if scale is None else scale)
+    # every query row's scores are held until its sums are known
+    step = Tq if 4 * B * Tq * Hq * W <= _SLAB_BYTES else max(1, _SLAB_BYTES // (4 * B * Hq * W))
+    with launch_device(device):
+        for t in range(0, Tq, step):
+            n = min(step, Tq - t)
+            part, pids, plens, plse = q, ids, lens, lse
+            if n != Tq:  # rows t .. t + n of every batch row
+                part = q[:, t:t + n].contiguous()
+                pids = ids.view(B, Tq, -1)[:, t:t + n].contiguous()
+                plens = lens.view(B, Tq, -1)[:, t:t + n].contiguous()
+                plse = None if lse is None else lse[:, t:t + n].contiguous()
+            nbytes = _abi.shape_size("lsa_key_mass_scratch_bytes", dt, B, n, caches, Tk, Hq, Hkv, D, W)
+            ws = _abi.scratch(device, "key_mass", nbytes)
+            _abi.call("lsa_key_mass", part.data_ptr(), k.data_ptr(), dt, B, n, caches, Tk, Hq, Hkv, D, sb, st, sh,
+                      pids.data_ptr(), plens.data_ptr(), W, 1 if per_head else 0, scale, _abi.ptr(plse),
+                      1 if fresh and t == 0 else 0, _abi.ptr(ws), nbytes, mass.data_ptr(),
+                      mass.stride(0) if caches > 1 else Hkv * Tk, mass.stride(1) if Hkv > 1 else Tk,
+                      _abi.stream(device))
+    return mass
+
+
+def _check_keep(what: str, T: int, budget: int, window: int, sink: int) -> None:
+    if not 1 <= budget <= T:
+        raise ValueError(f"{what}: a budget in 1..{T}, got {budget}")
+    if window < 0 or sink < 0 or window + sink > budget:
+        raise ValueError(f"{what}: window {window} and sink {sink} must fit the budget {budget}")
+
+
+def _row_lengths(what: str, lengths: torch.Tensor | None, B: int, device: torch.device) -> torch.Tensor | None:
+    if lengths is None:
+        return None
+    lens = int32_on(lengths, device)
+    if lens.numel() != B:
+        raise ValueError(f"{what}: {lens.numel()} lengths for {B} rows")
+    return lens
+
+
+def _dense_mass(what: str, mass: torch.Tensor, shape: tuple[int, int, int]) -> torch.Tensor:
+    if tuple(mass.shape) != shape or mass.dtype != torch.float32:
+        raise ValueError(f"{what}: mass must be fp32 {list(shape)}, got {mass.dtype} {tuple(mass.shape)}")
+    return mass if shape[2] <= 1 or mass.stride(2) == 1 else mass.contiguous()
+
+
+def _extent(t: torch.Tensor) -> tuple[int, int]:
+    """The addresses between which a tensor's elements lie."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def evict(
+    k: torch.Tensor,
+    v: torch.Tensor,
+    mass: torch.Tensor,
+    budget: int,
+    lengths: torch.Tensor | None = None,
+    window: int = 0,
+    sink: int = 0,
+    shared: bool = False,
+    out: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None,
+):
+    """The ``budget`` keys of each row and kv-head worth keeping, and the cache cut down to them.
+
+    k/v [B, T, Hkv, D], mass [B, Hkv, T] fp32 (``key_mass``'s, accumulated). Of a row's
+    ``lengths[b]`` positions (default T) the first ``sink`` and the last ``window`` stay, and of the
+    others those of largest mass; ties go to the lower position, a NaN weighs least; a row of at
+    most ``budget`` positions keeps all. ``shared``: the kv-heads keep the same positions, by the sum of their masses (as lists over an
+    index-space table need it).
+
+    Returns ``(k, v, mass, kept, lengths)``: the kept rows in their order, [B, budget, Hkv, D], their
+    masses [B, Hkv, budget], their positions in the old cache [B, Hkv, budget] int32 (shared:
+    [B, budget]; -1 past the row's new length) and the new lengths [B] int32. New tensors hold
+    zeros past the new length. ``out`` = (k, v, mass) buffers of ``budget`` rows or more (not the
+    inputs: two caches take turns), whose rows past the new length are left as they were.
+    """
+    device = one_device("evict", k, v, mass)
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError(f"evict: k/v [B, T, Hkv, D] of one dtype, got {k.dtype} {tuple(k.shape)} / {v.dtype} "
+                         f"{tuple(v.shape)}")
+    B, T, Hkv, D = k.shape
+    dt = _abi.dtype_code(k.dtype)
+    budget, window, sink = int(budget), int(window), int(sink)
+    _check_keep("evict", T, budget, window, sink)
+    mass = _dense_mass("evict", mass, (B, Hkv, T))
+    lens = _row_lengths("evict", lengths, B, device)
+    k, v, (sb, st, sh) = cache_pair(k, v)
+    if out is None:
+        k2, v2 = (torch.empty(B, budget, Hkv, D, dtype=k.dtype, device=device) for _ in range(2))
+        m2 = torch.empty(B, Hkv, budget, dtype=torch.float32, device=device)
+    else:
+        k2, v2, m2 = out
+        one_device("evict", k, k2, v2, m2)
+        if (k2.dim() != 4 or k2.shape != v2.shape or k2.shape[1] < budget or (k2.shape[0], *k2.shape[2:]) != (B, Hkv, D)
+                or k2.dtype != k.dtype or v2.dtype != k.dtype or k2.stride(-1) != 1 or v2.stride(-1) != 1
+                or cache_strides(k2) != cache_strides(v2) or k2.data_ptr() % 16 or v2.data_ptr() % 16):
+            raise ValueError(f"evict: out k/v must be {k.dtype} [{B}, >= {budget}, {Hkv}, {D}] of contiguous, 16-byte "
+                             f"aligned rows at the same strides, got {tuple(k2.shape)} / {tuple(v2.shape)}")
+        if (m2.dim() != 3 or tuple(m2.shape[:2]) != (B, Hkv) or m2.shape[2] < budget or m2.dtype != torch.float32
+                or (m2.shape[2] > 1 and m2.stride(2) != 1)):
+            raise ValueError(f"evict: out mass must be fp32 [{B}, {Hkv}, >= {budget}] with contiguous keys, got "
+                             f"{tuple(m2.shape)}")
+        for new in out:
+            a, b = _extent(new)
+            if any(a < hi and lo < b for lo, hi in map(_extent, (k, v, mass))):
+                raise ValueError("evict: out must not overlap the cache it is made from")
+        if k2.data_ptr() == v2.data_ptr() and k2.numel():
+            raise ValueError("evict: out k and v are the same buffer")
+    ob, ot, oh = cache_strides(k2)
+    kept = torch.empty((B, budget) if shared else (B, Hkv, budget), dtype=torch.int32, device=device)
+    new_lengths = torch.empty(B, dtype=torch.int32, device=device)
+    if B:
+        one = 1 if shared else 0
+        nbytes = _abi.shape_size("lsa_evict_scratch_bytes", B, T, one)
+        with launch_device(device):
+            ws = _abi.scratch(device, "evict", nbytes)
+            stream = _abi.stream(device)
+            _abi.call("lsa_evict_keep", mass.data_ptr(), B, Hkv, T, mass.stride(0), mass.stride(1), _abi.ptr(lens),
+                      budget, window, sink, one, None, 0, 0, _abi.ptr(ws), nbytes, kept.data_ptr(),
+                      new_lengths.data_ptr(), None, 0, stream)
+            _abi.call("lsa_evict_rows", k.data_ptr(), v.data_ptr(), mass.data_ptr(), dt, B, T, Hkv, D, sb, st, sh,
+                      mass.stride(0), mass.stride(1), kept.data_ptr(), one, budget, k2.data_ptr(), v2.data_ptr(), ob,
+                      ot, oh, m2.data_ptr(), m2.stride(0), m2.stride(1), 1 if out is None else 0, stream)
+    return k2, v2, m2, kept, new_lengths
+
+
+def evict_slots(
+    slot_table: torch.Tensor,
+    mass: torch.Tensor,
+    budget: int,
+    lengths: torch.Tensor | None = None,
+    window: int = 0,
+    sink: int = 0,
+):
+    """``evict`` for a paged cache: no K/V row moves, the slot table changes.
+
+    ``slot_table`` [R, T] int32 (a row a sequence: logical position -> cache row), mass
+    [1, Hkv, pool] fp32 (``key_mass``'s over the pool). What row r keeps of its ``lengths[r]``
+    positions (default T) is decided as in ``evict`` with ``shared``; a position without a cache row
+    (outside the pool) weighs least.
+
+    Returns ``(slot_table, lengths, kept)``: each row with the cache rows it keeps first, in their
+    order, then the ones it gave up, in theirs (the sequence's next tokens may take them, or an
+    allocator), then what was behind its length; the new lengths [R] and the kept positions
+    [R, budget] (-1 past the new length), int32. The masses stay with their cache rows: clear
+    those that are given to a new token.
+    """
+    device = one_device("evict_slots", slot_table, mass)
+    if slot_table.dim() != 2 or slot_table.shape[1] < 1:
+        raise ValueError(f"evict_slots: slot_table [R, T], got {tuple(slot_table.shape)}")
+    if mass.dim() != 3 or mass.shape[0] != 1 or mass.shape[1] < 1 or mass.shape[2] < 1:
+        raise ValueError(f"evict_slots: mass [1, Hkv, pool], got {tuple(mass.shape)}")
+    R, T = slot_table.shape
+    Hkv, pool = mass.shape[1:]
+    budget, window, sink = int(budget), int(window), int(sink)
+    _check_keep("evict_slots", T, budget, window, sink)
+    mass = _dense_mass("evict_slots", mass, (1, Hkv, pool))
+    lens = _row_lengths("evict_slots", lengths, R, device)
+    table = int32_on(slot_table, device)
+    new_table = torch.empty(R, T, dtype=torch.int32, device=device)
+    kept = torch.empty(R, budget, dtype=torch.int32, device=device)
+    new_lengths = torch.empty(R, dtype=torch.int32, device=device)
+    if R:
+        nbytes = _abi.shape_size("lsa_evict_scratch_bytes", R, T, 1)
+        with launch_device(device):
+            ws = _abi.scratch(device, "evict", nbytes)
+            _abi.call("lsa_evict_keep", mass.data_ptr(), R, Hkv, T, 0, mass.stride(1), _abi.ptr(lens), budget, window,
+                      sink, 1, table.data_ptr(), T, pool, _abi.ptr(ws), nbytes, kept.data_ptr(),
+                      new_lengths.data_ptr(), new_table.data_ptr(), T, _abi.stream(device))
+    return new_table, new_lengths, kept

@@ -1,0 +1,170 @@
+"""Attention of a decode batch over a prefix that its rows share.
+
+Requests behind one system prompt hold the same keys at its start. ``prefix_read`` keeps those
+once, reads them once for the whole batch, and joins them in one softmax with what each row
+reads of its own cache (a read list, as ``lsa_read``). No counterpart in the reference.
+"""
+
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from lsa_rocm_lab import _abi
+
+
+def launch_device(device: torch.device):
+    """A context in which a launch on ``device`` finds it current (nothing where it is)."""
+    index = _abi.device_index(device)
+    return contextlib.nullcontext() if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def one_device(what: str, *tensors: torch.Tensor | None) -> torch.device:
+    """The ROCm device that all of the tensors are on; anything else raises ``ValueError``."""
+    device = tensors[0].device
+    for t in tensors:
+        if t is not None and (t.device.type != "cuda" or t.device != device):
+            raise ValueError(f"{what} is a ROCm kernel over tensors of one device, got {device} and {t.device}")
+    return device
+
+
+def int32_on(t: torch.Tensor, device: torch.device) -> torch.Tensor:
+    """``t`` as a kernel reads it: int32, contiguous, on ``device``."""
+    if t.dtype == torch.int32 and t.device == device and t.is_contiguous():
+        return t
+    return t.to(device=device, dtype=torch.int32).contiguous()
+
+
+def cache_strides(x: torch.Tensor) -> tuple[int, int, int]:
+    """Batch, token and head strides of a cache [B, T, Hkv, D] (an axis of one has none of its own)."""
+    sb, st, sh = x.stride()[:3]
+    return (sb if x.shape[0] > 1 else 0, st if x.shape[1] > 1 else x.shape[3], sh if x.shape[2] > 1 else x.shape[3])
+
+
+def cache_pair(k: torch.Tensor, v: torch.Tensor):
+    """K and V as a kernel reads them (rows of contiguous elements at the same strides; other
+    layouts are made dense) and their strides."""
+    if (k.stride(-1) != 1 or v.stride(-1) != 1 or cache_strides(k) != cache_strides(v)
+            or k.data_ptr() % 16 or v.data_ptr() % 16):
+        k, v = k.contiguous(), v.contiguous()
+        if k.data_ptr() % 16 or v.data_ptr() % 16:  # a contiguous view that begins off a row's alignment
+            k, v = k.clone(), v.clone()
+    return k, v, cache_strides(k)
+
+
+def aligned(x: torch.Tensor) -> torch.Tensor:
+    x = x.contiguous()
+    return x.clone() if x.data_ptr() % 16 else x
+
+
+def lists_of(read_lists: torch.Tensor, lengths: torch.Tensor, rows: int, heads_kv: int, device: torch.device):
+    """Read lists of ``rows`` query rows as ``lsa_read`` takes them: ids [n, W], lengths [n], and
+    whether every kv-head has its own."""
+    width = read_lists.shape[-1]
+    ids, lens = int32_on(read_lists, device), int32_on(lengths, device)
+    n = lens.numel()
+    per_head = heads_kv > 1 and n == rows * heads_kv and n != rows
+    if n != (rows * heads_kv if per_head else rows) or ids.numel() != n * width:
+        raise ValueError(f"read lists {tuple(read_lists.shape)} / lengths {tuple(lengths.shape)} do not match "
+                         f"{rows} query rows (x {heads_kv} kv-heads)")
+    return ids, lens, width, per_head
+
+
+def prefix_read(
+    q: torch.Tensor,
+    k_prefix: torch.Tensor,
+    v_prefix: torch.Tensor,
+    k: torch.Tensor | None = None,
+    v: torch.Tensor | None = None,
+    read_lists: torch.Tensor | None = None,
+    lengths: torch.Tensor | None = None,
+    scale: float | None = None,
+    prefix_lengths: torch.Tensor | None = None,
+    prefix_rows: torch.Tensor | None = None,
+    prefix_slots: torch.Tensor | None = None,
+    return_lse: bool = False,
+):
+    """One softmax over a shared prefix and each row's own read list.
+
+    q [B, Tq, Hq, D] (fp32, bf16 or fp16; D 32, 64, 128 or 256; 1, 2, 4 or 8 query heads a
+    kv-head). ``k_prefix`` / ``v_prefix`` [P, Tp, Hkv, D] hold P prefixes, or, with
+    ``prefix_slots`` [P, Tp] (logical position -> cache row, as a slot table), are one pool
+    [1, slots, Hkv, D]; slots outside it are skipped. Every query row reads the first
+    ``prefix_lengths[p]`` keys (default: all) of prefix p = ``prefix_rows[b]`` of its batch row
+    (default: the only prefix, or prefix b where there are B; one outside [0, P) means none).
+    ``k``, ``v``, ``read_lists``, ``lengths``: the own part, as ``lsa_read`` (lists
+    [B, Tq, W] or [B, Tq, Hkv, W]; k/v [B or 1, Tk, Hkv, D]); all four or none.
+
+    Returns the output, like q, or with ``return_lse`` also the softmax's logarithm of sums
+    [B, Tq, Hq] in fp32 (``key_mass`` takes it). A row with no keys gives zeros and -inf.
+    """
+    own = (k, v, read_lists, lengths)
+    if any(t is None for t in own) and not all(t is None for t in own):
+        raise ValueError("prefix_read: k, v, read_lists and lengths come together")
+    device = one_device("prefix_read", q, k_prefix, v_prefix, k, v)
+    if q.dim() != 4 or k_prefix.dim() != 4 or k_prefix.shape != v_prefix.shape:
+        raise ValueError(f"prefix_read: q [B, Tq, Hq, D] and prefixes [P, Tp, Hkv, D], got {tuple(q.shape)}, "
+                         f"{tuple(k_prefix.shape)} / {tuple(v_prefix.shape)}")
+    B, Tq, Hq, D = q.shape
+    Hkv = k_prefix.shape[2]
+    if k_prefix.shape[3] != D or Hkv < 1 or Hq % Hkv:
+        raise ValueError(f"prefix_read: {Hq} query heads of {D} on prefixes {tuple(k_prefix.shape)}")
+    if any(t is not None and t.dtype != q.dtype for t in (k_prefix, v_prefix, k, v)):
+        raise ValueError("prefix_read: q, the prefixes and k/v must have one dtype")
+    dt = _abi.dtype_code(q.dtype)
+    slots = None
+    if prefix_slots is not None:
+        if prefix_slots.dim() != 2 or prefix_slots.shape[0] < 1 or k_prefix.shape[0] != 1:
+            raise ValueError(f"prefix_read: prefix_slots [P, Tp] over one pool, got {tuple(prefix_slots.shape)} over "
+                             f"{tuple(k_prefix.shape)}")
+        slots = int32_on(prefix_slots, device)
+        P, Tp = slots.shape
+        if k_prefix.shape[1] == 0:  # an empty pool: no slot names a row of it
+            Tp, slots = 0, None
+    else:
+        P, Tp = k_prefix.shape[:2]
+    if P < 1:
+        raise ValueError("prefix_read: no prefix")
+    plen = None if prefix_lengths is None else int32_on(prefix_lengths, device)
+    if plen is not None and plen.numel() != P:
+        raise ValueError(f"prefix_read: {plen.numel()} prefix lengths for {P} prefixes")
+    if prefix_rows is not None:
+        prow = int32_on(prefix_rows, device)
+        if prow.numel() != B:
+            raise ValueError(f"prefix_read: {prow.numel()} prefix rows for {B} batch rows")
+    elif P == 1:
+        prow = None
+    elif P == B:
+        from lsa_rocm_lab.port.pipeline import _row_index
+
+        prow = _row_index(device, B, shared=False)
+    else:
+        raise ValueError(f"prefix_read: prefix_rows is needed: {P} prefixes for {B} batch rows")
+    q = aligned(q)
+    k_prefix, v_prefix, (psb, pst, psh) = cache_pair(k_prefix, v_prefix)
+    Tk = W = sb = st = sh = 0
+    ids = lens = None
+    per_head = False
+    if k is not None:
+        if k.dim() != 4 or k.shape != v.shape or k.shape[0] not in (B, 1) or tuple(k.shape[2:]) != (Hkv, D):
+            raise ValueError(f"prefix_read: k/v must be [B={B} or 1, Tk, {Hkv}, {D}], got {tuple(k.shape)} / "
+                             f"{tuple(v.shape)}")
+        Tk = k.shape[1]
+        k, v, (sb, st, sh) = cache_pair(k, v)
+        ids, lens, W, per_head = lists_of(read_lists, lengths, B * Tq, Hkv, device)
+        if Tk == 0:
+            W = 0
+    out = torch.empty_like(q)
+    lse = torch.empty(B, Tq, Hq, dtype=torch.float32, device=device) if return_lse else None
+    if B * Tq:
+        nbytes = _abi.shape_size("lsa_prefix_read_scratch_bytes", dt, B, Tq, P, Tp, Hq, Hkv, D, W)
+        with launch_device(device):
+            ws = _abi.scratch(device, "prefix_read", nbytes)
+            _abi.call("lsa_prefix_read", q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), dt, B, Tq, P, Tp,
+                      k_prefix.shape[1], Hq, Hkv, D, psb, pst, psh, _abi.ptr(prow), _abi.ptr(plen), _abi.ptr(slots),
+                      slots.stride(0) if slots is not None else 0, _abi.ptr(k), _abi.ptr(v), Tk, sb, st, sh,
+                      _abi.ptr(ids), _abi.ptr(lens), W, 1 if per_head else 0,
+                      float(D ** -0.5 if scale is None else scale), _abi.ptr(ws), nbytes, out.data_ptr(),
+                      _abi.ptr(lse), _abi.stream(device))
+    return (out, lse) if return_lse else out
