@@ -1,5 +1,5 @@
-// The 32x32x16 matrix operations on 16-bit rows and the transposing LDS read, shared by the
-// prefill reads that run on the matrix cores.
+// The 32x32x16 matrix operations on 16-bit rows, the transposing LDS read and the loads that go
+// from memory straight to LDS, shared by the reads that run on the matrix cores.
 #pragma once
 
 #include "lsa_read_dev.h"
@@ -54,6 +54,32 @@ __device__ __forceinline__ uint2 v_column4(const lds_char* lane_base, int offset
   typedef __attribute__((address_space(3))) v4i16_t lds_v4;
   const v4i16_t r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)(lane_base + offset));
   return __builtin_bit_cast(uint2, r);
+}
+
+// Which LDS segment of row r holds its segment 0 (XOR): K rows are read 16 rows to a
+// 16-lane group at one segment, V rows (transposing reads) 8 rows at 64 bytes each.
+template <int D> __device__ __forceinline__ int kseg(int r) { return D == 128 ? r & 15 : (r >> 1) & 7; }
+template <int D> __device__ __forceinline__ int vseg(int r) { return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; }
+
+// 1024 (256) bytes from base + voff (a lane's) to LDS address `lds` + 16 (4) * lane, counted
+// by vmcnt. Written as instructions, so that the compiler does not drain the counter before
+// the LDS reads it cannot tell apart from these writes; the waits are wait_vm's.
+__device__ __forceinline__ void dma16(uint32_t lds, const void* base, uint32_t voff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(voff), "s"(base)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void dma4(uint32_t lds, const void* base, uint32_t voff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(voff), "s"(base)
+               : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void phase_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_barrier" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 }  // namespace lsa

@@ -4,74 +4,24 @@
 // The softmax over both parts is one: each part leaves partials (running maximum m, sum l and
 // weighted value row, in fp32, log2 domain), and the usual rescaling joins them.
 //
+//   prefix_mfma_kernel    (prefix_mfma.hip) a prefix's partials for 32 to 128 query columns at
+//                         once, 16-bit rows of head dim 64 or 128;
 //   prefix_gather_kernel  a prefix's partials row by row (any type and head dim);
 //   prefix_join_kernel    a row's own list (the gather read's span loop) and the join.
 //
 // A prefix of n keys is cut into pieces of whole 64-key tiles, a workgroup a piece, the same for
-// both kernels (prefix_pieces). Partials of (row, kv-head) unit i: piece s of n_p at
+// all of them (prefix_pieces). Partials of (row, kv-head) unit i: piece s of n_p at
 // [i][splits - n_p + s], the own list's spans behind them, so the join finds them in a line.
 #include <math.h>
 
 #include <algorithm>
 
 #include "lsa_abi_common.h"
-#include "lsa_read_dev.h"
+#include "lsa_prefix_dev.h"
 
 using namespace lsa;
 
 namespace {
-
-constexpr int kPieceTile = 64;  // keys; a piece is a multiple of it
-constexpr int kMaxPieces = 128;
-constexpr int kMaxOwn = 64;
-
-struct PrefixArgs {
-  const void* q;
-  const void* kp;
-  const void* vp;
-  const int32_t* prefix_rows;     // [B] or nullptr: 0
-  const int32_t* prefix_lengths;  // [P] or nullptr: Tp
-  const int32_t* slots;           // [P, Tp] cache rows of a pool, or nullptr
-  int64_t slot_stride, pool;      // rows the prefix cache holds a batch entry
-  int64_t p_sb, p_st, p_sh;
-  const void* k;
-  const void* v;
-  int64_t kv_sb, kv_st, kv_sh, Tk;
-  const int32_t* ids;
-  const int32_t* lengths;
-  int W, per_head;
-  int64_t B, Tq, Tp;
-  int P, Hq, Hkv;
-  float scale_log2;
-  int splits;      // pieces of a prefix at most
-  int own_splits;  // spans of an own list at most
-  int own_span;    // list slots of a span
-  int* counters;   // [units]: cleared by the prefix kernel, arrivals of the own spans
-  float* parts;    // [units][splits + own_splits][GQ (D + 2)]
-  void* out;
-  float* lse;      // [B, Tq, Hq] or nullptr
-};
-
-struct Pieces {
-  int n;      // keys
-  int count;  // pieces with keys in them
-  int keys;   // of a piece
-};
-
-__device__ __forceinline__ Pieces prefix_pieces(const PrefixArgs& a, int p) {
-  Pieces x{0, 0, kPieceTile};
-  if (p < 0 || p >= a.P) return x;  // no prefix
-  const int64_t n = a.prefix_lengths ? (int64_t)a.prefix_lengths[p] : a.Tp;
-  x.n = (int)(n < 0 ? 0 : (n > a.Tp ? a.Tp : n));
-  const int tiles = (x.n + kPieceTile - 1) / kPieceTile;
-  const int per = (tiles + a.splits - 1) / a.splits;
-  x.keys = (per > 0 ? per : 1) * kPieceTile;
-  x.count = (x.n + x.keys - 1) / x.keys;
-  return x;
-}
-__device__ __forceinline__ int prefix_of(const PrefixArgs& a, int64_t b) {
-  return a.prefix_rows ? a.prefix_rows[b] : 0;
-}
 
 // grid (row * Hkv, piece).
 template <typename T, int D, int GQ>
@@ -165,13 +115,25 @@ struct PrefixPlan {
   size_t parts, total;
 };
 
-// Pieces and own spans by size. About 512 workgroups of pieces; own spans of at least 256 slots,
-// as many as make 512 workgroups.
-PrefixPlan prefix_plan(int dtype, int64_t B, int64_t Tq, int64_t Tp, int32_t Hq, int32_t Hkv, int32_t D, int32_t W) {
+// Query columns a prefix has, if its rows are spread evenly.
+int64_t mean_columns(int64_t B, int64_t Tq, int64_t P, int32_t Hq, int32_t Hkv) {
+  return (B * Tq * (Hq / Hkv) + P - 1) / P;
+}
+
+// Pieces and own spans by size. On the matrix cores a workgroup has a CU to itself: as many pieces
+// as make one workgroup a CU, of at least 256 keys. The gather: about 512 workgroups. Own spans of at
+// least 256 slots, as many as make 512 workgroups.
+PrefixPlan prefix_plan(int dtype, int64_t B, int64_t Tq, int64_t P, int64_t Tp, int32_t Hq, int32_t Hkv, int32_t D, int32_t W) {
   PrefixPlan p;
   const int64_t units = B * Tq * Hkv;
   const int64_t tiles = (Tp + kPieceTile - 1) / kPieceTile;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({tiles, kMaxPieces, 512 / std::max<int64_t>(units, 1)}));
+  int64_t most = tiles, want_p = 512 / std::max<int64_t>(units, 1);
+  if (prefix_mfma_ok(dtype, D)) {
+    const int64_t cols = mean_columns(B, Tq, P, Hq, Hkv), wg = prefix_mfma_columns(cols);
+    most = (tiles + 3) / 4;
+    want_p = 256 / std::max<int64_t>(1, P * Hkv * ((cols + wg - 1) / wg));
+  }
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, kMaxPieces, want_p}));
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kMaxOwn, 512 / std::max<int64_t>(units, 1)));
   const int64_t per = std::max<int64_t>((W + want - 1) / want, 256);
   p.own_span = (int)((per + 63) / 64 * 64);
@@ -195,8 +157,10 @@ bool prefix_shape_ok(int dtype, int64_t B, int64_t Tq, int64_t P, int64_t Tp, in
 template <typename T, int D>
 void launch_prefix_gq(const PrefixArgs& a, int gq, int64_t units, hipStream_t s) {
   const dim3 gp((unsigned)units, (unsigned)a.splits), go((unsigned)units, (unsigned)a.own_splits);
-#define LSA_PREFIX(GQ)                                         \
-  prefix_gather_kernel<T, D, GQ><<<gp, LSA_BLOCK, 0, s>>>(a);  \
+  const bool done = launch_prefix_mfma(a, __is_same(T, float) ? LSA_F32 : (__is_same(T, bf16_t) ? LSA_BF16 : LSA_F16), D,
+                                       mean_columns(a.B, a.Tq, a.P, a.Hq, a.Hkv), s);
+#define LSA_PREFIX(GQ)                                                    \
+  if (!done) prefix_gather_kernel<T, D, GQ><<<gp, LSA_BLOCK, 0, s>>>(a);  \
   prefix_join_kernel<T, D, GQ><<<go, LSA_BLOCK, 0, s>>>(a)
   switch (gq) {
     case 1: LSA_PREFIX(1); break;
@@ -222,7 +186,7 @@ void launch_prefix(const PrefixArgs& a, int D, int gq, int64_t units, hipStream_
 extern "C" size_t lsa_prefix_read_scratch_bytes(int dtype, int64_t B, int64_t Tq, int64_t P, int64_t Tp, int32_t Hq,
                                                 int32_t Hkv, int32_t D, int32_t W) {
   if (!prefix_shape_ok(dtype, B, Tq, P, Tp, Hq, Hkv, D, W) || B * Tq == 0) return 0;
-  return prefix_plan(dtype, B, Tq, Tp, Hq, Hkv, D, W).total;
+  return prefix_plan(dtype, B, Tq, P, Tp, Hq, Hkv, D, W).total;
 }
 
 extern "C" int lsa_prefix_read(const void* q, const void* k_prefix, const void* v_prefix, int dtype, int64_t B,
@@ -258,7 +222,7 @@ extern "C" int lsa_prefix_read(const void* q, const void* k_prefix, const void* 
   LSA_REQUIRE(prefix_token_stride <= 0x7FFFFFFF && (!own || kv_token_stride <= 0x7FFFFFFF), LSA_ERR_SHAPE,
               "lsa_prefix_read: token strides past 2^31 elements");
   if (B * Tq == 0) return LSA_OK;
-  const PrefixPlan p = prefix_plan(dtype, B, Tq, Tp, Hq, Hkv, D, W);
+  const PrefixPlan p = prefix_plan(dtype, B, Tq, P, Tp, Hq, Hkv, D, W);
   LSA_REQUIRE(scratch && scratch_bytes >= p.total && ((uintptr_t)scratch & 15) == 0, LSA_ERR_WORKSPACE,
               "lsa_prefix_read: scratch missing, not 16-byte aligned or %zu < %zu bytes", scratch_bytes, p.total);
   PrefixArgs a = {};

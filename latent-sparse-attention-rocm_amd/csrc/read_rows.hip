@@ -299,32 +299,6 @@ struct alignas(1024) SweepLds {
   int n_act, left0;
 };
 
-// Which LDS segment of row r holds its segment 0 (XOR): K rows are read 16 rows to a
-// 16-lane group at one segment, V rows (transposing reads) 8 rows at 64 bytes each.
-template <int D> __device__ __forceinline__ int kseg(int r) { return D == 128 ? r & 15 : (r >> 1) & 7; }
-template <int D> __device__ __forceinline__ int vseg(int r) { return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; }
-
-// 1024 (256) bytes from base + voff (a lane's) to LDS address `lds` + 16 (4) * lane, counted
-// by vmcnt. Written as instructions, so that the compiler does not drain the counter before
-// the LDS reads it cannot tell apart from these writes; the waits are wait_vm's.
-__device__ __forceinline__ void dma16(uint32_t lds, const void* base, uint32_t voff) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(voff), "s"(base)
-               : "memory", "m0");
-}
-__device__ __forceinline__ void dma4(uint32_t lds, const void* base, uint32_t voff) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(voff), "s"(base)
-               : "memory", "m0");
-}
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void phase_barrier() {
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("s_barrier" ::: "memory");
-  __builtin_amdgcn_sched_barrier(0);
-}
-
 // What a weight's 16-bit half leaves out, exact in fp32: x - pair.lo (lo) and x - pair.hi (hi),
 // one dot product with (-1, 0) or (0, -1) each. The constants are kept opaque: as an inline
 // operand this compiler gives the packed bf16 pair (-1, 0) the encoding of -1.0, which the
