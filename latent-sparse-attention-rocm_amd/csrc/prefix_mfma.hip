@@ -4,11 +4,11 @@
 // S^T = K Q^T and O^T += V^T P^T. A workgroup takes up to 128 columns and one piece of the
 // prefix, so every key is read once per 128 columns, where the gather reads it once a row.
 //
-// Four groups of waves take the piece's 32-key tiles in turn, each with tile buffers of its own
-// (two of K and V, filled straight from memory a tile ahead), one wave or two waves of columns
-// (CG) a group and one or two blocks of 32 columns (QB) a wave. Few columns so still have four
-// tiles in flight a CU, and what bounds them is memory. At the end the four groups' states meet
-// in LDS and leave as one partial.
+// KG groups of CG waves, 32 columns a wave, take the piece's tiles in turn, each group with tile
+// buffers of its own (two of K and V, filled straight from memory a tile ahead): four groups on
+// 32-key tiles for up to 32 or 64 columns, two on 64-key tiles for up to 128. So few columns, too,
+// have 64 KB in flight a CU (D = 128), and what bounds them is memory. At the end the groups'
+// states meet in LDS and leave as one partial.
 //
 // A weight enters the matrix cores as one 16-bit number: half a step of it (2^-9 in bf16, 2^-12
 // in fp16), independent from key to key; the output is rounded by as much when it is stored.
@@ -27,23 +27,23 @@ using namespace lsa;
 
 namespace {
 
-constexpr int kKeys = 32;    // of a tile
-constexpr int kGroups = 4;   // wave groups, each on tiles of its own
 constexpr int kXcds = 8;
 
-template <int D, int QB, int CG>
+template <int KG> constexpr int tile_keys() { return 128 / KG; }
+
+template <int D, int KG, int CG>
 struct alignas(1024) PrefixLds {
   union {
     struct {
-      uint16_t k[kGroups][2][kKeys * D];  // 16-byte segments of a row permuted by kseg
-      uint16_t v[kGroups][2][kKeys * D];  // by vseg
+      uint16_t k[KG][2][tile_keys<KG>() * D];  // 16-byte segments of a row permuted by kseg
+      uint16_t v[KG][2][tile_keys<KG>() * D];  // by vseg
     };
-    float o[kGroups][CG][32][D + 4];      // a block of columns of every group (rows 4 banks apart)
+    float o[KG][CG][32][D + 4];  // every wave's state (rows 4 banks apart)
   };
-  float m[kGroups][CG][QB][32], l[kGroups][CG][QB][32];
-  int32_t ids[kGroups][CG][4][64];        // paged: cache rows of the tiles ahead, a wave's own
-  int32_t member[32 * QB * CG];           // batch rows whose columns these are
-  int count[kGroups * CG];
+  float m[KG][CG][32], l[KG][CG][32];
+  int32_t ids[KG][CG][4][64];    // paged: cache rows of the tiles ahead, a wave's own
+  int32_t member[32 * CG];       // batch rows whose columns these are
+  int count[KG * CG];
 };
 
 __device__ __forceinline__ void dma16_far(uint32_t lds, const void* p) {  // a lane's own 64-bit address
@@ -52,21 +52,22 @@ __device__ __forceinline__ void dma16_far(uint32_t lds, const void* p) {  // a l
 
 // grid: (kv-head, prefix, piece) units in groups of 8, the column blocks of a unit 8 apart, so that
 // those which read the same keys share an XCD and its L2.
-template <typename T, int D, int QB, int CG, bool PAGED>
-__global__ __launch_bounds__(64 * kGroups * CG) __attribute__((amdgpu_waves_per_eu(CG, CG)))
+template <typename T, int D, int KG, int CG, bool PAGED>
+__global__ __launch_bounds__(64 * KG * CG) __attribute__((amdgpu_waves_per_eu(KG * CG / 4, KG * CG / 4)))
 void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
   using M = Mfma<T>;
   using op_t = typename M::op_t;
   constexpr int KS = D / 16, DB = D / 32, SEGS = D / 8, ROWB = 2 * D;
+  constexpr int KT = tile_keys<KG>(), HT = KT / 32;
   constexpr int KPI = 1024 / ROWB;             // keys a dma16 moves
-  constexpr int NI = kKeys / KPI / CG;         // dma16s a wave a tile, K and V each
-  constexpr int NW = kGroups * CG, THREADS = 64 * NW, COLS = 32 * QB * CG;
+  constexpr int NI = KT / KPI / CG;            // dma16s a wave a tile, K and V each
+  constexpr int NW = KG * CG, THREADS = 64 * NW, COLS = 32 * CG;
   constexpr bool HALF = !__is_same(T, bf16_t);
   constexpr float BIAS = HALF ? 12.0f : 0.0f, TOP = HALF ? 15.0f : 8.0f;
-  __shared__ PrefixLds<D, QB, CG> sh;
+  __shared__ PrefixLds<D, KG, CG> sh;
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid / 64);
-  const int kg = w % kGroups, cg = w / kGroups;
+  const int kg = w % KG, cg = w / KG;
   const int hh = lane / 32, ln = lane % 32;
   const int GQ = a.Hq / a.Hkv;
   const int64_t clear = (int64_t)gridDim.x * THREADS;
@@ -119,36 +120,27 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
     h = r % GQ;
     return mi < found ? (int64_t)sh.member[mi] * a.Tq + r / GQ : -1;
   };
-  op_t qop[QB][KS];
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
+  op_t qop[KS];
+  {
     int h;
-    int64_t row = column((cg * QB + qb) * 32 + ln, h);
+    int64_t row = column(cg * 32 + ln, h);
     if (row < 0) row = (int64_t)sh.member[0] * a.Tq, h = 0;
     const T* src = (const T*)a.q + (row * a.Hq + (int64_t)g * GQ + h) * D + 8 * hh;
 #pragma unroll
-    for (int y = 0; y < KS; ++y) qop[qb][y] = __builtin_bit_cast(op_t, *(const uint4*)(src + 16 * y));
+    for (int y = 0; y < KS; ++y) qop[y] = __builtin_bit_cast(op_t, *(const uint4*)(src + 16 * y));
   }
 #pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
+  for (int y = 0; y < KS; ++y) asm volatile("" ::"v"(qop[y]));  // here: below, waits are counted by hand
+  f32x16_t o[DB];
+  float m_run = kNegBig, l_run = 0.0f;
 #pragma unroll
-    for (int y = 0; y < KS; ++y) asm volatile("" ::"v"(qop[qb][y]));  // here: below, waits are counted by hand
-  }
-  f32x16_t o[DB][QB];
-  float m_run[QB], l_run[QB];
+  for (int d = 0; d < DB; ++d) {
 #pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    m_run[qb] = kNegBig;
-    l_run[qb] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < DB; ++d) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[d][qb][r] = 0.0f;
-    }
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
   }
 
   const int k0 = s * pc.keys, n_keys = min(pc.keys, pc.n - k0);
-  const int n_tiles = (n_keys + kKeys - 1) / kKeys;
+  const int n_tiles = (n_keys + KT - 1) / KT;
   const int64_t head = (PAGED ? 0 : p * a.p_sb) + g * a.p_sh;
   const T* kb = (const T*)a.kp + head;
   const T* vb = (const T*)a.vp + head;
@@ -157,30 +149,31 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
   const uint32_t v_lds = (uint32_t)(uintptr_t)(lds_char*)&sh.v[kg][0][0];
   const uint32_t i_lds = (uint32_t)(uintptr_t)(lds_char*)&sh.ids[kg][cg][0][0];
   const int64_t st = a.p_st * 2;  // bytes
-  uint32_t live[2] = {0u, 0u};    // which keys of the two tiles in the buffers count
+  const float scale = a.scale_log2;
+  uint64_t live[2] = {0ull, 0ull};  // which keys of the two tiles in the buffers count
 
   // Tile i of the group's (i-th of its turn) into buffer i & 1; this wave moves its share of the rows.
   auto load_ids = [&](int i) {
-    const int t = kg + kGroups * i;
-    const int j = min(t, n_tiles - 1) * kKeys + ln;
+    const int t = kg + KG * i;
+    const int j = min(t, n_tiles - 1) * KT + lane % KT;
     dma4(i_lds + (uint32_t)(i & 3) * 256u, slots, 4u * (uint32_t)min(j, n_keys - 1));
   };
   auto load = [&](int i) {
-    const int t = kg + kGroups * i;
+    const int t = kg + KG * i;
     if (t >= n_tiles) return;  // wave-uniform
-    const int n = min(kKeys, n_keys - t * kKeys);
-    uint32_t ok = n == 32 ? ~0u : (1u << n) - 1u;
+    const int n = min(KT, n_keys - t * KT);
+    uint64_t ok = ~0ull >> (64 - n);
     int32_t mine = 0;
     if constexpr (PAGED) {
       typedef __attribute__((address_space(3))) const int32_t lds_int;
       const lds_char* at = (const lds_char*)&sh.ids[kg][cg][i & 3][0];
-      mine = *(lds_int*)(at + 4 * ln);
-      const bool in = mine >= 0 && mine < a.pool && ln < n;
-      ok = (uint32_t)__ballot(in);
+      mine = *(lds_int*)(at + 4 * lane);
+      const bool in = mine >= 0 && mine < a.pool && lane < n;
+      ok = __ballot(in);
       mine = in ? mine : 0;
     }
     live[i & 1] = ok;
-    const uint32_t to = (uint32_t)(i & 1) * (kKeys * ROWB);
+    const uint32_t to = (uint32_t)(i & 1) * (KT * ROWB);
 #pragma unroll
     for (int y = 0; y < NI; ++y) {
       const int part = cg * NI + y;
@@ -193,18 +186,18 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
         dma16_far(v_lds + dst, (const char*)vb + off + vo);
       } else {
         const uint32_t off = (uint32_t)min(r, n - 1) * (uint32_t)st;
-        const int64_t row0 = (int64_t)(k0 + t * kKeys) * st;
+        const int64_t row0 = (int64_t)(k0 + t * KT) * st;
         dma16(k_lds + dst, (const char*)kb + row0, off + ko);
         dma16(v_lds + dst, (const char*)vb + row0, off + vo);
       }
     }
   };
-  // Rows that do not count read as zeros, whatever their place in memory holds (both waves of a
-  // group write the same).
+  // Rows that do not count read as zeros, whatever their place in memory holds (every wave of a
+  // group writes the same).
   auto blank = [&](int i) {
-    const uint32_t ok = live[i & 1];
-    const uint32_t at = (uint32_t)(i & 1) * (kKeys * ROWB);
-    for (int y = lane; y < kKeys * SEGS; y += 64) {
+    const uint64_t ok = live[i & 1];
+    const uint32_t at = (uint32_t)(i & 1) * (KT * ROWB);
+    for (int y = lane; y < KT * SEGS; y += 64) {
       if (!(ok >> (y / SEGS) & 1u)) {
         *(uint4*)((char*)&sh.k[kg][0][0] + at + 16 * y) = make_uint4(0u, 0u, 0u, 0u);
         *(uint4*)((char*)&sh.v[kg][0][0] + at + 16 * y) = make_uint4(0u, 0u, 0u, 0u);
@@ -216,75 +209,61 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
   const uint32_t kbase = (uint32_t)(ln * ROWB) + (uint32_t)((hh ^ kseg<D>(ln)) * 16);
   const uint32_t vbase = (uint32_t)((4 * hh + jj) * ROWB + 32 * (ln / 16) + 8 * (lane % 4));
   auto compute = [&](int i) {
-    const uint32_t ok = live[i & 1];
-    const lds_char* kt = (const lds_char*)&sh.k[kg][i & 1][0];
-    const lds_char* vt = (const lds_char*)&sh.v[kg][i & 1][0] + vbase;
     typedef __attribute__((address_space(3))) const op_t lds_op;
-    f32x16_t sc[QB];
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
+    for (int half = 0; half < HT; ++half) {
+      const uint32_t ok = (uint32_t)(live[i & 1] >> (32 * half));
+      const lds_char* kt = (const lds_char*)&sh.k[kg][i & 1][0] + half * 32 * ROWB;
+      const lds_char* vt = (const lds_char*)&sh.v[kg][i & 1][0] + half * 32 * ROWB + vbase;
+      f32x16_t sc;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sc[qb][r] = 0.0f;
-    }
+      for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
 #pragma unroll
-    for (int y = 0; y < KS; ++y) {
-      const op_t ka = *(lds_op*)(kt + (kbase ^ (uint32_t)(32 * y)));
-#pragma unroll
-      for (int qb = 0; qb < QB; ++qb) sc[qb] = M::run(ka, qop[qb][y], sc[qb]);
-    }
-    uint32_t ph[QB][8];
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-      float mt = -INFINITY;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) sc[qb][r] *= a.scale_log2;
+      for (int y = 0; y < KS; ++y) sc = M::run(*(lds_op*)(kt + (kbase ^ (uint32_t)(32 * y))), qop[y], sc);
       if (ok != ~0u) {  // uniform
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sc[qb][r] = ok >> (8 * (r / 4) + 4 * hh + r % 4) & 1u ? sc[qb][r] : -INFINITY;
+        for (int r = 0; r < 16; ++r) sc[r] = ok >> (8 * (r / 4) + 4 * hh + r % 4) & 1u ? sc[r] : -INFINITY;
       }
+      float mt = sc[0];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) mt = fmaxf(mt, sc[qb][r]);
-      mt = fmaxf(mt, lane_xor(mt, 32));
-      const bool moves = mt > m_run[qb] + TOP;
+      for (int r = 1; r < 16; ++r) mt = fmaxf(mt, sc[r]);
+      mt = fmaxf(mt, lane_xor(mt, 32)) * scale;
+      const bool moves = mt > m_run + TOP;
       if (__any(moves)) {
-        const float mn = moves ? mt - BIAS : m_run[qb];
-        const float alpha = fast_exp2(m_run[qb] - mn);
-        m_run[qb] = mn;
-        l_run[qb] *= alpha;
+        const float mn = moves ? mt - BIAS : m_run;
+        const float alpha = fast_exp2(m_run - mn);
+        m_run = mn;
+        l_run *= alpha;
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) o[d][qb][r] *= alpha;
+          for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
         }
       }
       float ls[2] = {0.0f, 0.0f};
+      uint32_t ph[8];
 #pragma unroll
       for (int r = 0; r < 16; r += 2) {
-        const float p0 = fast_exp2(sc[qb][r] - m_run[qb]), p1 = fast_exp2(sc[qb][r + 1] - m_run[qb]);
+        const float p0 = fast_exp2(fmaf(sc[r], scale, -m_run)), p1 = fast_exp2(fmaf(sc[r + 1], scale, -m_run));
         ls[0] += p0;
         ls[1] += p1;
-        ph[qb][r / 2] = M::pack2(p0, p1);
+        ph[r / 2] = M::pack2(p0, p1);
       }
-      l_run[qb] += ls[0] + ls[1];
-    }
+      l_run += ls[0] + ls[1];
 #pragma unroll
-    for (int sp = 0; sp < 2; ++sp) {
+      for (int sp = 0; sp < 2; ++sp) {
+        const op_t pb = __builtin_bit_cast(op_t, make_uint4(ph[4 * sp], ph[4 * sp + 1], ph[4 * sp + 2], ph[4 * sp + 3]));
 #pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const lds_char* vd = vt + (uint32_t)(64 * (D == 128 ? (d ^ jj) : (d ^ (jj >> 1))));
-        const uint2 lo = v_column4(vd, 16 * sp * ROWB), hi = v_column4(vd, (16 * sp + 8) * ROWB);
-        const op_t va = __builtin_bit_cast(op_t, make_uint4(lo.x, lo.y, hi.x, hi.y));
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) {
-          const op_t pb = __builtin_bit_cast(op_t, make_uint4(ph[qb][4 * sp], ph[qb][4 * sp + 1], ph[qb][4 * sp + 2],
-                                                              ph[qb][4 * sp + 3]));
-          o[d][qb] = M::run(va, pb, o[d][qb]);
+        for (int d = 0; d < DB; ++d) {
+          const lds_char* vd = vt + (uint32_t)(64 * (D == 128 ? (d ^ jj) : (d ^ (jj >> 1))));
+          const uint2 lo = v_column4(vd, 16 * sp * ROWB), hi = v_column4(vd, (16 * sp + 8) * ROWB);
+          o[d] = M::run(__builtin_bit_cast(op_t, make_uint4(lo.x, lo.y, hi.x, hi.y)), pb, o[d]);
         }
       }
     }
   };
 
-  const int turns = (n_tiles + kGroups - 1) / kGroups;
+  const int turns = (n_tiles + KG - 1) / KG;
   if constexpr (PAGED) {
     load_ids(0);
     load_ids(1);
@@ -300,8 +279,8 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
       load(i + 1);
       if constexpr (PAGED) load_ids(i + 2);
     }
-    if (kg + kGroups * i < n_tiles) {  // wave-uniform
-      if (live[i & 1] != ~0u) {
+    if (kg + KG * i < n_tiles) {  // wave-uniform
+      if (live[i & 1] != ~0ull >> (64 - KT)) {
         blank(i);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
@@ -312,52 +291,47 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
   __syncthreads();
 
   // the groups' states into one partial a column
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    const float l = l_run[qb] + lane_xor(l_run[qb], 32);
+  {
+    const float l = l_run + lane_xor(l_run, 32);
     if (hh == 0) {
-      sh.m[kg][cg][qb][ln] = m_run[qb];
-      sh.l[kg][cg][qb][ln] = l;
+      sh.m[kg][cg][ln] = m_run;
+      sh.l[kg][cg][ln] = l;
     }
-  }
-  const int pstride = GQ * (D + 2);
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4)
         *(float4*)&sh.o[kg][cg][ln][32 * d + 8 * r4 + 4 * hh] =
-            make_float4(o[d][qb][4 * r4], o[d][qb][4 * r4 + 1], o[d][qb][4 * r4 + 2], o[d][qb][4 * r4 + 3]);
+            make_float4(o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]);
     }
-    __syncthreads();
-    for (int y = tid; y < CG * 32 * (D / 4); y += THREADS) {
-      const int c = y / (D / 4), d4 = y % (D / 4), oc = c / 32, cl = c % 32;
-      int h;
-      const int64_t row = column((oc * QB + qb) * 32 + cl, h);
-      if (row < 0) continue;
-      float mm = kNegBig;
+  }
+  __syncthreads();
+  const int pstride = GQ * (D + 2);
+  for (int y = tid; y < COLS * (D / 4); y += THREADS) {
+    const int c = y / (D / 4), d4 = y % (D / 4), oc = c / 32, cl = c % 32;
+    int h;
+    const int64_t row = column(c, h);
+    if (row < 0) continue;
+    float mm = kNegBig;
 #pragma unroll
-      for (int z = 0; z < kGroups; ++z) mm = fmaxf(mm, sh.m[z][oc][qb][cl]);
-      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      float ll = 0.0f;
+    for (int z = 0; z < KG; ++z) mm = fmaxf(mm, sh.m[z][oc][cl]);
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float ll = 0.0f;
 #pragma unroll
-      for (int z = 0; z < kGroups; ++z) {
-        const float f = fast_exp2(sh.m[z][oc][qb][cl] - mm);
-        const float4 v = *(const float4*)&sh.o[z][oc][cl][4 * d4];
-        acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
-        ll += f * sh.l[z][oc][qb][cl];
-      }
-      float* part = a.parts + ((row * a.Hkv + g) * (a.splits + a.own_splits) + a.splits - pc.count + s) * (int64_t)pstride;
-      float* to = part + 2 * GQ + h * D + 4 * d4;  // 8-byte aligned
-      *(float2*)to = make_float2(acc.x, acc.y);
-      *(float2*)(to + 2) = make_float2(acc.z, acc.w);
-      if (d4 == 0) {
-        part[h] = mm;
-        part[GQ + h] = ll;
-      }
+    for (int z = 0; z < KG; ++z) {
+      const float f = fast_exp2(sh.m[z][oc][cl] - mm);
+      const float4 v = *(const float4*)&sh.o[z][oc][cl][4 * d4];
+      acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+      ll += f * sh.l[z][oc][cl];
     }
-    __syncthreads();
+    float* part = a.parts + ((row * a.Hkv + g) * (a.splits + a.own_splits) + a.splits - pc.count + s) * (int64_t)pstride;
+    float* to = part + 2 * GQ + h * D + 4 * d4;  // 8-byte aligned
+    *(float2*)to = make_float2(acc.x, acc.y);
+    *(float2*)(to + 2) = make_float2(acc.z, acc.w);
+    if (d4 == 0) {
+      part[h] = mm;
+      part[GQ + h] = ll;
+    }
   }
 }
 
@@ -369,20 +343,20 @@ int64_t column_blocks(const PrefixArgs& a, int64_t columns) {
   return (a.B * a.Tq * (a.Hq / a.Hkv) + wg - 1) / wg;
 }
 
-template <typename T, int D, int QB, int CG>
+template <typename T, int D, int KG, int CG>
 void launch_mfma(const PrefixArgs& a, int n_cb, hipStream_t s) {
   const dim3 grid((unsigned)(prefix_units(a) * n_cb));
-  if (a.slots) prefix_mfma_kernel<T, D, QB, CG, true><<<grid, 64 * kGroups * CG, 0, s>>>(a, n_cb);
-  else prefix_mfma_kernel<T, D, QB, CG, false><<<grid, 64 * kGroups * CG, 0, s>>>(a, n_cb);
+  if (a.slots) prefix_mfma_kernel<T, D, KG, CG, true><<<grid, 64 * KG * CG, 0, s>>>(a, n_cb);
+  else prefix_mfma_kernel<T, D, KG, CG, false><<<grid, 64 * KG * CG, 0, s>>>(a, n_cb);
 }
 
 template <typename T, int D>
 void launch_mfma_cols(const PrefixArgs& a, int64_t columns, hipStream_t s) {
   const int64_t wg = prefix_mfma_columns(columns);
   const int n_cb = (int)column_blocks(a, columns);
-  if (wg == 32) launch_mfma<T, D, 1, 1>(a, n_cb, s);
-  else if (wg == 64) launch_mfma<T, D, 1, 2>(a, n_cb, s);
-  else launch_mfma<T, D, 2, 2>(a, n_cb, s);
+  if (wg == 32) launch_mfma<T, D, 4, 1>(a, n_cb, s);
+  else if (wg == 64) launch_mfma<T, D, 4, 2>(a, n_cb, s);
+  else launch_mfma<T, D, 2, 4>(a, n_cb, s);
 }
 
 }  // namespace
