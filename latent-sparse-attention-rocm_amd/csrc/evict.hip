@@ -63,16 +63,190 @@ __global__ __launch_bounds__(LSA_BLOCK) void seen_keys_kernel(KeepArgs a) {
   }
   const float* m = a.mass + b * a.mass_sb + (ok ? at : 0);
   double sum = 0.0;
-  for (int h = 0; h < a.Hkv; ++h) sum += (double)m[h * a.mass_sh];
+  for (int h0 = 0; h0 < a.Hkv; h0 += 8) {  // eight heads' loads in flight
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = m[min(h0 + e, a.Hkv - 1) * a.mass_sh];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += h0 + e < a.Hkv ? (double)f[e] : 0.0;
+  }
   a.keys_out[b * a.T + i] = ok ? seen_key((float)sum) : 0u;
 }
 
 // One workgroup a selection.
+//
+// The threshold, the budget's last key, comes from three histograms (11, 11 and 10 bits from the
+// top), each over the keys that share the digits found so far. Weights crowd into few bins (a third
+// of a cache may be exactly zero), and lanes that meet in one bin of LDS wait for each other, so there are four
+// copies of each histogram, a lane's by its number.
+//
+//   keep_kernel       rows of up to 32768 positions: a thread holds R in a line, turned through LDS
+//                     after coalesced loads. A CU's vector unit is what bounds it (one CU works on
+//                     a selection), so a key costs few instructions: the first and last positions
+//                     are the largest key, those past the row the least, and no loop asks which is
+//                     which; one scan over the threads' counts ranks everything.
+//   keep_long_kernel  longer rows: every pass reads the keys again, and ranks count slab by slab.
+constexpr int kBins = 2048, kCopies = 4;
+
+struct KeepLds {
+  int hist[kCopies][kBins];
+  int gt[kKeepThreads], eq[kKeepThreads];  // of a (slab, wave)
+  int wave_gt[kKeepWaves], wave_eq[kKeepWaves];
+  uint32_t digit;
+  int need;
+};
+
+// Exclusive sums over the workgroup's threads of two counts; every thread calls it.
+__device__ __forceinline__ void keep_scan(KeepLds& sh, int& gt, int& eq, int& all_gt, int& all_eq) {
+  const int lane = threadIdx.x & (LSA_WAVE - 1), w = threadIdx.x / LSA_WAVE;
+  const int ig = wave_inclusive_sum(gt), ie = wave_inclusive_sum(eq);
+  if (lane == LSA_WAVE - 1) {
+    sh.wave_gt[w] = ig;
+    sh.wave_eq[w] = ie;
+  }
+  __syncthreads();
+  int bg = 0, be = 0;
+  all_gt = all_eq = 0;
+#pragma unroll
+  for (int y = 0; y < kKeepWaves; ++y) {
+    const int cg = sh.wave_gt[y], ce = sh.wave_eq[y];
+    bg += y < w ? cg : 0;
+    be += y < w ? ce : 0;
+    all_gt += cg;
+    all_eq += ce;
+  }
+  __syncthreads();
+  gt = bg + ig - gt;
+  eq = be + ie - eq;
+}
+
+// The bin that the `need`-th key from the top is in, given every thread's share of the histogram
+// (bins 2047 - 2 t and 2046 - 2 t): its digit, and how many of its keys are needed.
+__device__ __forceinline__ void keep_digit(KeepLds& sh, int need) {
+  const int tid = threadIdx.x;
+  int c[2], none = 0, mine = 0, total, unused;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    c[e] = 0;
+#pragma unroll
+    for (int y = 0; y < kCopies; ++y) c[e] += sh.hist[y][kBins - 1 - 2 * tid - e];
+    mine += c[e];
+  }
+  const int own = mine;
+  keep_scan(sh, mine, none, total, unused);
+  if (mine < need && need <= mine + own) {
+    const int e = mine + c[0] < need ? 1 : 0;
+    sh.digit = (uint32_t)(kBins - 1 - 2 * tid - e);
+    sh.need = need - mine - (e ? c[0] : 0);
+  }
+  __syncthreads();
+}
+__device__ __forceinline__ void keep_clear(KeepLds& sh) {
+  for (int i = threadIdx.x; i < kCopies * kBins; i += kKeepThreads) (&sh.hist[0][0])[i] = 0;
+  __syncthreads();
+}
+
+template <int R>
+struct KeepTurn {
+  static constexpr int PAD = R > 4 ? 4 : 0;  // dwords a thread's run is kept apart: 16-byte reads without conflicts
+  union {
+    uint32_t key[kKeepThreads * (R + PAD)];
+    int32_t place[kKeepThreads * R];  // the positions in their new order
+    KeepLds sh;
+  };
+};
+
+template <int R>
 __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
-  __shared__ int hist[256];
-  __shared__ int wave_gt[kKeepWaves], wave_eq[kKeepWaves];
-  __shared__ uint32_t sh_prefix;
-  __shared__ int sh_need;
+  using Turn = KeepTurn<R>;
+  __shared__ __attribute__((aligned(16))) Turn turn;
+  KeepLds& sh = turn.sh;
+  const int tid = threadIdx.x, lane = tid & (LSA_WAVE - 1);
+  const int64_t u = blockIdx.x;
+  const int64_t b = u / a.G;
+  const int g = (int)(u % a.G);
+  const int n = row_length(a, b);
+  const int keep = n < a.budget ? n : a.budget;
+  if (g == 0 && tid == 0) a.new_lengths[b] = keep;
+  int32_t* kept = a.kept + u * a.budget;
+  const int32_t* table = a.table ? a.table + b * a.table_stride : nullptr;
+  int32_t* new_table = a.new_table ? a.new_table + b * a.new_stride : nullptr;
+  if (n <= a.budget) {  // uniform: all of it
+    for (int i = tid; i < a.budget; i += kKeepThreads) kept[i] = i < n ? i : -1;
+    if (new_table) {
+      for (int64_t i = tid; i < a.T; i += kKeepThreads) new_table[i] = table[i];
+    }
+    return;
+  }
+  {
+    const float* mass = a.mass + b * a.mass_sb + g * a.mass_sh;
+    const uint32_t* keys = a.keys ? a.keys + u * a.T : nullptr;
+    uint32_t in[R];
+#pragma unroll
+    for (int e = 0; e < R; ++e) {  // unconditional (clamped): all in flight
+      const int i = min(e * kKeepThreads + tid, n - 1);
+      in[e] = keys ? keys[i] : __float_as_uint(mass[i]);
+    }
+#pragma unroll
+    for (int e = 0; e < R; ++e) {
+      const int i = e * kKeepThreads + tid;
+      uint32_t x = keys ? in[e] : seen_key(__uint_as_float(in[e]));
+      x = i < a.sink || i >= n - a.window ? 0xFFFFFFFFu : x;  // no weight has this key
+      turn.key[i + i / R * Turn::PAD] = i < n ? x : 0u;
+    }
+  }
+  __syncthreads();
+  uint32_t x[R];
+#pragma unroll
+  for (int e = 0; e < R; e += 4) {
+    const uint4 y = *(const uint4*)&turn.key[tid * (R + Turn::PAD) + e];
+    x[e] = y.x; x[e + 1] = y.y; x[e + 2] = y.z; x[e + 3] = y.w;
+  }
+  __syncthreads();
+  uint32_t thr = 0, mask = 0;
+  int ties = a.budget;
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
+    keep_clear(sh);
+    int* hist = sh.hist[lane % kCopies];
+#pragma unroll
+    for (int e = 0; e < R; ++e) {
+      if ((x[e] & mask) == thr) atomicAdd(&hist[(x[e] >> shift) & (kBins - 1)], 1);
+    }
+    __syncthreads();
+    keep_digit(sh, ties);
+    thr |= sh.digit << shift;
+    ties = sh.need;
+    mask |= (pass == 2 ? 1023u : 2047u) << shift;
+  }
+  int gt = 0, eq = 0, all_gt, all_eq;
+#pragma unroll
+  for (int e = 0; e < R; ++e) {
+    gt += x[e] > thr;
+    eq += x[e] == thr;
+  }
+  keep_scan(sh, gt, eq, all_gt, all_eq);  // kept, and at the threshold, before this thread's positions
+  // positions past the row tie with NaN alone, and come after every position of the row
+#pragma unroll
+  for (int e = 0; e < R; ++e) {
+    const int i = tid * R + e, rank = gt + min(eq, ties);
+    const bool more = x[e] > thr, same = x[e] == thr;
+    const bool in = more || (same && eq < ties);
+    if (in || (new_table && i < n)) turn.place[in ? rank : keep + (i - rank)] = i;
+    gt += more;
+    eq += same;
+  }
+  __syncthreads();
+  for (int j = tid; j < keep; j += kKeepThreads) kept[j] = turn.place[j];
+  if (new_table) {
+    for (int64_t i = tid; i < a.T; i += kKeepThreads) new_table[i] = table[i < n ? turn.place[i] : i];
+  }
+}
+
+__global__ __launch_bounds__(kKeepThreads) void keep_long_kernel(KeepArgs a) {
+  __shared__ KeepLds sh;
+  constexpr int U = 8;  // keys of a thread at once
   const int tid = threadIdx.x, lane = tid & (LSA_WAVE - 1), w = tid / LSA_WAVE;
   const int64_t u = blockIdx.x;
   const int64_t b = u / a.G;
@@ -83,79 +257,106 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
   const bool all = n <= a.budget;
   const int lo = min(a.sink, n), hi = all ? lo : n - a.window;  // the positions that compete
   const float* mass = a.mass + b * a.mass_sb + g * a.mass_sh;
-  const uint32_t* keys = a.keys + u * a.T;
-  auto key = [&](int i) { return a.keys ? keys[i] : seen_key(mass[i]); };
-
+  const uint32_t* keys = a.keys ? a.keys + u * a.T : nullptr;
+  uint32_t x[U];
+  auto fetch = [&](int i0) {  // of positions i0 + tid + 1024 e; unconditional loads (clamped), n > 0
+    float f[U];
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      const int i = min(i0 + e * kKeepThreads + tid, n - 1);
+      if (keys) x[e] = keys[i];
+      else f[e] = mass[i];
+    }
+    if (!keys) {
+#pragma unroll
+      for (int e = 0; e < U; ++e) x[e] = seen_key(f[e]);
+    }
+  };
+  const int step = U * kKeepThreads;
   uint32_t thr = 0xFFFFFFFFu;
   int ties = 0;  // how many of the keys equal to the threshold stay
-  if (!all) {    // uniform
+  int need = a.budget - lo - (n - hi);
+  if (!all && need > 0) {  // uniform
     uint32_t prefix = 0, mask = 0;
-    int need = a.budget - lo - (n - hi);
-    if (need > 0) {
-      for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (int i = lo + tid; i < hi; i += kKeepThreads) {
-          const uint32_t x = key(i);
-          if ((x & mask) == prefix) atomicAdd(&hist[(x >> shift) & 255], 1);
-        }
-        __syncthreads();
-        if (w == 0) {  // lane l owns bins 255 - 4 l .. 252 - 4 l, from the top
-          int c[4], mine = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
+      keep_clear(sh);
+      for (int i0 = 0; i0 < n; i0 += step) {
+        fetch(i0);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mine += c[e] = hist[255 - 4 * lane - e];
-          const int inc = wave_inclusive_sum(mine);
-          int above = inc - mine;
-          if (above < need && need <= inc) {
-            int e = 0;
-            while (above + c[e] < need) above += c[e++];
-            sh_prefix = prefix | ((uint32_t)(255 - 4 * lane - e) << shift);
-            sh_need = need - above;
-          }
+        for (int e = 0; e < U; ++e) {
+          const int i = i0 + e * kKeepThreads + tid;
+          if (i >= lo && i < hi && (x[e] & mask) == prefix)
+            atomicAdd(&sh.hist[lane % kCopies][(x[e] >> shift) & (kBins - 1)], 1);
         }
-        __syncthreads();
-        prefix = sh_prefix;
-        need = sh_need;
-        mask |= 255u << shift;
       }
-      thr = prefix;
-      ties = need;
+      __syncthreads();
+      keep_digit(sh, need);
+      prefix |= sh.digit << shift;
+      need = sh.need;
+      mask |= (pass == 2 ? 1023u : 2047u) << shift;
     }
+    thr = prefix;
+    ties = need;
   }
   int32_t* kept = a.kept + u * a.budget;
   const int32_t* table = a.table ? a.table + b * a.table_stride : nullptr;
   int32_t* new_table = a.new_table ? a.new_table + b * a.new_stride : nullptr;
   const uint64_t below = lane == 0 ? 0ull : ~0ull >> (LSA_WAVE - lane);
-  int base = 0, base_eq = 0;  // kept for their place or weight, and at the threshold, before this chunk
-  for (int i0 = 0; i0 < n; i0 += kKeepThreads) {
-    const int i = i0 + tid;
-    const bool in = i < n;
-    const bool middle = in && !all && i >= lo && i < hi;
-    const uint32_t x = middle ? key(i) : 0u;
-    const bool gt = in && (!middle || x > thr);
-    const bool eq = middle && x == thr && ties > 0;
-    const uint64_t mg = __ballot(gt), me = __ballot(eq);
-    if (lane == 0) {
-      wave_gt[w] = __popcll(mg);
-      wave_eq[w] = __popcll(me);
-    }
+  // stays for its place or weight (gt), or may stay as one of the keys at the threshold (eq)
+  auto stays = [&](int e, int i, bool& gt, bool& eq) {
+    const bool middle = !all && i >= lo && i < hi;
+    gt = i < n && (!middle || x[e] > thr);
+    eq = middle && x[e] == thr && ties > 0;
+  };
+  constexpr int SLABS = kKeepThreads / kKeepWaves;  // counted in one scan
+  int base = 0, base_eq = 0;
+  for (int s0 = 0; s0 < n; s0 += SLABS * kKeepThreads) {
+    sh.gt[tid] = sh.eq[tid] = 0;
     __syncthreads();
-    int bg = base, be = base_eq;
+    const int s1 = min(n, s0 + SLABS * kKeepThreads);
+    for (int i0 = s0; i0 < s1; i0 += step) {
+      if (!all) fetch(i0);
 #pragma unroll
-    for (int y = 0; y < kKeepWaves; ++y) {
-      const int cg = wave_gt[y], ce = wave_eq[y];
-      bg += y < w ? cg : 0;
-      be += y < w ? ce : 0;
-      base += cg;
-      base_eq += ce;
+      for (int e = 0; e < U; ++e) {
+        const int j = i0 + e * kKeepThreads;
+        if (j >= s1) break;
+        bool gt, eq;
+        stays(e, j + tid, gt, eq);
+        const int cg = __popcll(__ballot(gt)), ce = __popcll(__ballot(eq));
+        if (lane == 0) {
+          const int at = (j - s0) / kKeepThreads * kKeepWaves + w;
+          sh.gt[at] = cg;
+          sh.eq[at] = ce;
+        }
+      }
     }
     __syncthreads();
-    bg += __popcll(mg & below);
-    be += __popcll(me & below);
-    const int rank = bg + min(be, ties);  // kept positions before i
-    const bool stays = gt || (eq && be < ties);
-    if (stays) kept[rank] = i;
-    if (in && new_table) new_table[stays ? rank : keep + (i - rank)] = table[i];
+    int cg = sh.gt[tid], ce = sh.eq[tid], tg, te;
+    keep_scan(sh, cg, ce, tg, te);
+    sh.gt[tid] = base + cg;
+    sh.eq[tid] = base_eq + ce;
+    base += tg;
+    base_eq += te;
+    __syncthreads();
+    for (int i0 = s0; i0 < s1; i0 += step) {
+      if (!all) fetch(i0);
+#pragma unroll
+      for (int e = 0; e < U; ++e) {
+        const int j = i0 + e * kKeepThreads, i = j + tid;
+        if (j >= s1) break;
+        bool gt, eq;
+        stays(e, i, gt, eq);
+        const int at = (j - s0) / kKeepThreads * kKeepWaves + w;
+        const int bg = sh.gt[at] + __popcll(__ballot(gt) & below), be = sh.eq[at] + __popcll(__ballot(eq) & below);
+        const int rank = bg + min(be, ties);  // kept positions before i
+        const bool in = gt || (eq && be < ties);
+        if (in) kept[rank] = i;
+        if (i < n && new_table) new_table[in ? rank : keep + (i - rank)] = table[i];
+      }
+    }
+    __syncthreads();
   }
   for (int j = keep + tid; j < a.budget; j += kKeepThreads) kept[j] = -1;
   if (new_table) {
@@ -254,7 +455,12 @@ extern "C" int lsa_evict_keep(const float* mass, int64_t B, int32_t Hkv, int64_t
     seen_keys_kernel<<<grid, LSA_BLOCK, 0, s>>>(a);
     LSA_LAUNCHED("lsa_evict_keep");
   }
-  keep_kernel<<<dim3((unsigned)(B * a.G)), kKeepThreads, 0, s>>>(a);
+  const dim3 grid((unsigned)(B * a.G));
+  if (T <= 4 * kKeepThreads) keep_kernel<4><<<grid, kKeepThreads, 0, s>>>(a);
+  else if (T <= 8 * kKeepThreads) keep_kernel<8><<<grid, kKeepThreads, 0, s>>>(a);
+  else if (T <= 16 * kKeepThreads) keep_kernel<16><<<grid, kKeepThreads, 0, s>>>(a);
+  else if (T <= 32 * kKeepThreads) keep_kernel<32><<<grid, kKeepThreads, 0, s>>>(a);
+  else keep_long_kernel<<<grid, kKeepThreads, 0, s>>>(a);
   LSA_LAUNCHED("lsa_evict_keep");
   return LSA_OK;
 }
