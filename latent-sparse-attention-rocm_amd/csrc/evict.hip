@@ -77,8 +77,8 @@ __global__ __launch_bounds__(LSA_BLOCK) void seen_keys_kernel(KeepArgs a) {
 //
 // The threshold, the budget's last key, comes from three histograms (11, 11 and 10 bits from the
 // top), each over the keys that share the digits found so far. Weights crowd into few bins (a third
-// of a cache may be exactly zero), and lanes that meet in one bin of LDS wait for each other, so there are four
-// copies of each histogram, a lane's by its number.
+// of a cache may be exactly zero), and lanes that meet in one bin of LDS wait for each other, so there are eight
+// copies of each histogram, a lane's by its number, side by side: a bin's copies lie in banks of their own.
 //
 //   keep_kernel       rows of up to 32768 positions: a thread holds R in a line, turned through LDS
 //                     after coalesced loads. A CU's vector unit is what bounds it (one CU works on
@@ -86,10 +86,10 @@ __global__ __launch_bounds__(LSA_BLOCK) void seen_keys_kernel(KeepArgs a) {
 //                     are the largest key, those past the row the least, and no loop asks which is
 //                     which; one scan over the threads' counts ranks everything.
 //   keep_long_kernel  longer rows: every pass reads the keys again, and ranks count slab by slab.
-constexpr int kBins = 2048, kCopies = 4;
+constexpr int kBins = 2048, kCopies = 8;
 
 struct KeepLds {
-  int hist[kCopies][kBins];
+  alignas(16) int hist[kBins][kCopies];
   int gt[kKeepThreads], eq[kKeepThreads];  // of a (slab, wave)
   int wave_gt[kKeepWaves], wave_eq[kKeepWaves];
   uint32_t digit;
@@ -129,7 +129,10 @@ __device__ __forceinline__ void keep_digit(KeepLds& sh, int need) {
   for (int e = 0; e < 2; ++e) {
     c[e] = 0;
 #pragma unroll
-    for (int y = 0; y < kCopies; ++y) c[e] += sh.hist[y][kBins - 1 - 2 * tid - e];
+    for (int y = 0; y < kCopies; y += 4) {
+      const int4 x = *(const int4*)&sh.hist[kBins - 1 - 2 * tid - e][y];
+      c[e] += x.x + x.y + x.z + x.w;
+    }
     mine += c[e];
   }
   const int own = mine;
@@ -142,13 +145,16 @@ __device__ __forceinline__ void keep_digit(KeepLds& sh, int need) {
   __syncthreads();
 }
 __device__ __forceinline__ void keep_clear(KeepLds& sh) {
-  for (int i = threadIdx.x; i < kCopies * kBins; i += kKeepThreads) (&sh.hist[0][0])[i] = 0;
+  int4* h = (int4*)&sh.hist[0][0];
+#pragma unroll
+  for (int i = 0; i < kCopies * kBins / 4 / kKeepThreads; ++i) h[i * kKeepThreads + threadIdx.x] = make_int4(0, 0, 0, 0);
   __syncthreads();
 }
 
 template <int R>
 struct KeepTurn {
   static constexpr int PAD = R > 4 ? 4 : 0;  // dwords a thread's run is kept apart: 16-byte reads without conflicts
+  static __host__ __device__ constexpr int at(int i) { return i + (int)((unsigned)i / R) * PAD; }
   union {
     uint32_t key[kKeepThreads * (R + PAD)];
     int32_t place[kKeepThreads * R];  // the positions in their new order
@@ -156,7 +162,7 @@ struct KeepTurn {
   };
 };
 
-template <int R>
+template <int R, bool TABLE>
 __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
   using Turn = KeepTurn<R>;
   __shared__ __attribute__((aligned(16))) Turn turn;
@@ -173,7 +179,7 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
   int32_t* new_table = a.new_table ? a.new_table + b * a.new_stride : nullptr;
   if (n <= a.budget) {  // uniform: all of it
     for (int i = tid; i < a.budget; i += kKeepThreads) kept[i] = i < n ? i : -1;
-    if (new_table) {
+    if (TABLE) {
       for (int64_t i = tid; i < a.T; i += kKeepThreads) new_table[i] = table[i];
     }
     return;
@@ -187,13 +193,15 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
       const int i = min(e * kKeepThreads + tid, n - 1);
       in[e] = keys ? keys[i] : __float_as_uint(mass[i]);
     }
+    uint32_t* to = &turn.key[Turn::at(tid)];
 #pragma unroll
-    for (int e = 0; e < R; ++e) {
-      const int i = e * kKeepThreads + tid;
-      uint32_t x = keys ? in[e] : seen_key(__uint_as_float(in[e]));
-      x = i < a.sink || i >= n - a.window ? 0xFFFFFFFFu : x;  // no weight has this key
-      turn.key[i + i / R * Turn::PAD] = i < n ? x : 0u;
-    }
+    for (int e = 0; e < R; ++e)
+      to[Turn::at(e * kKeepThreads)] = keys ? in[e] : seen_key(__uint_as_float(in[e]));
+    __syncthreads();
+    // the first and last positions, which no weight equals, and what is past the row
+    for (int i = tid; i < a.sink; i += kKeepThreads) turn.key[Turn::at(i)] = 0xFFFFFFFFu;
+    for (int i = n - a.window + tid; i < R * kKeepThreads; i += kKeepThreads)
+      turn.key[Turn::at(i)] = i < n ? 0xFFFFFFFFu : 0u;
   }
   __syncthreads();
   uint32_t x[R];
@@ -209,10 +217,10 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
     keep_clear(sh);
-    int* hist = sh.hist[lane % kCopies];
+    int* hist = &sh.hist[0][lane % kCopies];
 #pragma unroll
     for (int e = 0; e < R; ++e) {
-      if ((x[e] & mask) == thr) atomicAdd(&hist[(x[e] >> shift) & (kBins - 1)], 1);
+      if ((x[e] & mask) == thr) atomicAdd(&hist[((x[e] >> shift) & (kBins - 1)) * kCopies], 1);
     }
     __syncthreads();
     keep_digit(sh, ties);
@@ -228,18 +236,23 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
   }
   keep_scan(sh, gt, eq, all_gt, all_eq);  // kept, and at the threshold, before this thread's positions
   // positions past the row tie with NaN alone, and come after every position of the row
+  int rank = gt + min(eq, ties);  // kept positions before this one
 #pragma unroll
   for (int e = 0; e < R; ++e) {
-    const int i = tid * R + e, rank = gt + min(eq, ties);
-    const bool more = x[e] > thr, same = x[e] == thr;
-    const bool in = more || (same && eq < ties);
-    if (in || (new_table && i < n)) turn.place[in ? rank : keep + (i - rank)] = i;
-    gt += more;
+    const int i = tid * R + e;
+    const bool same = x[e] == thr;
+    const bool in = x[e] > thr || (same && eq < ties);
+    if (TABLE) {
+      if (i < n) turn.place[in ? rank : keep + (i - rank)] = i;
+    } else if (in) {
+      turn.place[rank] = i;
+    }
+    rank += in;
     eq += same;
   }
   __syncthreads();
   for (int j = tid; j < keep; j += kKeepThreads) kept[j] = turn.place[j];
-  if (new_table) {
+  if (TABLE) {
     for (int64_t i = tid; i < a.T; i += kKeepThreads) new_table[i] = table[i < n ? turn.place[i] : i];
   }
 }
@@ -288,7 +301,7 @@ __global__ __launch_bounds__(kKeepThreads) void keep_long_kernel(KeepArgs a) {
         for (int e = 0; e < U; ++e) {
           const int i = i0 + e * kKeepThreads + tid;
           if (i >= lo && i < hi && (x[e] & mask) == prefix)
-            atomicAdd(&sh.hist[lane % kCopies][(x[e] >> shift) & (kBins - 1)], 1);
+            atomicAdd(&sh.hist[(x[e] >> shift) & (kBins - 1)][lane % kCopies], 1);
         }
       }
       __syncthreads();
@@ -408,6 +421,12 @@ __global__ __launch_bounds__(LSA_BLOCK) void keep_rows_kernel(RowsArgs a, int ro
   }
 }
 
+template <int R>
+void launch_keep(const KeepArgs& a, dim3 grid, hipStream_t s) {
+  if (a.table) keep_kernel<R, true><<<grid, kKeepThreads, 0, s>>>(a);
+  else keep_kernel<R, false><<<grid, kKeepThreads, 0, s>>>(a);
+}
+
 int check_keep(const char* who, const void* mass, int64_t B, int32_t Hkv, int64_t T, int64_t mass_sb, int64_t mass_sh,
                int32_t budget, int32_t window, int32_t sink, const void* kept, const void* new_lengths) {
   LSA_REQUIRE(mass && kept && new_lengths, LSA_ERR_NULL, "%s: NULL pointer", who);
@@ -456,10 +475,10 @@ extern "C" int lsa_evict_keep(const float* mass, int64_t B, int32_t Hkv, int64_t
     LSA_LAUNCHED("lsa_evict_keep");
   }
   const dim3 grid((unsigned)(B * a.G));
-  if (T <= 4 * kKeepThreads) keep_kernel<4><<<grid, kKeepThreads, 0, s>>>(a);
-  else if (T <= 8 * kKeepThreads) keep_kernel<8><<<grid, kKeepThreads, 0, s>>>(a);
-  else if (T <= 16 * kKeepThreads) keep_kernel<16><<<grid, kKeepThreads, 0, s>>>(a);
-  else if (T <= 32 * kKeepThreads) keep_kernel<32><<<grid, kKeepThreads, 0, s>>>(a);
+  if (T <= 4 * kKeepThreads) launch_keep<4>(a, grid, s);
+  else if (T <= 8 * kKeepThreads) launch_keep<8>(a, grid, s);
+  else if (T <= 16 * kKeepThreads) launch_keep<16>(a, grid, s);
+  else if (T <= 32 * kKeepThreads) launch_keep<32>(a, grid, s);
   else keep_long_kernel<<<grid, kKeepThreads, 0, s>>>(a);
   LSA_LAUNCHED("lsa_evict_keep");
   return LSA_OK;
