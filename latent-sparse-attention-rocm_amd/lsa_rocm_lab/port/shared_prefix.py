@@ -14,17 +14,19 @@ import torch
 from lsa_rocm_lab import _abi
 
 
+_HERE = contextlib.nullcontext()
+
+
 def launch_device(device: torch.device):
-    """A context in which a launch on ``device`` finds it current (nothing where it is)."""
-    index = _abi.device_index(device)
-    return contextlib.nullcontext() if index == torch.cuda.current_device() else torch.cuda.device(index)
+    """A context in which a launch on a tensor's ``device`` finds it current (nothing where it is)."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def one_device(what: str, *tensors: torch.Tensor | None) -> torch.device:
     """The ROCm device that all of the tensors are on; anything else raises ``ValueError``."""
     device = tensors[0].device
     for t in tensors:
-        if t is not None and (t.device.type != "cuda" or t.device != device):
+        if t is not None and (t.device != device or device.type != "cuda"):
             raise ValueError(f"{what} is a ROCm kernel over tensors of one device, got {device} and {t.device}")
     return device
 
@@ -38,22 +40,23 @@ def int32_on(t: torch.Tensor, device: torch.device) -> torch.Tensor:
 
 def cache_strides(x: torch.Tensor) -> tuple[int, int, int]:
     """Batch, token and head strides of a cache [B, T, Hkv, D] (an axis of one has none of its own)."""
-    sb, st, sh = x.stride()[:3]
-    return (sb if x.shape[0] > 1 else 0, st if x.shape[1] > 1 else x.shape[3], sh if x.shape[2] > 1 else x.shape[3])
+    sb, st, sh, _ = x.stride()
+    nb, nt, nh, D = x.shape
+    return sb if nb > 1 else 0, st if nt > 1 else D, sh if nh > 1 else D
 
 
 def cache_pair(k: torch.Tensor, v: torch.Tensor):
     """K and V as a kernel reads them (rows of contiguous elements at the same strides; other
     layouts are made dense) and their strides."""
-    if (k.stride(-1) != 1 or v.stride(-1) != 1 or cache_strides(k) != cache_strides(v)
-            or k.data_ptr() % 16 or v.data_ptr() % 16):
-        k, v = k.contiguous(), v.contiguous()
-        if k.data_ptr() % 16 or v.data_ptr() % 16:  # a contiguous view that begins off a row's alignment
-            k, v = k.clone(), v.clone()
+    ks, vs = k.stride(), v.stride()
+    if (ks[3] != 1 or vs[3] != 1 or (ks != vs and cache_strides(k) != cache_strides(v))
+            or (k.data_ptr() | v.data_ptr()) % 16):
+        k, v = aligned(k), aligned(v)
     return k, v, cache_strides(k)
 
 
 def aligned(x: torch.Tensor) -> torch.Tensor:
+    """``x`` dense and 16-byte aligned (a contiguous view may begin off that)."""
     x = x.contiguous()
     return x.clone() if x.data_ptr() % 16 else x
 
@@ -99,8 +102,8 @@ def prefix_read(
     Returns the output, like q, or with ``return_lse`` also the softmax's logarithm of sums
     [B, Tq, Hq] in fp32 (``key_mass`` takes it). A row with no keys gives zeros and -inf.
     """
-    own = (k, v, read_lists, lengths)
-    if any(t is None for t in own) and not all(t is None for t in own):
+    none = k is None
+    if (v is None) != none or (read_lists is None) != none or (lengths is None) != none:
         raise ValueError("prefix_read: k, v, read_lists and lengths come together")
     device = one_device("prefix_read", q, k_prefix, v_prefix, k, v)
     if q.dim() != 4 or k_prefix.dim() != 4 or k_prefix.shape != v_prefix.shape:
@@ -110,9 +113,10 @@ def prefix_read(
     Hkv = k_prefix.shape[2]
     if k_prefix.shape[3] != D or Hkv < 1 or Hq % Hkv:
         raise ValueError(f"prefix_read: {Hq} query heads of {D} on prefixes {tuple(k_prefix.shape)}")
-    if any(t is not None and t.dtype != q.dtype for t in (k_prefix, v_prefix, k, v)):
+    dtype = q.dtype
+    if k_prefix.dtype != dtype or v_prefix.dtype != dtype or (k is not None and (k.dtype != dtype or v.dtype != dtype)):
         raise ValueError("prefix_read: q, the prefixes and k/v must have one dtype")
-    dt = _abi.dtype_code(q.dtype)
+    dt = _abi.dtype_code(dtype)
     slots = None
     if prefix_slots is not None:
         if prefix_slots.dim() != 2 or prefix_slots.shape[0] < 1 or k_prefix.shape[0] != 1:
