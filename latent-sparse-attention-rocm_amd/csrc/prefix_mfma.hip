@@ -46,12 +46,123 @@ struct alignas(1024) PrefixLds {
   int count[KG * CG];
 };
 
+// A workgroup's place: kv-head, prefix, piece, and the batch rows whose query rows times heads are
+// its columns (column: batch row of the prefix, query row, head). The grid's (kv-head, prefix, piece)
+// units come in groups of 8, the column blocks of a unit 8 apart, so that those which read the same
+// keys share an XCD and its L2.
+template <int COLS>
+struct PrefixBlock {
+  int GQ, g, p, s, found;
+  int64_t per, c0, first;
+  Pieces pc;
+  const int32_t* member;
+
+  // False: nothing to do (the whole workgroup). Clears the grid's share of the counters.
+  __device__ __forceinline__ bool init(const PrefixArgs& a, int n_cb, int threads, int32_t* members, int* count) {
+    const int tid = threadIdx.x, lane = tid & 63, w = tid / 64;
+    member = members;
+    GQ = a.Hq / a.Hkv;
+    const int64_t clear = (int64_t)gridDim.x * threads;
+    for (int64_t i = (int64_t)blockIdx.x * threads + tid; i < a.B * a.Tq * a.Hkv; i += clear) a.counters[i] = 0;
+    const int64_t x = blockIdx.x;
+    const int cb = (int)(x / kXcds % n_cb);
+    int64_t u = x / kXcds / n_cb * kXcds + x % kXcds;
+    s = (int)(u % a.splits); u /= a.splits;
+    g = (int)(u % a.Hkv); u /= a.Hkv;
+    if (u >= a.P) return false;
+    p = (int)u;
+    pc = prefix_pieces(a, p);
+    if (s >= pc.count) return false;
+    per = a.Tq * GQ;
+    c0 = (int64_t)cb * COLS;
+    first = c0 / per;
+    if (a.prefix_rows == nullptr) {
+      if (first >= a.B) return false;
+      found = (int)min(a.B - first, (int64_t)COLS);
+      if (tid < found) members[tid] = (int32_t)(first + tid);
+    } else {
+      int64_t seen = 0;
+      for (int64_t b0 = 0; b0 < a.B && seen < first + COLS; b0 += threads) {
+        const int64_t b = b0 + tid;
+        const bool is = b < a.B && a.prefix_rows[b < a.B ? b : 0] == p;
+        const uint64_t mask = __ballot(is);
+        if (lane == 0) count[w] = __popcll(mask);
+        __syncthreads();
+        int64_t at = seen;
+        for (int y = 0; y < threads / 64; ++y) {
+          at += y < w ? count[y] : 0;
+          seen += count[y];
+        }
+        at += __popcll(mask & ((1ull << lane) - 1)) - first;
+        if (is && at >= 0 && at < COLS) members[at] = (int32_t)b;
+        __syncthreads();
+      }
+      found = (int)max((int64_t)0, min(seen - first, (int64_t)COLS));
+      if (found == 0) return false;
+    }
+    __syncthreads();
+    return true;
+  }
+  // Column c's query row (b * Tq + t) and head in the group; -1 past the prefix's rows.
+  __device__ __forceinline__ int64_t column(const PrefixArgs& a, int c, int& h) const {
+    const int64_t e = c0 + c - first * per;  // below COLS + per
+    const int mi = (int)((uint32_t)e / (uint32_t)per), r = (int)((uint32_t)e % (uint32_t)per);
+    h = r % GQ;
+    return mi < found ? (int64_t)member[mi] * a.Tq + r / GQ : -1;
+  }
+};
+
 __device__ __forceinline__ void dma16_far(uint32_t lds, const void* p) {  // a lane's own 64-bit address
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
 }
 
-// grid: (kv-head, prefix, piece) units in groups of 8, the column blocks of a unit 8 apart, so that
-// those which read the same keys share an XCD and its L2.
+// The wave groups' states into one partial a column. Every thread calls it, after a barrier.
+template <int D, int KG, int CG, typename Lds>
+__device__ __forceinline__ void store_partials(const PrefixArgs& a, Lds& sh, const PrefixBlock<32 * CG>& blk, int kg, int cg,
+                                               const f32x16_t (&o)[D / 32], float m_run, float l_run) {
+  const int tid = threadIdx.x, lane = tid & 63, hh = lane / 32, ln = lane % 32;
+  const float l = l_run + lane_xor(l_run, 32);
+  if (hh == 0) {
+    sh.m[kg][cg][ln] = m_run;
+    sh.l[kg][cg][ln] = l;
+  }
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d) {
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4)
+      *(float4*)&sh.o[kg][cg][ln][32 * d + 8 * r4 + 4 * hh] =
+          make_float4(o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]);
+  }
+  __syncthreads();
+  const int GQ = blk.GQ, pstride = GQ * (D + 2);
+  for (int y = tid; y < 32 * CG * (D / 4); y += 64 * KG * CG) {
+    const int c = y / (D / 4), d4 = y % (D / 4), oc = c / 32, cl = c % 32;
+    int h;
+    const int64_t row = blk.column(a, c, h);
+    if (row < 0) continue;
+    float mm = kNegBig;
+#pragma unroll
+    for (int z = 0; z < KG; ++z) mm = fmaxf(mm, sh.m[z][oc][cl]);
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float ll = 0.0f;
+#pragma unroll
+    for (int z = 0; z < KG; ++z) {
+      const float f = fast_exp2(sh.m[z][oc][cl] - mm);
+      const float4 v = *(const float4*)&sh.o[z][oc][cl][4 * d4];
+      acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+      ll += f * sh.l[z][oc][cl];
+    }
+    float* part = a.parts + ((row * a.Hkv + blk.g) * (a.splits + a.own_splits) + a.splits - blk.pc.count + blk.s) * (int64_t)pstride;
+    float* to = part + 2 * GQ + h * D + 4 * d4;  // 8-byte aligned
+    *(float2*)to = make_float2(acc.x, acc.y);
+    *(float2*)(to + 2) = make_float2(acc.z, acc.w);
+    if (d4 == 0) {
+      part[h] = mm;
+      part[GQ + h] = ll;
+    }
+  }
+}
+
 template <typename T, int D, int KG, int CG, bool PAGED>
 __global__ __launch_bounds__(64 * KG * CG) __attribute__((amdgpu_waves_per_eu(KG * CG / 4, KG * CG / 4)))
 void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
@@ -69,61 +180,14 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid / 64);
   const int kg = w % KG, cg = w / KG;
   const int hh = lane / 32, ln = lane % 32;
-  const int GQ = a.Hq / a.Hkv;
-  const int64_t clear = (int64_t)gridDim.x * THREADS;
-  for (int64_t i = (int64_t)blockIdx.x * THREADS + tid; i < a.B * a.Tq * a.Hkv; i += clear) a.counters[i] = 0;
-  const int64_t x = blockIdx.x;
-  const int cb = (int)(x / kXcds % n_cb);
-  int64_t u = x / kXcds / n_cb * kXcds + x % kXcds;
-  const int s = (int)(u % a.splits); u /= a.splits;
-  const int g = (int)(u % a.Hkv);
-  const int64_t pp = u / a.Hkv;
-  if (pp >= a.P) return;
-  const int p = (int)pp;
-  const Pieces pc = prefix_pieces(a, p);
-  if (s >= pc.count) return;
-
-  // the batch rows of this block's columns (column: batch row of the prefix, query row, head)
-  const int64_t per = a.Tq * GQ, c0 = (int64_t)cb * COLS;
-  const int64_t first = c0 / per;
-  int found;
-  if (a.prefix_rows == nullptr) {
-    if (first >= a.B) return;
-    found = (int)min(a.B - first, (int64_t)COLS);
-    if (tid < found) sh.member[tid] = (int32_t)(first + tid);
-  } else {
-    int64_t seen = 0;
-    for (int64_t b0 = 0; b0 < a.B && seen < first + COLS; b0 += THREADS) {
-      const int64_t b = b0 + tid;
-      const bool is = b < a.B && a.prefix_rows[b < a.B ? b : 0] == p;
-      const uint64_t mask = __ballot(is);
-      if (lane == 0) sh.count[w] = __popcll(mask);
-      __syncthreads();
-      int64_t at = seen;
-#pragma unroll
-      for (int y = 0; y < NW; ++y) {
-        at += y < w ? sh.count[y] : 0;
-        seen += sh.count[y];
-      }
-      at += __popcll(mask & ((1ull << lane) - 1)) - first;
-      if (is && at >= 0 && at < COLS) sh.member[at] = (int32_t)b;
-      __syncthreads();
-    }
-    found = (int)max((int64_t)0, min(seen - first, (int64_t)COLS));
-    if (found == 0) return;
-  }
-  __syncthreads();
-  // column c of the block: its query row (b * Tq + t) and head in the group, or row -1
-  auto column = [&](int c, int& h) -> int64_t {
-    const int64_t e = c0 + c - first * per;  // 32-bit: below COLS + per
-    const int mi = (int)((uint32_t)e / (uint32_t)per), r = (int)((uint32_t)e % (uint32_t)per);
-    h = r % GQ;
-    return mi < found ? (int64_t)sh.member[mi] * a.Tq + r / GQ : -1;
-  };
+  PrefixBlock<COLS> blk;
+  if (!blk.init(a, n_cb, THREADS, sh.member, sh.count)) return;
+  const int GQ = blk.GQ, g = blk.g, p = blk.p, s = blk.s;
+  const Pieces pc = blk.pc;
   op_t qop[KS];
   {
     int h;
-    int64_t row = column(cg * 32 + ln, h);
+    int64_t row = blk.column(a, cg * 32 + ln, h);
     if (row < 0) row = (int64_t)sh.member[0] * a.Tq, h = 0;
     const T* src = (const T*)a.q + (row * a.Hq + (int64_t)g * GQ + h) * D + 8 * hh;
 #pragma unroll
@@ -290,49 +354,311 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // nothing lands after this
   __syncthreads();
 
-  // the groups' states into one partial a column
+  store_partials<D, KG, CG>(a, sh, blk, kg, cg, o, m_run, l_run);
+}
+
+// ---------------------------------------------------------------- 256 columns
+//
+// Eight waves of 32 columns share 64-key tiles, four buffers each of K and V. A wave's step is two
+// phases: M, the last tile's P V products and this tile's scores (matrix cores, LDS reads, and the loads
+// ahead between the matrix operations, where their issue costs least), and V, this tile's weights (vector
+// unit). Two groups of four waves, one of each on every SIMD, run half a step apart (a barrier after each
+// phase), so one's matrix work runs beside the other's vector work.
+//
+// What a load straight to LDS costs a CU is about 39 cycles a KB wherever it stands (measured: eight of a
+// wave, four waves at once, 1240 cycles), which is why the many-column form shares a tile between all
+// waves: 32 KB a step of 2048 cycles of matrix work, where two groups on tiles of their own would load
+// 64 KB.
+//
+// M(i) loads K(i + 3) over K(i - 1) and V(i + 2) over V(i - 2), both read for the last time a phase of
+// either group before. K(i) is read in M(i), V(i) from the end of V(i) on: both were loaded in M(i - 2) or
+// earlier, and at the end of V(i - 1) only the loads of M(i - 1) may be outstanding.
+constexpr int kWideBuf = 4;
+
+template <int D>
+struct alignas(1024) WideLds {
+  union {
+    struct {
+      uint16_t k[kWideBuf][64 * D];  // 16-byte segments of a row permuted by kseg
+      uint16_t v[kWideBuf][64 * D];  // by vseg
+    };
+    float o[1][8][32][D + 4];
+  };
+  float m[1][8][32], l[1][8][32];
+  int32_t ids[8][8][64];  // paged: cache rows of eight tiles, a wave's own
+  int32_t member[256];
+  int count[8];
+};
+
+template <typename T, int D, bool PAGED>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void prefix_wide_kernel(PrefixArgs a, int n_cb) {
+  using M = Mfma<T>;
+  using op_t = typename M::op_t;
+  constexpr int KG = 1, CG = 8, KT = 64, COLS = 256, THREADS = 512, NB = kWideBuf;
+  constexpr int KS = D / 16, DB = D / 32, SEGS = D / 8, ROWB = 2 * D;
+  constexpr int KPI = 1024 / ROWB, NI = KT / KPI / CG;
+  constexpr int PER = 2 * NI + (PAGED ? 1 : 0);  // loads of a step
+  constexpr int NG = 4 + KS / 2;                 // groups of matrix operations of an M: 4 of P V, the scores
+  constexpr bool HALF = !__is_same(T, bf16_t);
+  constexpr float BIAS = HALF ? 12.0f : 0.0f, TOP = HALF ? 15.0f : 8.0f;
+  typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+  __shared__ WideLds<D> sh;
+
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid / 64);
+  const int hh = lane / 32, ln = lane % 32;
+  PrefixBlock<COLS> blk;
+  if (!blk.init(a, n_cb, THREADS, sh.member, sh.count)) return;
+  op_t qop[KS];
   {
-    const float l = l_run + lane_xor(l_run, 32);
-    if (hh == 0) {
-      sh.m[kg][cg][ln] = m_run;
-      sh.l[kg][cg][ln] = l;
-    }
-#pragma unroll
-    for (int d = 0; d < DB; ++d) {
-#pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4)
-        *(float4*)&sh.o[kg][cg][ln][32 * d + 8 * r4 + 4 * hh] =
-            make_float4(o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]);
-    }
-  }
-  __syncthreads();
-  const int pstride = GQ * (D + 2);
-  for (int y = tid; y < COLS * (D / 4); y += THREADS) {
-    const int c = y / (D / 4), d4 = y % (D / 4), oc = c / 32, cl = c % 32;
     int h;
-    const int64_t row = column(c, h);
-    if (row < 0) continue;
-    float mm = kNegBig;
+    int64_t row = blk.column(a, w * 32 + ln, h);
+    if (row < 0) row = (int64_t)sh.member[0] * a.Tq, h = 0;
+    const T* src = (const T*)a.q + (row * a.Hq + (int64_t)blk.g * blk.GQ + h) * D + 8 * hh;
 #pragma unroll
-    for (int z = 0; z < KG; ++z) mm = fmaxf(mm, sh.m[z][oc][cl]);
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float ll = 0.0f;
+    for (int y = 0; y < KS; ++y) qop[y] = __builtin_bit_cast(op_t, *(const uint4*)(src + 16 * y));
+  }
 #pragma unroll
-    for (int z = 0; z < KG; ++z) {
-      const float f = fast_exp2(sh.m[z][oc][cl] - mm);
-      const float4 v = *(const float4*)&sh.o[z][oc][cl][4 * d4];
-      acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
-      ll += f * sh.l[z][oc][cl];
+  for (int y = 0; y < KS; ++y) asm volatile("" ::"v"(qop[y]));  // here: below, waits are counted by hand
+
+  const int k0 = blk.s * blk.pc.keys, n_keys = min(blk.pc.keys, blk.pc.n - k0);
+  const int n_tiles = (n_keys + KT - 1) / KT;
+  const int64_t head = (PAGED ? 0 : blk.p * a.p_sb) + blk.g * a.p_sh;
+  const T* kb = (const T*)a.kp + head;
+  const T* vb = (const T*)a.vp + head;
+  const int32_t* slots = PAGED ? a.slots + blk.p * a.slot_stride + k0 : nullptr;
+  const uint32_t k_lds = (uint32_t)(uintptr_t)(lds_char*)&sh.k[0][0];
+  const uint32_t v_lds = (uint32_t)(uintptr_t)(lds_char*)&sh.v[0][0];
+  const uint32_t i_lds = (uint32_t)(uintptr_t)(lds_char*)&sh.ids[w][0][0];
+  const int64_t st = a.p_st * 2;  // bytes
+  const float scale = a.scale_log2;
+  typedef __attribute__((address_space(3))) const int32_t lds_int;
+
+  // past the last tile: that one again, loaded and not used
+  auto tile_of = [&](int i) { return min(i, n_tiles - 1); };
+  auto keys_of = [&](int t) { return min(KT, n_keys - t * KT); };
+  auto load_ids = [&](int i) {
+    dma4(i_lds + (uint32_t)(i & 7) * 256u, slots, 4u * (uint32_t)min(tile_of(i) * KT + lane, n_keys - 1));
+  };
+  // Move y of this wave's eighth of tile i's K or V rows. A lane's offset within the rows of one move is the
+  // same for every move but for two bits of K's segment.
+  const uint32_t lrow = (uint32_t)(lane / SEGS) * (uint32_t)st;
+  const uint32_t kseg0 = (uint32_t)(((lane % SEGS) ^ kseg<D>(lane / SEGS)) * 16);
+  const uint32_t vseg0 = (uint32_t)(((lane % SEGS) ^ vseg<D>(lane / SEGS)) * 16);
+  auto load = [&](bool values, int i, int y) {
+    static_assert(KPI == 512 / D && (D == 64 || D == 128), "K's segments differ from move to move by 64 bytes times this");
+    const int t = tile_of(i), n = keys_of(t), part = w * NI + y;
+    const char* src = (const char*)(values ? vb : kb);
+    const uint32_t dst = (values ? v_lds : k_lds) + (uint32_t)(i & (NB - 1)) * (KT * ROWB) + (uint32_t)part * 1024u;
+    const uint32_t seg = values ? vseg0 : kseg0 ^ (uint32_t)(part % (D == 128 ? 4 : 2) * 64);
+    if constexpr (PAGED) {
+      const int32_t id = *(lds_int*)((const lds_char*)&sh.ids[w][i & 7][0] + 4 * (part * KPI + lane / SEGS));
+      dma16_far(dst, src + (int64_t)(id >= 0 && id < a.pool ? id : 0) * st + seg);
+    } else {
+      const int64_t row0 = (int64_t)(k0 + t * KT) * st;
+      if (n == KT) {  // uniform
+        dma16(dst, src + row0 + (int64_t)(part * KPI) * st, lrow + seg);
+      } else {  // rows past the last read the last
+        dma16(dst, src + row0, (uint32_t)min(part * KPI + lane / SEGS, n - 1) * (uint32_t)st + seg);
+      }
     }
-    float* part = a.parts + ((row * a.Hkv + g) * (a.splits + a.own_splits) + a.splits - pc.count + s) * (int64_t)pstride;
-    float* to = part + 2 * GQ + h * D + 4 * d4;  // 8-byte aligned
-    *(float2*)to = make_float2(acc.x, acc.y);
-    *(float2*)(to + 2) = make_float2(acc.z, acc.w);
-    if (d4 == 0) {
-      part[h] = mm;
-      part[GQ + h] = ll;
+  };
+  // which keys of tile i count
+  auto live_of = [&](int i) -> uint64_t {
+    const int n = keys_of(tile_of(i));
+    if constexpr (PAGED) {
+      const int32_t id = *(lds_int*)((const lds_char*)&sh.ids[w][i & 7][0] + 4 * lane);
+      return __ballot(id >= 0 && id < a.pool && lane < n);
+    }
+    return ~0ull >> (64 - n);
+  };
+  // V rows of tile i that do not count become zeros, whatever their place in memory holds: this
+  // wave's own eighth, landed.
+  auto blank = [&](int i) {
+    const uint64_t ok = live_of(i);
+    if (ok == ~0ull) return;  // uniform
+    for (int y = lane; y < KT / CG * SEGS; y += 64) {
+      const int r = w * (KT / CG) + y / SEGS;
+      if (!(ok >> r & 1u))
+        *(uint4*)((char*)&sh.v[i & (NB - 1)][0] + r * ROWB + 16 * (y % SEGS)) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  };
+
+  f32x16_t o[DB], sc[2];
+  uint32_t ph[2][8];  // a tile's weights, two a word
+  float m_run = kNegBig, l_run = 0.0f;
+#pragma unroll
+  for (int d = 0; d < DB; ++d) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+  }
+  const int jj = (lane % 16) / 4;
+  const uint32_t kbase = (uint32_t)(ln * ROWB) + (uint32_t)((hh ^ kseg<D>(ln)) * 16);
+  const uint32_t vbase = (uint32_t)((4 * hh + jj) * ROWB + 32 * (ln / 16) + 8 * (lane % 4));
+  // Groups of matrix operations with their LDS operands, read while the two groups before compute:
+  // 0 .. 3 are O^T += V^T P^T of 16 keys each, 4 .. the scores at two 16-dim steps each.
+  op_t op[3][4];
+  auto load_group = [&](int gi, int tile_v, int tile_k) {
+    if (gi < 4) {
+      const lds_char* vt = (const lds_char*)&sh.v[tile_v & (NB - 1)][0] + vbase;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const lds_char* vd = vt + (uint32_t)(64 * (D == 128 ? (d ^ jj) : (d ^ (jj >> 1))));
+        const uint2 lo = v_column4(vd, 16 * gi * ROWB), hi = v_column4(vd, (16 * gi + 8) * ROWB);
+        op[gi % 3][d] = __builtin_bit_cast(op_t, make_uint4(lo.x, lo.y, hi.x, hi.y));
+      }
+    } else if (gi < NG) {
+      typedef __attribute__((address_space(3))) const op_t lds_op;
+      const lds_char* kt = (const lds_char*)&sh.k[tile_k & (NB - 1)][0];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        op[gi % 3][e] = *(lds_op*)(kt + (kbase ^ (uint32_t)(32 * (2 * (gi - 4) + e / 2))) + (e % 2) * 32 * ROWB);
+    }
+  };
+  auto run_group = [&](int gi) {
+    if (gi < 4) {
+      const uint32_t* x = &ph[gi / 2][4 * (gi % 2)];
+      const op_t pb = __builtin_bit_cast(op_t, make_uint4(x[0], x[1], x[2], x[3]));
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[d] = M::run(op[gi % 3][d], pb, o[d]);
+    } else {
+      f32x16_t none;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) none[r] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        sc[e % 2] = M::run(op[gi % 3][e], qop[2 * (gi - 4) + e / 2], gi == 4 && e < 2 ? none : sc[e % 2]);
+    }
+  };
+  // Groups g0 .. g1 - 1, the first two's operands loaded; hook(x) between them: loads ahead.
+  auto run_groups = [&](int g0, int g1, int tile_v, int tile_k, auto&& hook) {
+#pragma unroll
+    for (int gi = g0; gi < g1; ++gi) {
+      load_group(gi + 2, tile_v, tile_k);
+      hook(gi - g0);
+      __builtin_amdgcn_sched_barrier(0);
+      run_group(gi);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // p = exp2(s scale - m) against the reference as it is, eight at a time (one wave a SIMD makes weights:
+  // a chain of dependent instructions would leave the unit idle), and their sum. top: fp16, the largest
+  // of the packed halves as bits.
+  u16x2_t top;
+  auto weights = [&](float (&ls)[2]) {
+    ls[0] = ls[1] = 0.0f;
+    top = {0, 0};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int r0 = 0; r0 < 16; r0 += 8) {
+        float x[8];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = fmaf(sc[h][r0 + e], scale, -m_run);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = fast_exp2(x[e]);
+        __builtin_amdgcn_sched_barrier(0);
+        uint32_t* pair = &ph[h][r0 / 2];
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) pair[e / 2] = M::pack2(x[e], x[e + 1]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ls[e & 1] += x[e];
+        if constexpr (HALF) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, pair[e]));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+  // The reference moves lazily: weights are made against it as it is, and only where one may have
+  // reached 2^TOP (bf16: a lane's 32 together) are the column maxima taken, the state rescaled and
+  // the weights made again. Most tiles take no maximum.
+  auto softmax = [&](uint64_t ok) {
+    if (ok != ~0ull) {  // uniform: a tile with keys that do not count
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t wd = (uint32_t)(ok >> (32 * h)) >> (4 * hh);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[h][r] = wd >> (8 * (r / 4) + r % 4) & 1u ? sc[h][r] : -INFINITY;
+      }
+    }
+    float ls[2];
+    weights(ls);
+    static_assert(TOP == (HALF ? 15.0f : 8.0f), "the test is against 2^TOP");
+    const bool over = HALF ? max(top.x, top.y) >= 0x7800 : !(ls[0] + ls[1] < 256.0f);
+    if (__builtin_expect(__any(over), 0)) {
+      float mx = sc[0][0];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[h][r]);
+      }
+      const float mt = fmaxf(mx, lane_xor(mx, 32)) * scale;
+      const bool moves = mt > m_run + TOP;
+      if (__any(moves)) {
+        const float mn = moves ? mt - BIAS : m_run;
+        const float alpha = fast_exp2(m_run - mn);
+        m_run = mn;
+        l_run *= alpha;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+        }
+        weights(ls);
+      }
+    }
+    l_run += ls[0] + ls[1];
+  };
+
+  if constexpr (PAGED) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) load_ids(i);
+    wait_vm<0>();
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+#pragma unroll
+    for (int y = 0; y < NI; ++y) {
+      load(false, i, y);
+      if (i < 2) load(true, i, y);
     }
   }
+  wait_vm<0>();
+  blank(0);
+#pragma unroll
+  for (int y = 0; y < NI; ++y) load(false, 3, y);  // M(0)'s
+  phase_barrier();
+  const bool late = w >= 4;
+  if (late) phase_barrier();
+  load_group(4, 0, 0);
+  load_group(5, 0, 0);
+  for (int i = 0;;) {
+    run_groups(4, NG, i, i, [&](int x) {
+      if (x < NI) load(true, i + 2, x);
+      if (PAGED && x == NG - 5) load_ids(i + 6);
+    });
+    wait_vm<2 * PER>();
+    phase_barrier();
+    softmax(live_of(i));
+    __builtin_amdgcn_sched_barrier(0);
+    load_group(0, i, i);
+    load_group(1, i, i);
+    wait_vm<PER>();
+    blank(i + 1);
+    phase_barrier();
+    run_groups(0, 4, i, i + 1, [&](int x) {
+      if (x < NI) load(false, i + 4, x);
+    });
+    if (++i == n_tiles) break;
+  }
+  if (!late) phase_barrier();
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // nothing lands after this
+  __syncthreads();
+  store_partials<D, KG, CG>(a, sh, blk, 0, w, o, m_run, l_run);
 }
 
 int64_t prefix_units(const PrefixArgs& a) { return ((int64_t)a.P * a.Hkv * a.splits + kXcds - 1) / kXcds * kXcds; }
@@ -356,7 +682,12 @@ void launch_mfma_cols(const PrefixArgs& a, int64_t columns, hipStream_t s) {
   const int n_cb = (int)column_blocks(a, columns);
   if (wg == 32) launch_mfma<T, D, 4, 1>(a, n_cb, s);
   else if (wg == 64) launch_mfma<T, D, 4, 2>(a, n_cb, s);
-  else launch_mfma<T, D, 2, 4>(a, n_cb, s);
+  else if (wg == 128) launch_mfma<T, D, 2, 4>(a, n_cb, s);
+  else {
+    const dim3 grid((unsigned)(prefix_units(a) * n_cb));
+    if (a.slots) prefix_wide_kernel<T, D, true><<<grid, 512, 0, s>>>(a, n_cb);
+    else prefix_wide_kernel<T, D, false><<<grid, 512, 0, s>>>(a, n_cb);
+  }
 }
 
 }  // namespace
@@ -365,11 +696,11 @@ namespace lsa {
 
 bool prefix_mfma_ok(int dtype, int D) { return dtype != LSA_F32 && (D == 64 || D == 128); }
 
-int64_t prefix_mfma_columns(int64_t columns) { return columns <= 32 ? 32 : (columns <= 64 ? 64 : 128); }
+int64_t prefix_mfma_columns(int64_t columns) { return columns <= 32 ? 32 : (columns <= 64 ? 64 : (columns <= 128 ? 128 : 256)); }
 
 bool launch_prefix_mfma(const PrefixArgs& a, int dtype, int D, int64_t columns, hipStream_t s) {
-  // a lane's offset within a tile is 32 bits of bytes
-  if (!prefix_mfma_ok(dtype, D) || a.p_st >= (int64_t)1 << 25 || prefix_units(a) * column_blocks(a, columns) > 0x7FFFFFFF)
+  // a lane's offset within a tile is 32 bits of bytes; a column's largest score is its largest dot product
+  if (!prefix_mfma_ok(dtype, D) || !(a.scale_log2 > 0.0f && a.scale_log2 < INFINITY) || a.p_st >= (int64_t)1 << 25 || prefix_units(a) * column_blocks(a, columns) > 0x7FFFFFFF)
     return false;
   if (dtype == LSA_BF16) {
     if (D == 64) launch_mfma_cols<bf16_t, 64>(a, columns, s);
