@@ -360,19 +360,20 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
 // ---------------------------------------------------------------- 256 columns
 //
 // Eight waves of 32 columns share 64-key tiles, four buffers each of K and V. A wave's step is two
-// phases: M, the last tile's P V products and this tile's scores (matrix cores, LDS reads, and the loads
-// ahead between the matrix operations, where their issue costs least), and V, this tile's weights (vector
-// unit). Two groups of four waves, one of each on every SIMD, run half a step apart (a barrier after each
-// phase), so one's matrix work runs beside the other's vector work.
+// phases: M, the last tile's P V products and this tile's scores (matrix cores and LDS reads), and V, the
+// loads ahead and this tile's weights (vector unit). Two groups of four waves, one of each on every SIMD, run
+// half a step apart (a barrier after each phase), so one's matrix work runs beside the other's vector work.
 //
-// What a load straight to LDS costs a CU is about 39 cycles a KB wherever it stands (measured: eight of a
-// wave, four waves at once, 1240 cycles), which is why the many-column form shares a tile between all
-// waves: 32 KB a step of 2048 cycles of matrix work, where two groups on tiles of their own would load
-// 64 KB.
+// A load straight to LDS holds its wave for about 155 cycles (four waves at once: 39 cycles a KB of the CU).
+// In M, between the matrix operations, four of them cost 500 cycles, in V they fill time that V has left
+// (131072 keys, 512 columns of 128 on 8 kv-heads: a step of 4850 cycles with them in M, 3720 in V; under load the clock falls as the
+// cycles do, and both take 310 us). That is also why the
+// many-column form shares a tile between all waves: 32 KB a step of 2048 cycles of matrix work, where two
+// groups on tiles of their own load 64 KB (350 us).
 //
-// M(i) loads K(i + 3) over K(i - 1) and V(i + 2) over V(i - 2), both read for the last time a phase of
-// either group before. K(i) is read in M(i), V(i) from the end of V(i) on: both were loaded in M(i - 2) or
-// earlier, and at the end of V(i - 1) only the loads of M(i - 1) may be outstanding.
+// V(i) loads K(i + 3) over K(i - 1) and V(i + 2) over V(i - 2), both read for the last time in M(i - 1) of
+// either group. K(i) is read in M(i), V(i) from the end of V(i) on: both were loaded in V(i - 2) or
+// earlier, and at the end of V(i - 1) only the loads of that phase may be outstanding.
 constexpr int kWideBuf = 4;
 
 template <int D>
@@ -531,12 +532,10 @@ void prefix_wide_kernel(PrefixArgs a, int n_cb) {
         sc[e % 2] = M::run(op[gi % 3][e], qop[2 * (gi - 4) + e / 2], gi == 4 && e < 2 ? none : sc[e % 2]);
     }
   };
-  // Groups g0 .. g1 - 1, the first two's operands loaded; hook(x) between them: loads ahead.
-  auto run_groups = [&](int g0, int g1, int tile_v, int tile_k, auto&& hook) {
+  auto run_groups = [&](int g0, int g1, int tile_v, int tile_k) {  // g0 .. g1 - 1, the first two's operands loaded
 #pragma unroll
     for (int gi = g0; gi < g1; ++gi) {
       load_group(gi + 2, tile_v, tile_k);
-      hook(gi - g0);
       __builtin_amdgcn_sched_barrier(0);
       run_group(gi);
       __builtin_amdgcn_sched_barrier(0);
@@ -629,20 +628,20 @@ void prefix_wide_kernel(PrefixArgs a, int n_cb) {
   }
   wait_vm<0>();
   blank(0);
-#pragma unroll
-  for (int y = 0; y < NI; ++y) load(false, 3, y);  // M(0)'s
   phase_barrier();
   const bool late = w >= 4;
   if (late) phase_barrier();
   load_group(4, 0, 0);
   load_group(5, 0, 0);
   for (int i = 0;;) {
-    run_groups(4, NG, i, i, [&](int x) {
-      if (x < NI) load(true, i + 2, x);
-      if (PAGED && x == NG - 5) load_ids(i + 6);
-    });
-    wait_vm<2 * PER>();
+    run_groups(4, NG, i, i);
     phase_barrier();
+#pragma unroll
+    for (int y = 0; y < NI; ++y) {
+      load(false, i + 3, y);
+      load(true, i + 2, y);
+    }
+    if constexpr (PAGED) load_ids(i + 6);
     softmax(live_of(i));
     __builtin_amdgcn_sched_barrier(0);
     load_group(0, i, i);
@@ -650,9 +649,7 @@ void prefix_wide_kernel(PrefixArgs a, int n_cb) {
     wait_vm<PER>();
     blank(i + 1);
     phase_barrier();
-    run_groups(0, 4, i, i + 1, [&](int x) {
-      if (x < NI) load(false, i + 4, x);
-    });
+    run_groups(0, 4, i, i + 1);
     if (++i == n_tiles) break;
   }
   if (!late) phase_barrier();
