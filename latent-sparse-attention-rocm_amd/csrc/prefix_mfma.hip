@@ -29,6 +29,80 @@ namespace {
 
 constexpr int kXcds = 8;
 
+// A workgroup's place: kv-head, prefix, piece, and the batch rows whose query rows times heads are
+// its columns (column: batch row of the prefix, query row, head). The grid's (kv-head, prefix, piece)
+// units come in groups of 8, the column blocks of a unit 8 apart, so that those which read the same
+// keys share an XCD and its L2.
+template <int COLS>
+struct PrefixBlock {
+  struct Lds {
+    int32_t member[COLS];  // the batch rows
+    int32_t row[COLS];     // a column's query row (b * Tq + t), -1 past the prefix's rows
+    int32_t head[COLS];    // and head in the group
+    int count[16];
+  };
+  int GQ, g, p, s;
+  Pieces pc;
+
+  // False: nothing to do (the whole workgroup). Clears the grid's share of the counters.
+  __device__ __forceinline__ bool init(const PrefixArgs& a, uint32_t n_cb, int threads, Lds& sh) {
+    const int tid = threadIdx.x, lane = tid & 63, w = tid / 64;
+    GQ = a.Hq / a.Hkv;
+    const int64_t clear = (int64_t)gridDim.x * threads;
+    for (int64_t i = (int64_t)blockIdx.x * threads + tid; i < a.B * a.Tq * a.Hkv; i += clear) a.counters[i] = 0;
+    const uint32_t x = blockIdx.x, x8 = x / kXcds, cb = x8 % n_cb;
+    uint32_t u = x8 / n_cb * kXcds + x % kXcds;
+    s = (int)(u % (uint32_t)a.splits); u /= (uint32_t)a.splits;
+    g = (int)(u % (uint32_t)a.Hkv); u /= (uint32_t)a.Hkv;
+    if (u >= (uint32_t)a.P) return false;
+    p = (int)u;
+    pc = prefix_pieces(a, p);
+    if (s >= pc.count) return false;
+    // columns and rows are fewer than 2^31
+    const uint32_t per = (uint32_t)a.Tq * (uint32_t)GQ, c0 = cb * COLS, first = c0 / per;
+    int found;
+    if (a.prefix_rows == nullptr) {
+      if (first >= a.B) return false;
+      found = (int)min(a.B - first, (int64_t)COLS);
+      if (tid < found) sh.member[tid] = (int32_t)first + tid;
+    } else {
+      int64_t seen = 0;
+      for (int64_t b0 = 0; b0 < a.B && seen < (int64_t)first + COLS; b0 += threads) {
+        const int64_t b = b0 + tid;
+        const bool is = b < a.B && a.prefix_rows[b < a.B ? b : 0] == p;
+        const uint64_t mask = __ballot(is);
+        if (lane == 0) sh.count[w] = __popcll(mask);
+        __syncthreads();
+        int64_t at = seen;
+        for (int y = 0; y < threads / 64; ++y) {
+          at += y < w ? sh.count[y] : 0;
+          seen += sh.count[y];
+        }
+        at += __popcll(mask & ((1ull << lane) - 1)) - (int64_t)first;
+        if (is && at >= 0 && at < COLS) sh.member[at] = (int32_t)b;
+        __syncthreads();
+      }
+      found = (int)max((int64_t)0, min(seen - (int64_t)first, (int64_t)COLS));
+      if (found == 0) return false;
+    }
+    __syncthreads();
+    if (tid < COLS) {
+      const uint32_t e = c0 + tid - first * per, r = e % per;
+      const int mi = (int)(e / per);
+      sh.row[tid] = mi < found ? sh.member[mi] * (int32_t)a.Tq + (int32_t)(r / (uint32_t)GQ) : -1;
+      sh.head[tid] = (int)(r % (uint32_t)GQ);
+    }
+    __syncthreads();
+    return true;
+  }
+  // Column c's query row in q; past the prefix's rows the first column's.
+  template <typename T, int D>
+  __device__ __forceinline__ const T* query(const PrefixArgs& a, const Lds& sh, int c) const {
+    const int e = sh.row[c] < 0 ? 0 : c;
+    return (const T*)a.q + ((int64_t)sh.row[e] * a.Hq + (int64_t)g * GQ + sh.head[e]) * D;
+  }
+};
+
 template <int KG> constexpr int tile_keys() { return 128 / KG; }
 
 template <int D, int KG, int CG>
@@ -42,74 +116,7 @@ struct alignas(1024) PrefixLds {
   };
   float m[KG][CG][32], l[KG][CG][32];
   int32_t ids[KG][CG][4][64];    // paged: cache rows of the tiles ahead, a wave's own
-  int32_t member[32 * CG];       // batch rows whose columns these are
-  int count[KG * CG];
-};
-
-// A workgroup's place: kv-head, prefix, piece, and the batch rows whose query rows times heads are
-// its columns (column: batch row of the prefix, query row, head). The grid's (kv-head, prefix, piece)
-// units come in groups of 8, the column blocks of a unit 8 apart, so that those which read the same
-// keys share an XCD and its L2.
-template <int COLS>
-struct PrefixBlock {
-  int GQ, g, p, s, found;
-  int64_t per, c0, first;
-  Pieces pc;
-  const int32_t* member;
-
-  // False: nothing to do (the whole workgroup). Clears the grid's share of the counters.
-  __device__ __forceinline__ bool init(const PrefixArgs& a, int n_cb, int threads, int32_t* members, int* count) {
-    const int tid = threadIdx.x, lane = tid & 63, w = tid / 64;
-    member = members;
-    GQ = a.Hq / a.Hkv;
-    const int64_t clear = (int64_t)gridDim.x * threads;
-    for (int64_t i = (int64_t)blockIdx.x * threads + tid; i < a.B * a.Tq * a.Hkv; i += clear) a.counters[i] = 0;
-    const int64_t x = blockIdx.x;
-    const int cb = (int)(x / kXcds % n_cb);
-    int64_t u = x / kXcds / n_cb * kXcds + x % kXcds;
-    s = (int)(u % a.splits); u /= a.splits;
-    g = (int)(u % a.Hkv); u /= a.Hkv;
-    if (u >= a.P) return false;
-    p = (int)u;
-    pc = prefix_pieces(a, p);
-    if (s >= pc.count) return false;
-    per = a.Tq * GQ;
-    c0 = (int64_t)cb * COLS;
-    first = c0 / per;
-    if (a.prefix_rows == nullptr) {
-      if (first >= a.B) return false;
-      found = (int)min(a.B - first, (int64_t)COLS);
-      if (tid < found) members[tid] = (int32_t)(first + tid);
-    } else {
-      int64_t seen = 0;
-      for (int64_t b0 = 0; b0 < a.B && seen < first + COLS; b0 += threads) {
-        const int64_t b = b0 + tid;
-        const bool is = b < a.B && a.prefix_rows[b < a.B ? b : 0] == p;
-        const uint64_t mask = __ballot(is);
-        if (lane == 0) count[w] = __popcll(mask);
-        __syncthreads();
-        int64_t at = seen;
-        for (int y = 0; y < threads / 64; ++y) {
-          at += y < w ? count[y] : 0;
-          seen += count[y];
-        }
-        at += __popcll(mask & ((1ull << lane) - 1)) - first;
-        if (is && at >= 0 && at < COLS) members[at] = (int32_t)b;
-        __syncthreads();
-      }
-      found = (int)max((int64_t)0, min(seen - first, (int64_t)COLS));
-      if (found == 0) return false;
-    }
-    __syncthreads();
-    return true;
-  }
-  // Column c's query row (b * Tq + t) and head in the group; -1 past the prefix's rows.
-  __device__ __forceinline__ int64_t column(const PrefixArgs& a, int c, int& h) const {
-    const int64_t e = c0 + c - first * per;  // below COLS + per
-    const int mi = (int)((uint32_t)e / (uint32_t)per), r = (int)((uint32_t)e % (uint32_t)per);
-    h = r % GQ;
-    return mi < found ? (int64_t)member[mi] * a.Tq + r / GQ : -1;
-  }
+  typename PrefixBlock<32 * CG>::Lds block;
 };
 
 __device__ __forceinline__ void dma16_far(uint32_t lds, const void* p) {  // a lane's own 64-bit address
@@ -137,8 +144,8 @@ __device__ __forceinline__ void store_partials(const PrefixArgs& a, Lds& sh, con
   const int GQ = blk.GQ, pstride = GQ * (D + 2);
   for (int y = tid; y < 32 * CG * (D / 4); y += 64 * KG * CG) {
     const int c = y / (D / 4), d4 = y % (D / 4), oc = c / 32, cl = c % 32;
-    int h;
-    const int64_t row = blk.column(a, c, h);
+    const int h = sh.block.head[c];
+    const int64_t row = sh.block.row[c];
     if (row < 0) continue;
     float mm = kNegBig;
 #pragma unroll
@@ -181,15 +188,12 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
   const int kg = w % KG, cg = w / KG;
   const int hh = lane / 32, ln = lane % 32;
   PrefixBlock<COLS> blk;
-  if (!blk.init(a, n_cb, THREADS, sh.member, sh.count)) return;
-  const int GQ = blk.GQ, g = blk.g, p = blk.p, s = blk.s;
+  if (!blk.init(a, (uint32_t)n_cb, THREADS, sh.block)) return;
+  const int g = blk.g, p = blk.p, s = blk.s;
   const Pieces pc = blk.pc;
   op_t qop[KS];
   {
-    int h;
-    int64_t row = blk.column(a, cg * 32 + ln, h);
-    if (row < 0) row = (int64_t)sh.member[0] * a.Tq, h = 0;
-    const T* src = (const T*)a.q + (row * a.Hq + (int64_t)g * GQ + h) * D + 8 * hh;
+    const T* src = blk.template query<T, D>(a, sh.block, cg * 32 + ln) + 8 * hh;
 #pragma unroll
     for (int y = 0; y < KS; ++y) qop[y] = __builtin_bit_cast(op_t, *(const uint4*)(src + 16 * y));
   }
@@ -387,8 +391,7 @@ struct alignas(1024) WideLds {
   };
   float m[1][8][32], l[1][8][32];
   int32_t ids[8][8][64];  // paged: cache rows of eight tiles, a wave's own
-  int32_t member[256];
-  int count[8];
+  typename PrefixBlock<256>::Lds block;
 };
 
 template <typename T, int D, bool PAGED>
@@ -409,13 +412,10 @@ void prefix_wide_kernel(PrefixArgs a, int n_cb) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid / 64);
   const int hh = lane / 32, ln = lane % 32;
   PrefixBlock<COLS> blk;
-  if (!blk.init(a, n_cb, THREADS, sh.member, sh.count)) return;
+  if (!blk.init(a, (uint32_t)n_cb, THREADS, sh.block)) return;
   op_t qop[KS];
   {
-    int h;
-    int64_t row = blk.column(a, w * 32 + ln, h);
-    if (row < 0) row = (int64_t)sh.member[0] * a.Tq, h = 0;
-    const T* src = (const T*)a.q + (row * a.Hq + (int64_t)blk.g * blk.GQ + h) * D + 8 * hh;
+    const T* src = blk.template query<T, D>(a, sh.block, w * 32 + ln) + 8 * hh;
 #pragma unroll
     for (int y = 0; y < KS; ++y) qop[y] = __builtin_bit_cast(op_t, *(const uint4*)(src + 16 * y));
   }
