@@ -44,20 +44,27 @@ struct PrefixBlock {
   int GQ, g, p, s;
   Pieces pc;
 
+  uint32_t cb;
+
   // False: nothing to do (the whole workgroup). Clears the grid's share of the counters.
-  __device__ __forceinline__ bool init(const PrefixArgs& a, uint32_t n_cb, int threads, Lds& sh) {
-    const int tid = threadIdx.x, lane = tid & 63, w = tid / 64;
+  __device__ __forceinline__ bool place(const PrefixArgs& a, uint32_t n_cb, int threads) {
+    const int tid = threadIdx.x;
     GQ = a.Hq / a.Hkv;
     const int64_t clear = (int64_t)gridDim.x * threads;
     for (int64_t i = (int64_t)blockIdx.x * threads + tid; i < a.B * a.Tq * a.Hkv; i += clear) a.counters[i] = 0;
-    const uint32_t x = blockIdx.x, x8 = x / kXcds, cb = x8 % n_cb;
+    const uint32_t x = blockIdx.x, x8 = x / kXcds;
+    cb = x8 % n_cb;
     uint32_t u = x8 / n_cb * kXcds + x % kXcds;
     s = (int)(u % (uint32_t)a.splits); u /= (uint32_t)a.splits;
     g = (int)(u % (uint32_t)a.Hkv); u /= (uint32_t)a.Hkv;
     if (u >= (uint32_t)a.P) return false;
     p = (int)u;
     pc = prefix_pieces(a, p);
-    if (s >= pc.count) return false;
+    return s < pc.count;
+  }
+  // The columns; false: none. Contains barriers.
+  __device__ __forceinline__ bool columns(const PrefixArgs& a, int threads, Lds& sh) const {
+    const int tid = threadIdx.x, lane = tid & 63, w = tid / 64;
     // columns and rows are fewer than 2^31
     const uint32_t per = (uint32_t)a.Tq * (uint32_t)GQ, c0 = cb * COLS, first = c0 / per;
     int found;
@@ -142,8 +149,11 @@ __device__ __forceinline__ void store_partials(const PrefixArgs& a, Lds& sh, con
   }
   __syncthreads();
   const int GQ = blk.GQ, pstride = GQ * (D + 2);
-  for (int y = tid; y < 32 * CG * (D / 4); y += 64 * KG * CG) {
-    const int c = y / (D / 4), d4 = y % (D / 4), oc = c / 32, cl = c % 32;
+  constexpr int STEP = 64 * KG * CG / (D / 4);  // columns of the workgroup at once
+  const int d4 = tid % (D / 4);
+#pragma unroll 4
+  for (int n = 0; n < 32 * CG / STEP; ++n) {
+    const int c = tid / (D / 4) + STEP * n, oc = c / 32, cl = c % 32;
     const int h = sh.block.head[c];
     const int64_t row = sh.block.row[c];
     if (row < 0) continue;
@@ -188,25 +198,9 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
   const int kg = w % KG, cg = w / KG;
   const int hh = lane / 32, ln = lane % 32;
   PrefixBlock<COLS> blk;
-  if (!blk.init(a, (uint32_t)n_cb, THREADS, sh.block)) return;
+  if (!blk.place(a, (uint32_t)n_cb, THREADS)) return;
   const int g = blk.g, p = blk.p, s = blk.s;
   const Pieces pc = blk.pc;
-  op_t qop[KS];
-  {
-    const T* src = blk.template query<T, D>(a, sh.block, cg * 32 + ln) + 8 * hh;
-#pragma unroll
-    for (int y = 0; y < KS; ++y) qop[y] = __builtin_bit_cast(op_t, *(const uint4*)(src + 16 * y));
-  }
-#pragma unroll
-  for (int y = 0; y < KS; ++y) asm volatile("" ::"v"(qop[y]));  // here: below, waits are counted by hand
-  f32x16_t o[DB];
-  float m_run = kNegBig, l_run = 0.0f;
-#pragma unroll
-  for (int d = 0; d < DB; ++d) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
-  }
-
   const int k0 = s * pc.keys, n_keys = min(pc.keys, pc.n - k0);
   const int n_tiles = (n_keys + KT - 1) / KT;
   const int64_t head = (PAGED ? 0 : p * a.p_sb) + g * a.p_sh;
@@ -273,6 +267,33 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
     }
   };
 
+  if constexpr (PAGED) {
+    load_ids(0);
+    load_ids(1);
+    wait_vm<0>();
+  }
+  load(0);
+  // the first tile is on its way while the columns are looked up
+  if (!blk.columns(a, THREADS, sh.block)) {
+    wait_vm<0>();  // nothing lands after the workgroup's LDS is given back
+    return;
+  }
+  op_t qop[KS];
+  {
+    const T* src = blk.template query<T, D>(a, sh.block, cg * 32 + ln) + 8 * hh;
+#pragma unroll
+    for (int y = 0; y < KS; ++y) qop[y] = __builtin_bit_cast(op_t, *(const uint4*)(src + 16 * y));
+  }
+#pragma unroll
+  for (int y = 0; y < KS; ++y) asm volatile("" ::"v"(qop[y]));  // here: below, waits are counted by hand
+  f32x16_t o[DB];
+  float m_run = kNegBig, l_run = 0.0f;
+#pragma unroll
+  for (int d = 0; d < DB; ++d) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+  }
+
   const int jj = (lane % 16) / 4;
   const uint32_t kbase = (uint32_t)(ln * ROWB) + (uint32_t)((hh ^ kseg<D>(ln)) * 16);
   const uint32_t vbase = (uint32_t)((4 * hh + jj) * ROWB + 32 * (ln / 16) + 8 * (lane % 4));
@@ -332,12 +353,6 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
   };
 
   const int turns = (n_tiles + KG - 1) / KG;
-  if constexpr (PAGED) {
-    load_ids(0);
-    load_ids(1);
-    wait_vm<0>();
-  }
-  load(0);
   for (int i = 0; i < turns; ++i) {
     // tile i (and the cache rows of the next) landed, by this wave and its neighbour, and both
     // through with tile i - 1
@@ -412,16 +427,7 @@ void prefix_wide_kernel(PrefixArgs a, int n_cb) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid / 64);
   const int hh = lane / 32, ln = lane % 32;
   PrefixBlock<COLS> blk;
-  if (!blk.init(a, (uint32_t)n_cb, THREADS, sh.block)) return;
-  op_t qop[KS];
-  {
-    const T* src = blk.template query<T, D>(a, sh.block, w * 32 + ln) + 8 * hh;
-#pragma unroll
-    for (int y = 0; y < KS; ++y) qop[y] = __builtin_bit_cast(op_t, *(const uint4*)(src + 16 * y));
-  }
-#pragma unroll
-  for (int y = 0; y < KS; ++y) asm volatile("" ::"v"(qop[y]));  // here: below, waits are counted by hand
-
+  if (!blk.place(a, (uint32_t)n_cb, THREADS)) return;
   const int k0 = blk.s * blk.pc.keys, n_keys = min(blk.pc.keys, blk.pc.n - k0);
   const int n_tiles = (n_keys + KT - 1) / KT;
   const int64_t head = (PAGED ? 0 : blk.p * a.p_sb) + blk.g * a.p_sh;
@@ -485,6 +491,33 @@ void prefix_wide_kernel(PrefixArgs a, int n_cb) {
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   };
+
+  if constexpr (PAGED) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) load_ids(i);
+    wait_vm<0>();
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+#pragma unroll
+    for (int y = 0; y < NI; ++y) {
+      load(false, i, y);
+      if (i < 2) load(true, i, y);
+    }
+  }
+  // the first tiles are on their way while the columns are looked up
+  if (!blk.columns(a, THREADS, sh.block)) {
+    wait_vm<0>();  // nothing lands after the workgroup's LDS is given back
+    return;
+  }
+  op_t qop[KS];
+  {
+    const T* src = blk.template query<T, D>(a, sh.block, w * 32 + ln) + 8 * hh;
+#pragma unroll
+    for (int y = 0; y < KS; ++y) qop[y] = __builtin_bit_cast(op_t, *(const uint4*)(src + 16 * y));
+  }
+#pragma unroll
+  for (int y = 0; y < KS; ++y) asm volatile("" ::"v"(qop[y]));  // here: below, waits are counted by hand
 
   f32x16_t o[DB], sc[2];
   uint32_t ph[2][8];  // a tile's weights, two a word
@@ -613,19 +646,6 @@ void prefix_wide_kernel(PrefixArgs a, int n_cb) {
     l_run += ls[0] + ls[1];
   };
 
-  if constexpr (PAGED) {
-#pragma unroll
-    for (int i = 0; i < 6; ++i) load_ids(i);
-    wait_vm<0>();
-  }
-#pragma unroll
-  for (int i = 0; i < 3; ++i) {
-#pragma unroll
-    for (int y = 0; y < NI; ++y) {
-      load(false, i, y);
-      if (i < 2) load(true, i, y);
-    }
-  }
   wait_vm<0>();
   blank(0);
   phase_barrier();
