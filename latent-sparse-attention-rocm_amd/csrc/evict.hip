@@ -253,7 +253,20 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
   __syncthreads();
   for (int j = tid; j < keep; j += kKeepThreads) kept[j] = turn.place[j];
   if (TABLE) {
-    for (int64_t i = tid; i < a.T; i += kKeepThreads) new_table[i] = table[i < n ? turn.place[i] : i];
+    constexpr int E = 8;  // entries of a thread in flight
+    for (int64_t i0 = tid; i0 < a.T; i0 += E * kKeepThreads) {
+      int32_t y[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int64_t i = min(i0 + e * kKeepThreads, a.T - 1);
+        y[e] = table[i < n ? turn.place[i] : i];
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int64_t i = i0 + e * kKeepThreads;
+        if (i < a.T) new_table[i] = y[e];
+      }
+    }
   }
 }
 
