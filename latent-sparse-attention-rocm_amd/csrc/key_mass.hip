@@ -71,26 +71,34 @@ __device__ __forceinline__ void join(float& m, float& l, float mo, float lo) {
   m = mn;
 }
 
+typedef uint32_t raw_t __attribute__((ext_vector_type(4)));  // 16 bytes of a row, kept in registers
+
 template <typename T, int D>
 struct MassShape {
   static constexpr bool MM = sizeof(T) == 2;             // scores on the matrix cores
   static constexpr int VEC = Row16<T>::N;
-  static constexpr int LPT = MM ? 4 : D / VEC;           // lanes a token
-  static constexpr int TPW = LSA_WAVE / LPT;             // tokens of a wave's step
-  static constexpr int LD = MM ? D / 32 : 1;             // 16-byte loads a lane a token
-  static constexpr int U = 16 / LD;                      // steps in flight: 16 loads a lane
-  static constexpr int NT = LSA_WAVES * TPW * U;
+  static constexpr int LPT = D / VEC;                    // lanes that load a token
+  static constexpr int TPW = MM ? 16 : LSA_WAVE / LPT;   // tokens of a wave's step
+  static constexpr int LD = MM ? D / 32 : 1;             // 16-byte loads a lane a step
+  static constexpr int U = MM ? (D == 256 ? 2 : 4) : 16; // steps in flight
+  static constexpr int TW = TPW * U;                     // tokens of a wave's turn
+  static constexpr int NT = LSA_WAVES * TW;
 };
 
 // grid (row * Hkv, span). Matrix-core form: 16 tokens a wave's step, Q as the A operand (heads
-// past the group are zero rows), K as the B operand: lane (row, col) loads dims 32 i + 8 row ..
-// + 8 of token col and receives the scores of heads 4 row .. + 3 against it.
+// past the group are zero rows), K as the B operand: lane (row, col) holds dims 32 i + 8 row .. + 8 of
+// token col and receives the scores of heads 4 row .. + 3 against it. Loading K so would touch 16 tokens
+// with every 16 lanes, which the cache serves a line a lane: 53 cycles a load of 1 KB where 16 would do,
+// 69 us for 64 rows of 4096 keys on 8 kv-heads. So lanes load whole rows, D / 8 lanes a token, and the wave
+// turns them through LDS of its own: 50 us.
 template <typename T, int D, int GQ>
-__global__ __launch_bounds__(LSA_BLOCK) void mass_scores_kernel(MassArgs a) {
+__global__ __launch_bounds__(LSA_BLOCK) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 && D <= 128 ? 4 : 1)))
+void mass_scores_kernel(MassArgs a) {
   using S = MassShape<T, D>;
-  constexpr int U = S::U, TPW = S::TPW, NT = S::NT;
+  constexpr int U = S::U, TPW = S::TPW, NT = S::NT, TW = S::TW;
   constexpr int HL = S::MM ? (GQ < 4 ? GQ : 4) : GQ;  // heads of a lane
   __shared__ float sm[LSA_WAVES][GQ], sl[LSA_WAVES][GQ];
+  __shared__ __attribute__((aligned(16))) uint16_t turn[S::MM ? LSA_WAVES : 1][16][S::MM ? D + 8 : 8];
   const int tid = threadIdx.x, lane = tid & (LSA_WAVE - 1), w = tid / LSA_WAVE;
   const int64_t unit = blockIdx.x;
   const int sp = blockIdx.y;
@@ -123,7 +131,7 @@ __global__ __launch_bounds__(LSA_BLOCK) void mass_scores_kernel(MassArgs a) {
     l[h] = 0.0f;
   }
   const int rowq = lane >> 4, col = lane & 15;                   // matrix-core form
-  const int tg = S::MM ? col : lane / S::LPT, lp = S::MM ? rowq : lane % S::LPT;
+  const int tg = S::MM ? col : lane / S::LPT, lp = lane % S::LPT;
   uint4 qm[S::LD];
   float qf[S::MM ? 1 : GQ][S::VEC];
   if constexpr (S::MM) {
@@ -136,31 +144,62 @@ __global__ __launch_bounds__(LSA_BLOCK) void mass_scores_kernel(MassArgs a) {
 #pragma unroll
     for (int h = 0; h < GQ; ++h) Row16<T>::cvt(*(const uint4*)(qrow + (int64_t)h * D + lp * S::VEC), qf[h]);
   }
+  // slot of token tg of step u: the wave's turn of TW slots (matrix cores), or steps of all waves
+  auto slot = [&](int base, int u) {
+    return S::MM ? base + w * TW + u * TPW + tg : base + (u * LSA_WAVES + w) * TPW + tg;
+  };
+  auto id_of = [&](int base) {  // matrix-core form: one id a lane, fetched a turn ahead
+    const int j = base + w * TW + lane % TW;
+    return list.ids[j < hi ? j : hi - 1];
+  };
+  int32_t next = S::MM ? id_of(lo) : 0;
   for (int base = lo; base < hi; base += NT) {
     bool ok[U];
-    uint4 kr[U][S::LD];
+    raw_t kr[U][S::LD];
+    if constexpr (S::MM) {
+      // handed to the lanes that load its row
+      int32_t id = next;
+      const bool in = base + w * TW + lane % TW < hi && id >= 0 && id < a.Tk;
+      if (fixed && in && lane < TW) fixed[id] = 0;
+      const uint64_t live = __ballot(in);
+      id = in ? id : 0;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = base + (u * LSA_WAVES + w) * TPW + tg;
-      const int32_t id = list.ids[j < hi ? j : hi - 1];
-      ok[u] = j < hi && id >= 0 && id < a.Tk;
-      const T* src = kb + (int64_t)(ok[u] ? id : 0) * a.k_st + (S::MM ? 8 : S::VEC) * lp;
+      for (int u = 0; u < U; ++u) {
+        ok[u] = live >> (u * TPW + col) & 1;
 #pragma unroll
-      for (int i = 0; i < S::LD; ++i) kr[u][i] = *(const uint4*)(src + 32 * i);
-      if (fixed && ok[u] && lp == 0) fixed[id] = 0;
+        for (int i = 0; i < S::LD; ++i) {
+          const int32_t mine = __shfl(id, u * TPW + i * (16 / S::LD) + lane / S::LPT, LSA_WAVE);
+          kr[u][i] = *(const raw_t*)(kb + (int64_t)mine * a.k_st + 8 * lp);
+        }
+      }
+      next = id_of(base + NT);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = slot(base, u);
+        const int32_t id = list.ids[j < hi ? j : hi - 1];
+        ok[u] = j < hi && id >= 0 && id < a.Tk;
+        kr[u][0] = *(const raw_t*)(kb + (int64_t)(ok[u] ? id : 0) * a.k_st + S::VEC * lp);
+        if (fixed && ok[u] && lp == 0) fixed[id] = 0;
+      }
     }
     float s[U][HL];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if constexpr (S::MM) {
+        __builtin_amdgcn_wave_barrier();  // the last step's reads before these writes
+#pragma unroll
+        for (int i = 0; i < S::LD; ++i)
+          *(raw_t*)&turn[w][i * (16 / S::LD) + lane / S::LPT][8 * lp] = kr[u][i];
+        __builtin_amdgcn_wave_barrier();  // and these before the reads (a wave's LDS operations keep their order)
         f32x4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < S::LD; ++i) x = Mfma16<T>::run(qm[i], kr[u][i], x);
+        for (int i = 0; i < S::LD; ++i) x = Mfma16<T>::run(qm[i], __builtin_bit_cast(uint4, *(const raw_t*)&turn[w][col][32 * i + 8 * rowq]), x);
 #pragma unroll
         for (int h = 0; h < HL; ++h) s[u][h] = ok[u] ? x[h] * a.scale_log2 : -INFINITY;
       } else {
         float kf[S::VEC];
-        Row16<T>::cvt(kr[u][0], kf);
+        Row16<T>::cvt(__builtin_bit_cast(uint4, kr[u][0]), kf);
 #pragma unroll
         for (int h = 0; h < HL; ++h) {
           float p = 0.0f;
@@ -185,7 +224,7 @@ __global__ __launch_bounds__(LSA_BLOCK) void mass_scores_kernel(MassArgs a) {
     if (S::MM ? HL * rowq < GQ : lp == 0) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int j = base + (u * LSA_WAVES + w) * TPW + tg;
+        const int j = slot(base, u);
         if (j < hi) {
           float* to = scores + (int64_t)j * GQ + (S::MM ? HL * rowq : 0);
 #pragma unroll
@@ -295,9 +334,7 @@ __global__ __launch_bounds__(LSA_BLOCK) void mass_fold_kernel(MassArgs a) {
 }
 
 int mass_span(int dtype, int D, int64_t units, int W) {
-  const int loads = dtype == LSA_F32 ? 1 : D / 32;
-  const int tokens = dtype == LSA_F32 ? LSA_WAVE / (D / 4) : 16;
-  const int nt = LSA_WAVES * tokens * (16 / loads);
+  const int nt = LSA_WAVES * (dtype == LSA_F32 ? LSA_WAVE / (D / 4) * 16 : (D == 256 ? 32 : 64));  // MassShape::NT
   const int64_t want = std::max<int64_t>(1, 1024 / std::max<int64_t>(units, 1));  // workgroups a list
   const int tiles = (W + nt - 1) / nt;
   const int per = (int)((tiles + want - 1) / want);
