@@ -33,6 +33,7 @@ struct PrefixArgs {
   int own_span;    // list slots of a span
   int* counters;   // [units]: cleared by the prefix kernel, arrivals of the own spans
   float* parts;    // [units][splits + own_splits][GQ (D + 2)]
+  float* sums;     // [units][splits][GQ]: the pieces' sums for lse (where lse is wanted)
   void* out;
   float* lse;      // [B, Tq, Hq] or nullptr
 };

@@ -11,8 +11,9 @@
 // states meet in LDS and leave as one partial.
 //
 // A weight enters the matrix cores as one 16-bit number: half a step of it (2^-9 in bf16, 2^-12
-// in fp16), independent from key to key; the output is rounded by as much when it is stored.
-// The sum l, which lse shows, adds the weights before that rounding. fp16 weights are kept high
+// in fp16), independent from key to key; the output is rounded by as much when it is stored. The sum
+// it is divided by adds the same rounded weights, so a row that one key fills returns that key's value;
+// the sum that lse shows adds them unrounded, in fp32. fp16 weights are kept high
 // in their range (the largest is 2^12 when the reference moves and stays below 2^15), so the smallest step
 // is 2^-36 of it and many small weights beside a large one are not lost.
 #include <math.h>
@@ -121,7 +122,7 @@ struct alignas(1024) PrefixLds {
     };
     float o[KG][CG][32][D + 4];  // every wave's state (rows 4 banks apart)
   };
-  float m[KG][CG][32], l[KG][CG][32];
+  float m[KG][CG][32], l[KG][CG][32], l32[KG][CG][32];
   int32_t ids[KG][CG][4][64];    // paged: cache rows of the tiles ahead, a wave's own
   typename PrefixBlock<32 * CG>::Lds block;
 };
@@ -133,12 +134,13 @@ __device__ __forceinline__ void dma16_far(uint32_t lds, const void* p) {  // a l
 // The wave groups' states into one partial a column. Every thread calls it, after a barrier.
 template <int D, int KG, int CG, typename Lds>
 __device__ __forceinline__ void store_partials(const PrefixArgs& a, Lds& sh, const PrefixBlock<32 * CG>& blk, int kg, int cg,
-                                               const f32x16_t (&o)[D / 32], float m_run, float l_run) {
+                                               const f32x16_t (&o)[D / 32], float m_run, float l_run, float l32_run) {
   const int tid = threadIdx.x, lane = tid & 63, hh = lane / 32, ln = lane % 32;
-  const float l = l_run + lane_xor(l_run, 32);
+  const float l = l_run + lane_xor(l_run, 32), l32 = l32_run + lane_xor(l32_run, 32);
   if (hh == 0) {
     sh.m[kg][cg][ln] = m_run;
     sh.l[kg][cg][ln] = l;
+    sh.l32[kg][cg][ln] = l32;
   }
 #pragma unroll
   for (int d = 0; d < D / 32; ++d) {
@@ -161,21 +163,25 @@ __device__ __forceinline__ void store_partials(const PrefixArgs& a, Lds& sh, con
 #pragma unroll
     for (int z = 0; z < KG; ++z) mm = fmaxf(mm, sh.m[z][oc][cl]);
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float ll = 0.0f;
+    float ll = 0.0f, ll32 = 0.0f;
 #pragma unroll
     for (int z = 0; z < KG; ++z) {
       const float f = fast_exp2(sh.m[z][oc][cl] - mm);
       const float4 v = *(const float4*)&sh.o[z][oc][cl][4 * d4];
       acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
       ll += f * sh.l[z][oc][cl];
+      ll32 += f * sh.l32[z][oc][cl];
     }
-    float* part = a.parts + ((row * a.Hkv + blk.g) * (a.splits + a.own_splits) + a.splits - blk.pc.count + blk.s) * (int64_t)pstride;
+    const int64_t unit = row * a.Hkv + blk.g;
+    const int at = a.splits - blk.pc.count + blk.s;
+    float* part = a.parts + (unit * (a.splits + a.own_splits) + at) * (int64_t)pstride;
     float* to = part + 2 * GQ + h * D + 4 * d4;  // 8-byte aligned
     *(float2*)to = make_float2(acc.x, acc.y);
     *(float2*)(to + 2) = make_float2(acc.z, acc.w);
     if (d4 == 0) {
       part[h] = mm;
       part[GQ + h] = ll;
+      if (a.lse) a.sums[(unit * a.splits + at) * GQ + h] = ll32;
     }
   }
 }
@@ -287,7 +293,7 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
 #pragma unroll
   for (int y = 0; y < KS; ++y) asm volatile("" ::"v"(qop[y]));  // here: below, waits are counted by hand
   f32x16_t o[DB];
-  float m_run = kNegBig, l_run = 0.0f;
+  float m_run = kNegBig, l_run = 0.0f, l32_run = 0.0f;
 #pragma unroll
   for (int d = 0; d < DB; ++d) {
 #pragma unroll
@@ -323,22 +329,25 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
         const float alpha = fast_exp2(m_run - mn);
         m_run = mn;
         l_run *= alpha;
+        l32_run *= alpha;
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
         }
       }
-      float ls[2] = {0.0f, 0.0f};
+      float ls[2] = {0.0f, 0.0f}, l32[2] = {0.0f, 0.0f};
       uint32_t ph[8];
 #pragma unroll
       for (int r = 0; r < 16; r += 2) {
         const float p0 = fast_exp2(fmaf(sc[r], scale, -m_run)), p1 = fast_exp2(fmaf(sc[r + 1], scale, -m_run));
-        ls[0] += p0;
-        ls[1] += p1;
+        l32[0] += p0;
+        l32[1] += p1;
         ph[r / 2] = M::pack2(p0, p1);
+        ls[r / 2 & 1] = M::sum2(ph[r / 2], ls[r / 2 & 1]);
       }
       l_run += ls[0] + ls[1];
+      l32_run += l32[0] + l32[1];
 #pragma unroll
       for (int sp = 0; sp < 2; ++sp) {
         const op_t pb = __builtin_bit_cast(op_t, make_uint4(ph[4 * sp], ph[4 * sp + 1], ph[4 * sp + 2], ph[4 * sp + 3]));
@@ -373,7 +382,7 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // nothing lands after this
   __syncthreads();
 
-  store_partials<D, KG, CG>(a, sh, blk, kg, cg, o, m_run, l_run);
+  store_partials<D, KG, CG>(a, sh, blk, kg, cg, o, m_run, l_run, l32_run);
 }
 
 // ---------------------------------------------------------------- 256 columns
@@ -404,7 +413,7 @@ struct alignas(1024) WideLds {
     };
     float o[1][8][32][D + 4];
   };
-  float m[1][8][32], l[1][8][32];
+  float m[1][8][32], l[1][8][32], l32[1][8][32];
   int32_t ids[8][8][64];  // paged: cache rows of eight tiles, a wave's own
   typename PrefixBlock<256>::Lds block;
 };
@@ -521,7 +530,7 @@ void prefix_wide_kernel(PrefixArgs a, int n_cb) {
 
   f32x16_t o[DB], sc[2];
   uint32_t ph[2][8];  // a tile's weights, two a word
-  float m_run = kNegBig, l_run = 0.0f;
+  float m_run = kNegBig, l_run = 0.0f, l32_run = 0.0f;
 #pragma unroll
   for (int d = 0; d < DB; ++d) {
 #pragma unroll
@@ -578,8 +587,10 @@ void prefix_wide_kernel(PrefixArgs a, int n_cb) {
   // a chain of dependent instructions would leave the unit idle), and their sum. top: fp16, the largest
   // of the packed halves as bits.
   u16x2_t top;
+  const bool want_lse = a.lse != nullptr;
+  float l32;
   auto weights = [&](float (&ls)[2]) {
-    ls[0] = ls[1] = 0.0f;
+    ls[0] = ls[1] = l32 = 0.0f;
     top = {0, 0};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -596,7 +607,8 @@ void prefix_wide_kernel(PrefixArgs a, int n_cb) {
 #pragma unroll
         for (int e = 0; e < 8; e += 2) pair[e / 2] = M::pack2(x[e], x[e + 1]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ls[e & 1] += x[e];
+        for (int e = 0; e < 4; ++e) ls[e & 1] = M::sum2(pair[e], ls[e & 1]);
+        if (want_lse) l32 += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));  // uniform
         if constexpr (HALF) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, pair[e]));
@@ -635,6 +647,7 @@ void prefix_wide_kernel(PrefixArgs a, int n_cb) {
         const float alpha = fast_exp2(m_run - mn);
         m_run = mn;
         l_run *= alpha;
+        l32_run *= alpha;
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
 #pragma unroll
@@ -644,6 +657,7 @@ void prefix_wide_kernel(PrefixArgs a, int n_cb) {
       }
     }
     l_run += ls[0] + ls[1];
+    l32_run += l32;
   };
 
   wait_vm<0>();
@@ -675,7 +689,7 @@ void prefix_wide_kernel(PrefixArgs a, int n_cb) {
   if (!late) phase_barrier();
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // nothing lands after this
   __syncthreads();
-  store_partials<D, KG, CG>(a, sh, blk, 0, w, o, m_run, l_run);
+  store_partials<D, KG, CG>(a, sh, blk, 0, w, o, m_run, l_run, l32_run);
 }
 
 int64_t prefix_units(const PrefixArgs& a) { return ((int64_t)a.P * a.Hkv * a.splits + kXcds - 1) / kXcds * kXcds; }

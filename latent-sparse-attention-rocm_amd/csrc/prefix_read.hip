@@ -49,6 +49,14 @@ __global__ __launch_bounds__(LSA_BLOCK) void prefix_gather_kernel(PrefixArgs a) 
                         a.scale_log2, st);
   float* part = a.parts + (i * (a.splits + a.own_splits) + a.splits - pc.count + s) * (int64_t)PSTRIDE;
   finish_span<T, D, GQ, kMaxPieces + kMaxOwn, true>(sh, st, false, (T*)nullptr, part, 0);
+  if (a.lse && threadIdx.x < GQ) {  // weights are fp32 here: one sum serves both
+    float m = kNegBig, l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < LSA_WAVES; ++w) m = fmaxf(m, sh.m[w][threadIdx.x]);
+#pragma unroll
+    for (int w = 0; w < LSA_WAVES; ++w) l += sh.l[w][threadIdx.x] * fast_exp2(sh.m[w][threadIdx.x] - m);
+    a.sums[(i * a.splits + a.splits - pc.count + s) * GQ + threadIdx.x] = l;
+  }
 }
 
 // grid (row * Hkv, own span). The last span of a unit to arrive joins the unit's partials.
@@ -97,12 +105,17 @@ __global__ __launch_bounds__(LSA_BLOCK) void prefix_join_kernel(PrefixArgs a) {
   }
   if (a.lse) {
     const int lane = threadIdx.x & (LSA_WAVE - 1);
+    const float* sums = a.sums + (i * a.splits + a.splits - pc.count) * GQ;
     for (int h = threadIdx.x / LSA_WAVE; h < GQ; h += LSA_WAVES) {
-      float M = kNegBig;
+      float M = kNegBig, L = 0.0f;
       for (int x = lane; x < total; x += LSA_WAVE) M = fmaxf(M, coherent_load(parts + (int64_t)x * PSTRIDE + h));
       M = wave_max(M);
+      for (int x = lane; x < total; x += LSA_WAVE) {
+        const float* part = parts + (int64_t)x * PSTRIDE;
+        L += (x < pc.count ? sums[x * GQ + h] : coherent_load(part + GQ + h)) * fast_exp2(coherent_load(part + h) - M);
+      }
+      L = wave_sum(L);
       if (lane == 0) {
-        const float L = total ? sh.ltot[h] : 0.0f;
         // no keys, or a sum that is not a number, which counts as none
         a.lse[row * a.Hq + g * GQ + h] = L > 0.0f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
       }
@@ -112,7 +125,7 @@ __global__ __launch_bounds__(LSA_BLOCK) void prefix_join_kernel(PrefixArgs a) {
 
 struct PrefixPlan {
   int splits, own_splits, own_span;
-  size_t parts, total;
+  size_t parts, sums, total;
 };
 
 // Query columns a prefix has, if its rows are spread evenly.
@@ -140,7 +153,8 @@ PrefixPlan prefix_plan(int dtype, int64_t B, int64_t Tq, int64_t P, int64_t Tp, 
   p.own_splits = std::max(1, (W + p.own_span - 1) / p.own_span);
   const int64_t gq = Hq / Hkv;
   p.parts = (size_t)units * (p.splits + p.own_splits) * (size_t)(gq * (D + 2)) * sizeof(float);
-  p.total = p.parts + (size_t)units * sizeof(int);
+  p.sums = (size_t)units * p.splits * gq * sizeof(float);
+  p.total = p.parts + p.sums + (size_t)units * sizeof(int);
   return p;
 }
 
@@ -234,7 +248,8 @@ extern "C" int lsa_prefix_read(const void* q, const void* k_prefix, const void* 
   a.B = B; a.Tq = Tq; a.Tp = Tp; a.P = (int)P; a.Hq = Hq; a.Hkv = Hkv; a.scale_log2 = scale * kLog2e;
   a.splits = p.splits; a.own_splits = p.own_splits; a.own_span = p.own_span;
   a.parts = (float*)scratch;
-  a.counters = (int*)((char*)scratch + p.parts);
+  a.sums = (float*)((char*)scratch + p.parts);
+  a.counters = (int*)((char*)scratch + p.parts + p.sums);
   a.out = out; a.lse = lse;
   hipStream_t s = (hipStream_t)stream;
   const int64_t units = B * Tq * Hkv;

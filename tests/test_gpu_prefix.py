@@ -204,6 +204,24 @@ def test_one_large_and_many_small_weights(dtype):
     compare(call(c, scale=1.0), want(c, scale=1.0), c)
 
 
+@pytest.mark.parametrize("dtype,B", [(torch.bfloat16, 3), (torch.bfloat16, 150), (torch.float16, 30), (torch.float16, 150)])
+def test_a_key_that_fills_its_row_returns_its_value(dtype, B):
+    """One score far above the rest: the output is that key's value, bit for bit."""
+    g = torch.Generator().manual_seed(2)
+    q = torch.randn(B, 1, 2, 128, generator=g)
+    q = (q / q.norm(dim=-1, keepdim=True)).to(dtype)
+    kp, vp = (torch.randn(1, 300, 1, 128, generator=g).to(dtype) for _ in range(2))
+    kp[0, 7::11] = 0
+    at = torch.randint(0, 300, (B,), generator=g)
+    kp[0, at, 0] = q[:, 0, 0]
+    out = pipeline.prefix_read(q[:, :, :1].to(DEV), kp.to(DEV), vp.to(DEV), scale=1000.0).cpu()
+    s = 1000.0 * q[:, 0, :1].double() @ kp[0, :, 0].double().T
+    gap = s.topk(2, -1).values  # where no other key has 2^-60 of the weight
+    sure = (gap[:, 0, 0] - gap[:, 0, 1] > 42.0).nonzero()[:, 0]
+    assert len(sure) > B // 2
+    assert torch.equal(out[sure, 0, 0], vp[0, s[sure, 0].argmax(-1), 0])
+
+
 @pytest.mark.parametrize("dtype,D", [(torch.float32, 64), (torch.bfloat16, 128), (torch.float16, 128)])
 def test_views_strides_and_a_shared_pool(dtype, D):
     """Caches as views of wider buffers, K and V halves of one, the own cache a pool of every row."""
