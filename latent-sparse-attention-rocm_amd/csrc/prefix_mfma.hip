@@ -273,6 +273,8 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
     }
   };
 
+  // a block past the first may have no columns: looked up before anything loads
+  if (blk.cb != 0 && !blk.columns(a, THREADS, sh.block)) return;
   if constexpr (PAGED) {
     load_ids(0);
     load_ids(1);
@@ -280,7 +282,7 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
   }
   load(0);
   // the first tile is on its way while the columns are looked up
-  if (!blk.columns(a, THREADS, sh.block)) {
+  if (blk.cb == 0 && !blk.columns(a, THREADS, sh.block)) {
     wait_vm<0>();  // nothing lands after the workgroup's LDS is given back
     return;
   }
@@ -501,6 +503,8 @@ void prefix_wide_kernel(PrefixArgs a, int n_cb) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   };
 
+  // a block past the first may have no columns: looked up before anything loads
+  if (blk.cb != 0 && !blk.columns(a, THREADS, sh.block)) return;
   if constexpr (PAGED) {
 #pragma unroll
     for (int i = 0; i < 6; ++i) load_ids(i);
@@ -515,7 +519,7 @@ void prefix_wide_kernel(PrefixArgs a, int n_cb) {
     }
   }
   // the first tiles are on their way while the columns are looked up
-  if (!blk.columns(a, THREADS, sh.block)) {
+  if (blk.cb == 0 && !blk.columns(a, THREADS, sh.block)) {
     wait_vm<0>();  // nothing lands after the workgroup's LDS is given back
     return;
   }
