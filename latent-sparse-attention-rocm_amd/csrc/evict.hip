@@ -443,8 +443,8 @@ void launch_keep(const KeepArgs& a, dim3 grid, hipStream_t s) {
 int check_keep(const char* who, const void* mass, int64_t B, int32_t Hkv, int64_t T, int64_t mass_sb, int64_t mass_sh,
                int32_t budget, int32_t window, int32_t sink, const void* kept, const void* new_lengths) {
   LSA_REQUIRE(mass && kept && new_lengths, LSA_ERR_NULL, "%s: NULL pointer", who);
-  LSA_REQUIRE(B >= 0 && B <= 65535 && Hkv >= 1 && T >= 1 && T <= 0x7FFFFFFF, LSA_ERR_SHAPE,
-              "%s: needs 0..65535 rows of 1..2^31-1 positions and a kv-head", who);
+  LSA_REQUIRE(B >= 0 && B <= 65535 && Hkv >= 1 && T >= 1 && T <= 1 << 30, LSA_ERR_SHAPE,
+              "%s: needs 0..65535 rows of 1..2^30 positions and a kv-head", who);
   LSA_REQUIRE(mass_sb >= 0 && mass_sh >= 0, LSA_ERR_SHAPE, "%s: weight strides must be >= 0", who);
   LSA_REQUIRE(budget >= 1 && budget <= T, LSA_ERR_SHAPE, "%s: budget %d not in 1..%lld", who, budget, (long long)T);
   LSA_REQUIRE(window >= 0 && sink >= 0 && (int64_t)window + sink <= budget, LSA_ERR_SHAPE,

@@ -17,6 +17,16 @@ from lsa_rocm_lab.port.shared_prefix import aligned, cache_pair, cache_strides, 
 _SLAB_BYTES = 256 << 20  # scores of query rows held at once (more rows go through in slabs)
 
 
+def _apart(t: torch.Tensor) -> bool:
+    """Whether a tensor that is written has every element in a place of its own."""
+    reach = 1
+    for step, n in sorted((step, n) for step, n in zip(t.stride(), t.shape) if n > 1):
+        if step < reach:
+            return False
+        reach = step * n
+    return True
+
+
 def key_mass(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -55,9 +65,9 @@ def key_mass(
     if fresh:
         mass = torch.empty(caches, Hkv, Tk, dtype=torch.float32, device=device)
     elif (tuple(mass.shape) != (caches, Hkv, Tk) or mass.dtype != torch.float32 or (Tk > 1 and mass.stride(2) != 1)
-          or (Hkv > 1 and mass.stride(1) < Tk) or (caches > 1 and mass.stride(0) < Tk)):
-        raise ValueError(f"key_mass: mass must be fp32 [{caches}, {Hkv}, {Tk}] with contiguous keys, got {mass.dtype} "
-                         f"{tuple(mass.shape)} at strides {mass.stride()}")
+          or not _apart(mass)):
+        raise ValueError(f"key_mass: mass must be fp32 [{caches}, {Hkv}, {Tk}] with contiguous keys, each in a place of "
+                         f"its own, got {mass.dtype} {tuple(mass.shape)} at strides {mass.stride()}")
     if B * Tq == 0 or W == 0 or Tk == 0:
         return mass.zero_() if fresh else mass
     q = aligned(q)
@@ -170,8 +180,8 @@ def evict(
             a, b = _extent(new)
             if any(a < hi and lo < b for lo, hi in map(_extent, (k, v, mass))):
                 raise ValueError("evict: out must not overlap the cache it is made from")
-        if k2.data_ptr() == v2.data_ptr() and k2.numel():
-            raise ValueError("evict: out k and v are the same buffer")
+        if not (_apart(k2) and _apart(v2) and _apart(m2)) or (k2.data_ptr() == v2.data_ptr() and k2.numel()):
+            raise ValueError("evict: out k, v and mass need a place of their own for every element")
     ob, ot, oh = cache_strides(k2)
     kept = torch.empty((B, budget) if shared else (B, Hkv, budget), dtype=torch.int32, device=device)
     new_lengths = torch.empty(B, dtype=torch.int32, device=device)

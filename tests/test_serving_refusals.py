@@ -78,7 +78,7 @@ def keep(**over):
 @pytest.mark.parametrize("over,match", [
     (dict(mass=None), "NULL"), (dict(kept=None), "NULL"), (dict(budget=0), "budget"), (dict(budget=101), "budget"),
     (dict(window=9), "fit the budget"), (dict(window=-1), "fit the budget"), (dict(sink=-1), "fit the budget"),
-    (dict(B=70000), "rows"), (dict(T=0), "positions"), (dict(table=P, stride=100, pool=5), "come together"),
+    (dict(B=70000), "rows"), (dict(T=0), "positions"), (dict(T=(1 << 30) + 1), "positions"), (dict(table=P, stride=100, pool=5), "come together"),
     (dict(table=P, new_table=P, stride=100, new_stride=100, pool=5), "shared"),
     (dict(table=P, new_table=P, stride=99, new_stride=100, pool=5, shared=1), "strides"),
 ])
@@ -166,7 +166,8 @@ def test_key_mass_arguments():
         ((q, k, ids, lens), dict(lse=fake(3, 8, dtype=f32)), "lse must be fp32"),
         ((q, k, ids, lens), dict(mass=fake(3, 2, 8, dtype=f32)), "mass must be fp32"),
         ((q, k, ids, lens), dict(mass=fake(3, 2, 9)), "mass must be fp32"),
-        ((q, k, ids, lens), dict(mass=fake(3, 1, 9, dtype=f32).expand(3, 2, 9)), "mass must be fp32"),
+        ((q, k, ids, lens), dict(mass=fake(3, 1, 9, dtype=f32).expand(3, 2, 9)), "place of its own"),
+        ((q, k, ids, lens), dict(mass=fake(99, dtype=f32).as_strided((3, 2, 9), (9, 9, 1))), "place of its own"),
         ((q, k, ids, lens), dict(mass=fake(3, 9, 2, dtype=f32).transpose(1, 2)), "contiguous keys"),
     ]:
         with pytest.raises(ValueError, match=match):
@@ -187,6 +188,9 @@ def test_evict_arguments():
         ((k, k, m, 4), dict(out=(fake(2, 4, 2, 64), fake(2, 4, 2, 64), fake(2, 2, 3, dtype=torch.float32))), "out mass"),
         ((k, k, m, 4), dict(out=(k[:, :4], fake(2, 4, 2, 64), fake(2, 2, 4, dtype=torch.float32))), "strides|overlap"),
         ((k, k, m, 4), dict(out=(k, k, fake(2, 2, 4, dtype=torch.float32))), "overlap"),
+        ((k, k, m, 4), dict(out=(*[fake(2, 4, 2, 64)] * 2, fake(2, 2, 4, dtype=torch.float32))), "place of their own"),
+        ((k, k, m, 4), dict(out=(fake(2, 4, 2, 64), fake(2, 4, 2, 64), fake(1, 2, 4, dtype=torch.float32).expand(2, 2, 4))),
+         "place of their own"),
     ]:
         with pytest.raises(ValueError, match=match):
             eviction.evict(*args, **kw)
