@@ -484,9 +484,10 @@ int lsa_key_mass(const void* q, const void* k, int dtype, int64_t B, int64_t Tq,
  * (in fp64, head by head, rounded to fp32). With a slot table [B, T] (shared; rows table_stride
  * apart) mass is a pool's, [Hkv, pool_rows], and new_table [B, T] receives each table row with
  * its kept entries first, then the others of its length, then what was behind it (entries
- * outside the pool weigh least). scratch: lsa_evict_scratch_bytes(B, T, shared). No counterpart
- * in the reference. */
-size_t lsa_evict_scratch_bytes(int64_t B, int64_t T, int summed);
+ * outside the pool weigh least). scratch: lsa_evict_scratch_bytes(), 16-byte aligned, no
+ * initialisation (0 bytes where selections are not shared and T <= 32768). No counterpart in the
+ * reference. */
+size_t lsa_evict_scratch_bytes(int64_t B, int32_t Hkv, int64_t T, int shared);
 int lsa_evict_keep(const float* mass, int64_t B, int32_t Hkv, int64_t T, int64_t mass_batch_stride,
                    int64_t mass_head_stride, const int32_t* lengths, int32_t budget, int32_t window, int32_t sink,
                    int shared, const int32_t* table, int64_t table_stride, int64_t pool_rows, void* scratch,

@@ -43,6 +43,8 @@ struct KeepArgs {
   int64_t new_stride;
   int64_t pool;           // paged: cache rows the weights hold
   uint32_t* keys_out;
+  int* hist;              // rows in slabs: [3][units][slabs][2048]
+  int2* state;            // [units][2]
 };
 
 __device__ __forceinline__ int row_length(const KeepArgs& a, int64_t b) {
@@ -85,12 +87,12 @@ __global__ __launch_bounds__(LSA_BLOCK) void seen_keys_kernel(KeepArgs a) {
 //                     a selection), so a key costs few instructions: the first and last positions
 //                     are the largest key, those past the row the least, and no loop asks which is
 //                     which; one scan over the threads' counts ranks everything.
-//   keep_long_kernel  longer rows: every pass reads the keys again, and ranks count slab by slab.
+//   keep_slab_kernel  longer rows, a workgroup a slab of 32768, four launches: a histogram each, then the
+//                     ranks.
 constexpr int kBins = 2048, kCopies = 8;
 
 struct KeepLds {
   alignas(16) int hist[kBins][kCopies];
-  int gt[kKeepThreads], eq[kKeepThreads];  // of a (slab, wave)
   int wave_gt[kKeepWaves], wave_eq[kKeepWaves];
   uint32_t digit;
   int need;
@@ -120,21 +122,11 @@ __device__ __forceinline__ void keep_scan(KeepLds& sh, int& gt, int& eq, int& al
   eq = be + ie - eq;
 }
 
-// The bin that the `need`-th key from the top is in, given every thread's share of the histogram
-// (bins 2047 - 2 t and 2046 - 2 t): its digit, and how many of its keys are needed.
-__device__ __forceinline__ void keep_digit(KeepLds& sh, int need) {
+// The bin that the `need`-th key from the top is in, given every thread's counts (bins 2047 - 2 t and
+// 2046 - 2 t): its digit, and how many of its keys are needed.
+__device__ __forceinline__ void keep_digit(KeepLds& sh, int need, const int (&c)[2]) {
   const int tid = threadIdx.x;
-  int c[2], none = 0, mine = 0, total, unused;
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    c[e] = 0;
-#pragma unroll
-    for (int y = 0; y < kCopies; y += 4) {
-      const int4 x = *(const int4*)&sh.hist[kBins - 1 - 2 * tid - e][y];
-      c[e] += x.x + x.y + x.z + x.w;
-    }
-    mine += c[e];
-  }
+  int none = 0, mine = c[0] + c[1], total, unused;
   const int own = mine;
   keep_scan(sh, mine, none, total, unused);
   if (mine < need && need <= mine + own) {
@@ -162,12 +154,57 @@ struct KeepTurn {
   };
 };
 
+// The thread's run of R keys of the positions from p0 on: the first and last of the row are the largest
+// key, which no weight equals, positions past it the least. Contains barriers.
+template <int R>
+__device__ __forceinline__ void keep_load(KeepTurn<R>& turn, const KeepArgs& a, int64_t u, int64_t b, int g, int n, int p0,
+                                          uint32_t (&x)[R]) {
+  using Turn = KeepTurn<R>;
+  const int tid = threadIdx.x;
+  const float* mass = a.mass + b * a.mass_sb + g * a.mass_sh;
+  const uint32_t* keys = a.keys ? a.keys + u * a.T : nullptr;
+  uint32_t in[R];
+#pragma unroll
+  for (int e = 0; e < R; ++e) {  // unconditional (clamped): all in flight
+    const int i = min(p0 + e * kKeepThreads + tid, n - 1);
+    in[e] = keys ? keys[i] : __float_as_uint(mass[i]);
+  }
+  uint32_t* to = &turn.key[Turn::at(tid)];
+#pragma unroll
+  for (int e = 0; e < R; ++e)
+    to[Turn::at(e * kKeepThreads)] = keys ? in[e] : seen_key(__uint_as_float(in[e]));
+  __syncthreads();
+  const int end = R * kKeepThreads;
+  for (int i = tid; i < min(a.sink - p0, end); i += kKeepThreads) turn.key[Turn::at(i)] = 0xFFFFFFFFu;
+  for (int i = max(n - a.window - p0, 0) + tid; i < end; i += kKeepThreads)
+    turn.key[Turn::at(i)] = p0 + i < n ? 0xFFFFFFFFu : 0u;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < R; e += 4) {
+    const uint4 y = *(const uint4*)&turn.key[tid * (R + Turn::PAD) + e];
+    x[e] = y.x; x[e + 1] = y.y; x[e + 2] = y.z; x[e + 3] = y.w;
+  }
+  __syncthreads();
+}
+
+// Counts the digits at `shift` of the keys that share `thr` under `mask`. Ends with a barrier. Positions past the
+// row are counted, as the least key; there are enough of the row's own before they would matter.
+template <int R>
+__device__ __forceinline__ void keep_count(KeepLds& sh, const uint32_t (&x)[R], uint32_t mask, uint32_t thr, int shift) {
+  int* hist = &sh.hist[0][threadIdx.x % kCopies];
+#pragma unroll
+  for (int e = 0; e < R; ++e) {
+    if ((x[e] & mask) == thr) atomicAdd(&hist[((x[e] >> shift) & (kBins - 1)) * kCopies], 1);
+  }
+  __syncthreads();
+}
+
 template <int R, bool TABLE>
 __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
   using Turn = KeepTurn<R>;
   __shared__ __attribute__((aligned(16))) Turn turn;
   KeepLds& sh = turn.sh;
-  const int tid = threadIdx.x, lane = tid & (LSA_WAVE - 1);
+  const int tid = threadIdx.x;
   const int64_t u = blockIdx.x;
   const int64_t b = u / a.G;
   const int g = (int)(u % a.G);
@@ -184,46 +221,25 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
     }
     return;
   }
-  {
-    const float* mass = a.mass + b * a.mass_sb + g * a.mass_sh;
-    const uint32_t* keys = a.keys ? a.keys + u * a.T : nullptr;
-    uint32_t in[R];
-#pragma unroll
-    for (int e = 0; e < R; ++e) {  // unconditional (clamped): all in flight
-      const int i = min(e * kKeepThreads + tid, n - 1);
-      in[e] = keys ? keys[i] : __float_as_uint(mass[i]);
-    }
-    uint32_t* to = &turn.key[Turn::at(tid)];
-#pragma unroll
-    for (int e = 0; e < R; ++e)
-      to[Turn::at(e * kKeepThreads)] = keys ? in[e] : seen_key(__uint_as_float(in[e]));
-    __syncthreads();
-    // the first and last positions, which no weight equals, and what is past the row
-    for (int i = tid; i < a.sink; i += kKeepThreads) turn.key[Turn::at(i)] = 0xFFFFFFFFu;
-    for (int i = n - a.window + tid; i < R * kKeepThreads; i += kKeepThreads)
-      turn.key[Turn::at(i)] = i < n ? 0xFFFFFFFFu : 0u;
-  }
-  __syncthreads();
   uint32_t x[R];
-#pragma unroll
-  for (int e = 0; e < R; e += 4) {
-    const uint4 y = *(const uint4*)&turn.key[tid * (R + Turn::PAD) + e];
-    x[e] = y.x; x[e + 1] = y.y; x[e + 2] = y.z; x[e + 3] = y.w;
-  }
-  __syncthreads();
+  keep_load<R>(turn, a, u, b, g, n, 0, x);
   uint32_t thr = 0, mask = 0;
   int ties = a.budget;
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
     keep_clear(sh);
-    int* hist = &sh.hist[0][lane % kCopies];
+    keep_count<R>(sh, x, mask, thr, shift);
+    int c[2] = {0, 0};
 #pragma unroll
-    for (int e = 0; e < R; ++e) {
-      if ((x[e] & mask) == thr) atomicAdd(&hist[((x[e] >> shift) & (kBins - 1)) * kCopies], 1);
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int y = 0; y < kCopies; y += 4) {
+        const int4 z = *(const int4*)&sh.hist[kBins - 1 - 2 * tid - e][y];
+        c[e] += z.x + z.y + z.z + z.w;
+      }
     }
-    __syncthreads();
-    keep_digit(sh, ties);
+    keep_digit(sh, ties, c);
     thr |= sh.digit << shift;
     ties = sh.need;
     mask |= (pass == 2 ? 1023u : 2047u) << shift;
@@ -270,123 +286,137 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
   }
 }
 
-__global__ __launch_bounds__(kKeepThreads) void keep_long_kernel(KeepArgs a) {
-  __shared__ KeepLds sh;
-  constexpr int U = 8;  // keys of a thread at once
-  const int tid = threadIdx.x, lane = tid & (LSA_WAVE - 1), w = tid / LSA_WAVE;
+// A row in slabs of 32768 positions, a workgroup a slab; grid (selection, slab). Phases 0, 1 and 2 leave
+// each slab's histogram of their digit, and phases 1, 2 and 3 add the slabs' up and find the digit
+// (slab 0 keeps it for the phases after the next). Phase 3 ranks: what is kept before a slab follows from
+// the earlier slabs' histograms.
+constexpr int kSlabRun = 32, kSlab = kSlabRun * kKeepThreads;
+
+template <int PHASE, bool TABLE>
+__global__ __launch_bounds__(kKeepThreads) void keep_slab_kernel(KeepArgs a) {
+  constexpr int R = kSlabRun;
+  using Turn = KeepTurn<R>;
+  __shared__ __attribute__((aligned(16))) Turn turn;
+  KeepLds& sh = turn.sh;
+  const int tid = threadIdx.x, lane = tid & (LSA_WAVE - 1);
   const int64_t u = blockIdx.x;
+  const int slab = blockIdx.y, slabs = gridDim.y;
   const int64_t b = u / a.G;
   const int g = (int)(u % a.G);
-  const int n = row_length(a, b);
+  const int n = row_length(a, b), p0 = slab * kSlab, p1 = (int)min((int64_t)p0 + kSlab, a.T);
   const int keep = n < a.budget ? n : a.budget;
-  if (g == 0 && tid == 0) a.new_lengths[b] = keep;
-  const bool all = n <= a.budget;
-  const int lo = min(a.sink, n), hi = all ? lo : n - a.window;  // the positions that compete
-  const float* mass = a.mass + b * a.mass_sb + g * a.mass_sh;
-  const uint32_t* keys = a.keys ? a.keys + u * a.T : nullptr;
-  uint32_t x[U];
-  auto fetch = [&](int i0) {  // of positions i0 + tid + 1024 e; unconditional loads (clamped), n > 0
-    float f[U];
-#pragma unroll
-    for (int e = 0; e < U; ++e) {
-      const int i = min(i0 + e * kKeepThreads + tid, n - 1);
-      if (keys) x[e] = keys[i];
-      else f[e] = mass[i];
-    }
-    if (!keys) {
-#pragma unroll
-      for (int e = 0; e < U; ++e) x[e] = seen_key(f[e]);
-    }
-  };
-  const int step = U * kKeepThreads;
-  uint32_t thr = 0xFFFFFFFFu;
-  int ties = 0;  // how many of the keys equal to the threshold stay
-  int need = a.budget - lo - (n - hi);
-  if (!all && need > 0) {  // uniform
-    uint32_t prefix = 0, mask = 0;
-#pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
-      keep_clear(sh);
-      for (int i0 = 0; i0 < n; i0 += step) {
-        fetch(i0);
-#pragma unroll
-        for (int e = 0; e < U; ++e) {
-          const int i = i0 + e * kKeepThreads + tid;
-          if (i >= lo && i < hi && (x[e] & mask) == prefix)
-            atomicAdd(&sh.hist[(x[e] >> shift) & (kBins - 1)][lane % kCopies], 1);
-        }
-      }
-      __syncthreads();
-      keep_digit(sh, need);
-      prefix |= sh.digit << shift;
-      need = sh.need;
-      mask |= (pass == 2 ? 1023u : 2047u) << shift;
-    }
-    thr = prefix;
-    ties = need;
-  }
   int32_t* kept = a.kept + u * a.budget;
   const int32_t* table = a.table ? a.table + b * a.table_stride : nullptr;
   int32_t* new_table = a.new_table ? a.new_table + b * a.new_stride : nullptr;
-  const uint64_t below = lane == 0 ? 0ull : ~0ull >> (LSA_WAVE - lane);
-  // stays for its place or weight (gt), or may stay as one of the keys at the threshold (eq)
-  auto stays = [&](int e, int i, bool& gt, bool& eq) {
-    const bool middle = !all && i >= lo && i < hi;
-    gt = i < n && (!middle || x[e] > thr);
-    eq = middle && x[e] == thr && ties > 0;
-  };
-  constexpr int SLABS = kKeepThreads / kKeepWaves;  // counted in one scan
-  int base = 0, base_eq = 0;
-  for (int s0 = 0; s0 < n; s0 += SLABS * kKeepThreads) {
-    sh.gt[tid] = sh.eq[tid] = 0;
-    __syncthreads();
-    const int s1 = min(n, s0 + SLABS * kKeepThreads);
-    for (int i0 = s0; i0 < s1; i0 += step) {
-      if (!all) fetch(i0);
-#pragma unroll
-      for (int e = 0; e < U; ++e) {
-        const int j = i0 + e * kKeepThreads;
-        if (j >= s1) break;
-        bool gt, eq;
-        stays(e, j + tid, gt, eq);
-        const int cg = __popcll(__ballot(gt)), ce = __popcll(__ballot(eq));
-        if (lane == 0) {
-          const int at = (j - s0) / kKeepThreads * kKeepWaves + w;
-          sh.gt[at] = cg;
-          sh.eq[at] = ce;
-        }
+  if (PHASE == 3) {
+    if (g == 0 && slab == 0 && tid == 0) a.new_lengths[b] = keep;
+    for (int i = max(p0, keep) + tid; i < min(p1, a.budget); i += kKeepThreads) kept[i] = -1;
+    if (TABLE) {
+      for (int i = max(p0, n) + tid; i < p1; i += kKeepThreads) new_table[i] = table[i];
+    }
+    if (n <= a.budget) {  // uniform: all of it
+      for (int i = p0 + tid; i < min(p1, n); i += kKeepThreads) {
+        kept[i] = i;
+        if (TABLE) new_table[i] = table[i];
       }
     }
-    __syncthreads();
-    int cg = sh.gt[tid], ce = sh.eq[tid], tg, te;
-    keep_scan(sh, cg, ce, tg, te);
-    sh.gt[tid] = base + cg;
-    sh.eq[tid] = base_eq + ce;
-    base += tg;
-    base_eq += te;
-    __syncthreads();
-    for (int i0 = s0; i0 < s1; i0 += step) {
-      if (!all) fetch(i0);
-#pragma unroll
-      for (int e = 0; e < U; ++e) {
-        const int j = i0 + e * kKeepThreads, i = j + tid;
-        if (j >= s1) break;
-        bool gt, eq;
-        stays(e, i, gt, eq);
-        const int at = (j - s0) / kKeepThreads * kKeepWaves + w;
-        const int bg = sh.gt[at] + __popcll(__ballot(gt) & below), be = sh.eq[at] + __popcll(__ballot(eq) & below);
-        const int rank = bg + min(be, ties);  // kept positions before i
-        const bool in = gt || (eq && be < ties);
-        if (in) kept[rank] = i;
-        if (i < n && new_table) new_table[in ? rank : keep + (i - rank)] = table[i];
-      }
-    }
-    __syncthreads();
   }
-  for (int j = keep + tid; j < a.budget; j += kKeepThreads) kept[j] = -1;
-  if (new_table) {
-    for (int64_t i = n + tid; i < a.T; i += kKeepThreads) new_table[i] = table[i];
+  if (n <= a.budget) return;
+  int* hist = a.hist + u * slabs * kBins;             // of phase 0, [slab][bin]
+  const int64_t phase_hist = (int64_t)gridDim.x * slabs * kBins;
+  int2* state = a.state + u * 2;                      // digits (and what they leave needed) of phases 0, 1
+  uint32_t thr = 0, mask = 0;
+  int ties = a.budget, gt0 = 0, eq0 = 0;  // phase 3: above and at the threshold in the slabs before
+#pragma unroll
+  for (int q = 0; q < PHASE; ++q) {
+    const int shift = q == 0 ? 21 : (q == 1 ? 10 : 0);
+    int c[2] = {0, 0}, before[2] = {0, 0};
+    if (q == PHASE - 1 || PHASE == 3) {  // bins 2047 - 2 t and 2046 - 2 t of all slabs, and of the ones before
+      const int2* h = (const int2*)(hist + q * phase_hist + kBins - 2 - 2 * tid);
+      for (int y = 0; y < slabs; ++y) {
+        const int2 x = h[(int64_t)y * kBins / 2];
+        c[0] += x.y;
+        c[1] += x.x;
+        before[0] += y < slab ? x.y : 0;
+        before[1] += y < slab ? x.x : 0;
+      }
+    }
+    if (q == PHASE - 1) {
+      keep_digit(sh, ties, c);
+      if (PHASE < 3 && slab == 0 && tid == 0) state[q] = make_int2((int)sh.digit, sh.need);
+    } else {
+      if (tid == 0) {
+        const int2 x = state[q];
+        sh.digit = (uint32_t)x.x;
+        sh.need = x.y;
+      }
+      __syncthreads();
+    }
+    const uint32_t digit = sh.digit;
+    ties = sh.need;
+    thr |= digit << shift;
+    mask |= (q == 2 ? 1023u : 2047u) << shift;
+    if (PHASE == 3) {
+      int more = 0, same = 0, all_more, all_same;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t bin = (uint32_t)(kBins - 1 - 2 * tid - e);
+        more += bin > digit ? before[e] : 0;
+        same += q == 2 && bin == digit ? before[e] : 0;
+      }
+      keep_scan(sh, more, same, all_more, all_same);
+      gt0 += all_more;
+      eq0 += all_same;
+    }
+    __syncthreads();  // the digit is read before the next takes its place
+  }
+  uint32_t x[R];
+  keep_load<R>(turn, a, u, b, g, n, p0, x);
+  if (PHASE < 3) {
+    const int shift = PHASE == 0 ? 21 : (PHASE == 1 ? 10 : 0);
+    keep_clear(sh);
+    keep_count<R>(sh, x, mask, thr, shift);
+    int* out = hist + PHASE * phase_hist + (int64_t)slab * kBins;
+    for (int i = tid; i < kBins; i += kKeepThreads) {
+      int c = 0;
+#pragma unroll
+      for (int y = 0; y < kCopies; y += 4) {
+        const int4 z = *(const int4*)&sh.hist[i][y];
+        c += z.x + z.y + z.z + z.w;
+      }
+      out[i] = c;
+    }
+    return;
+  }
+  int gt = 0, eq = 0, all_gt, all_eq;
+#pragma unroll
+  for (int e = 0; e < R; ++e) {
+    gt += x[e] > thr;
+    eq += x[e] == thr;
+  }
+  keep_scan(sh, gt, eq, all_gt, all_eq);
+  const int first = gt0 + min(eq0, ties);                                  // kept before this slab,
+  const int mine = gt0 + all_gt + min(eq0 + all_eq, ties) - first;         // and in it
+  eq += eq0;
+  int rank = gt0 + gt + min(eq, ties) - first;
+#pragma unroll
+  for (int e = 0; e < R; ++e) {
+    const int i = tid * R + e;
+    const bool same = x[e] == thr;
+    const bool in = x[e] > thr || (same && eq < ties);
+    if (TABLE) {
+      if (p0 + i < n) turn.place[in ? rank : mine + (i - rank)] = p0 + i;
+    } else if (in) {
+      turn.place[rank] = p0 + i;
+    }
+    rank += in;
+    eq += same;
+  }
+  __syncthreads();
+  for (int j = tid; j < mine; j += kKeepThreads) kept[first + j] = turn.place[j];
+  if (TABLE) {
+    const int live = max(0, min(p1, n) - p0), rest = keep + (p0 - first) - mine;  // where what it gives up goes
+    for (int j = tid; j < live; j += kKeepThreads) new_table[j < mine ? first + j : rest + j] = table[turn.place[j]];
   }
 }
 
@@ -440,6 +470,21 @@ void launch_keep(const KeepArgs& a, dim3 grid, hipStream_t s) {
   else keep_kernel<R, false><<<grid, kKeepThreads, 0, s>>>(a);
 }
 
+int64_t keep_slabs(int64_t T) { return T > kSlab ? (T + kSlab - 1) / kSlab : 0; }
+
+template <bool TABLE>
+void launch_keep_slabs(const KeepArgs& a, int64_t units, hipStream_t s) {
+  const dim3 grid((unsigned)units, (unsigned)keep_slabs(a.T));
+  keep_slab_kernel<0, TABLE><<<grid, kKeepThreads, 0, s>>>(a);
+  keep_slab_kernel<1, TABLE><<<grid, kKeepThreads, 0, s>>>(a);
+  keep_slab_kernel<2, TABLE><<<grid, kKeepThreads, 0, s>>>(a);
+  keep_slab_kernel<3, TABLE><<<grid, kKeepThreads, 0, s>>>(a);
+}
+
+size_t summed_bytes(int64_t B, int64_t T, int shared) {
+  return shared ? ((size_t)B * (size_t)T * sizeof(uint32_t) + 15) / 16 * 16 : 0;
+}
+
 int check_keep(const char* who, const void* mass, int64_t B, int32_t Hkv, int64_t T, int64_t mass_sb, int64_t mass_sh,
                int32_t budget, int32_t window, int32_t sink, const void* kept, const void* new_lengths) {
   LSA_REQUIRE(mass && kept && new_lengths, LSA_ERR_NULL, "%s: NULL pointer", who);
@@ -455,8 +500,10 @@ int check_keep(const char* who, const void* mass, int64_t B, int32_t Hkv, int64_
 
 }  // namespace
 
-extern "C" size_t lsa_evict_scratch_bytes(int64_t B, int64_t T, int summed) {
-  return summed && B > 0 && T > 0 ? (size_t)B * (size_t)T * sizeof(uint32_t) : 0;
+extern "C" size_t lsa_evict_scratch_bytes(int64_t B, int32_t Hkv, int64_t T, int shared) {
+  if (B <= 0 || T <= 0 || Hkv <= 0) return 0;
+  const size_t units = (size_t)B * (shared ? 1 : Hkv), slabs = (size_t)keep_slabs(T);
+  return summed_bytes(B, T, shared) + units * (3 * slabs * kBins * sizeof(int) + (slabs ? 2 * sizeof(int2) : 0));
 }
 
 extern "C" int lsa_evict_keep(const float* mass, int64_t B, int32_t Hkv, int64_t T, int64_t mass_batch_stride,
@@ -471,9 +518,9 @@ extern "C" int lsa_evict_keep(const float* mass, int64_t B, int32_t Hkv, int64_t
   LSA_REQUIRE(table == nullptr || (shared && table_stride >= T && new_table_stride >= T && pool_rows >= 1),
               LSA_ERR_SHAPE, "lsa_evict_keep: a slot table needs shared selection, strides >= %lld and a pool",
               (long long)T);
-  const size_t need = lsa_evict_scratch_bytes(B, T, shared);
-  LSA_REQUIRE(need == 0 || (scratch && scratch_bytes >= need), LSA_ERR_WORKSPACE,
-              "lsa_evict_keep: scratch missing or %zu < %zu bytes", scratch_bytes, need);
+  const size_t need = lsa_evict_scratch_bytes(B, Hkv, T, shared);
+  LSA_REQUIRE(need == 0 || (scratch && scratch_bytes >= need && ((uintptr_t)scratch & 15) == 0), LSA_ERR_WORKSPACE,
+              "lsa_evict_keep: scratch missing, not 16-byte aligned or %zu < %zu bytes", scratch_bytes, need);
   if (B == 0) return LSA_OK;
   KeepArgs a = {};
   a.mass = mass; a.mass_sb = mass_batch_stride; a.mass_sh = mass_head_stride; a.lengths = lengths; a.T = T;
@@ -481,18 +528,22 @@ extern "C" int lsa_evict_keep(const float* mass, int64_t B, int32_t Hkv, int64_t
   a.kept = kept; a.new_lengths = new_lengths; a.table = table; a.table_stride = table_stride;
   a.new_table = new_table; a.new_stride = new_table_stride; a.pool = pool_rows;
   hipStream_t s = (hipStream_t)stream;
+  a.hist = (int*)((char*)scratch + summed_bytes(B, T, shared));
+  a.state = (int2*)(a.hist + 3 * B * a.G * keep_slabs(T) * kBins);
   if (shared) {
     a.keys = a.keys_out = (uint32_t*)scratch;
     const dim3 grid((unsigned)((T + LSA_BLOCK - 1) / LSA_BLOCK), (unsigned)B);
     seen_keys_kernel<<<grid, LSA_BLOCK, 0, s>>>(a);
     LSA_LAUNCHED("lsa_evict_keep");
   }
-  const dim3 grid((unsigned)(B * a.G));
+  const int64_t units = B * a.G;
+  const dim3 grid((unsigned)units);
   if (T <= 4 * kKeepThreads) launch_keep<4>(a, grid, s);
   else if (T <= 8 * kKeepThreads) launch_keep<8>(a, grid, s);
   else if (T <= 16 * kKeepThreads) launch_keep<16>(a, grid, s);
   else if (T <= 32 * kKeepThreads) launch_keep<32>(a, grid, s);
-  else keep_long_kernel<<<grid, kKeepThreads, 0, s>>>(a);
+  else if (a.table) launch_keep_slabs<true>(a, units, s);
+  else launch_keep_slabs<false>(a, units, s);
   LSA_LAUNCHED("lsa_evict_keep");
   return LSA_OK;
 }

@@ -112,7 +112,7 @@ SIGNATURES = {
     "lsa_key_mass_scratch_bytes": (_sz, [_int, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32]),
     "lsa_key_mass": (_int, [_p, _p, _int, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _i64, _p, _p, _i32,
                             _int, _f32, _p, _int, _p, _sz, _p, _i64, _i64, _p]),
-    "lsa_evict_scratch_bytes": (_sz, [_i64, _i64, _int]),
+    "lsa_evict_scratch_bytes": (_sz, [_i64, _i32, _i64, _int]),
     "lsa_evict_keep": (_int, [_p, _i64, _i32, _i64, _i64, _i64, _p, _i32, _i32, _i32, _int, _p, _i64, _i64, _p, _sz, _p,
                               _p, _p, _i64, _p]),
     "lsa_evict_rows": (_int, [_p, _p, _p, _int, _i64, _i64, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _p, _int, _i32,

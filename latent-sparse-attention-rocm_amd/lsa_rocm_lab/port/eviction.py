@@ -187,7 +187,7 @@ def evict(
     new_lengths = torch.empty(B, dtype=torch.int32, device=device)
     if B:
         one = 1 if shared else 0
-        nbytes = _abi.shape_size("lsa_evict_scratch_bytes", B, T, one)
+        nbytes = _abi.shape_size("lsa_evict_scratch_bytes", B, Hkv, T, one)
         with launch_device(device):
             ws = _abi.scratch(device, "evict", nbytes)
             stream = _abi.stream(device)
@@ -237,7 +237,7 @@ def evict_slots(
     kept = torch.empty(R, budget, dtype=torch.int32, device=device)
     new_lengths = torch.empty(R, dtype=torch.int32, device=device)
     if R:
-        nbytes = _abi.shape_size("lsa_evict_scratch_bytes", R, T, 1)
+        nbytes = _abi.shape_size("lsa_evict_scratch_bytes", R, Hkv, T, 1)
         with launch_device(device):
             ws = _abi.scratch(device, "evict", nbytes)
             _abi.call("lsa_evict_keep", mass.data_ptr(), R, Hkv, T, 0, mass.stride(1), _abi.ptr(lens), budget, window,

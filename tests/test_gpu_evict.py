@@ -193,6 +193,9 @@ EVICT = [
     (4, 3000, 2, 128, torch.bfloat16, 700, 700, 0),
     (2, 5000, 8, 96, torch.bfloat16, 1234, 64, 64),
     (1, 40000, 2, 64, torch.float16, 20000, 512, 4),
+    (2, 32769, 2, 32, torch.bfloat16, 32768, 1, 0),
+    (2, 100001, 3, 32, torch.bfloat16, 33000, 32800, 70),
+    (3, 70000, 1, 32, torch.float16, 40000, 0, 33000),
 ]
 
 
@@ -243,7 +246,8 @@ def test_evict(case, shared):
 
 
 @pytest.mark.parametrize("R,T,Hkv,budget,window,sink", [(1, 1, 1, 1, 0, 0), (3, 700, 2, 100, 20, 4), (2, 1024, 8, 1023, 0, 1),
-                                                        (4, 5000, 3, 2000, 512, 4), (2, 33000, 2, 9000, 0, 0)])
+                                                        (4, 5000, 3, 2000, 512, 4), (2, 33000, 2, 9000, 0, 0),
+                                                        (3, 98304, 2, 50000, 512, 4), (2, 70001, 1, 1, 0, 0)])
 def test_evict_slots(R, T, Hkv, budget, window, sink):
     rng = np.random.default_rng(T)
     pool = R * T + 50
@@ -269,6 +273,25 @@ def test_evict_slots(R, T, Hkv, budget, window, sink):
         at = keep(seen, n, budget, window, sink)
         assert n2[r] == len(at) and kept[r].tolist() == at + [-1] * (budget - len(at))
         assert np.array_equal(new[r], np.concatenate([table[r, at], np.delete(table[r, :n], at), table[r, n:]]))
+
+
+@pytest.mark.parametrize("T", [3000, 70000])
+@pytest.mark.parametrize("kind", ["equal", "nan", "zero and one"])
+def test_evict_of_ties_alone(T, kind):
+    """All masses the same, none a number, or two values: the lower positions of the heavier ones."""
+    m = torch.zeros(2, 2, T)
+    if kind == "nan":
+        m += math.nan
+    if kind == "zero and one":
+        m[:, :, T // 2:] = 1.0
+    k = torch.zeros(2, T, 2, 32, dtype=torch.bfloat16, device=DEV)
+    budget = T // 3
+    lens = torch.tensor([T, T - 7], dtype=torch.int32, device=DEV)
+    for shared in (False, True):
+        kept = pipeline.evict(k, k, m.to(DEV), budget, lens, window=5, sink=2, shared=shared)[3].cpu()
+        for b, n in enumerate((T, T - 7)):
+            at = keep(m[b, 0].tolist(), n, budget, 5, 2)
+            assert (kept[b] if shared else kept[b, 1]).tolist() == at
 
 
 def test_evict_of_views_and_in_a_graph():

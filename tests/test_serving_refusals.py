@@ -88,9 +88,11 @@ def test_evict_keep_abi(over, match):
 
 
 def test_evict_scratch():
-    assert _abi.size("lsa_evict_scratch_bytes", 3, 100, 1) == 1200 and _abi.size("lsa_evict_scratch_bytes", 3, 100, 0) == 0
-    with pytest.raises(_abi.LsaError, match="scratch"):
-        keep(shared=1, nbytes=799)
+    size = lambda *a: _abi.size("lsa_evict_scratch_bytes", *a)  # noqa: E731
+    assert size(3, 2, 100, 1) == 1200 and size(3, 2, 100, 0) == 0 and size(3, 2, 32768, 0) == 0 < size(3, 2, 32769, 0)
+    for over in (dict(nbytes=799), dict(ws=None), dict(ws=P + 8)):
+        with pytest.raises(_abi.LsaError, match="scratch"):
+            keep(shared=1, **over)
 
 
 def rows(**over):
