@@ -465,15 +465,18 @@ int lsa_prefix_read(const void* q, const void* k_prefix, const void* v_prefix, i
  * those of the softmax over the row's own list, or exp(score - lse) with lse [B, Tq, Hq] (a
  * wider softmax's, as lsa_prefix_read gives it; -inf and NaN: no weight). A softmax whose sum
  * is not a number gives none. The result does not depend on the order in which workgroups run.
- * zero_first != 0: mass (dense) begins at zero. No counterpart in the reference. scratch:
+ * zero_first != 0: mass (dense) begins at zero. counters (or NULL): B * Tq * Hkv int32 that read
+ * zero at launch and are left zero; with one query row a cache they make the call one launch instead
+ * of two. No counterpart in the reference. scratch:
  * lsa_key_mass_scratch_bytes(), 16-byte aligned, no initialisation. */
 size_t lsa_key_mass_scratch_bytes(int dtype, int64_t B, int64_t Tq, int64_t caches, int64_t Tk, int32_t Hq, int32_t Hkv,
                                   int32_t D, int32_t W);
 int lsa_key_mass(const void* q, const void* k, int dtype, int64_t B, int64_t Tq, int64_t caches, int64_t Tk,
                  int32_t Hq, int32_t Hkv, int32_t D, int64_t k_batch_stride, int64_t k_token_stride,
                  int64_t k_head_stride, const int32_t* ids, const int32_t* lengths, int32_t W, int ids_per_head,
-                 float scale, const float* lse, int zero_first, void* scratch, size_t scratch_bytes, float* mass,
-                 int64_t mass_batch_stride, int64_t mass_head_stride, void* stream);
+                 float scale, const float* lse, int zero_first, int32_t* counters, void* scratch,
+                 size_t scratch_bytes, float* mass, int64_t mass_batch_stride, int64_t mass_head_stride,
+                 void* stream);
 
 /* Which positions of a cache to keep. mass [B, Hkv, T] fp32 (element strides, positions
  * contiguous). Of row b's lengths[b] positions (NULL: T) the first `sink` and the last `window`

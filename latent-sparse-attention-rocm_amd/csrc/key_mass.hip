@@ -7,7 +7,10 @@
 //
 //   mass_scores_kernel  gathers the listed K rows and leaves their scores and each span's
 //                       (maximum, sum) a head;
-//   mass_add_kernel     turns the scores into weights and adds them.
+//   mass_add_kernel     turns the scores into weights and adds them. With one query row a cache the last span
+//                       of a list to finish does that within the first launch, if it has counters
+//                       to tell which that is (a launch costs the host 3 us, as much as the rest of a small
+//                       call).
 //
 // A key that a list names twice counts twice; several query rows of one cache add to the same
 // keys. Sums must not depend on the order in which workgroups arrive. With one query row a cache, all
@@ -47,9 +50,22 @@ struct MassArgs {
   int64_t m_sb, m_sh;     // batch stride 0: one pool for every batch row
   int64_t m_n;            // caches * Hkv * Tk (zero: fresh weights are written whole)
   int caches;
+  int* counters;          // one launch: arrivals of a unit's spans, zero before and after; or nullptr
   int zero;               // the weights begin at zero
   uint64_t* fixed;        // [caches, Hkv, Tk] or nullptr
   int whole;              // fixed is cleared and folded whole, not by the lists
+};
+
+// 16 bytes written through (visible to the workgroup that adds), from a workgroup-uniform base
+struct CoherentOut {
+  __amdgpu_buffer_rsrc_t rsrc;
+  __device__ __forceinline__ explicit CoherentOut(float* base)
+      : rsrc(__builtin_amdgcn_make_buffer_rsrc(base, 0, 0x7FFFFFFF, 0x00020000)) {}
+  __device__ __forceinline__ void store4(int byte_offset, const float (&x)[4]) const {
+    typedef int i4v __attribute__((ext_vector_type(4)));
+    const i4v v = {__float_as_int(x[0]), __float_as_int(x[1]), __float_as_int(x[2]), __float_as_int(x[3])};
+    __builtin_amdgcn_raw_buffer_store_b128(v, rsrc, byte_offset, 0, 16 /* sc1 */);
+  }
 };
 
 struct MassList {
@@ -69,6 +85,52 @@ __device__ __forceinline__ void join(float& m, float& l, float mo, float lo) {
   const float mn = fmaxf(m, mo);
   l = l * fast_exp2(m - mn) + lo * fast_exp2(mo - mn);
   m = mn;
+}
+
+// What the unit's weights are measured by, a head a thread: the reference m and one over the sum.
+template <int GQ, bool COHERENT>
+__device__ __forceinline__ void weigh_by(const MassArgs& a, int64_t unit, int64_t row, int g, const MassList& list,
+                                         float* sm, float* sinv) {
+  const int tid = threadIdx.x;
+  if (tid >= GQ) return;
+  float m = kNegBig, l = 0.0f;
+  if (a.lse) {
+    m = a.lse[row * a.Hq + g * GQ + tid] * kLog2e;
+    l = m > -INFINITY ? 1.0f : 0.0f;  // no keys at all, or not a number: no weight
+  } else {
+    const int n_act = (list.n + a.span - 1) / a.span;
+#pragma unroll 4
+    for (int s = 0; s < n_act; ++s) {
+      const float* st = a.stats + ((unit * a.n_span + s) * GQ + tid) * 2;
+      if constexpr (COHERENT) join(m, l, coherent_load(st), coherent_load(st + 1));
+      else join(m, l, st[0], st[1]);
+    }
+  }
+  sm[tid] = m;
+  sinv[tid] = l > 0.0f ? 1.0f / l : 0.0f;  // a sum that is not a number counts as none, as in the read
+}
+
+// Slot j's weight, the heads together.
+template <int GQ, bool COHERENT>
+__device__ __forceinline__ float weight_of(const float* scores, int64_t j, const float* sm, const float* sinv) {
+  float s[GQ];
+  if constexpr (COHERENT && GQ % 4 == 0) {
+#pragma unroll
+    for (int h = 0; h < GQ; h += 4) {
+      const float4 x = CoherentRows(scores).load4(4 * ((int)j * GQ + h));
+      s[h] = x.x; s[h + 1] = x.y; s[h + 2] = x.z; s[h + 3] = x.w;
+    }
+  } else {
+#pragma unroll
+    for (int h = 0; h < GQ; ++h) s[h] = COHERENT ? coherent_load(scores + j * GQ + h) : scores[j * GQ + h];
+  }
+  float sum = 0.0f;
+#pragma unroll
+  for (int h = 0; h < GQ; ++h) {
+    const float x = fast_exp2(s[h] - sm[h]) * sinv[h];
+    sum += sinv[h] > 0.0f && x > 0.0f ? fminf(x, kMaxWeight) : 0.0f;
+  }
+  return sum;
 }
 
 typedef uint32_t raw_t __attribute__((ext_vector_type(4)));  // 16 bytes of a row, kept in registers
@@ -104,7 +166,17 @@ void mass_scores_kernel(MassArgs a) {
   const int sp = blockIdx.y;
   const int64_t row = unit / a.Hkv;
   const int g = (int)(unit % a.Hkv);
-  if (a.zero || a.whole) {  // this workgroup's share of the weights, and of the integers
+  const MassList list = mass_list(a, row, g);
+  const int lo = sp * a.span, hi = min(lo + a.span, list.n);
+  const int n_act = (list.n + a.span - 1) / a.span;
+  if (a.counters) {
+    if (sp >= max(n_act, 1)) return;
+    if (a.zero) {  // this span's share of the unit's own weights, which no other unit adds to
+      float* m = a.mass + (a.caches > 1 ? row / a.Tq : 0) * a.m_sb + g * a.m_sh;
+      const int64_t share = (a.Tk + max(n_act, 1) - 1) / max(n_act, 1), k1 = min(share * (sp + 1), a.Tk);
+      for (int64_t i = share * sp + tid; i < k1; i += LSA_BLOCK) coherent_store(m + i, 0.0f);
+    }
+  } else if (a.zero || a.whole) {  // this workgroup's share of the weights, and of the integers
     const int64_t grid = (int64_t)gridDim.x * gridDim.y * LSA_BLOCK;
     const int64_t at = ((int64_t)sp * gridDim.x + unit) * LSA_BLOCK + tid;
     if (a.zero) {
@@ -114,8 +186,6 @@ void mass_scores_kernel(MassArgs a) {
       for (int64_t i = at; i < a.m_n; i += grid) a.fixed[i] = 0;
     }
   }
-  const MassList list = mass_list(a, row, g);
-  const int lo = sp * a.span, hi = min(lo + a.span, list.n);
   if (lo >= hi) return;
   const int64_t b = row / a.Tq;
   const int64_t c = a.caches > 1 ? b : 0;
@@ -226,9 +296,23 @@ void mass_scores_kernel(MassArgs a) {
       for (int u = 0; u < U; ++u) {
         const int j = slot(base, u);
         if (j < hi) {
-          float* to = scores + (int64_t)j * GQ + (S::MM ? HL * rowq : 0);
+          const int h0 = S::MM ? HL * rowq : 0;
+          if (a.counters) {
+            if constexpr (HL % 4 == 0) {
 #pragma unroll
-          for (int h = 0; h < HL; ++h) to[h] = s[u][h];
+              for (int h = 0; h < HL; h += 4) {
+                const float x[4] = {s[u][h], s[u][h + 1], s[u][h + 2], s[u][h + 3]};
+                CoherentOut(scores).store4(4 * (j * GQ + h0 + h), x);
+              }
+            } else {
+#pragma unroll
+              for (int h = 0; h < HL; ++h) coherent_store(scores + (int64_t)j * GQ + h0 + h, s[u][h]);
+            }
+          } else {
+            float* to = scores + (int64_t)j * GQ + h0;
+#pragma unroll
+            for (int h = 0; h < HL; ++h) to[h] = s[u][h];
+          }
         }
       }
     }
@@ -253,8 +337,25 @@ void mass_scores_kernel(MassArgs a) {
 #pragma unroll
     for (int x = 1; x < LSA_WAVES; ++x) join(mm, ll, sm[x][tid], sl[x][tid]);
     float* st = a.stats + ((unit * a.n_span + sp) * GQ + tid) * 2;
-    st[0] = mm;
-    st[1] = ll;
+    if (a.counters) {
+      coherent_store(st, mm);
+      coherent_store(st + 1, ll);
+    } else {
+      st[0] = mm;
+      st[1] = ll;
+    }
+  }
+  if (!a.counters) return;
+  __shared__ int flag;
+  __shared__ float wm[GQ], winv[GQ];
+  if (!arrive_last(&a.counters[unit], n_act, &flag)) return;
+  weigh_by<GQ, true>(a, unit, row, g, list, wm, winv);
+  __syncthreads();
+  float* mass = a.mass + c * a.m_sb + g * a.m_sh;
+  for (int j = tid; j < list.n; j += LSA_BLOCK) {
+    const int32_t id = list.ids[j];
+    const float sum = weight_of<GQ, true>(scores, j, wm, winv);
+    if (id >= 0 && id < a.Tk && sum > 0.0f) atomicAdd(mass + id, sum);
   }
 }
 
@@ -269,32 +370,12 @@ __global__ __launch_bounds__(LSA_BLOCK) void mass_add_kernel(MassArgs a) {
   const MassList list = mass_list(a, row, g);
   const int j = blockIdx.y * LSA_BLOCK + tid;
   if (blockIdx.y * LSA_BLOCK >= list.n) return;
-  if (tid < GQ) {
-    float m = kNegBig, l = 0.0f;
-    if (a.lse) {
-      m = a.lse[row * a.Hq + g * GQ + tid] * kLog2e;
-      l = m > -INFINITY ? 1.0f : 0.0f;  // no keys at all, or not a number: no weight
-    } else {
-      const int n_act = (list.n + a.span - 1) / a.span;
-      for (int s = 0; s < n_act; ++s) {
-        const float* st = a.stats + ((unit * a.n_span + s) * GQ + tid) * 2;
-        join(m, l, st[0], st[1]);
-      }
-    }
-    sm[tid] = m;
-    sinv[tid] = l > 0.0f ? 1.0f / l : 0.0f;  // a sum that is not a number counts as none, as in the read
-  }
+  weigh_by<GQ, false>(a, unit, row, g, list, sm, sinv);
   __syncthreads();
   if (j >= list.n) return;
   const int32_t id = list.ids[j];
   if (id < 0 || id >= a.Tk) return;
-  const float* s = a.scores + (unit * (int64_t)a.W + j) * GQ;
-  float sum = 0.0f;
-#pragma unroll
-  for (int h = 0; h < GQ; ++h) {
-    const float x = fast_exp2(s[h] - sm[h]) * sinv[h];
-    sum += sinv[h] > 0.0f && x > 0.0f ? fminf(x, kMaxWeight) : 0.0f;
-  }
+  const float sum = weight_of<GQ, false>(a.scores + unit * (int64_t)a.W * GQ, j, sm, sinv);
   if (!(sum > 0.0f)) return;
   const int64_t b = row / a.Tq;
   const int64_t c = a.caches > 1 ? b : 0;
@@ -405,8 +486,8 @@ extern "C" size_t lsa_key_mass_scratch_bytes(int dtype, int64_t B, int64_t Tq, i
 extern "C" int lsa_key_mass(const void* q, const void* k, int dtype, int64_t B, int64_t Tq, int64_t caches, int64_t Tk,
                             int32_t Hq, int32_t Hkv, int32_t D, int64_t k_batch_stride, int64_t k_token_stride,
                             int64_t k_head_stride, const int32_t* ids, const int32_t* lengths, int32_t W,
-                            int ids_per_head, float scale, const float* lse, int zero_first, void* scratch,
-                            size_t scratch_bytes, float* mass, int64_t mass_batch_stride, int64_t mass_head_stride,
+                            int ids_per_head, float scale, const float* lse, int zero_first, int32_t* counters,
+                            void* scratch, size_t scratch_bytes, float* mass, int64_t mass_batch_stride, int64_t mass_head_stride,
                             void* stream) {
   LSA_REQUIRE(q && k && ids && lengths && mass, LSA_ERR_NULL, "lsa_key_mass: NULL pointer");
   LSA_TRY(check_dtype(dtype));
@@ -438,6 +519,8 @@ extern "C" int lsa_key_mass(const void* q, const void* k, int dtype, int64_t B, 
   a.fixed = p.fixed ? (uint64_t*)((char*)scratch + p.scores + p.stats) : nullptr;
   a.whole = p.whole ? 1 : 0;
   a.mass = mass; a.m_sb = caches > 1 ? mass_batch_stride : 0; a.m_sh = mass_head_stride;
+  // offsets within a unit's scores are 32 bits of bytes
+  a.counters = !p.fixed && (int64_t)W * (Hq / Hkv) * 4 <= 0x7FFFFFFF ? counters : nullptr;
   a.m_n = caches * Hkv * Tk; a.caches = (int)caches; a.zero = zero_first ? 1 : 0;
   hipStream_t s = (hipStream_t)stream;
   const int gq = Hq / Hkv;
@@ -446,6 +529,7 @@ extern "C" int lsa_key_mass(const void* q, const void* k, int dtype, int64_t B, 
   else if (dtype == LSA_F16) launch_scores_d<_Float16>(a, D, gq, grid, s);
   else launch_scores_d<float>(a, D, gq, grid, s);
   LSA_LAUNCHED("lsa_key_mass");
+  if (a.counters) return LSA_OK;
   const dim3 add((unsigned)units, (unsigned)chunks);
   switch (gq) {
     case 1: mass_add_kernel<1><<<add, LSA_BLOCK, 0, s>>>(a); break;

@@ -111,7 +111,7 @@ SIGNATURES = {
                                _p]),
     "lsa_key_mass_scratch_bytes": (_sz, [_int, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32]),
     "lsa_key_mass": (_int, [_p, _p, _int, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _i64, _p, _p, _i32,
-                            _int, _f32, _p, _int, _p, _sz, _p, _i64, _i64, _p]),
+                            _int, _f32, _p, _int, _p, _p, _sz, _p, _i64, _i64, _p]),
     "lsa_evict_scratch_bytes": (_sz, [_i64, _i32, _i64, _int]),
     "lsa_evict_keep": (_int, [_p, _i64, _i32, _i64, _i64, _i64, _p, _i32, _i32, _i32, _int, _p, _i64, _i64, _p, _sz, _p,
                               _p, _p, _i64, _p]),
@@ -265,6 +265,12 @@ def scratch(device: torch.device, purpose: str, nbytes: int) -> torch.Tensor | N
     if nbytes > 0 and torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     return Workspace.get(device, purpose, nbytes)
+
+
+def counters(device: torch.device, n: int) -> torch.Tensor | None:
+    """Counters of one call, or None while a HIP graph is captured: ``Counters``' belong to the
+    stream, and graphs that hold them must not be replayed on several at once."""
+    return None if torch.cuda.is_current_stream_capturing() else Counters.get(device, n)
 
 
 class Counters:

@@ -89,9 +89,10 @@ def key_mass(
                 plse = None if lse is None else lse[:, t:t + n].contiguous()
             nbytes = _abi.shape_size("lsa_key_mass_scratch_bytes", dt, B, n, caches, Tk, Hq, Hkv, D, W)
             ws = _abi.scratch(device, "key_mass", nbytes)
+            counters = _abi.counters(device, B * Hkv) if n == 1 and caches == B else None
             _abi.call("lsa_key_mass", part.data_ptr(), k.data_ptr(), dt, B, n, caches, Tk, Hq, Hkv, D, sb, st, sh,
                       pids.data_ptr(), plens.data_ptr(), W, 1 if per_head else 0, scale, _abi.ptr(plse),
-                      1 if fresh and t == 0 else 0, _abi.ptr(ws), nbytes, mass.data_ptr(),
+                      1 if fresh and t == 0 else 0, _abi.ptr(counters), _abi.ptr(ws), nbytes, mass.data_ptr(),
                       mass.stride(0) if caches > 1 else Hkv * Tk, mass.stride(1) if Hkv > 1 else Tk,
                       _abi.stream(device))
     return mass

@@ -41,7 +41,7 @@ def test_prefix_read_needs_its_scratch():
 
 def mass(**over):
     a = dict(q=P, k=P, dt=BF16, B=2, Tq=1, caches=2, Tk=32, Hq=8, Hkv=2, D=128, sb=8192, st=256, sh=128, ids=P, lens=P, W=4,
-             per=0, scale=0.1, lse=None, zero=0, ws=P, nbytes=1 << 40, mass=P, mb=64, mh=32, stream=None)
+             per=0, scale=0.1, lse=None, zero=0, counters=None, ws=P, nbytes=1 << 40, mass=P, mb=64, mh=32, stream=None)
     a.update(over)
     return _abi.call("lsa_key_mass", *a.values())
 
