@@ -445,8 +445,10 @@ int lsa_decode_flat_noalloc(const void* q, const void* k, const void* v, int dty
  * none where it is outside [0, P)). The own part as lsa_read (W == 0: none; k, v, ids and
  * lengths may be NULL then). A row without any key gives zeros. lse (NULL: not wanted) [B, Tq,
  * Hq] fp32: the natural logarithm of the softmax's sum, -inf for a row without keys.
- * scratch: lsa_prefix_read_scratch_bytes(), 16-byte aligned, no initialisation; nothing of it
- * is needed after the call's kernels. */
+ * counters (or NULL): B * Tq * Hkv int32 that read zero at launch and are left zero; where the
+ * matrix cores do not serve they make the call one launch instead of two. scratch:
+ * lsa_prefix_read_scratch_bytes(), 16-byte aligned, no initialisation; nothing of it is needed
+ * after the call's kernels. */
 size_t lsa_prefix_read_scratch_bytes(int dtype, int64_t B, int64_t Tq, int64_t P, int64_t Tp, int32_t Hq, int32_t Hkv,
                                      int32_t D, int32_t W);
 int lsa_prefix_read(const void* q, const void* k_prefix, const void* v_prefix, int dtype, int64_t B, int64_t Tq,
@@ -455,8 +457,8 @@ int lsa_prefix_read(const void* q, const void* k_prefix, const void* v_prefix, i
                     const int32_t* prefix_rows, const int32_t* prefix_lengths, const int32_t* prefix_slots,
                     int64_t prefix_slot_stride, const void* k, const void* v, int64_t Tk, int64_t kv_batch_stride,
                     int64_t kv_token_stride, int64_t kv_head_stride, const int32_t* ids, const int32_t* lengths,
-                    int32_t W, int ids_per_head, float scale, void* scratch, size_t scratch_bytes, void* out,
-                    float* lse, void* stream);
+                    int32_t W, int ids_per_head, float scale, int32_t* counters, void* scratch, size_t scratch_bytes,
+                    void* out, float* lse, void* stream);
 
 /* Adds to mass [caches, Hkv, Tk] (fp32, element strides, keys contiguous) the softmax weight
  * that each listed key receives from batch row b's query rows, summed over them and over the

@@ -4,10 +4,10 @@
 // The softmax over both parts is one: each part leaves partials (running maximum m, sum l and
 // weighted value row, in fp32, log2 domain), and the usual rescaling joins them.
 //
-//   prefix_mfma_kernel    (prefix_mfma.hip) a prefix's partials for 32 to 128 query columns at
-//                         once, 16-bit rows of head dim 64 or 128;
-//   prefix_gather_kernel  a prefix's partials row by row (any type and head dim);
-//   prefix_join_kernel    a row's own list (the gather read's span loop) and the join.
+//   prefix_mfma_kernel,  (prefix_mfma.hip) a prefix's partials for up to 256 query columns at once,
+//   prefix_wide_kernel   16-bit rows of head dim 64 or 128;
+//   prefix_rows_kernel   row by row with the gather read's span loop: the pieces of a prefix (any type and
+//                        head dim), a row's own list, and the join, by the last of a unit to finish.
 //
 // A prefix of n keys is cut into pieces of whole 64-key tiles, a workgroup a piece, the same for
 // all of them (prefix_pieces). Partials of (row, kv-head) unit i: piece s of n_p at
@@ -23,80 +23,56 @@ using namespace lsa;
 
 namespace {
 
-// grid (row * Hkv, piece).
+// grid (row * Hkv, span): spans [0, splits) are the pieces of the row's prefix, the rest its own list's.
+enum Arrive { kNone, kOwn, kAll };  // whose arrival the join waits for (kNone: another launch joins)
 template <typename T, int D, int GQ>
-__global__ __launch_bounds__(LSA_BLOCK) void prefix_gather_kernel(PrefixArgs a) {
+__global__ __launch_bounds__(LSA_BLOCK) void prefix_rows_kernel(PrefixArgs a, int first, int arrive) {
   __shared__ ReadLds<D, GQ, kMaxPieces + kMaxOwn> sh;
   constexpr int PSTRIDE = GQ * (D + 2);
   const int64_t i = blockIdx.x, row = i / a.Hkv;
-  const int g = (int)(i % a.Hkv), s = blockIdx.y;
-  if (s == 0 && threadIdx.x == 0) a.counters[i] = 0;
-  const int p = prefix_of(a, row / a.Tq);
-  const Pieces pc = prefix_pieces(a, p);
-  if (s >= pc.count) return;
-  const int lo = s * pc.keys, hi = min(lo + pc.keys, pc.n);
-  const int lp = (threadIdx.x & (LSA_WAVE - 1)) % ReadShape<T, D, GQ>::LPT;
-  const int64_t at = (a.slots ? 0 : p * a.p_sb) + g * a.p_sh + lp * ReadShape<T, D, GQ>::VEC;
-  const int32_t* slots = a.slots ? a.slots + p * a.slot_stride : nullptr;
-  AttnState<T, D, GQ> st;
-  attend_span<T, D, GQ, true>((const T*)a.q + (row * a.Hq + (int64_t)g * GQ) * D, (const T*)a.kp + at, (const T*)a.vp + at,
-                        a.p_st, a.pool, lo, hi,
-                        [&](int j) {
-                          const int jc = j < hi ? j : hi - 1;
-                          const int32_t id = slots ? slots[jc] : jc;
-                          return j < hi ? id : -1;
-                        },
-                        a.scale_log2, st);
-  float* part = a.parts + (i * (a.splits + a.own_splits) + a.splits - pc.count + s) * (int64_t)PSTRIDE;
-  finish_span<T, D, GQ, kMaxPieces + kMaxOwn, true>(sh, st, false, (T*)nullptr, part, 0);
-  if (a.lse && threadIdx.x < GQ) {  // weights are fp32 here: one sum serves both
-    float m = kNegBig, l = 0.0f;
-#pragma unroll
-    for (int w = 0; w < LSA_WAVES; ++w) m = fmaxf(m, sh.m[w][threadIdx.x]);
-#pragma unroll
-    for (int w = 0; w < LSA_WAVES; ++w) l += sh.l[w][threadIdx.x] * fast_exp2(sh.m[w][threadIdx.x] - m);
-    a.sums[(i * a.splits + a.splits - pc.count + s) * GQ + threadIdx.x] = l;
-  }
-}
-
-// grid (row * Hkv, own span). The last span of a unit to arrive joins the unit's partials.
-template <typename T, int D, int GQ>
-__global__ __launch_bounds__(LSA_BLOCK) void prefix_join_kernel(PrefixArgs a) {
-  __shared__ ReadLds<D, GQ, kMaxPieces + kMaxOwn> sh;
-  constexpr int PSTRIDE = GQ * (D + 2);
-  const int64_t i = blockIdx.x, row = i / a.Hkv;
-  const int g = (int)(i % a.Hkv), s = blockIdx.y;
+  const int g = (int)(i % a.Hkv), s = (int)blockIdx.y + first;
   const int64_t b = row / a.Tq;
+  if (arrive == kNone && s == 0 && threadIdx.x == 0) a.counters[i] = 0;
+  const bool piece = s < a.splits;
+  const int p = prefix_of(a, b);
+  const Pieces pc = prefix_pieces(a, p);
   int n = 0;
-  const int32_t* list = nullptr;
-  if (a.W > 0) {
+  const int32_t* ids = nullptr;  // the keys' rows (a prefix's own order without)
+  if (a.W > 0 && !(arrive == kNone && piece)) {
     const int64_t li = a.per_head ? row * a.Hkv + g : row;
     n = a.lengths[li];
     n = (n < 0 || a.Tk <= 0) ? 0 : (n > a.W ? a.W : n);
-    list = a.ids + li * a.W;
+    ids = a.ids + li * a.W;
   }
-  const int n_own = (n + a.own_span - 1) / a.own_span;
-  if (s >= max(n_own, 1)) return;
-  const Pieces pc = prefix_pieces(a, prefix_of(a, b));
+  const int n_own = (n + a.own_span - 1) / a.own_span, total = pc.count + n_own;
+  const int at = piece ? s : s - a.splits;
+  const bool active = at < (piece ? pc.count : n_own);
   float* parts = a.parts + (i * (a.splits + a.own_splits) + a.splits - pc.count) * (int64_t)PSTRIDE;
-  if (n > 0) {
-    const int lo = s * a.own_span, hi = min(lo + a.own_span, n);
+  if (!active) {  // a unit without spans to wait for still joins: its first workgroup
+    if (arrive == kNone || blockIdx.y != 0 || (arrive == kAll ? total : n_own) > 0) return;
+  } else {
+    const int span = piece ? pc.keys : a.own_span;
+    const int lo = at * span, hi = min(lo + span, piece ? pc.n : n);
     const int lp = (threadIdx.x & (LSA_WAVE - 1)) % ReadShape<T, D, GQ>::LPT;
-    const int64_t at = b * a.kv_sb + g * a.kv_sh + lp * ReadShape<T, D, GQ>::VEC;
+    if (piece) ids = a.slots ? a.slots + p * a.slot_stride : nullptr;
+    const int64_t off = (piece ? (a.slots ? 0 : p * a.p_sb) + g * a.p_sh : b * a.kv_sb + g * a.kv_sh) +
+                        lp * ReadShape<T, D, GQ>::VEC;
     AttnState<T, D, GQ> st;
-    attend_span<T, D, GQ, true>((const T*)a.q + (row * a.Hq + (int64_t)g * GQ) * D, (const T*)a.k + at, (const T*)a.v + at,
-                          a.kv_st, a.Tk, lo, hi,
-                          [&](int j) {
-                            const int32_t id = list[j < hi ? j : hi - 1];
-                            return j < hi ? id : -1;
-                          },
-                          a.scale_log2, st);
+    attend_span<T, D, GQ, true>((const T*)a.q + (row * a.Hq + (int64_t)g * GQ) * D,
+                                (const T*)(piece ? a.kp : a.k) + off, (const T*)(piece ? a.vp : a.v) + off,
+                                piece ? a.p_st : a.kv_st, piece ? a.pool : a.Tk, lo, hi,
+                                [&](int j) {
+                                  const int jc = j < hi ? j : hi - 1;
+                                  const int32_t id = ids ? ids[jc] : jc;
+                                  return j < hi ? id : -1;
+                                },
+                                a.scale_log2, st);
     finish_span<T, D, GQ, kMaxPieces + kMaxOwn, true>(sh, st, false, (T*)nullptr,
-                                                      parts + (int64_t)(pc.count + s) * PSTRIDE, 0);
+                                                      parts + (int64_t)(piece ? at : pc.count + at) * PSTRIDE, 0);
+    if (arrive == kNone) return;
     // the partials complete before they are read back, by this workgroup or the last one
-    if (!arrive_last(&a.counters[i], n_own, &sh.flag)) return;
+    if (!arrive_last(&a.counters[i], arrive == kAll ? total : n_own, &sh.flag)) return;
   }
-  const int total = pc.count + n_own;
   T* outp = (T*)a.out + (row * a.Hq + (int64_t)g * GQ) * D;
   if (total == 0) {
     for (int j = threadIdx.x; j < GQ * D; j += LSA_BLOCK) store_out<T>(outp + j, 0.0f);
@@ -105,14 +81,14 @@ __global__ __launch_bounds__(LSA_BLOCK) void prefix_join_kernel(PrefixArgs a) {
   }
   if (a.lse) {
     const int lane = threadIdx.x & (LSA_WAVE - 1);
-    const float* sums = a.sums + (i * a.splits + a.splits - pc.count) * GQ;
+    const float* sums = a.sums ? a.sums + (i * a.splits + a.splits - pc.count) * GQ : nullptr;
     for (int h = threadIdx.x / LSA_WAVE; h < GQ; h += LSA_WAVES) {
       float M = kNegBig, L = 0.0f;
       for (int x = lane; x < total; x += LSA_WAVE) M = fmaxf(M, coherent_load(parts + (int64_t)x * PSTRIDE + h));
       M = wave_max(M);
       for (int x = lane; x < total; x += LSA_WAVE) {
         const float* part = parts + (int64_t)x * PSTRIDE;
-        L += (x < pc.count ? sums[x * GQ + h] : coherent_load(part + GQ + h)) * fast_exp2(coherent_load(part + h) - M);
+        L += (sums && x < pc.count ? sums[x * GQ + h] : coherent_load(part + GQ + h)) * fast_exp2(coherent_load(part + h) - M);
       }
       L = wave_sum(L);
       if (lane == 0) {
@@ -169,13 +145,22 @@ bool prefix_shape_ok(int dtype, int64_t B, int64_t Tq, int64_t P, int64_t Tp, in
 }
 
 template <typename T, int D>
-void launch_prefix_gq(const PrefixArgs& a, int gq, int64_t units, hipStream_t s) {
-  const dim3 gp((unsigned)units, (unsigned)a.splits), go((unsigned)units, (unsigned)a.own_splits);
-  const bool done = launch_prefix_mfma(a, __is_same(T, float) ? LSA_F32 : (__is_same(T, bf16_t) ? LSA_BF16 : LSA_F16), D,
+void launch_prefix_gq(PrefixArgs a, int gq, int64_t units, int* counters, hipStream_t s) {
+  const dim3 pieces((unsigned)units, (unsigned)a.splits), own((unsigned)units, (unsigned)a.own_splits);
+  const dim3 all((unsigned)units, (unsigned)(a.splits + a.own_splits));
+  const bool mfma = launch_prefix_mfma(a, __is_same(T, float) ? LSA_F32 : (__is_same(T, bf16_t) ? LSA_BF16 : LSA_F16), D,
                                        mean_columns(a.B, a.Tq, a.P, a.Hq, a.Hkv), s);
-#define LSA_PREFIX(GQ)                                                    \
-  if (!done) prefix_gather_kernel<T, D, GQ><<<gp, LSA_BLOCK, 0, s>>>(a);  \
-  prefix_join_kernel<T, D, GQ><<<go, LSA_BLOCK, 0, s>>>(a)
+  if (!mfma) a.sums = nullptr;  // row by row the weights are fp32: one sum serves both
+  if (!mfma && counters) a.counters = counters;
+#define LSA_PREFIX(GQ)                                                                        \
+  if (mfma) {                                                                                 \
+    prefix_rows_kernel<T, D, GQ><<<own, LSA_BLOCK, 0, s>>>(a, a.splits, kOwn);                \
+  } else if (counters) {                                                                      \
+    prefix_rows_kernel<T, D, GQ><<<all, LSA_BLOCK, 0, s>>>(a, 0, kAll);                       \
+  } else {                                                                                    \
+    prefix_rows_kernel<T, D, GQ><<<pieces, LSA_BLOCK, 0, s>>>(a, 0, kNone);                   \
+    prefix_rows_kernel<T, D, GQ><<<own, LSA_BLOCK, 0, s>>>(a, a.splits, kOwn);                \
+  }
   switch (gq) {
     case 1: LSA_PREFIX(1); break;
     case 2: LSA_PREFIX(2); break;
@@ -186,12 +171,12 @@ void launch_prefix_gq(const PrefixArgs& a, int gq, int64_t units, hipStream_t s)
 }
 
 template <typename T>
-void launch_prefix(const PrefixArgs& a, int D, int gq, int64_t units, hipStream_t s) {
+void launch_prefix(const PrefixArgs& a, int D, int gq, int64_t units, int* counters, hipStream_t s) {
   switch (D) {
-    case 32: launch_prefix_gq<T, 32>(a, gq, units, s); break;
-    case 64: launch_prefix_gq<T, 64>(a, gq, units, s); break;
-    case 128: launch_prefix_gq<T, 128>(a, gq, units, s); break;
-    default: launch_prefix_gq<T, 256>(a, gq, units, s); break;
+    case 32: launch_prefix_gq<T, 32>(a, gq, units, counters, s); break;
+    case 64: launch_prefix_gq<T, 64>(a, gq, units, counters, s); break;
+    case 128: launch_prefix_gq<T, 128>(a, gq, units, counters, s); break;
+    default: launch_prefix_gq<T, 256>(a, gq, units, counters, s); break;
   }
 }
 
@@ -210,7 +195,8 @@ extern "C" int lsa_prefix_read(const void* q, const void* k_prefix, const void* 
                                const int32_t* prefix_slots, int64_t prefix_slot_stride, const void* k, const void* v,
                                int64_t Tk, int64_t kv_batch_stride, int64_t kv_token_stride, int64_t kv_head_stride,
                                const int32_t* ids, const int32_t* lengths, int32_t W, int ids_per_head, float scale,
-                               void* scratch, size_t scratch_bytes, void* out, float* lse, void* stream) {
+                               int32_t* counters, void* scratch, size_t scratch_bytes, void* out, float* lse,
+                               void* stream) {
   LSA_REQUIRE(q && out && (Tp == 0 || (k_prefix && v_prefix)), LSA_ERR_NULL, "lsa_prefix_read: NULL pointer");
   LSA_TRY(check_dtype(dtype));
   LSA_REQUIRE(prefix_shape_ok(dtype, B, Tq, P, Tp, Hq, Hkv, D, W), LSA_ERR_SHAPE,
@@ -254,9 +240,9 @@ extern "C" int lsa_prefix_read(const void* q, const void* k_prefix, const void* 
   hipStream_t s = (hipStream_t)stream;
   const int64_t units = B * Tq * Hkv;
   const int gq = Hq / Hkv;
-  if (dtype == LSA_BF16) launch_prefix<bf16_t>(a, D, gq, units, s);
-  else if (dtype == LSA_F16) launch_prefix<_Float16>(a, D, gq, units, s);
-  else launch_prefix<float>(a, D, gq, units, s);
+  if (dtype == LSA_BF16) launch_prefix<bf16_t>(a, D, gq, units, counters, s);
+  else if (dtype == LSA_F16) launch_prefix<_Float16>(a, D, gq, units, counters, s);
+  else launch_prefix<float>(a, D, gq, units, counters, s);
   LSA_LAUNCHED("lsa_prefix_read");
   return LSA_OK;
 }

@@ -107,8 +107,8 @@ SIGNATURES = {
                                        _f32, _i32, _i32, _i32, _p, _p, _p, _p, _p]),
     "lsa_prefix_read_scratch_bytes": (_sz, [_int, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32]),
     "lsa_prefix_read": (_int, [_p, _p, _p, _int, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _i64, _p,
-                               _p, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _i32, _int, _f32, _p, _sz, _p, _p,
-                               _p]),
+                               _p, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _i32, _int, _f32, _p, _p, _sz, _p,
+                               _p, _p]),
     "lsa_key_mass_scratch_bytes": (_sz, [_int, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32]),
     "lsa_key_mass": (_int, [_p, _p, _int, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _i64, _p, _p, _i32,
                             _int, _f32, _p, _int, _p, _p, _sz, _p, _i64, _i64, _p]),

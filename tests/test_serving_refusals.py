@@ -12,7 +12,7 @@ BF16, P = _abi.LSA_BF16, 4096  # P: an aligned address that is never read
 def prefix(**over):
     a = dict(q=P, kp=P, vp=P, dt=BF16, B=2, Tq=1, P=1, Tp=64, rows=64, Hq=8, Hkv=2, D=128, sb=0, st=256, sh=128, prow=None,
              plen=None, slots=None, slot_stride=0, k=P, v=P, Tk=32, kb=8192, kt=256, kh=128, ids=P, lens=P, W=4, per=0,
-             scale=0.1, ws=P, nbytes=1 << 40, out=P, lse=None, stream=None)
+             scale=0.1, counters=None, ws=P, nbytes=1 << 40, out=P, lse=None, stream=None)
     a.update(over)
     return _abi.call("lsa_prefix_read", *a.values())
 
