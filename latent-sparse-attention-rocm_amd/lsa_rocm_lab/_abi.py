@@ -258,19 +258,24 @@ class Workspace:
         return buf
 
 
-def scratch(device: torch.device, purpose: str, nbytes: int) -> torch.Tensor | None:
-    """Scratch of one call whose kernels need nothing of it afterwards: ``Workspace``'s, or,
-    while a HIP graph is captured, memory of that graph's own pool, so that graphs captured on
-    one stream may be replayed on several at once."""
-    if nbytes > 0 and torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return Workspace.get(device, purpose, nbytes)
-
-
-def counters(device: torch.device, n: int) -> torch.Tensor | None:
-    """Counters of one call, or None while a HIP graph is captured: ``Counters``' belong to the
-    stream, and graphs that hold them must not be replayed on several at once."""
-    return None if torch.cuda.is_current_stream_capturing() else Counters.get(device, n)
+def call_memory(device: torch.device, purpose: str, nbytes: int, n_counters: int = 0):
+    """What one call on a tensor's ``device`` hands its kernels: (scratch that they need nothing of
+    afterwards or None, counters or None, the stream). They are ``Workspace``'s and ``Counters``',
+    or, while a HIP graph is captured, scratch of that graph's own pool and no counters, so that
+    graphs captured on one stream may be replayed on several at once."""
+    here = stream(device)
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None, None, here
+    ws = count = None
+    if nbytes:
+        ws = Workspace._buffers.get((device.index, here, purpose))
+        if ws is None or ws.numel() < nbytes:
+            ws = Workspace.get(device, purpose, nbytes)
+    if n_counters:
+        count = Counters._buffers.get((device.index, here))
+        if count is None or count.numel() < n_counters:
+            count = Counters.get(device, n_counters)
+    return ws, count, here
 
 
 class Counters:

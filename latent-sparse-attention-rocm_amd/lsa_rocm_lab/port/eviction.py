@@ -88,13 +88,11 @@ def key_mass(
                 plens = lens.view(B, Tq, -1)[:, t:t + n].contiguous()
                 plse = None if lse is None else lse[:, t:t + n].contiguous()
             nbytes = _abi.shape_size("lsa_key_mass_scratch_bytes", dt, B, n, caches, Tk, Hq, Hkv, D, W)
-            ws = _abi.scratch(device, "key_mass", nbytes)
-            counters = _abi.counters(device, B * Hkv) if n == 1 and caches == B else None
+            ws, counters, stream = _abi.call_memory(device, "key_mass", nbytes, B * Hkv if n == 1 and caches == B else 0)
             _abi.call("lsa_key_mass", part.data_ptr(), k.data_ptr(), dt, B, n, caches, Tk, Hq, Hkv, D, sb, st, sh,
                       pids.data_ptr(), plens.data_ptr(), W, 1 if per_head else 0, scale, _abi.ptr(plse),
                       1 if fresh and t == 0 else 0, _abi.ptr(counters), _abi.ptr(ws), nbytes, mass.data_ptr(),
-                      mass.stride(0) if caches > 1 else Hkv * Tk, mass.stride(1) if Hkv > 1 else Tk,
-                      _abi.stream(device))
+                      mass.stride(0) if caches > 1 else Hkv * Tk, mass.stride(1) if Hkv > 1 else Tk, stream)
     return mass
 
 
@@ -190,8 +188,7 @@ def evict(
         one = 1 if shared else 0
         nbytes = _abi.shape_size("lsa_evict_scratch_bytes", B, Hkv, T, one)
         with launch_device(device):
-            ws = _abi.scratch(device, "evict", nbytes)
-            stream = _abi.stream(device)
+            ws, _, stream = _abi.call_memory(device, "evict", nbytes)
             _abi.call("lsa_evict_keep", mass.data_ptr(), B, Hkv, T, mass.stride(0), mass.stride(1), _abi.ptr(lens),
                       budget, window, sink, one, None, 0, 0, _abi.ptr(ws), nbytes, kept.data_ptr(),
                       new_lengths.data_ptr(), None, 0, stream)
@@ -240,8 +237,8 @@ def evict_slots(
     if R:
         nbytes = _abi.shape_size("lsa_evict_scratch_bytes", R, Hkv, T, 1)
         with launch_device(device):
-            ws = _abi.scratch(device, "evict", nbytes)
+            ws, _, stream = _abi.call_memory(device, "evict", nbytes)
             _abi.call("lsa_evict_keep", mass.data_ptr(), R, Hkv, T, 0, mass.stride(1), _abi.ptr(lens), budget, window,
                       sink, 1, table.data_ptr(), T, pool, _abi.ptr(ws), nbytes, kept.data_ptr(),
-                      new_lengths.data_ptr(), new_table.data_ptr(), T, _abi.stream(device))
+                      new_lengths.data_ptr(), new_table.data_ptr(), T, stream)
     return new_table, new_lengths, kept

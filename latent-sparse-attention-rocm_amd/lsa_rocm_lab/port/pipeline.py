@@ -54,6 +54,8 @@ import torch.nn.functional as F
 
 from lsa_rocm_lab import _abi
 from lsa_rocm_lab.port import keys as keys_mod
+from lsa_rocm_lab.port.eviction import evict, evict_slots, key_mass  # noqa: F401
+from lsa_rocm_lab.port.shared_prefix import prefix_read  # noqa: F401
 
 
 @dataclass(frozen=True)
@@ -610,38 +612,6 @@ def lsa_read(q, k, v, read_lists, lengths, scale):
     from lsa_rocm_lab.port.read_kernel_tiled import sparse_read_auto
 
     return sparse_read_auto(q, k, v, read_lists, lengths, scale)
-
-
-def prefix_read(q, k_prefix, v_prefix, k=None, v=None, read_lists=None, lengths=None, scale=None,
-                prefix_lengths=None, prefix_rows=None, prefix_slots=None, return_lse: bool = False):
-    """Attention of a batch over prefixes its rows share and over each row's own read list.
-
-    See ``shared_prefix.prefix_read``; the own part as ``lsa_read``."""
-    from lsa_rocm_lab.port import shared_prefix
-
-    return shared_prefix.prefix_read(q, k_prefix, v_prefix, k, v, read_lists, lengths, scale, prefix_lengths,
-                                     prefix_rows, prefix_slots, return_lse)
-
-
-def key_mass(q, k, read_lists, lengths, scale=None, lse=None, mass=None):
-    """The attention weight each listed key received, added up (``eviction.key_mass``)."""
-    from lsa_rocm_lab.port import eviction
-
-    return eviction.key_mass(q, k, read_lists, lengths, scale, lse, mass)
-
-
-def evict(k, v, mass, budget: int, lengths=None, window: int = 0, sink: int = 0, shared: bool = False, out=None):
-    """A cache cut down to the keys of largest weight (``eviction.evict``)."""
-    from lsa_rocm_lab.port import eviction
-
-    return eviction.evict(k, v, mass, budget, lengths, window, sink, shared, out)
-
-
-def evict_slots(slot_table, mass, budget: int, lengths=None, window: int = 0, sink: int = 0):
-    """The same for a paged cache, by its slot table alone (``eviction.evict_slots``)."""
-    from lsa_rocm_lab.port import eviction
-
-    return eviction.evict_slots(slot_table, mass, budget, lengths, window, sink)
 
 
 def flat_decode(
