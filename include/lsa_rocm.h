@@ -441,8 +441,8 @@ int lsa_decode_flat_noalloc(const void* q, const void* k, const void* v, int dty
  * strides; prefix_cache_rows >= Tp rows a batch entry) or, with prefix_slots [P, Tp] (rows
  * prefix_slot_stride apart), the cache rows it names of one pool of prefix_cache_rows rows
  * (prefix_batch_stride unused; a slot outside the pool is skipped). Of prefix p the first
- * prefix_lengths[p] keys count (NULL: Tp); batch row b reads prefix prefix_rows[b] (NULL: 0;
- * none where it is outside [0, P)). The own part as lsa_read (W == 0: none; k, v, ids and
+ * prefix_lengths[p] keys count (NULL: Tp); batch row b reads prefix prefix_rows[b] (none
+ * where it is outside [0, P); NULL: the only one, or prefix b of B). The own part as lsa_read (W == 0: none; k, v, ids and
  * lengths may be NULL then). A row without any key gives zeros. lse (NULL: not wanted) [B, Tq,
  * Hq] fp32: the natural logarithm of the softmax's sum, -inf for a row without keys.
  * counters (or NULL): B * Tq * Hkv int32 that read zero at launch and are left zero; where the

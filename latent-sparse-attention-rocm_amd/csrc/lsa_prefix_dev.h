@@ -14,7 +14,7 @@ struct PrefixArgs {
   const void* q;
   const void* kp;
   const void* vp;
-  const int32_t* prefix_rows;     // [B] or nullptr: 0
+  const int32_t* prefix_rows;     // [B] or nullptr: the only prefix, or prefix b of B
   const int32_t* prefix_lengths;  // [P] or nullptr: Tp
   const int32_t* slots;           // [P, Tp] cache rows of a pool, or nullptr
   int64_t slot_stride, pool;      // rows the prefix cache holds a batch entry
@@ -56,7 +56,7 @@ __device__ __forceinline__ Pieces prefix_pieces(const PrefixArgs& a, int p) {
   return x;
 }
 __device__ __forceinline__ int prefix_of(const PrefixArgs& a, int64_t b) {
-  return a.prefix_rows ? a.prefix_rows[b] : 0;
+  return a.prefix_rows ? a.prefix_rows[b] : (a.P > 1 ? (int)b : 0);
 }
 
 // Partials of the prefixes from the matrix cores (16-bit rows, head dim 64 or 128); clears the

@@ -1,21 +1,23 @@
 // A shared prefix's partials on the matrix cores (16-bit rows, head dim 64 or 128).
 //
 // The query rows of a prefix's batch rows, times the kv-head's query group, are the columns of
-// S^T = K Q^T and O^T += V^T P^T. A workgroup takes up to 128 columns and one piece of the
-// prefix, so every key is read once per 128 columns, where the gather reads it once a row.
+// S^T = K Q^T and O^T += V^T P^T. A workgroup takes up to 256 columns and one piece of the
+// prefix, so every key is read once per block of columns, where the gather reads it once a row.
 //
-// KG groups of CG waves, 32 columns a wave, take the piece's tiles in turn, each group with tile
-// buffers of its own (two of K and V, filled straight from memory a tile ahead): four groups on
-// 32-key tiles for up to 32 or 64 columns, two on 64-key tiles for up to 128. So few columns, too,
-// have 64 KB in flight a CU (D = 128), and what bounds them is memory. At the end the groups'
-// states meet in LDS and leave as one partial.
+// Up to 128 columns: KG groups of CG waves, 32 columns a wave, take the piece's tiles in turn, each
+// group with tile buffers of its own (two of K and V, filled straight from memory a tile ahead): four
+// groups on 32-key tiles for up to 32 or 64 columns, two on 64-key tiles for up to 128. So few columns,
+// too, have 64 KB in flight a CU (D = 128), and what bounds them is memory: 32768 bf16 keys of 128 on 8
+// kv-heads (134 MB) for 128 columns take 34 to 36 us, 10 of them the start and the joining of states.
+// (128 columns as four waves of 64 spilled 45 registers: 102 us.) At the end the groups' states meet in
+// LDS and leave as one partial. More than 128 columns: the second kernel below.
 //
-// A weight enters the matrix cores as one 16-bit number: half a step of it (2^-9 in bf16, 2^-12
-// in fp16), independent from key to key; the output is rounded by as much when it is stored. The sum
-// it is divided by adds the same rounded weights, so a row that one key fills returns that key's value;
-// the sum that lse shows adds them unrounded, in fp32. fp16 weights are kept high
-// in their range (the largest is 2^12 when the reference moves and stays below 2^15), so the smallest step
-// is 2^-36 of it and many small weights beside a large one are not lost.
+// A weight enters the matrix cores as one 16-bit number: off by at most half a step of it (2^-8 in bf16,
+// 2^-11 in fp16), independent from key to key; the output is rounded by as much when it is stored. The
+// sum it is divided by adds the same rounded weights, so a row that one key fills returns that key's
+// value; the sum that lse shows adds them unrounded, in fp32. fp16 weights are kept high in their range
+// (the largest is 2^12 when the reference moves and stays below 2^15), so the smallest step is 2^-36 of
+// it and many small weights beside a large one are not lost.
 #include <math.h>
 
 #include <algorithm>
@@ -30,12 +32,16 @@ namespace {
 
 constexpr int kXcds = 8;
 
-// A workgroup's place: kv-head, prefix, piece, and the batch rows whose query rows times heads are
-// its columns (column: batch row of the prefix, query row, head). The grid's (kv-head, prefix, piece)
-// units come in groups of 8, the column blocks of a unit 8 apart, so that those which read the same
-// keys share an XCD and its L2.
+// A workgroup's place: kv-head, piece, prefix, and the batch rows whose query rows times heads are
+// its columns (column: batch row of the prefix, query row, head). The column blocks of all prefixes
+// stand in one line, and the grid is that line times the (kv-head, piece) units: which prefix a block
+// belongs to follows from how many rows each has, counted here. (A grid of every prefix times the most
+// blocks one may have is nearly all empty where prefixes are many: 512 rows over 128 prefixes of 2048
+// keys took 820 us so, and take 242; 64 rows over 4000 of 256 keys 1922 and 42.) Units come in groups
+// of 8, the blocks of a unit 8 apart, so that those which read the same keys share an XCD and its L2.
 template <int COLS>
 struct PrefixBlock {
+  static constexpr int kCount = 1024;  // prefixes counted at once
   struct Lds {
     int32_t member[COLS];  // the batch rows
     int32_t row[COLS];     // a column's query row (b * Tq + t), -1 past the prefix's rows
@@ -45,21 +51,59 @@ struct PrefixBlock {
   int GQ, g, p, s;
   Pieces pc;
 
-  uint32_t cb;
+  uint32_t cb;  // the prefix's column block
 
-  // False: nothing to do (the whole workgroup). Clears the grid's share of the counters.
-  __device__ __forceinline__ bool place(const PrefixArgs& a, uint32_t n_cb, int threads) {
-    const int tid = threadIdx.x;
+  // False: nothing to do (the whole workgroup). Clears the grid's share of the counters. Contains
+  // barriers; `rows`: kCount ints of LDS, free again after it.
+  __device__ __forceinline__ bool place(const PrefixArgs& a, uint32_t blocks, int threads, int* rows) {
+    const int tid = threadIdx.x, lane = tid & 63;
     GQ = a.Hq / a.Hkv;
     const int64_t clear = (int64_t)gridDim.x * threads;
     for (int64_t i = (int64_t)blockIdx.x * threads + tid; i < a.B * a.Tq * a.Hkv; i += clear) a.counters[i] = 0;
-    const uint32_t x = blockIdx.x, x8 = x / kXcds;
-    cb = x8 % n_cb;
-    uint32_t u = x8 / n_cb * kXcds + x % kXcds;
-    s = (int)(u % (uint32_t)a.splits); u /= (uint32_t)a.splits;
-    g = (int)(u % (uint32_t)a.Hkv); u /= (uint32_t)a.Hkv;
-    if (u >= (uint32_t)a.P) return false;
-    p = (int)u;
+    const uint32_t units = (uint32_t)(a.Hkv * a.splits), together = min(units, (uint32_t)kXcds);
+    const uint32_t x = blockIdx.x, xu = x / together;
+    cb = xu % blocks;
+    const uint32_t u = xu / blocks * together + x % together;
+    s = (int)(u % (uint32_t)a.splits);
+    g = (int)(u / (uint32_t)a.splits);
+    if (g >= a.Hkv) return false;
+    const uint32_t per = (uint32_t)a.Tq * (uint32_t)GQ;  // columns of a batch row; all are fewer than 2^31
+    p = 0;
+    if (a.prefix_rows == nullptr) {
+      if (a.P > 1) {
+        const uint32_t each = (per + COLS - 1) / COLS;
+        p = (int)(cb / each);
+        cb %= each;
+      }
+    } else if (a.P > 1) {
+      bool found = false;  // uniform, as every wave finds the same
+      uint32_t base = 0;   // blocks of the prefixes before
+      for (int p0 = 0; p0 < a.P && !found; p0 += kCount) {
+        const int np = min(kCount, a.P - p0);
+        for (int i = tid; i < np; i += threads) rows[i] = 0;
+        __syncthreads();
+        for (int64_t b = tid; b < a.B; b += threads) {
+          const int64_t r = (int64_t)a.prefix_rows[b] - p0;
+          if (r >= 0 && r < np) atomicAdd(&rows[r], 1);
+        }
+        __syncthreads();
+        for (int i0 = 0; i0 < np && !found; i0 += 64) {
+          const uint32_t n = i0 + lane < np ? (uint32_t)rows[i0 + lane] * per : 0u;
+          const int own = (int)((n + COLS - 1) / COLS), to = wave_inclusive_sum(own);
+          const uint64_t after = __ballot(base + (uint32_t)to > cb);
+          if (after != 0ull) {
+            const int l = __builtin_ctzll(after);
+            found = true;
+            p = p0 + i0 + l;
+            cb -= base + (uint32_t)__shfl(to - own, l, 64);
+          } else {
+            base += (uint32_t)__shfl(to, 63, 64);
+          }
+        }
+        __syncthreads();  // before the counts' place is used again
+      }
+      if (!found) return false;
+    }
     pc = prefix_pieces(a, p);
     return s < pc.count;
   }
@@ -70,9 +114,10 @@ struct PrefixBlock {
     const uint32_t per = (uint32_t)a.Tq * (uint32_t)GQ, c0 = cb * COLS, first = c0 / per;
     int found;
     if (a.prefix_rows == nullptr) {
-      if (first >= a.B) return false;
-      found = (int)min(a.B - first, (int64_t)COLS);
-      if (tid < found) sh.member[tid] = (int32_t)first + tid;
+      const int64_t of = a.P > 1 ? 1 : a.B;  // batch rows: p, or all of them
+      if (first >= of) return false;
+      found = (int)min(of - first, (int64_t)COLS);
+      if (tid < found) sh.member[tid] = (a.P > 1 ? p : (int32_t)first) + tid;
     } else {
       int64_t seen = 0;
       for (int64_t b0 = 0; b0 < a.B && seen < (int64_t)first + COLS; b0 += threads) {
@@ -204,7 +249,7 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
   const int kg = w % KG, cg = w / KG;
   const int hh = lane / 32, ln = lane % 32;
   PrefixBlock<COLS> blk;
-  if (!blk.place(a, (uint32_t)n_cb, THREADS)) return;
+  if (!blk.place(a, (uint32_t)n_cb, THREADS, (int*)&sh)) return;
   const int g = blk.g, p = blk.p, s = blk.s;
   const Pieces pc = blk.pc;
   const int k0 = s * pc.keys, n_keys = min(pc.keys, pc.n - k0);
@@ -394,12 +439,12 @@ void prefix_mfma_kernel(PrefixArgs a, int n_cb) {
 // loads ahead and this tile's weights (vector unit). Two groups of four waves, one of each on every SIMD, run
 // half a step apart (a barrier after each phase), so one's matrix work runs beside the other's vector work.
 //
-// A load straight to LDS holds its wave for about 155 cycles (four waves at once: 39 cycles a KB of the CU).
-// In M, between the matrix operations, four of them cost 500 cycles, in V they fill time that V has left
-// (131072 keys, 512 columns of 128 on 8 kv-heads: a step of 4850 cycles with them in M, 3720 in V; under load the clock falls as the
-// cycles do, and both take 310 us). That is also why the
-// many-column form shares a tile between all waves: 32 KB a step of 2048 cycles of matrix work, where two
-// groups on tiles of their own load 64 KB (350 us).
+// A load straight to LDS holds its wave for about 155 cycles (four waves at once: 39 cycles a KB of the
+// CU). In M, between the matrix operations, four of them cost 500 cycles; in V they fill time that V has
+// left. 131072 keys, 512 columns of 128 on 8 kv-heads: a step takes 4850 cycles with them in M, 3720 in V
+// (2048 of them matrix work). At that load the card lowers its clock as the cycles fall, and both take 310
+// us, 920 TFLOP/s: power bounds it. A tile is shared by all waves for the same reason: 32 KB a step,
+// where two groups on tiles of their own load 64 KB (350 us).
 //
 // V(i) loads K(i + 3) over K(i - 1) and V(i + 2) over V(i - 2), both read for the last time in M(i - 1) of
 // either group. K(i) is read in M(i), V(i) from the end of V(i) on: both were loaded in V(i - 2) or
@@ -438,7 +483,7 @@ void prefix_wide_kernel(PrefixArgs a, int n_cb) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid / 64);
   const int hh = lane / 32, ln = lane % 32;
   PrefixBlock<COLS> blk;
-  if (!blk.place(a, (uint32_t)n_cb, THREADS)) return;
+  if (!blk.place(a, (uint32_t)n_cb, THREADS, (int*)&sh)) return;
   const int k0 = blk.s * blk.pc.keys, n_keys = min(blk.pc.keys, blk.pc.n - k0);
   const int n_tiles = (n_keys + KT - 1) / KT;
   const int64_t head = (PAGED ? 0 : blk.p * a.p_sb) + blk.g * a.p_sh;
@@ -464,7 +509,7 @@ void prefix_wide_kernel(PrefixArgs a, int n_cb) {
   const uint32_t kseg0 = (uint32_t)(((lane % SEGS) ^ kseg<D>(lane / SEGS)) * 16);
   const uint32_t vseg0 = (uint32_t)(((lane % SEGS) ^ vseg<D>(lane / SEGS)) * 16);
   auto load = [&](bool values, int i, int y) {
-    static_assert(KPI == 512 / D && (D == 64 || D == 128), "K's segments differ from move to move by 64 bytes times this");
+    static_assert(KPI == 512 / D && (D == 64 || D == 128), "moves differ by 64-byte steps of K's segment");
     const int t = tile_of(i), n = keys_of(t), part = w * NI + y;
     const char* src = (const char*)(values ? vb : kb);
     const uint32_t dst = (values ? v_lds : k_lds) + (uint32_t)(i & (NB - 1)) * (KT * ROWB) + (uint32_t)part * 1024u;
@@ -696,17 +741,21 @@ void prefix_wide_kernel(PrefixArgs a, int n_cb) {
   store_partials<D, KG, CG>(a, sh, blk, 0, w, o, m_run, l_run, l32_run);
 }
 
-int64_t prefix_units(const PrefixArgs& a) { return ((int64_t)a.P * a.Hkv * a.splits + kXcds - 1) / kXcds * kXcds; }
+// Column blocks of all prefixes, at most.
+int64_t column_blocks(const PrefixArgs& a, int64_t wg) {
+  const int64_t per = a.Tq * (a.Hq / a.Hkv);
+  if (a.prefix_rows == nullptr && a.P > 1) return a.P * ((per + wg - 1) / wg);
+  return (a.B * per + std::min<int64_t>(a.P, a.B) * (wg - 1)) / wg;
+}
 
-// Column blocks of a prefix, at most (it has as many as it has rows).
-int64_t column_blocks(const PrefixArgs& a, int64_t columns) {
-  const int64_t wg = prefix_mfma_columns(columns);
-  return (a.B * a.Tq * (a.Hq / a.Hkv) + wg - 1) / wg;
+int64_t prefix_grid(const PrefixArgs& a, int64_t wg) {
+  const int64_t units = (int64_t)a.Hkv * a.splits, together = std::min<int64_t>(units, kXcds);
+  return (units + together - 1) / together * together * column_blocks(a, wg);
 }
 
 template <typename T, int D, int KG, int CG>
 void launch_mfma(const PrefixArgs& a, int n_cb, hipStream_t s) {
-  const dim3 grid((unsigned)(prefix_units(a) * n_cb));
+  const dim3 grid((unsigned)prefix_grid(a, 32 * CG));
   if (a.slots) prefix_mfma_kernel<T, D, KG, CG, true><<<grid, 64 * KG * CG, 0, s>>>(a, n_cb);
   else prefix_mfma_kernel<T, D, KG, CG, false><<<grid, 64 * KG * CG, 0, s>>>(a, n_cb);
 }
@@ -714,12 +763,12 @@ void launch_mfma(const PrefixArgs& a, int n_cb, hipStream_t s) {
 template <typename T, int D>
 void launch_mfma_cols(const PrefixArgs& a, int64_t columns, hipStream_t s) {
   const int64_t wg = prefix_mfma_columns(columns);
-  const int n_cb = (int)column_blocks(a, columns);
+  const int n_cb = (int)column_blocks(a, wg);
   if (wg == 32) launch_mfma<T, D, 4, 1>(a, n_cb, s);
   else if (wg == 64) launch_mfma<T, D, 4, 2>(a, n_cb, s);
   else if (wg == 128) launch_mfma<T, D, 2, 4>(a, n_cb, s);
   else {
-    const dim3 grid((unsigned)(prefix_units(a) * n_cb));
+    const dim3 grid((unsigned)prefix_grid(a, wg));
     if (a.slots) prefix_wide_kernel<T, D, true><<<grid, 512, 0, s>>>(a, n_cb);
     else prefix_wide_kernel<T, D, false><<<grid, 512, 0, s>>>(a, n_cb);
   }
@@ -731,11 +780,14 @@ namespace lsa {
 
 bool prefix_mfma_ok(int dtype, int D) { return dtype != LSA_F32 && (D == 64 || D == 128); }
 
-int64_t prefix_mfma_columns(int64_t columns) { return columns <= 32 ? 32 : (columns <= 64 ? 64 : (columns <= 128 ? 128 : 256)); }
+int64_t prefix_mfma_columns(int64_t columns) {
+  return columns <= 32 ? 32 : (columns <= 64 ? 64 : (columns <= 128 ? 128 : 256));
+}
 
 bool launch_prefix_mfma(const PrefixArgs& a, int dtype, int D, int64_t columns, hipStream_t s) {
   // a lane's offset within a tile is 32 bits of bytes; a column's largest score is its largest dot product
-  if (!prefix_mfma_ok(dtype, D) || !(a.scale_log2 > 0.0f && a.scale_log2 < INFINITY) || a.p_st >= (int64_t)1 << 25 || prefix_units(a) * column_blocks(a, columns) > 0x7FFFFFFF)
+  if (!prefix_mfma_ok(dtype, D) || !(a.scale_log2 > 0.0f && a.scale_log2 < INFINITY) ||
+      a.p_st >= (int64_t)1 << 25 || prefix_grid(a, prefix_mfma_columns(columns)) > 0xFFFFFFFFll / 512)
     return false;
   if (dtype == LSA_BF16) {
     if (D == 64) launch_mfma_cols<bf16_t, 64>(a, columns, s);

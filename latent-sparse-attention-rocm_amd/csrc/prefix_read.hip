@@ -104,9 +104,11 @@ struct PrefixPlan {
   size_t parts, sums, total;
 };
 
-// Query columns a prefix has, if its rows are spread evenly.
+// Prefixes that rows read, at most, and the query columns of each if the rows are spread evenly.
+int64_t read_prefixes(int64_t B, int64_t P) { return std::max<int64_t>(1, std::min(B, P)); }
 int64_t mean_columns(int64_t B, int64_t Tq, int64_t P, int32_t Hq, int32_t Hkv) {
-  return (B * Tq * (Hq / Hkv) + P - 1) / P;
+  const int64_t n = read_prefixes(B, P);
+  return (B * Tq * (Hq / Hkv) + n - 1) / n;
 }
 
 // Pieces and own spans by size. On the matrix cores a workgroup has a CU to itself: as many pieces
@@ -120,7 +122,7 @@ PrefixPlan prefix_plan(int dtype, int64_t B, int64_t Tq, int64_t P, int64_t Tp, 
   if (prefix_mfma_ok(dtype, D)) {
     const int64_t cols = mean_columns(B, Tq, P, Hq, Hkv), wg = prefix_mfma_columns(cols);
     most = (tiles + 3) / 4;
-    want_p = 256 / std::max<int64_t>(1, P * Hkv * ((cols + wg - 1) / wg));
+    want_p = 256 / std::max<int64_t>(1, read_prefixes(B, P) * Hkv * ((cols + wg - 1) / wg));
   }
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, kMaxPieces, want_p}));
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kMaxOwn, 512 / std::max<int64_t>(units, 1)));
@@ -140,8 +142,10 @@ bool prefix_shape_ok(int dtype, int64_t B, int64_t Tq, int64_t P, int64_t Tp, in
   if (!(D == 32 || D == 64 || D == 128 || D == 256) || Hq < 1 || Hkv < 1 || Hq % Hkv) return false;
   const int gq = Hq / Hkv;
   if (!(gq == 1 || gq == 2 || gq == 4 || gq == 8)) return false;
-  return B >= 0 && Tq >= 0 && B <= 0x7FFFFFFF && Tq <= 0x7FFFFFFF && B * Tq <= 0x7FFFFFFF / Hq && P >= 1 && P <= 65535 &&
-         Tp >= 0 && Tp <= 0x7FFFFFC0 && W >= 0 && W <= 0x7FFFFFC0;
+  // a launch holds fewer than 2^32 threads along an axis
+  return B >= 0 && Tq >= 0 && B <= 0x7FFFFFFF && Tq <= 0x7FFFFFFF && B * Tq <= 0x7FFFFFFF / Hq &&
+         B * Tq * Hkv <= 0xFFFFFFFFll / LSA_BLOCK && P >= 1 && P <= 65535 && Tp >= 0 &&
+         Tp <= 0x7FFFFFC0 && W >= 0 && W <= 0x7FFFFFC0;
 }
 
 template <typename T, int D>
@@ -201,7 +205,9 @@ extern "C" int lsa_prefix_read(const void* q, const void* k_prefix, const void* 
   LSA_TRY(check_dtype(dtype));
   LSA_REQUIRE(prefix_shape_ok(dtype, B, Tq, P, Tp, Hq, Hkv, D, W), LSA_ERR_SHAPE,
               "lsa_prefix_read: B %lld Tq %lld P %lld Tp %lld Hq %d Hkv %d D %d W %d (D in {32,64,128,256}, groups of "
-              "1/2/4/8, 1..65535 prefixes)", (long long)B, (long long)Tq, (long long)P, (long long)Tp, Hq, Hkv, D, W);
+              "1/2/4/8, 1..65535 prefixes, rows x kv-heads under 2^24)", (long long)B, (long long)Tq, (long long)P, (long long)Tp, Hq, Hkv, D, W);
+  LSA_REQUIRE(prefix_rows || P == 1 || P == B, LSA_ERR_NULL, "lsa_prefix_read: %lld prefixes for %lld rows need "
+              "prefix_rows", (long long)P, (long long)B);
   LSA_REQUIRE(W == 0 || (k && v && ids && lengths && Tk >= 0 && Tk <= 0x7FFFFFFF), LSA_ERR_NULL,
               "lsa_prefix_read: own lists need K, V, ids and lengths");
   LSA_REQUIRE(prefix_cache_rows >= 0 && prefix_cache_rows <= 0x7FFFFFFF && (prefix_slots || prefix_cache_rows >= Tp),

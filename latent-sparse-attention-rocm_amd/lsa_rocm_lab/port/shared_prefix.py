@@ -137,12 +137,8 @@ def prefix_read(
         prow = int32_on(prefix_rows, device)
         if prow.numel() != B:
             raise ValueError(f"prefix_read: {prow.numel()} prefix rows for {B} batch rows")
-    elif P == 1:
+    elif P in (1, B):
         prow = None
-    elif P == B:
-        from lsa_rocm_lab.port.pipeline import _row_index
-
-        prow = _row_index(device, B, shared=False)
     else:
         raise ValueError(f"prefix_read: prefix_rows is needed: {P} prefixes for {B} batch rows")
     q = aligned(q)

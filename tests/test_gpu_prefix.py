@@ -305,3 +305,42 @@ def test_a_row_does_not_depend_on_its_neighbours_prefix():
     c["plen"] = torch.tensor([400, 17, 230], dtype=torch.int32)
     c["prow"] = torch.tensor([2, 0, 1, 1, 2, 0, -1, 2, 0, 0, 1, 7], dtype=torch.int32)
     compare(call(c), want(c), c)
+
+
+@pytest.mark.parametrize("dtype,B,Tq,P,Hq,paged", [
+    (torch.bfloat16, 5, 1, 1500, 8, 0),   # more prefixes than rows, some past the first thousand
+    (torch.bfloat16, 600, 1, 9, 8, 16),   # several blocks a prefix
+    (torch.float16, 70, 3, 40, 4, 0),
+    (torch.float32, 20, 1, 1100, 4, 0),
+])
+def test_many_prefixes(dtype, B, Tq, P, Hq, paged):
+    """Rows spread unevenly over prefixes, some of which none reads."""
+    c = make(dtype, B, Tq, P, 40, Hq, 2, 64, 30, 6, paged=paged, seed=17)
+    rng = np.random.default_rng(18)
+    c["prow"] = torch.from_numpy((P * rng.random(B) ** 3).astype(np.int32))
+    c["prow"][:4] = torch.tensor([P - 1, -1, P, P - 1], dtype=torch.int32)
+    compare(call(c), want(c), c)
+
+
+@pytest.mark.parametrize("dtype,B,Tq,paged", [(torch.bfloat16, 7, 1, 0), (torch.float16, 4, 40, 16), (torch.float32, 6, 2, 0)])
+def test_a_prefix_a_row(dtype, B, Tq, paged):
+    """Without prefix_rows row b reads prefix b; also from a graph that a first call is captured into."""
+    c = make(dtype, B, Tq, B, 130, 8, 2, 64, 30, 6, paged=paged, seed=19)
+    c["prow"] = torch.arange(B, dtype=torch.int32)
+    exact = want(c)
+    c["prow"] = None
+    t = {n: dev(c[n]) for n in ("q", "kp", "vp", "k", "v", "ids", "lens", "plen", "slots")}
+    print("a prefix a row", dtype, B, Tq, paged, flush=True)
+
+    def step():
+        return pipeline.prefix_read(t["q"], t["kp"], t["vp"], t["k"], t["v"], t["ids"], t["lens"], return_lse=True,
+                                    prefix_lengths=t["plen"], prefix_slots=t["slots"])
+
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    compare(step(), exact, c)
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        compare(out, exact, c)

@@ -30,6 +30,14 @@ def test_prefix_read_abi(over, match):
         prefix(**over)
 
 
+def test_prefix_read_of_several_prefixes_needs_their_rows():
+    for over in (dict(P=3), dict(P=3, B=1)):
+        with pytest.raises(ValueError, match="need prefix_rows"):
+            prefix(**over)
+    with pytest.raises(ValueError, match="LSA_ERR_SHAPE"):
+        prefix(B=1 << 23)  # 2^24 rows of kv-heads
+
+
 def test_prefix_read_needs_its_scratch():
     need = _abi.size("lsa_prefix_read_scratch_bytes", BF16, 2, 1, 1, 64, 8, 2, 128, 4)
     assert need > 0
