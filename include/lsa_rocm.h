@@ -467,6 +467,7 @@ int lsa_prefix_read(const void* q, const void* k_prefix, const void* v_prefix, i
  * those of the softmax over the row's own list, or exp(score - lse) with lse [B, Tq, Hq] (a
  * wider softmax's, as lsa_prefix_read gives it; -inf and NaN: no weight). A softmax whose sum
  * is not a number gives none. The result does not depend on the order in which workgroups run.
+ * Several rows of one cache: at most 2^19 rows times the group's heads a cache in one call.
  * zero_first != 0: mass (dense) begins at zero. counters (or NULL): B * Tq * Hkv int32 that read
  * zero at launch and are left zero; with one query row a cache they make the call one launch instead
  * of two. No counterpart in the reference. scratch:

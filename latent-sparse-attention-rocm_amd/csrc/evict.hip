@@ -494,7 +494,9 @@ int check_keep(const char* who, const void* mass, int64_t B, int32_t Hkv, int64_
   LSA_REQUIRE(budget >= 1 && budget <= T, LSA_ERR_SHAPE, "%s: budget %d not in 1..%lld", who, budget, (long long)T);
   LSA_REQUIRE(window >= 0 && sink >= 0 && (int64_t)window + sink <= budget, LSA_ERR_SHAPE,
               "%s: window %d and sink %d must fit the budget %d", who, window, sink, budget);
-  LSA_REQUIRE(B * (int64_t)Hkv <= 0x7FFFFFFF, LSA_ERR_SHAPE, "%s: too many rows", who);
+  // a launch holds fewer than 2^32 threads along an axis
+  LSA_REQUIRE(B * (int64_t)Hkv <= 0xFFFFFFFFll / kKeepThreads, LSA_ERR_SHAPE, "%s: %lld rows of %d kv-heads are too many",
+              who, (long long)B, Hkv);
   return LSA_OK;
 }
 

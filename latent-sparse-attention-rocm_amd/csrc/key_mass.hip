@@ -29,7 +29,8 @@ using namespace lsa;
 
 namespace {
 
-constexpr float kFix = 17592186044416.0f;  // 2^44: weights up to 2^19 in all
+constexpr float kFix = 17592186044416.0f;  // 2^44: a key's weights add up to less than 2^20
+constexpr int64_t kMaxRows = 1 << 19;      // so of softmaxes (one a row and head) at most this a cache
 constexpr float kMaxWeight = 65536.0f;     // a given lse may be off; a weight is at most this
 
 struct MassArgs {
@@ -471,8 +472,10 @@ bool mass_shape_ok(int dtype, int64_t B, int64_t Tq, int64_t caches, int64_t Tk,
   if (!(D == 32 || D == 64 || D == 128 || D == 256) || Hq < 1 || Hkv < 1 || Hq % Hkv) return false;
   const int gq = Hq / Hkv;
   if (!(gq == 1 || gq == 2 || gq == 4 || gq == 8)) return false;
-  return B >= 0 && Tq >= 0 && Tk >= 0 && Tk <= 0x7FFFFFFF && W >= 0 && (caches == B || caches == 1) &&
-         B * Tq <= 0x7FFFFFFF / Hkv;
+  // a launch holds fewer than 2^32 threads along an axis
+  return B >= 0 && Tq >= 0 && B <= 0x7FFFFFFF && Tq <= 0x7FFFFFFF && Tk >= 0 && Tk <= 0x7FFFFFFF && W >= 0 &&
+         (caches == B || caches == 1) && B * Tq <= 0xFFFFFFFFll / LSA_BLOCK / Hkv &&
+         (B * Tq <= caches || B * Tq <= caches * (kMaxRows / gq));
 }
 
 }  // namespace
@@ -493,7 +496,7 @@ extern "C" int lsa_key_mass(const void* q, const void* k, int dtype, int64_t B, 
   LSA_TRY(check_dtype(dtype));
   LSA_REQUIRE(mass_shape_ok(dtype, B, Tq, caches, Tk, Hq, Hkv, D, W), LSA_ERR_SHAPE,
               "lsa_key_mass: B %lld Tq %lld caches %lld Tk %lld Hq %d Hkv %d D %d W %d (D in {32,64,128,256}, groups of "
-              "1/2/4/8, B caches or 1)", (long long)B, (long long)Tq, (long long)caches, (long long)Tk, Hq, Hkv, D, W);
+              "1/2/4/8, B caches or 1, rows x kv-heads under 2^24, rows x group of a cache up to 2^19)", (long long)B, (long long)Tq, (long long)caches, (long long)Tk, Hq, Hkv, D, W);
   const int64_t e = dtype == LSA_F32 ? 4 : 2;
   LSA_REQUIRE(k_batch_stride >= 0 && k_token_stride >= D && k_head_stride >= D && mass_batch_stride >= 0 &&
                   mass_head_stride >= 0, LSA_ERR_SHAPE, "lsa_key_mass: strides must leave rows apart");

@@ -14,7 +14,9 @@ import torch
 from lsa_rocm_lab import _abi
 from lsa_rocm_lab.port.shared_prefix import aligned, cache_pair, cache_strides, int32_on, launch_device, lists_of, one_device
 
-_SLAB_BYTES = 256 << 20  # scores of query rows held at once (more rows go through in slabs)
+# Query rows go through in slabs: of so many bytes of scores, so many softmaxes a cache (their sums are
+# 64-bit integers) and so many kv-heads of rows (a launch's limit)
+_SLAB_BYTES, _SLAB_SUMS, _SLAB_UNITS = 256 << 20, 1 << 19, (1 << 24) - 1
 
 
 def _apart(t: torch.Tensor) -> bool:
@@ -77,7 +79,10 @@ def key_mass(
     lse = None if lse is None else lse.contiguous()
     scale = float(D ** -0.5 if scale is None else scale)
     # every query row's scores are held until its sums are known
-    step = Tq if 4 * B * Tq * Hq * W <= _SLAB_BYTES else max(1, _SLAB_BYTES // (4 * B * Hq * W))
+    step = Tq
+    if 4 * B * Tq * Hq * W > _SLAB_BYTES or B * Tq * Hq > _SLAB_SUMS:
+        step = max(1, min(Tq, _SLAB_BYTES // (4 * B * Hq * W), _SLAB_SUMS * caches // (B * (Hq // Hkv)),
+                          _SLAB_UNITS // (B * Hkv)))
     with launch_device(device):
         for t in range(0, Tq, step):
             n = min(step, Tq - t)
@@ -140,8 +145,8 @@ def evict(
     k/v [B, T, Hkv, D], mass [B, Hkv, T] fp32 (``key_mass``'s, accumulated). Of a row's
     ``lengths[b]`` positions (default T) the first ``sink`` and the last ``window`` stay, and of the
     others those of largest mass; ties go to the lower position, a NaN weighs least; a row of at
-    most ``budget`` positions keeps all. ``shared``: the kv-heads keep the same positions, by the sum of their masses (as lists over an
-    index-space table need it).
+    most ``budget`` positions keeps all. ``shared``: the kv-heads keep the same positions, by the sum
+    of their masses (as lists over an index-space table need it).
 
     Returns ``(k, v, mass, kept, lengths)``: the kept rows in their order, [B, budget, Hkv, D], their
     masses [B, Hkv, budget], their positions in the old cache [B, Hkv, budget] int32 (shared:

@@ -139,6 +139,16 @@ def test_key_mass_in_slabs_of_rows(monkeypatch):
         monkeypatch.undo()
 
 
+def test_key_mass_of_a_key_that_a_million_softmaxes_list():
+    """More of them than a 64-bit sum of 2^-44 holds: every one counts (integers, exact in fp32)."""
+    n = 131080
+    q = torch.zeros(1, n, 8, 32, dtype=torch.bfloat16, device=DEV)
+    k = torch.zeros(1, 5, 1, 32, dtype=torch.bfloat16, device=DEV)
+    ids = torch.full((1, n, 1), 3, dtype=torch.int32, device=DEV)
+    got = pipeline.key_mass(q, k, ids, torch.ones(1, n, dtype=torch.int32, device=DEV))
+    assert got.flatten().tolist() == [0.0, 0.0, 0.0, 8.0 * n, 0.0]
+
+
 @pytest.mark.parametrize("Tq", [1, 6])
 def test_key_mass_in_a_graph(Tq):
     q, k, ids, lens = make(torch.bfloat16, 3, Tq, 8, 2, 128, 500, 200, seed=8)

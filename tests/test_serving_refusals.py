@@ -64,6 +64,14 @@ def test_key_mass_abi(over, match):
         mass(**over)
 
 
+def test_key_mass_of_too_many_rows():
+    """Their sums, and a launch's threads, have limits."""
+    for over in (dict(Tq=(1 << 17) + 1), dict(caches=1, Tq=(1 << 16) + 1), dict(B=1 << 23, caches=1 << 23)):
+        with pytest.raises(ValueError, match="LSA_ERR_SHAPE"):
+            mass(**over)
+    assert _abi.size("lsa_key_mass_scratch_bytes", BF16, 2, 1 << 17, 2, 32, 8, 2, 128, 4) > 0
+
+
 def test_key_mass_needs_its_scratch():
     need = _abi.size("lsa_key_mass_scratch_bytes", BF16, 2, 1, 2, 32, 8, 2, 128, 4)
     assert need > 0
