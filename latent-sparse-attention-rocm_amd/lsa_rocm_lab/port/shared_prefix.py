@@ -15,6 +15,7 @@ from lsa_rocm_lab import _abi
 
 
 _HERE = contextlib.nullcontext()
+_SLAB_BYTES = 256 << 20  # partials held at once (more query rows go through in slabs)
 
 
 def launch_device(device: torch.device):
@@ -159,6 +160,25 @@ def prefix_read(
     lse = torch.empty(B, Tq, Hq, dtype=torch.float32, device=device) if return_lse else None
     if B * Tq:
         nbytes = _abi.shape_size("lsa_prefix_read_scratch_bytes", dt, B, Tq, P, Tp, Hq, Hkv, D, W)
+        if nbytes > _SLAB_BYTES and B * Tq > 1:  # in halves: query rows, then batch rows
+            axis = 1 if Tq > 1 else 0
+            if prow is None and P > 1:
+                prow = torch.arange(B, dtype=torch.int32, device=device)
+            own = [None] * 4
+            if W:
+                heads = (Hkv,) if per_head else ()
+                own = [k, v, ids.view(B, Tq, *heads, W), lens.view(B, Tq, *heads)]
+            n = q.shape[axis]
+            for at, m in ((0, n // 2), (n // 2, n - n // 2)):
+                cut = [x if x is None or (i < 2 and (axis == 1 or x.shape[0] == 1)) else x.narrow(axis, at, m)
+                       for i, x in enumerate(own)]
+                rows = prow if prow is None or axis == 1 else prow.narrow(0, at, m)
+                part = prefix_read(q.narrow(axis, at, m), k_prefix, v_prefix, *cut, scale, plen if Tp else None, rows,
+                                   slots, return_lse=True)
+                out.narrow(axis, at, m).copy_(part[0])
+                if return_lse:
+                    lse.narrow(axis, at, m).copy_(part[1])
+            return (out, lse) if return_lse else out
         with launch_device(device):
             ws, counters, stream = _abi.call_memory(device, "prefix_read", nbytes, B * Tq * Hkv)
             _abi.call("lsa_prefix_read", q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), dt, B, Tq, P, Tp,

@@ -371,3 +371,24 @@ def test_a_server_s_round():
     assert (lengths == budget).all()
     whole = pipeline.lsa_read(q[:1], k2[:1], v2[:1], short[:1], n[:1], D ** -0.5)
     assert ((dec.float() - whole.float()).abs() <= 2.0 ** -8 * whole.float().abs() + 2.0 ** -11).all()
+
+
+def test_offsets_past_32_bits():
+    """Token rows 2^24 elements apart: 300 of them span 10 GB."""
+    n, apart = 300, 1 << 24
+    whole = torch.empty(n * apart, dtype=torch.bfloat16, device=DEV)
+    for Tq in (1, 5):
+        q, k, ids, lens = make(torch.bfloat16, 2, Tq, 8, 2, 64, n, 40, pool=True, seed=41)
+        far = whole.as_strided((1, n, 2, 64), (n * apart, apart, 64, 1))
+        far.copy_(k)
+        mass = pipeline.key_mass(q.to(DEV), far, ids.to(DEV), lens.to(DEV))
+        close(mass, want(q, k, ids, lens), 2 * Tq, 4)
+    v = whole.as_strided((1, n, 2, 64), (n * apart, apart, 64, 1), 128)
+    v.copy_(-k)
+    k2, v2, m2, kept, length = pipeline.evict(far, v, mass, 120, window=9, sink=2)
+    assert length.tolist() == [120]
+    for h in range(2):
+        at = kept[0, h].long().cpu()
+        assert torch.equal(k2[0, :, h].cpu(), k[0, at, h]) and torch.equal(v2[0, :, h].cpu(), -k[0, at, h])
+        assert torch.equal(m2[0, h].cpu(), mass[0, h].cpu()[at])
+    assert kept[0, :, -1].tolist() == [n - 1] * 2

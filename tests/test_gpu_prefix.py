@@ -13,7 +13,7 @@ import numpy as np
 import pytest
 import torch
 
-from lsa_rocm_lab.port import pipeline
+from lsa_rocm_lab.port import pipeline, shared_prefix
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -344,3 +344,55 @@ def test_a_prefix_a_row(dtype, B, Tq, paged):
         g.replay()
         torch.cuda.synchronize()
         compare(out, exact, c)
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.float32, 64), (torch.bfloat16, 128), (torch.float16, 32)])
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+def test_scales_that_are_not_positive(dtype, D, scale):
+    c = make(dtype, 5, 2, 1, 150, 8, 2, D, 40, 9, seed=23)
+    compare(call(c, scale=scale), want(c, scale=scale), c)
+
+
+@pytest.mark.parametrize("B", [2, 80])
+@pytest.mark.parametrize("paged", [False, True])
+def test_offsets_past_32_bits(B, paged):
+    """Token rows 2^24 elements apart: 300 of them span 10 GB."""
+    n, apart = 300, 1 << 24
+    c = make(torch.bfloat16, B, 1, 1, n, 4, 1, 64, n, 40, seed=29)
+    c["k"], c["v"] = c["k"][:1], c["v"][:1]
+    whole = torch.empty(n * apart, dtype=torch.bfloat16, device=DEV)
+    views = []
+    for i, x in enumerate((c["kp"], c["vp"], c["k"], c["v"])):
+        views.append(whole.as_strided((1, n, 1, 64), (n * apart, apart, 64, 1), 64 * i))
+        views[-1].copy_(x)
+    if paged:
+        c["slots"] = torch.from_numpy(np.random.default_rng(1).permutation(n).astype(np.int32))[None]
+    got = pipeline.prefix_read(dev(c["q"]), views[0], views[1], views[2], views[3], dev(c["ids"]), dev(c["lens"]),
+                               prefix_slots=dev(c["slots"]), return_lse=True)
+    compare(got, want(c), c)
+
+
+def test_a_chunk_of_a_prompt():
+    """Query rows by the thousand (a few checked): many column blocks."""
+    c = make(torch.bfloat16, 1, 2500, 1, 500, 8, 2, 128, 30, 6, seed=31)
+    got = call(c)
+    rows = [0, 1, 77, 1023, 1024, 2047, 2499]
+    few = dict(c, q=c["q"][:, rows], ids=c["ids"][:, rows], lens=c["lens"][:, rows])
+    compare((got[0][:, rows], got[1][:, rows]), want(few), few)
+
+
+@pytest.mark.parametrize("B,Tq,P,per_head,pool,own", [(5, 3, 1, False, False, True), (6, 1, 6, True, False, True),
+                                                      (4, 2, 3, True, True, True), (5, 1, 5, False, False, False)])
+def test_in_slabs_of_rows(monkeypatch, B, Tq, P, per_head, pool, own):
+    c = make(torch.bfloat16, B, Tq, P, 90, 8, 2, 64, 30, 9, per_head, seed=37)
+    if pool:
+        c["k"], c["v"] = c["k"][:1], c["v"][:1]
+    if not own:
+        c["k"] = None
+    if P == B:
+        c["prow"] = torch.arange(B, dtype=torch.int32)
+    exact = want(c)
+    if P == B:
+        c["prow"] = None
+    monkeypatch.setattr(shared_prefix, "_SLAB_BYTES", 1)
+    compare(call(c), exact, c)
