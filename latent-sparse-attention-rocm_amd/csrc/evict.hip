@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kKeepThreads = 1024;
 constexpr int kKeepWaves = kKeepThreads / LSA_WAVE;
+constexpr int kSlabRun = 32, kSlab = kSlabRun * kKeepThreads;
 
 // A weight as an unsigned key of the same order: NaN (0) below -inf, -0 as +0.
 __device__ __forceinline__ uint32_t seen_key(float w) {
@@ -52,7 +53,8 @@ __device__ __forceinline__ int row_length(const KeepArgs& a, int64_t b) {
   return (int)(n < 0 ? 0 : (n > a.T ? a.T : n));
 }
 
-// grid (chunks of T, B). A paged cache's weights are gathered, one 64-byte sector a page and head.
+// grid (chunks of T, B). A paged cache's weights are gathered, one 64-byte sector a page and head: 32 rows
+// of 32768 positions over 8 kv-heads in 10 us (34 MB, 3.4 TB/s).
 __global__ __launch_bounds__(LSA_BLOCK) void seen_keys_kernel(KeepArgs a) {
   const int64_t b = blockIdx.y;
   const int64_t i = (int64_t)blockIdx.x * LSA_BLOCK + threadIdx.x;
@@ -77,133 +79,242 @@ __global__ __launch_bounds__(LSA_BLOCK) void seen_keys_kernel(KeepArgs a) {
 
 // One workgroup a selection.
 //
-// The threshold, the budget's last key, comes from three histograms (11, 11 and 10 bits from the
+// The threshold, the budget's last key, comes from three histograms (10, 11 and 11 bits from the
 // top), each over the keys that share the digits found so far. Weights crowd into few bins (a third
-// of a cache may be exactly zero), and lanes that meet in one bin of LDS wait for each other, so there are eight
-// copies of each histogram, a lane's by its number, side by side: a bin's copies lie in banks of their own.
+// of a cache may be exactly zero), and lanes that meet in one bin of LDS wait for each other, so there
+// are 16 copies of the first histogram and 8 of the others, a lane's by its number, side by side: a bin's
+// copies lie in banks of their own.
 //
-//   keep_kernel       rows of up to 32768 positions: a thread holds R in a line, turned through LDS
-//                     after coalesced loads. A CU's vector unit is what bounds it (one CU works on
+//   keep_kernel       rows of up to 32768 positions: a wave holds R times 64 in a line, a lane every 64th,
+//                     so ranks are bit counts of what the wave's comparisons leave and no key moves
+//                     between threads. A CU's vector unit is what bounds it (one CU works on
 //                     a selection), so a key costs few instructions: the first and last positions
 //                     are the largest key, those past the row the least, and no loop asks which is
-//                     which; one scan over the threads' counts ranks everything.
+//                     which; one scan over the waves' counts ranks everything. 8 selections of 8192 from
+//                     32768 take 15 us, 128 take 17: in the kernel 2.5 us until the keys are there, 2.0,
+//                     2.3 and 1.4 for the digits, 2.5 to rank and write. (With a line of positions a thread,
+//                     turned through LDS, and eight copies of 11 bits first: 21 us.)
 //   keep_slab_kernel  longer rows, a workgroup a slab of 32768, four launches: a histogram each, then the
-//                     ranks.
-constexpr int kBins = 2048, kCopies = 8;
+//                     ranks. 131072 positions of 8 kv-heads: about 30 us.
+constexpr int kBins = 2048, kHist = 8 * kBins;  // bins at most, and ints of a histogram's copies
+
+template <int PASS>
+struct KeepDigit {
+  static constexpr int BITS = PASS == 0 ? 10 : 11, SHIFT = PASS == 0 ? 22 : (PASS == 1 ? 11 : 0);
+  static constexpr int BINS = 1 << BITS, COPIES = kHist / BINS;
+  static constexpr int PER = BINS / kKeepThreads;  // bins of a thread: BINS - 1 - PER tid, and the one below
+};
 
 struct KeepLds {
-  alignas(16) int hist[kBins][kCopies];
-  int wave_gt[kKeepWaves], wave_eq[kKeepWaves];
+  alignas(16) int hist[2][kHist];  // one is cleared while the other counts
+  int wave[2][kKeepWaves];
   uint32_t digit;
   int need;
 };
 
-// Exclusive sums over the workgroup's threads of two counts; every thread calls it.
-__device__ __forceinline__ void keep_scan(KeepLds& sh, int& gt, int& eq, int& all_gt, int& all_eq) {
-  const int lane = threadIdx.x & (LSA_WAVE - 1), w = threadIdx.x / LSA_WAVE;
-  const int ig = wave_inclusive_sum(gt), ie = wave_inclusive_sum(eq);
-  if (lane == LSA_WAVE - 1) {
-    sh.wave_gt[w] = ig;
-    sh.wave_eq[w] = ie;
-  }
+// Of a value that each wave has (the same in its lanes): the sum over the waves before this one, and over all.
+// Every thread calls them; a barrier lies between two uses of one `slot`.
+__device__ __forceinline__ int keep_wave_values(KeepLds& sh, int slot, int value) {
+  const int lane = threadIdx.x % LSA_WAVE;
+  if (lane == 0) sh.wave[slot][threadIdx.x / LSA_WAVE] = value;
   __syncthreads();
-  int bg = 0, be = 0;
-  all_gt = all_eq = 0;
-#pragma unroll
-  for (int y = 0; y < kKeepWaves; ++y) {
-    const int cg = sh.wave_gt[y], ce = sh.wave_eq[y];
-    bg += y < w ? cg : 0;
-    be += y < w ? ce : 0;
-    all_gt += cg;
-    all_eq += ce;
-  }
-  __syncthreads();
-  gt = bg + ig - gt;
-  eq = be + ie - eq;
+  return lane < kKeepWaves ? sh.wave[slot][lane] : 0;
+}
+__device__ __forceinline__ int keep_waves_before(KeepLds& sh, int slot, int value) {
+  const int x = keep_wave_values(sh, slot, value);
+  return wave_sum(threadIdx.x % LSA_WAVE < threadIdx.x / LSA_WAVE ? x : 0);
+}
+__device__ __forceinline__ int keep_waves_all(KeepLds& sh, int slot, int value) {
+  return wave_sum(keep_wave_values(sh, slot, value));
 }
 
-// The bin that the `need`-th key from the top is in, given every thread's counts (bins 2047 - 2 t and
-// 2046 - 2 t): its digit, and how many of its keys are needed.
+// The bin that the `need`-th key from the top is in, given every thread's counts: its digit, and how
+// many of its keys are needed. Ends with a barrier.
+template <int PASS>
 __device__ __forceinline__ void keep_digit(KeepLds& sh, int need, const int (&c)[2]) {
-  const int tid = threadIdx.x;
-  int none = 0, mine = c[0] + c[1], total, unused;
-  const int own = mine;
-  keep_scan(sh, mine, none, total, unused);
+  using D = KeepDigit<PASS>;
+  const int own = D::PER == 2 ? c[0] + c[1] : c[0], to = wave_inclusive_sum(own);
+  const int mine = keep_waves_before(sh, 0, __builtin_amdgcn_readlane(to, LSA_WAVE - 1)) + to - own;
   if (mine < need && need <= mine + own) {
-    const int e = mine + c[0] < need ? 1 : 0;
-    sh.digit = (uint32_t)(kBins - 1 - 2 * tid - e);
+    const int e = D::PER == 2 && mine + c[0] < need ? 1 : 0;
+    sh.digit = (uint32_t)(D::BINS - 1 - D::PER * (int)threadIdx.x - e);
     sh.need = need - mine - (e ? c[0] : 0);
   }
   __syncthreads();
 }
-__device__ __forceinline__ void keep_clear(KeepLds& sh) {
-  int4* h = (int4*)&sh.hist[0][0];
+__device__ __forceinline__ void keep_clear(int* hist) {  // no barrier
+  int4* h = (int4*)hist;
 #pragma unroll
-  for (int i = 0; i < kCopies * kBins / 4 / kKeepThreads; ++i) h[i * kKeepThreads + threadIdx.x] = make_int4(0, 0, 0, 0);
-  __syncthreads();
+  for (int i = 0; i < kHist / 4 / kKeepThreads; ++i) h[i * kKeepThreads + threadIdx.x] = make_int4(0, 0, 0, 0);
 }
 
+// The first of the wave's positions, and a lane's e-th.
 template <int R>
-struct KeepTurn {
-  static constexpr int PAD = R > 4 ? 4 : 0;  // dwords a thread's run is kept apart: 16-byte reads without conflicts
-  static __host__ __device__ constexpr int at(int i) { return i + (int)((unsigned)i / R) * PAD; }
-  union {
-    uint32_t key[kKeepThreads * (R + PAD)];
-    int32_t place[kKeepThreads * R];  // the positions in their new order
-    KeepLds sh;
-  };
-};
+__device__ __forceinline__ int keep_base(int p0) {
+  return p0 + __builtin_amdgcn_readfirstlane(threadIdx.x / LSA_WAVE) * (R * LSA_WAVE);
+}
+__device__ __forceinline__ int keep_at(int base, int e) { return base + e * LSA_WAVE + (int)(threadIdx.x % LSA_WAVE); }
 
-// The thread's run of R keys of the positions from p0 on: the first and last of the row are the largest
-// key, which no weight equals, positions past it the least. Contains barriers.
+// The keys of the thread's R positions (keep_at) from p0 on: the first and last of the row are the largest
+// key, which no weight equals, positions past it the least. The histograms are cleared while the keys are on
+// their way.
 template <int R>
-__device__ __forceinline__ void keep_load(KeepTurn<R>& turn, const KeepArgs& a, int64_t u, int64_t b, int g, int n, int p0,
+__device__ __forceinline__ void keep_load(KeepLds& sh, const KeepArgs& a, int64_t u, int64_t b, int g, int n, int p0,
                                           uint32_t (&x)[R]) {
-  using Turn = KeepTurn<R>;
-  const int tid = threadIdx.x;
-  const float* mass = a.mass + b * a.mass_sb + g * a.mass_sh;
-  const uint32_t* keys = a.keys ? a.keys + u * a.T : nullptr;
-  uint32_t in[R];
+  const int base = keep_base<R>(p0);
+  const uint32_t* src = a.keys ? a.keys + u * a.T : (const uint32_t*)(a.mass + b * a.mass_sb + g * a.mass_sh);
+  if ((int64_t)base + R * LSA_WAVE <= a.T) {  // uniform
+    src += base;
 #pragma unroll
-  for (int e = 0; e < R; ++e) {  // unconditional (clamped): all in flight
-    const int i = min(p0 + e * kKeepThreads + tid, n - 1);
-    in[e] = keys ? keys[i] : __float_as_uint(mass[i]);
+    for (int e = 0; e < R; ++e) x[e] = src[keep_at(0, e)];
+  } else {
+#pragma unroll
+    for (int e = 0; e < R; ++e) x[e] = src[min((int64_t)keep_at(base, e), a.T - 1)];
   }
-  uint32_t* to = &turn.key[Turn::at(tid)];
-#pragma unroll
-  for (int e = 0; e < R; ++e)
-    to[Turn::at(e * kKeepThreads)] = keys ? in[e] : seen_key(__uint_as_float(in[e]));
+  keep_clear(sh.hist[0]);
+  keep_clear(sh.hist[1]);
   __syncthreads();
-  const int end = R * kKeepThreads;
-  for (int i = tid; i < min(a.sink - p0, end); i += kKeepThreads) turn.key[Turn::at(i)] = 0xFFFFFFFFu;
-  for (int i = max(n - a.window - p0, 0) + tid; i < end; i += kKeepThreads)
-    turn.key[Turn::at(i)] = p0 + i < n ? 0xFFFFFFFFu : 0u;
-  __syncthreads();
+  if (!a.keys) {
+    uint32_t top = 0;
 #pragma unroll
-  for (int e = 0; e < R; e += 4) {
-    const uint4 y = *(const uint4*)&turn.key[tid * (R + Turn::PAD) + e];
-    x[e] = y.x; x[e + 1] = y.y; x[e + 2] = y.z; x[e + 3] = y.w;
+    for (int e = 0; e < R; ++e) top = max(top, x[e]);
+    if (!__any(top > 0x7F800000u)) {  // neither NaN nor a sign
+#pragma unroll
+      for (int e = 0; e < R; ++e) x[e] |= 0x80000000u;
+    } else {
+#pragma unroll
+      for (int e = 0; e < R; ++e) x[e] = seen_key(__uint_as_float(x[e]));
+    }
+  }
+  const int last = n - a.window;
+  if (base < a.sink || base + R * LSA_WAVE > last) {  // uniform
+#pragma unroll
+    for (int e = 0; e < R; ++e) {
+      const int i = keep_at(base, e);
+      x[e] = i < a.sink || i >= last ? 0xFFFFFFFFu : x[e];
+      x[e] = i < n ? x[e] : 0u;
+    }
+  }
+}
+
+// Counts digit PASS of the keys that share `thr` in the ones before. Ends with a barrier. Positions past
+// the row are counted, as the least key; there are enough of the row's own before they would matter.
+template <int R, int PASS>
+__device__ __forceinline__ void keep_count(KeepLds& sh, const uint32_t (&x)[R], uint32_t thr) {
+  using D = KeepDigit<PASS>;
+  int* hist = &sh.hist[PASS % 2][threadIdx.x % D::COPIES];
+  constexpr int E = PASS == 2 ? 4 : 1;  // few share two digits: four keys are asked at once
+  constexpr uint32_t UP = PASS == 0 ? ~0u : (1u << KeepDigit<PASS == 0 ? 0 : PASS - 1>::SHIFT) - 1;
+#pragma unroll
+  for (int e0 = 0; e0 < R; e0 += E) {
+    uint32_t off = x[e0] ^ thr;
+#pragma unroll
+    for (int e = 1; e < E; ++e) off = min(off, x[e0 + e] ^ thr);
+    if (PASS == 0 || off <= UP) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (E == 1 || (x[e0 + e] ^ thr) <= UP) atomicAdd(&hist[((x[e0 + e] >> D::SHIFT) & (D::BINS - 1)) * D::COPIES], 1);
+      }
+    }
   }
   __syncthreads();
 }
 
-// Counts the digits at `shift` of the keys that share `thr` under `mask`. Ends with a barrier. Positions past the
-// row are counted, as the least key; there are enough of the row's own before they would matter.
+// What the wave holds above and at the threshold.
 template <int R>
-__device__ __forceinline__ void keep_count(KeepLds& sh, const uint32_t (&x)[R], uint32_t mask, uint32_t thr, int shift) {
-  int* hist = &sh.hist[0][threadIdx.x % kCopies];
+__device__ __forceinline__ void keep_above(const uint32_t (&x)[R], uint32_t thr, int& gt, int& eq) {
+  gt = eq = 0;
 #pragma unroll
   for (int e = 0; e < R; ++e) {
-    if ((x[e] & mask) == thr) atomicAdd(&hist[((x[e] >> shift) & (kBins - 1)) * kCopies], 1);
+    gt += x[e] > thr;
+    eq += x[e] == thr;
   }
-  __syncthreads();
+  const int both = wave_sum(gt | eq << 16);  // of 2048 at most
+  gt = both & 0xFFFF;
+  eq = both >> 16;
+}
+
+// Writes what the wave's positions become, given how many positions before them are above the threshold
+// and at it (TIES: some of its own are). Positions past the row tie with NaN alone, and come after every
+// position of the row.
+template <int R, bool TABLE, bool TIES>
+__device__ __forceinline__ void keep_place(const KeepArgs& a, const uint32_t (&x)[R], int base, int n, int keep, uint32_t thr,
+                                           int ties, int gt, int eq, int32_t* kept, const int32_t* table,
+                                           int32_t* new_table) {
+  int first = gt + min(eq, ties);  // kept positions before these
+  constexpr int E = R < 8 ? R : 8;
+#pragma unroll
+  for (int e0 = 0; e0 < R; e0 += E) {
+    int32_t y[E];
+    if (TABLE) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[e] = table[min((int64_t)keep_at(base, e0 + e), a.T - 1)];
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint32_t z = x[e0 + e];
+      const int i = keep_at(base, e0 + e);
+      bool in = z > thr;
+      if (TIES) {
+        const uint64_t same = __ballot(z == thr);
+        const int tie = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, eq));
+        in = z >= thr && (z != thr || tie < ties);
+        eq += __popcll(same);
+      }
+      const uint64_t take = __ballot(in);
+      const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(take >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)take, first));
+      first += __popcll(take);
+      if (in) kept[rank] = i;
+      if (TABLE && i < a.T) new_table[in ? rank : (i < n ? keep + (i - rank) : i)] = y[e];
+    }
+  }
+}
+
+// Ranks and writes, given how many are above the threshold and at it before the workgroup's positions.
+template <int R, bool TABLE>
+__device__ __forceinline__ void keep_write(KeepLds& sh, const KeepArgs& a, const uint32_t (&x)[R], int base, int n, int keep,
+                                           uint32_t thr, int ties, int gt0, int eq0, int32_t* kept, const int32_t* table,
+                                           int32_t* new_table) {
+  int gt, eq;
+  keep_above<R>(x, thr, gt, eq);
+  static_assert(kSlab < 1 << 16, "two counts in a word");
+  const uint32_t before = (uint32_t)keep_waves_before(sh, 0, gt | eq << 16);
+  gt0 += (int)(before & 0xFFFFu);
+  eq0 += (int)(before >> 16);
+  if (eq == 0) keep_place<R, TABLE, false>(a, x, base, n, keep, thr, ties, gt0, eq0, kept, table, new_table);  // uniform
+  else keep_place<R, TABLE, true>(a, x, base, n, keep, thr, ties, gt0, eq0, kept, table, new_table);
+}
+
+// The thread's bins' counts, summed over the copies.
+template <int PASS>
+__device__ __forceinline__ void keep_bins(const KeepLds& sh, int (&c)[2]) {
+  using D = KeepDigit<PASS>;
+  c[1] = 0;
+#pragma unroll
+  for (int e = 0; e < D::PER; ++e) {
+    c[e] = 0;
+#pragma unroll
+    for (int y = 0; y < D::COPIES; y += 4) {
+      const int4 z = *(const int4*)&sh.hist[PASS % 2][(D::BINS - 1 - D::PER * (int)threadIdx.x - e) * D::COPIES + y];
+      c[e] += z.x + z.y + z.z + z.w;
+    }
+  }
+}
+
+template <int R, int PASS>
+__device__ __forceinline__ void keep_pass(KeepLds& sh, const uint32_t (&x)[R], uint32_t& thr, int& ties) {
+  if (PASS == 1) keep_clear(sh.hist[0]);
+  keep_count<R, PASS>(sh, x, thr);
+  int c[2];
+  keep_bins<PASS>(sh, c);
+  keep_digit<PASS>(sh, ties, c);
+  thr |= sh.digit << KeepDigit<PASS>::SHIFT;
+  ties = sh.need;
 }
 
 template <int R, bool TABLE>
 __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
-  using Turn = KeepTurn<R>;
-  __shared__ __attribute__((aligned(16))) Turn turn;
-  KeepLds& sh = turn.sh;
+  __shared__ KeepLds sh;
   const int tid = threadIdx.x;
   const int64_t u = blockIdx.x;
   const int64_t b = u / a.G;
@@ -222,83 +333,85 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
     return;
   }
   uint32_t x[R];
-  keep_load<R>(turn, a, u, b, g, n, 0, x);
-  uint32_t thr = 0, mask = 0;
+  keep_load<R>(sh, a, u, b, g, n, 0, x);
+  uint32_t thr = 0;
   int ties = a.budget;
-#pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
-    keep_clear(sh);
-    keep_count<R>(sh, x, mask, thr, shift);
-    int c[2] = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-#pragma unroll
-      for (int y = 0; y < kCopies; y += 4) {
-        const int4 z = *(const int4*)&sh.hist[kBins - 1 - 2 * tid - e][y];
-        c[e] += z.x + z.y + z.z + z.w;
-      }
-    }
-    keep_digit(sh, ties, c);
-    thr |= sh.digit << shift;
-    ties = sh.need;
-    mask |= (pass == 2 ? 1023u : 2047u) << shift;
-  }
-  int gt = 0, eq = 0, all_gt, all_eq;
-#pragma unroll
-  for (int e = 0; e < R; ++e) {
-    gt += x[e] > thr;
-    eq += x[e] == thr;
-  }
-  keep_scan(sh, gt, eq, all_gt, all_eq);  // kept, and at the threshold, before this thread's positions
-  // positions past the row tie with NaN alone, and come after every position of the row
-  int rank = gt + min(eq, ties);  // kept positions before this one
-#pragma unroll
-  for (int e = 0; e < R; ++e) {
-    const int i = tid * R + e;
-    const bool same = x[e] == thr;
-    const bool in = x[e] > thr || (same && eq < ties);
-    if (TABLE) {
-      if (i < n) turn.place[in ? rank : keep + (i - rank)] = i;
-    } else if (in) {
-      turn.place[rank] = i;
-    }
-    rank += in;
-    eq += same;
-  }
-  __syncthreads();
-  for (int j = tid; j < keep; j += kKeepThreads) kept[j] = turn.place[j];
-  if (TABLE) {
-    constexpr int E = 8;  // entries of a thread in flight
-    for (int64_t i0 = tid; i0 < a.T; i0 += E * kKeepThreads) {
-      int32_t y[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int64_t i = min(i0 + e * kKeepThreads, a.T - 1);
-        y[e] = table[i < n ? turn.place[i] : i];
-      }
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int64_t i = i0 + e * kKeepThreads;
-        if (i < a.T) new_table[i] = y[e];
-      }
-    }
-  }
+  keep_pass<R, 0>(sh, x, thr, ties);
+  keep_pass<R, 1>(sh, x, thr, ties);
+  keep_pass<R, 2>(sh, x, thr, ties);
+  keep_write<R, TABLE>(sh, a, x, keep_base<R>(0), n, keep, thr, ties, 0, 0, kept, table, new_table);
 }
 
 // A row in slabs of 32768 positions, a workgroup a slab; grid (selection, slab). Phases 0, 1 and 2 leave
 // each slab's histogram of their digit, and phases 1, 2 and 3 add the slabs' up and find the digit
 // (slab 0 keeps it for the phases after the next). Phase 3 ranks: what is kept before a slab follows from
 // the earlier slabs' histograms.
-constexpr int kSlabRun = 32, kSlab = kSlabRun * kKeepThreads;
+struct KeepFound {
+  uint32_t thr;  // the digits so far
+  int ties;      // keys needed of those that share them
+  int gt, eq;    // phase 3: above and at the threshold in the slabs before
+};
+
+// Digit Q from the slabs' histograms of it, or as an earlier phase left it.
+template <int Q, int PHASE>
+__device__ __forceinline__ void keep_found(KeepLds& sh, const int* hist, int slab, int slabs, int2* state, KeepFound& f) {
+  using D = KeepDigit<Q>;
+  const int tid = threadIdx.x;
+  int c[2] = {0, 0}, before[2] = {0, 0};  // of all slabs, and of the ones before
+  if (Q == PHASE - 1 || PHASE == 3) {
+    const int* h = hist + D::BINS - D::PER * (tid + 1);
+#pragma unroll 4
+    for (int y = 0; y < slabs; ++y) {
+      int x[2] = {0, 0};
+      if constexpr (D::PER == 2) {
+        const int2 z = *(const int2*)(h + (int64_t)y * kBins);
+        x[0] = z.y; x[1] = z.x;
+      } else {
+        x[0] = h[(int64_t)y * kBins];
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        c[e] += x[e];
+        before[e] += y < slab ? x[e] : 0;
+      }
+    }
+  }
+  if (Q == PHASE - 1) {
+    keep_digit<Q>(sh, f.ties, c);
+    if (PHASE < 3 && slab == 0 && tid == 0) state[Q] = make_int2((int)sh.digit, sh.need);
+  } else {
+    if (tid == 0) {
+      const int2 x = state[Q];
+      sh.digit = (uint32_t)x.x;
+      sh.need = x.y;
+    }
+    __syncthreads();
+  }
+  const uint32_t digit = sh.digit;
+  f.ties = sh.need;
+  f.thr |= digit << D::SHIFT;
+  if (PHASE == 3) {
+    int more = 0, same = 0;
+#pragma unroll
+    for (int e = 0; e < D::PER; ++e) {
+      const uint32_t bin = (uint32_t)(D::BINS - 1 - D::PER * tid - e);
+      more += bin > digit ? before[e] : 0;
+      same += Q == 2 && bin == digit ? before[e] : 0;
+    }
+    f.gt += keep_waves_all(sh, 1, wave_sum(more));
+    if (Q == 2) {
+      __syncthreads();
+      f.eq = keep_waves_all(sh, 1, wave_sum(same));
+    }
+  }
+  __syncthreads();  // the digit is read before the next takes its place
+}
 
 template <int PHASE, bool TABLE>
 __global__ __launch_bounds__(kKeepThreads) void keep_slab_kernel(KeepArgs a) {
   constexpr int R = kSlabRun;
-  using Turn = KeepTurn<R>;
-  __shared__ __attribute__((aligned(16))) Turn turn;
-  KeepLds& sh = turn.sh;
-  const int tid = threadIdx.x, lane = tid & (LSA_WAVE - 1);
+  __shared__ KeepLds sh;
+  const int tid = threadIdx.x;
   const int64_t u = blockIdx.x;
   const int slab = blockIdx.y, slabs = gridDim.y;
   const int64_t b = u / a.G;
@@ -311,12 +424,9 @@ __global__ __launch_bounds__(kKeepThreads) void keep_slab_kernel(KeepArgs a) {
   if (PHASE == 3) {
     if (g == 0 && slab == 0 && tid == 0) a.new_lengths[b] = keep;
     for (int i = max(p0, keep) + tid; i < min(p1, a.budget); i += kKeepThreads) kept[i] = -1;
-    if (TABLE) {
-      for (int i = max(p0, n) + tid; i < p1; i += kKeepThreads) new_table[i] = table[i];
-    }
     if (n <= a.budget) {  // uniform: all of it
-      for (int i = p0 + tid; i < min(p1, n); i += kKeepThreads) {
-        kept[i] = i;
+      for (int i = p0 + tid; i < p1; i += kKeepThreads) {
+        if (i < n) kept[i] = i;
         if (TABLE) new_table[i] = table[i];
       }
     }
@@ -325,98 +435,22 @@ __global__ __launch_bounds__(kKeepThreads) void keep_slab_kernel(KeepArgs a) {
   int* hist = a.hist + u * slabs * kBins;             // of phase 0, [slab][bin]
   const int64_t phase_hist = (int64_t)gridDim.x * slabs * kBins;
   int2* state = a.state + u * 2;                      // digits (and what they leave needed) of phases 0, 1
-  uint32_t thr = 0, mask = 0;
-  int ties = a.budget, gt0 = 0, eq0 = 0;  // phase 3: above and at the threshold in the slabs before
-#pragma unroll
-  for (int q = 0; q < PHASE; ++q) {
-    const int shift = q == 0 ? 21 : (q == 1 ? 10 : 0);
-    int c[2] = {0, 0}, before[2] = {0, 0};
-    if (q == PHASE - 1 || PHASE == 3) {  // bins 2047 - 2 t and 2046 - 2 t of all slabs, and of the ones before
-      const int2* h = (const int2*)(hist + q * phase_hist + kBins - 2 - 2 * tid);
-      for (int y = 0; y < slabs; ++y) {
-        const int2 x = h[(int64_t)y * kBins / 2];
-        c[0] += x.y;
-        c[1] += x.x;
-        before[0] += y < slab ? x.y : 0;
-        before[1] += y < slab ? x.x : 0;
-      }
-    }
-    if (q == PHASE - 1) {
-      keep_digit(sh, ties, c);
-      if (PHASE < 3 && slab == 0 && tid == 0) state[q] = make_int2((int)sh.digit, sh.need);
-    } else {
-      if (tid == 0) {
-        const int2 x = state[q];
-        sh.digit = (uint32_t)x.x;
-        sh.need = x.y;
-      }
-      __syncthreads();
-    }
-    const uint32_t digit = sh.digit;
-    ties = sh.need;
-    thr |= digit << shift;
-    mask |= (q == 2 ? 1023u : 2047u) << shift;
-    if (PHASE == 3) {
-      int more = 0, same = 0, all_more, all_same;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t bin = (uint32_t)(kBins - 1 - 2 * tid - e);
-        more += bin > digit ? before[e] : 0;
-        same += q == 2 && bin == digit ? before[e] : 0;
-      }
-      keep_scan(sh, more, same, all_more, all_same);
-      gt0 += all_more;
-      eq0 += all_same;
-    }
-    __syncthreads();  // the digit is read before the next takes its place
-  }
+  KeepFound f{0, a.budget, 0, 0};
+  if constexpr (PHASE > 0) keep_found<0, PHASE>(sh, hist, slab, slabs, state, f);
+  if constexpr (PHASE > 1) keep_found<1, PHASE>(sh, hist + phase_hist, slab, slabs, state, f);
+  if constexpr (PHASE > 2) keep_found<2, PHASE>(sh, hist + 2 * phase_hist, slab, slabs, state, f);
   uint32_t x[R];
-  keep_load<R>(turn, a, u, b, g, n, p0, x);
-  if (PHASE < 3) {
-    const int shift = PHASE == 0 ? 21 : (PHASE == 1 ? 10 : 0);
-    keep_clear(sh);
-    keep_count<R>(sh, x, mask, thr, shift);
-    int* out = hist + PHASE * phase_hist + (int64_t)slab * kBins;
-    for (int i = tid; i < kBins; i += kKeepThreads) {
-      int c = 0;
-#pragma unroll
-      for (int y = 0; y < kCopies; y += 4) {
-        const int4 z = *(const int4*)&sh.hist[i][y];
-        c += z.x + z.y + z.z + z.w;
-      }
-      out[i] = c;
-    }
-    return;
-  }
-  int gt = 0, eq = 0, all_gt, all_eq;
-#pragma unroll
-  for (int e = 0; e < R; ++e) {
-    gt += x[e] > thr;
-    eq += x[e] == thr;
-  }
-  keep_scan(sh, gt, eq, all_gt, all_eq);
-  const int first = gt0 + min(eq0, ties);                                  // kept before this slab,
-  const int mine = gt0 + all_gt + min(eq0 + all_eq, ties) - first;         // and in it
-  eq += eq0;
-  int rank = gt0 + gt + min(eq, ties) - first;
-#pragma unroll
-  for (int e = 0; e < R; ++e) {
-    const int i = tid * R + e;
-    const bool same = x[e] == thr;
-    const bool in = x[e] > thr || (same && eq < ties);
-    if (TABLE) {
-      if (p0 + i < n) turn.place[in ? rank : mine + (i - rank)] = p0 + i;
-    } else if (in) {
-      turn.place[rank] = p0 + i;
-    }
-    rank += in;
-    eq += same;
-  }
-  __syncthreads();
-  for (int j = tid; j < mine; j += kKeepThreads) kept[first + j] = turn.place[j];
-  if (TABLE) {
-    const int live = max(0, min(p1, n) - p0), rest = keep + (p0 - first) - mine;  // where what it gives up goes
-    for (int j = tid; j < live; j += kKeepThreads) new_table[j < mine ? first + j : rest + j] = table[turn.place[j]];
+  keep_load<R>(sh, a, u, b, g, n, p0, x);
+  if constexpr (PHASE < 3) {
+    using D = KeepDigit<PHASE>;
+    keep_count<R, PHASE>(sh, x, f.thr);
+    int c[2];
+    keep_bins<PHASE>(sh, c);
+    int* to = hist + PHASE * phase_hist + (int64_t)slab * kBins + D::BINS - D::PER * (tid + 1);
+    if constexpr (D::PER == 2) *(int2*)to = make_int2(c[1], c[0]);
+    else *to = c[0];
+  } else {
+    keep_write<R, TABLE>(sh, a, x, keep_base<R>(p0), n, keep, f.thr, f.ties, f.gt, f.eq, kept, table, new_table);
   }
 }
 
@@ -438,7 +472,8 @@ struct RowsArgs {
   int zero;               // rows past the new length: zeros (else left as they were)
 };
 
-// HBM-bound: each kept row read and written once. grid (rows of the new cache a workgroup, B).
+// HBM-bound: each kept row read and written once (16 caches of 32768 cut to 8192, 1.07 GB moved: 222 us,
+// 4.8 TB/s; one: 12 us). grid (rows of the new cache a workgroup, B).
 __global__ __launch_bounds__(LSA_BLOCK) void keep_rows_kernel(RowsArgs a, int rows_per_block) {
   const int64_t b = blockIdx.y;
   const int j0 = blockIdx.x * rows_per_block;
