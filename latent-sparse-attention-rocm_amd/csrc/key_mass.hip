@@ -10,7 +10,10 @@
 //   mass_add_kernel     turns the scores into weights and adds them. With one query row a cache the last span
 //                       of a list to finish does that within the first launch, if it has counters
 //                       to tell which that is (a launch costs the host 3 us, as much as the rest of a small
-//                       call).
+//                       call). A small call is one chain of latencies: 2564 keys of 8 kv-heads, 9.5 us (1.2
+//                       until the keys' rows are asked for, 2 for their scores, 1.6 to tell who is last, 1 for
+//                       the sums, 4 to add), 640 fp32 keys of 2 kv-heads 7.4.
+//                       32 such rows: 35.5 us, the gather's 4.8 TB/s.
 //
 // A key that a list names twice counts twice; several query rows of one cache add to the same
 // keys. Sums must not depend on the order in which workgroups arrive. With one query row a cache, all
@@ -88,33 +91,54 @@ __device__ __forceinline__ void join(float& m, float& l, float mo, float lo) {
   m = mn;
 }
 
-// What the unit's weights are measured by, a head a thread: the reference m and one over the sum.
+template <int GQ>
+struct WeighLds {
+  float pm[LSA_WAVES][GQ], pl[LSA_WAVES][GQ];
+  float m[GQ], inv[GQ];  // the reference, and one over the sum
+};
+
+// What the unit's weights are measured by, the spans' statistics a span and head a thread. Every thread calls
+// it; a barrier before `sh` is read.
 template <int GQ, bool COHERENT>
 __device__ __forceinline__ void weigh_by(const MassArgs& a, int64_t unit, int64_t row, int g, const MassList& list,
-                                         float* sm, float* sinv) {
-  const int tid = threadIdx.x;
-  if (tid >= GQ) return;
+                                         WeighLds<GQ>& sh) {
+  const int tid = threadIdx.x, lane = tid & (LSA_WAVE - 1), w = tid / LSA_WAVE;
   float m = kNegBig, l = 0.0f;
   if (a.lse) {
-    m = a.lse[row * a.Hq + g * GQ + tid] * kLog2e;
-    l = m > -INFINITY ? 1.0f : 0.0f;  // no keys at all, or not a number: no weight
+    if (tid < GQ) {
+      m = a.lse[row * a.Hq + g * GQ + tid] * kLog2e;
+      l = m > -INFINITY ? 1.0f : 0.0f;  // no keys at all, or not a number: no weight
+    }
   } else {
     const int n_act = (list.n + a.span - 1) / a.span;
-#pragma unroll 4
-    for (int s = 0; s < n_act; ++s) {
-      const float* st = a.stats + ((unit * a.n_span + s) * GQ + tid) * 2;
-      if constexpr (COHERENT) join(m, l, coherent_load(st), coherent_load(st + 1));
-      else join(m, l, st[0], st[1]);
+    const float* st = a.stats + unit * a.n_span * (GQ * 2);
+    for (int i = tid; i < n_act * GQ; i += LSA_BLOCK) {
+      if constexpr (COHERENT) join(m, l, coherent_load(st + 2 * i), coherent_load(st + 2 * i + 1));
+      else join(m, l, st[2 * i], st[2 * i + 1]);
+    }
+#pragma unroll
+    for (int x = GQ; x < LSA_WAVE; x <<= 1) join(m, l, lane_xor(m, x), lane_xor(l, x));
+    if (n_act * GQ > LSA_WAVE) {  // uniform: more than the first wave's
+      if (lane < GQ) {
+        sh.pm[w][lane] = m;
+        sh.pl[w][lane] = l;
+      }
+      __syncthreads();
+      if (tid < GQ) {
+#pragma unroll
+        for (int y = 1; y < LSA_WAVES; ++y) join(m, l, sh.pm[y][tid], sh.pl[y][tid]);
+      }
     }
   }
-  sm[tid] = m;
-  sinv[tid] = l > 0.0f ? 1.0f / l : 0.0f;  // a sum that is not a number counts as none, as in the read
+  if (tid < GQ) {
+    sh.m[tid] = m;
+    sh.inv[tid] = l > 0.0f ? 1.0f / l : 0.0f;  // a sum that is not a number counts as none, as in the read
+  }
 }
 
-// Slot j's weight, the heads together.
+// Slot j's scores, and its weight, the heads together.
 template <int GQ, bool COHERENT>
-__device__ __forceinline__ float weight_of(const float* scores, int64_t j, const float* sm, const float* sinv) {
-  float s[GQ];
+__device__ __forceinline__ void scores_of(const float* scores, int64_t j, float (&s)[GQ]) {
   if constexpr (COHERENT && GQ % 4 == 0) {
 #pragma unroll
     for (int h = 0; h < GQ; h += 4) {
@@ -125,11 +149,14 @@ __device__ __forceinline__ float weight_of(const float* scores, int64_t j, const
 #pragma unroll
     for (int h = 0; h < GQ; ++h) s[h] = COHERENT ? coherent_load(scores + j * GQ + h) : scores[j * GQ + h];
   }
+}
+template <int GQ>
+__device__ __forceinline__ float weight_of(const float (&s)[GQ], const WeighLds<GQ>& sh) {
   float sum = 0.0f;
 #pragma unroll
   for (int h = 0; h < GQ; ++h) {
-    const float x = fast_exp2(s[h] - sm[h]) * sinv[h];
-    sum += sinv[h] > 0.0f && x > 0.0f ? fminf(x, kMaxWeight) : 0.0f;
+    const float x = fast_exp2(s[h] - sh.m[h]) * sh.inv[h];
+    sum += sh.inv[h] > 0.0f && x > 0.0f ? fminf(x, kMaxWeight) : 0.0f;
   }
   return sum;
 }
@@ -143,7 +170,7 @@ struct MassShape {
   static constexpr int LPT = D / VEC;                    // lanes that load a token
   static constexpr int TPW = MM ? 16 : LSA_WAVE / LPT;   // tokens of a wave's step
   static constexpr int LD = MM ? D / 32 : 1;             // 16-byte loads a lane a step
-  static constexpr int U = MM ? (D == 256 ? 2 : 4) : 16; // steps in flight
+  static constexpr int U = MM ? (D == 256 ? 2 : 4) : 4;  // steps in flight
   static constexpr int TW = TPW * U;                     // tokens of a wave's turn
   static constexpr int NT = LSA_WAVES * TW;
 };
@@ -174,8 +201,9 @@ void mass_scores_kernel(MassArgs a) {
     if (sp >= max(n_act, 1)) return;
     if (a.zero) {  // this span's share of the unit's own weights, which no other unit adds to
       float* m = a.mass + (a.caches > 1 ? row / a.Tq : 0) * a.m_sb + g * a.m_sh;
-      const int64_t share = (a.Tk + max(n_act, 1) - 1) / max(n_act, 1), k1 = min(share * (sp + 1), a.Tk);
-      for (int64_t i = share * sp + tid; i < k1; i += LSA_BLOCK) coherent_store(m + i, 0.0f);
+      const uint32_t n_all = (uint32_t)a.Tk, share = (n_all - 1) / (uint32_t)max(n_act, 1) + 1;  // 32 bits
+      const int64_t k0 = (int64_t)share * sp, k1 = min(k0 + share, a.Tk);
+      for (int64_t i = k0 + tid; i < k1; i += LSA_BLOCK) coherent_store(m + i, 0.0f);
     }
   } else if (a.zero || a.whole) {  // this workgroup's share of the weights, and of the integers
     const int64_t grid = (int64_t)gridDim.x * gridDim.y * LSA_BLOCK;
@@ -348,22 +376,47 @@ void mass_scores_kernel(MassArgs a) {
   }
   if (!a.counters) return;
   __shared__ int flag;
-  __shared__ float wm[GQ], winv[GQ];
+  __shared__ WeighLds<GQ> by;
   if (!arrive_last(&a.counters[unit], n_act, &flag)) return;
-  weigh_by<GQ, true>(a, unit, row, g, list, wm, winv);
-  __syncthreads();
+  // E slots of a thread at once, and two steps' scores loaded ahead: a load comes back after the atomics
+  // issued before it (one slot at a time: 8 us of 12 for a list of 2564)
+  constexpr int E = GQ == 8 ? 2 : 4, AHEAD = 3, STEP = E * LSA_BLOCK;
   float* mass = a.mass + c * a.m_sb + g * a.m_sh;
-  for (int j = tid; j < list.n; j += LSA_BLOCK) {
-    const int32_t id = list.ids[j];
-    const float sum = weight_of<GQ, true>(scores, j, wm, winv);
-    if (id >= 0 && id < a.Tk && sum > 0.0f) atomicAdd(mass + id, sum);
+  int32_t id[AHEAD][E];
+  float s[AHEAD][E][GQ];
+  auto load = [&](int j0, int (&id)[E], float (&s)[E][GQ]) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int j = min(j0 + e * LSA_BLOCK + tid, list.n - 1);
+      id[e] = list.ids[j];
+      scores_of<GQ, true>(scores, j, s[e]);
+    }
+  };
+  load(0, id[0], s[0]);
+  load(STEP, id[1], s[1]);
+  weigh_by<GQ, true>(a, unit, row, g, list, by);
+  __syncthreads();
+  for (int i = 0; i < list.n; i += AHEAD * STEP) {
+#pragma unroll
+    for (int x = 0; x < AHEAD; ++x) {
+      const int j0 = i + x * STEP;
+      if (j0 >= list.n) break;  // uniform
+      load(j0 + 2 * STEP, id[(x + 2) % AHEAD], s[(x + 2) % AHEAD]);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float sum = weight_of<GQ>(s[x][e], by);
+        if (j0 + e * LSA_BLOCK + tid < list.n && id[x][e] >= 0 && id[x][e] < a.Tk && sum > 0.0f)
+          atomicAdd(mass + id[x][e], sum);
+      }
+    }
   }
 }
 
-// grid (row * Hkv, slots / 256).
+// grid (row * Hkv, slots / 256). Bound by the rate of 64-bit atomics: 64 rows of about 4096 keys on 8
+// kv-heads, 2.1 M additions, take 19 us (four slots a thread 20).
 template <int GQ>
 __global__ __launch_bounds__(LSA_BLOCK) void mass_add_kernel(MassArgs a) {
-  __shared__ float sm[GQ], sinv[GQ];
+  __shared__ WeighLds<GQ> by;
   const int tid = threadIdx.x;
   const int64_t unit = blockIdx.x;
   const int64_t row = unit / a.Hkv;
@@ -371,15 +424,16 @@ __global__ __launch_bounds__(LSA_BLOCK) void mass_add_kernel(MassArgs a) {
   const MassList list = mass_list(a, row, g);
   const int j = blockIdx.y * LSA_BLOCK + tid;
   if (blockIdx.y * LSA_BLOCK >= list.n) return;
-  weigh_by<GQ, false>(a, unit, row, g, list, sm, sinv);
+  float s[GQ];
+  const int at = min(j, list.n - 1);
+  const int32_t id = list.ids[at];
+  scores_of<GQ, false>(a.scores + unit * (int64_t)a.W * GQ, at, s);
+  weigh_by<GQ, false>(a, unit, row, g, list, by);
   __syncthreads();
-  if (j >= list.n) return;
-  const int32_t id = list.ids[j];
-  if (id < 0 || id >= a.Tk) return;
-  const float sum = weight_of<GQ, false>(a.scores + unit * (int64_t)a.W * GQ, j, sm, sinv);
+  if (j >= list.n || id < 0 || id >= a.Tk) return;
+  const float sum = weight_of<GQ>(s, by);
   if (!(sum > 0.0f)) return;
-  const int64_t b = row / a.Tq;
-  const int64_t c = a.caches > 1 ? b : 0;
+  const int64_t c = a.caches > 1 ? row / a.Tq : 0;
   if (a.fixed) {
     atomicAdd((unsigned long long*)a.fixed + (c * a.Hkv + g) * a.Tk + id,
               (unsigned long long)__float2ull_rn(sum * kFix));
@@ -416,7 +470,7 @@ __global__ __launch_bounds__(LSA_BLOCK) void mass_fold_kernel(MassArgs a) {
 }
 
 int mass_span(int dtype, int D, int64_t units, int W) {
-  const int nt = LSA_WAVES * (dtype == LSA_F32 ? LSA_WAVE / (D / 4) * 16 : (D == 256 ? 32 : 64));  // MassShape::NT
+  const int nt = LSA_WAVES * (dtype == LSA_F32 ? LSA_WAVE / (D / 4) * 4 : (D == 256 ? 32 : 64));  // MassShape::NT
   const int64_t want = std::max<int64_t>(1, 1024 / std::max<int64_t>(units, 1));  // workgroups a list
   const int tiles = (W + nt - 1) / nt;
   const int per = (int)((tiles + want - 1) / want);
