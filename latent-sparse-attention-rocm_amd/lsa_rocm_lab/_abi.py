@@ -200,8 +200,11 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-# torch's own query of a stream's handle; not part of its public interface
+# torch's own queries (a stream's handle, the current device, a capture), without the check that the GPU
+# runtime is up, which a tensor on it has shown; not part of its public interface
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
 
 def stream(device: torch.device | None = None) -> int:
@@ -263,8 +266,8 @@ def call_memory(device: torch.device, purpose: str, nbytes: int, n_counters: int
     afterwards or None, counters or None, the stream). They are ``Workspace``'s and ``Counters``',
     or, while a HIP graph is captured, scratch of that graph's own pool and no counters, so that
     graphs captured on one stream may be replayed on several at once."""
-    here = stream(device)
-    if torch.cuda.is_current_stream_capturing():
+    here = stream(device) if _raw_stream is None else _raw_stream(device.index)
+    if _capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None, None, here
     ws = count = None
     if nbytes:

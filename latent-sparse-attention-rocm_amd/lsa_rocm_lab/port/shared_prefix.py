@@ -20,21 +20,22 @@ _SLAB_BYTES = 256 << 20  # partials held at once (more query rows go through in 
 
 def launch_device(device: torch.device):
     """A context in which a launch on a tensor's ``device`` finds it current (nothing where it is)."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == _abi.current_device() else torch.cuda.device(device)
 
 
 def one_device(what: str, *tensors: torch.Tensor | None) -> torch.device:
     """The ROCm device that all of the tensors are on; anything else raises ``ValueError``."""
     device = tensors[0].device
-    for t in tensors:
-        if t is not None and (t.device != device or device.type != "cuda"):
+    index = device.index if device.type == "cuda" else -1
+    for t in tensors:  # an int compares in a fraction of a device's time
+        if t is not None and (index < 0 or (t.get_device() != index and t.device != device)):
             raise ValueError(f"{what} is a ROCm kernel over tensors of one device, got {device} and {t.device}")
     return device
 
 
 def int32_on(t: torch.Tensor, device: torch.device) -> torch.Tensor:
     """``t`` as a kernel reads it: int32, contiguous, on ``device``."""
-    if t.dtype == torch.int32 and t.device == device and t.is_contiguous():
+    if t.dtype is torch.int32 and t.get_device() == device.index and t.is_contiguous():
         return t
     return t.to(device=device, dtype=torch.int32).contiguous()
 
