@@ -35,7 +35,7 @@ def one_device(what: str, *tensors: torch.Tensor | None) -> torch.device:
 
 def int32_on(t: torch.Tensor, device: torch.device) -> torch.Tensor:
     """``t`` as a kernel reads it: int32, contiguous, on ``device``."""
-    if t.dtype is torch.int32 and t.get_device() == device.index and t.is_contiguous():
+    if t.dtype is torch.int32 and (t.get_device() == device.index or t.device == device) and t.is_contiguous():
         return t
     return t.to(device=device, dtype=torch.int32).contiguous()
 
