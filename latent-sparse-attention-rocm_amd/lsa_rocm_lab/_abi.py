@@ -170,6 +170,16 @@ def call(name: str, *args):
     return rc
 
 
+_in_order = threading.Lock()
+
+
+def call_in_order(name: str, *args):
+    """``call`` for an entry point of several launches over scratch that a stream's calls share: no
+    other thread's launches on that stream come between this call's (ctypes drops the GIL)."""
+    with _in_order:
+        return call(name, *args)
+
+
 def size(name: str, *args) -> int:
     return int(getattr(load(), name)(*args))
 

@@ -94,10 +94,11 @@ def key_mass(
                 plse = None if lse is None else lse[:, t:t + n].contiguous()
             nbytes = _abi.shape_size("lsa_key_mass_scratch_bytes", dt, B, n, caches, Tk, Hq, Hkv, D, W)
             ws, counters, stream = _abi.call_memory(device, "key_mass", nbytes, B * Hkv if n == 1 and caches == B else 0)
-            _abi.call("lsa_key_mass", part.data_ptr(), k.data_ptr(), dt, B, n, caches, Tk, Hq, Hkv, D, sb, st, sh,
-                      pids.data_ptr(), plens.data_ptr(), W, 1 if per_head else 0, scale, _abi.ptr(plse),
-                      1 if fresh and t == 0 else 0, _abi.ptr(counters), _abi.ptr(ws), nbytes, mass.data_ptr(),
-                      mass.stride(0) if caches > 1 else Hkv * Tk, mass.stride(1) if Hkv > 1 else Tk, stream)
+            _abi.call_in_order("lsa_key_mass", part.data_ptr(), k.data_ptr(), dt, B, n, caches, Tk, Hq, Hkv, D, sb, st,
+                               sh, pids.data_ptr(), plens.data_ptr(), W, 1 if per_head else 0, scale, _abi.ptr(plse),
+                               1 if fresh and t == 0 else 0, _abi.ptr(counters), _abi.ptr(ws), nbytes,
+                               mass.data_ptr(), mass.stride(0) if caches > 1 else Hkv * Tk,
+                               mass.stride(1) if Hkv > 1 else Tk, stream)
     return mass
 
 
@@ -194,9 +195,9 @@ def evict(
         nbytes = _abi.shape_size("lsa_evict_scratch_bytes", B, Hkv, T, one)
         with launch_device(device):
             ws, _, stream = _abi.call_memory(device, "evict", nbytes)
-            _abi.call("lsa_evict_keep", mass.data_ptr(), B, Hkv, T, mass.stride(0), mass.stride(1), _abi.ptr(lens),
-                      budget, window, sink, one, None, 0, 0, _abi.ptr(ws), nbytes, kept.data_ptr(),
-                      new_lengths.data_ptr(), None, 0, stream)
+            _abi.call_in_order("lsa_evict_keep", mass.data_ptr(), B, Hkv, T, mass.stride(0), mass.stride(1),
+                               _abi.ptr(lens), budget, window, sink, one, None, 0, 0, _abi.ptr(ws), nbytes,
+                               kept.data_ptr(), new_lengths.data_ptr(), None, 0, stream)
             _abi.call("lsa_evict_rows", k.data_ptr(), v.data_ptr(), mass.data_ptr(), dt, B, T, Hkv, D, sb, st, sh,
                       mass.stride(0), mass.stride(1), kept.data_ptr(), one, budget, k2.data_ptr(), v2.data_ptr(), ob,
                       ot, oh, m2.data_ptr(), m2.stride(0), m2.stride(1), 1 if out is None else 0, stream)
@@ -243,7 +244,7 @@ def evict_slots(
         nbytes = _abi.shape_size("lsa_evict_scratch_bytes", R, Hkv, T, 1)
         with launch_device(device):
             ws, _, stream = _abi.call_memory(device, "evict", nbytes)
-            _abi.call("lsa_evict_keep", mass.data_ptr(), R, Hkv, T, 0, mass.stride(1), _abi.ptr(lens), budget, window,
-                      sink, 1, table.data_ptr(), T, pool, _abi.ptr(ws), nbytes, kept.data_ptr(),
-                      new_lengths.data_ptr(), new_table.data_ptr(), T, stream)
+            _abi.call_in_order("lsa_evict_keep", mass.data_ptr(), R, Hkv, T, 0, mass.stride(1), _abi.ptr(lens), budget,
+                               window, sink, 1, table.data_ptr(), T, pool, _abi.ptr(ws), nbytes, kept.data_ptr(),
+                               new_lengths.data_ptr(), new_table.data_ptr(), T, stream)
     return new_table, new_lengths, kept

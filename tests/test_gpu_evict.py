@@ -139,6 +139,19 @@ def test_key_mass_in_slabs_of_rows(monkeypatch):
         monkeypatch.undo()
 
 
+@pytest.mark.parametrize("dtype,Hq,Hkv,D", [(torch.bfloat16, 4, 1, 64), (torch.float16, 8, 1, 128), (torch.float32, 8, 2, 64),
+                                            (torch.bfloat16, 2, 2, 32)])
+@pytest.mark.parametrize("Tq", [1, 3])
+def test_key_mass_of_long_lists(dtype, Hq, Hkv, D, Tq):
+    """Lists of many spans: their sums join, and one workgroup adds slots in several steps."""
+    q, k, ids, lens = make(dtype, 1, Tq, Hq, Hkv, D, 9000, 7777, seed=43)
+    lens[:] = torch.tensor([7777, 3100, 1025])[:Tq]
+    args = [x.to(DEV) for x in (q, k, ids, lens)]
+    got = pipeline.key_mass(*args)
+    close(got, want(q, k, ids, lens), Tq, Hq // Hkv)
+    assert torch.equal(pipeline.key_mass(*args), got)
+
+
 def test_key_mass_of_a_key_that_a_million_softmaxes_list():
     """More of them than a 64-bit sum of 2^-44 holds: every one counts (integers, exact in fp32)."""
     n = 131080
@@ -304,6 +317,25 @@ def test_evict_of_ties_alone(T, kind):
             assert (kept[b] if shared else kept[b, 1]).tolist() == at
 
 
+@pytest.mark.parametrize("T", [4096, 8191, 10000, 16384, 20001, 32768, 33000, 65537])
+@pytest.mark.parametrize("odd", [False, True])
+def test_evict_of_masses_as_they_accumulate(T, odd):
+    """A third exactly zero, the rest spread over decades; odd: one row's end holds a NaN and a negative one."""
+    rng = np.random.default_rng(T)
+    m = np.where(rng.random((2, 2, T)) < 0.33, 0.0, np.exp(3 * rng.standard_normal((2, 2, T)) - 5)).astype(np.float32)
+    if odd:
+        m[1, 0, T - 40], m[1, 0, T - 41] = math.nan, -1.0
+    k = torch.zeros(2, T, 2, 32, dtype=torch.bfloat16, device=DEV)
+    lens = torch.tensor([T, T - 9], dtype=torch.int32, device=DEV)
+    print("evict", T, odd, flush=True)
+    for budget in (T // 5, T - T // 4):  # the threshold is a weight, or zero
+        kept, n2 = pipeline.evict(k, k, torch.from_numpy(m).to(DEV), budget, lens, window=33, sink=4)[3:]
+        assert n2.tolist() == [budget] * 2
+        for b, n in enumerate((T, T - 9)):
+            for h in range(2):
+                assert kept[b, h].tolist() == keep(m[b, h], n, budget, 33, 4)
+
+
 def test_evict_of_views_and_in_a_graph():
     """A cache's first rows (a view), masses of a longer buffer, replayed with new masses."""
     B, T, Hkv, D, budget = 2, 600, 2, 64, 200
@@ -392,3 +424,29 @@ def test_offsets_past_32_bits():
         assert torch.equal(k2[0, :, h].cpu(), k[0, at, h]) and torch.equal(v2[0, :, h].cpu(), -k[0, at, h])
         assert torch.equal(m2[0, h].cpu(), mass[0, h].cpu()[at])
     assert kept[0, :, -1].tolist() == [n - 1] * 2
+
+
+def test_threads_on_one_stream():
+    """Calls of several threads share a stream's scratch and counters: each gets its own results."""
+    import concurrent.futures
+
+    jobs = []
+    for seed in range(4):
+        q, k, ids, lens = make(torch.bfloat16, 2, 1 + seed % 2 * 4, 8, 2, 64, 40000, 300, seed=50 + seed)
+        args = [x.to(DEV) for x in (q, k, ids, lens)]
+        v = args[1] * 2
+        table = torch.randperm(40000, device=DEV, dtype=torch.int64).to(torch.int32)[None]
+
+        def job(args=args, v=v, table=table):
+            mass = pipeline.key_mass(*args)
+            read = pipeline.prefix_read(args[0], args[1][:1, :700], v[:1, :700], args[1], v, *args[2:])
+            return (mass, read, pipeline.evict(args[1], v, mass, 9000)[3],
+                    pipeline.evict_slots(table, mass[:1], 9000)[0])
+
+        jobs.append(job)
+    alone = [job() for job in jobs]
+    torch.cuda.synchronize()
+    with concurrent.futures.ThreadPoolExecutor(4) as pool:
+        for _ in range(10):
+            for job, got in [(i, f.result()) for i, f in enumerate([pool.submit(j) for j in jobs])]:
+                assert all(torch.equal(x, y) for x, y in zip(got, alone[job]))
