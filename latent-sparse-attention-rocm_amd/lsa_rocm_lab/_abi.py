@@ -163,11 +163,15 @@ def call(name: str, *args):
     """Calls an entry point; a nonzero status raises (ValueError for argument errors)."""
     rc = getattr(load(), name)(*args)
     if rc != 0:
-        msg = load().lsa_last_error().decode(errors="replace")
-        if rc in (-1, -2, -3, -4, -7):
-            raise ValueError(f"{name}: {_ERRORS.get(rc, rc)}: {msg}")
-        raise LsaError(rc, f"{name}: {msg}")
+        _raise(name, rc)
     return rc
+
+
+def _raise(name: str, rc: int):
+    msg = load().lsa_last_error().decode(errors="replace")
+    if rc in (-1, -2, -3, -4, -7):
+        raise ValueError(f"{name}: {_ERRORS.get(rc, rc)}: {msg}")
+    raise LsaError(rc, f"{name}: {msg}")
 
 
 _in_order = threading.Lock()
@@ -176,8 +180,12 @@ _in_order = threading.Lock()
 def call_in_order(name: str, *args):
     """``call`` for an entry point of several launches over scratch that a stream's calls share: no
     other thread's launches on that stream come between this call's (ctypes drops the GIL)."""
+    entry = getattr(load(), name)
     with _in_order:
-        return call(name, *args)
+        rc = entry(*args)
+    if rc != 0:
+        _raise(name, rc)
+    return rc
 
 
 def size(name: str, *args) -> int:

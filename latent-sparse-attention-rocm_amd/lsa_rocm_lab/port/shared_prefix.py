@@ -26,9 +26,9 @@ def launch_device(device: torch.device):
 def one_device(what: str, *tensors: torch.Tensor | None) -> torch.device:
     """The ROCm device that all of the tensors are on; anything else raises ``ValueError``."""
     device = tensors[0].device
-    index = device.index if device.type == "cuda" else -1
-    for t in tensors:  # an int compares in a fraction of a device's time
-        if t is not None and (index < 0 or (t.get_device() != index and t.device != device)):
+    index = device.index  # compared in a fraction of a device's time
+    for t in tensors:
+        if t is not None and t.get_device() != index and (t.device != device or device.type != "cuda"):
             raise ValueError(f"{what} is a ROCm kernel over tensors of one device, got {device} and {t.device}")
     return device
 
