@@ -203,18 +203,12 @@ def prepare(case, seed):
 # ------------------------------------------------------------------------------- one pass, as a user calls it
 
 
-_LOADED = []  # the framework's module, imported once as a program does
-
-
 def _pipeline():
-    if _LOADED:
-        return _LOADED[0]
     path = str(pathlib.Path(__file__).resolve().parents[1] / "latent-sparse-attention-rocm_amd")
     if path not in sys.path:
         sys.path.insert(0, path)
     from lsa_rocm_lab.port import pipeline
 
-    _LOADED.append(pipeline)
     return pipeline
 
 
