@@ -293,23 +293,25 @@ def call_memory(device: torch.device, purpose: str, nbytes: int, n_counters: int
         if ws is None or ws.numel() < nbytes:
             ws = Workspace.get(device, purpose, nbytes)
     if n_counters:
-        count = Counters._buffers.get((device.index, here))
+        count = Counters._buffers.get((device.index, here, purpose))
         if count is None or count.numel() < n_counters:
-            count = Counters.get(device, n_counters)
+            count = Counters.get(device, n_counters, purpose)
     return ws, count, here
 
 
 class Counters:
-    """Split-arrival counters per (device, stream): int32 that every kernel finds zero at
-    launch and leaves zero, so the buffer is zero-filled only when it is (re)allocated.
+    """Split-arrival counters per (device, stream, purpose): int32 that every kernel finds zero at
+    launch and leaves zero, so the buffer is zero-filled only when it is (re)allocated. A fused
+    decode that gives up waiting may leave words in its own ("decode", which ``reset`` zeroes);
+    purposes whose kernels never wait share none with it.
     Outgrown buffers are retired, never freed (a captured graph may hold them)."""
 
     _buffers: dict[tuple, torch.Tensor] = {}
     _retired: list[torch.Tensor] = []
 
     @classmethod
-    def get(cls, device: torch.device, n: int) -> torch.Tensor:
-        key = (device_index(device), stream(device))
+    def get(cls, device: torch.device, n: int, purpose: str = "decode") -> torch.Tensor:
+        key = (device_index(device), stream(device), purpose)
         buf = cls._buffers.get(key)
         if buf is None or buf.numel() < n:
             if buf is not None:
@@ -320,10 +322,10 @@ class Counters:
 
     @classmethod
     def reset(cls, device: torch.device) -> None:
-        """Zeroes every counter buffer of the device (after a decode gave up waiting)."""
+        """Zeroes the device's "decode" counter buffers (after a decode gave up waiting)."""
         index = device_index(device)
-        for (dev, _), buf in cls._buffers.items():
-            if dev == index:
+        for (dev, _, purpose), buf in cls._buffers.items():
+            if dev == index and purpose == "decode":
                 buf.zero_()
 
 

@@ -1,0 +1,37 @@
+"""The memory that prefix_read, key_mass and the evictions hand their kernels: host logic, nothing is launched."""
+
+import pytest
+import torch
+
+from lsa_rocm_lab import _abi
+
+GPU = torch.device("cuda", 0)
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """Buffers in host memory where a call asks for the device's; one stream, no capture."""
+    for name in ("zeros", "empty"):
+        make = getattr(torch, name)
+        monkeypatch.setattr(torch, name, lambda *a, _make=make, device=None, **k: _make(*a, **k))
+    monkeypatch.setattr(_abi, "_raw_stream", lambda index=None: 7)
+    monkeypatch.setattr(_abi, "_capturing", lambda: False)
+    for cls in (_abi.Workspace, _abi.Counters):
+        monkeypatch.setattr(cls, "_buffers", {})
+        monkeypatch.setattr(cls, "_retired", [])
+    return monkeypatch
+
+
+def test_counters_are_not_the_decodes(host):
+    """A fused decode that gave up waiting may leave words in its counters; the calls around it, which do
+    not ask whether one did, find theirs zero."""
+    decode = _abi.Counters.get(GPU, 64)
+    decode.fill_(3)
+    for purpose in ("key_mass", "prefix_read"):
+        _, counters, _ = _abi.call_memory(GPU, purpose, 16, 64)
+        assert counters.data_ptr() != decode.data_ptr() and not counters.any()
+        assert _abi.call_memory(GPU, purpose, 16, 64)[1] is counters  # kept from call to call
+        assert _abi.call_memory(GPU, purpose, 16, 5000)[1].numel() >= 5000
+    assert _abi.Counters.get(GPU, 64) is decode
+    _abi.Counters.reset(GPU)
+    assert not decode.any()
