@@ -464,10 +464,12 @@ int lsa_prefix_read(const void* q, const void* k_prefix, const void* v_prefix, i
  * that each listed key receives from batch row b's query rows, summed over them and over the
  * query heads of its kv-head. q [B, Tq, Hq, D], K as lsa_read's, `caches` = B caches or one
  * pool for every row; lists as lsa_read's (a key listed twice counts twice). The weights are
- * those of the softmax over the row's own list, or exp(score - lse) with lse [B, Tq, Hq] (a
- * wider softmax's, as lsa_prefix_read gives it; -inf and NaN: no weight). A softmax whose sum
- * is not a number gives none. The result does not depend on the order in which workgroups run.
- * Several rows of one cache: at most 2^19 rows times the group's heads a cache in one call.
+ * those of the softmax over the row's own list, or min(1, exp(score - lse)) with lse [B, Tq, Hq] (a
+ * wider softmax's, as lsa_prefix_read gives it, whose weights are at most 1; -inf and NaN: no weight).
+ * A softmax whose sum is not a number gives none. The result does not depend on the order in which
+ * workgroups run. Several rows of one cache: at most 2^19 rows times the group's heads a cache in one
+ * call, and a weight is rounded to a multiple of 2^-44 (with lse and n > 2^19 list slots times heads a
+ * cache, of n 2^-63, n rounded up to a power of two).
  * zero_first != 0: mass (dense) begins at zero. counters (or NULL): B * Tq * Hkv int32 that read
  * zero at launch and are left zero; with one query row a cache they make the call one launch instead
  * of two. No counterpart in the reference. scratch:

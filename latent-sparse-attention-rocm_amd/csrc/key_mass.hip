@@ -19,8 +19,11 @@
 // keys. Sums must not depend on the order in which workgroups arrive. With one query row a cache, all
 // additions to a key come from one list and are the same number, so fp32 atomics will do.
 // With more, the weights go to 64-bit integers of 2^-44 first (integer sums have no order;
-// 2^-45 of rounding a weight, against 2^-24 of the fp32 sum), and mass_fold_kernel adds those to
-// the fp32 weights.
+// 2^-45 of rounding a weight, against 2^-24 of the fp32 sum: a weight below that counts as none), and
+// mass_fold_kernel adds those to the fp32 weights. The weights that a softmax gives a key are 1 together at most,
+// and 2^19 softmaxes fit. Those by a given lse are so only if it is a wider softmax's: each is held to 1, and
+// the integers' unit is as large as it has to be for every slot of every list to hold 1 for one key (2^-44 up to
+// 2^19 slots times heads a cache, 2^-37 at 2^26).
 #include <math.h>
 
 #include <algorithm>
@@ -32,9 +35,9 @@ using namespace lsa;
 
 namespace {
 
-constexpr float kFix = 17592186044416.0f;  // 2^44: a key's weights add up to less than 2^20
-constexpr int64_t kMaxRows = 1 << 19;      // so of softmaxes (one a row and head) at most this a cache
-constexpr float kMaxWeight = 65536.0f;     // a given lse may be off; a weight is at most this
+constexpr int kFixBits = 44;           // a key's weights add up to less than 2^20 in units of 2^-44
+constexpr int64_t kMaxRows = 1 << 19;  // so of softmaxes (one a row and head) at most this a cache
+constexpr float kMaxWeight = 1.0f;     // a given lse may be off; a weight is at most this
 
 struct MassArgs {
   const void* q;
@@ -57,6 +60,7 @@ struct MassArgs {
   int* counters;          // one launch: arrivals of a unit's spans, zero before and after; or nullptr
   int zero;               // the weights begin at zero
   uint64_t* fixed;        // [caches, Hkv, Tk] or nullptr
+  float fix;              // of them, one over the unit
   int whole;              // fixed is cleared and folded whole, not by the lists
 };
 
@@ -436,7 +440,7 @@ __global__ __launch_bounds__(LSA_BLOCK) void mass_add_kernel(MassArgs a) {
   const int64_t c = a.caches > 1 ? row / a.Tq : 0;
   if (a.fixed) {
     atomicAdd((unsigned long long*)a.fixed + (c * a.Hkv + g) * a.Tk + id,
-              (unsigned long long)__float2ull_rn(sum * kFix));
+              (unsigned long long)__float2ull_rn(sum * a.fix));
   } else {
     atomicAdd(a.mass + c * a.m_sb + g * a.m_sh + id, sum);
   }
@@ -452,7 +456,7 @@ __global__ __launch_bounds__(LSA_BLOCK) void mass_fold_kernel(MassArgs a) {
       if (x == 0) continue;
       const int64_t cg = i / a.Tk;
       float* m = a.mass + (cg / a.Hkv) * a.m_sb + (cg % a.Hkv) * a.m_sh + i % a.Tk;
-      *m += (float)((double)x / (double)kFix);
+      *m += (float)((double)x / (double)a.fix);
     }
     return;
   }
@@ -466,7 +470,16 @@ __global__ __launch_bounds__(LSA_BLOCK) void mass_fold_kernel(MassArgs a) {
   if (id < 0 || id >= a.Tk) return;
   const int64_t c = a.caches > 1 ? row / a.Tq : 0;
   const uint64_t x = atomicExch((unsigned long long*)a.fixed + (c * a.Hkv + g) * a.Tk + id, 0ull);
-  if (x) a.mass[c * a.m_sb + g * a.m_sh + id] += (float)((double)x / (double)kFix);
+  if (x) a.mass[c * a.m_sb + g * a.m_sh + id] += (float)((double)x / (double)a.fix);
+}
+
+// Bits below one of the integers. rows: query rows of a cache.
+int mass_fix_bits(int64_t rows, int gq, int32_t W, bool given) {
+  int slots = 0;
+  if (given) {
+    while (slots < 62 && (int64_t)1 << slots < rows * gq * W) ++slots;
+  }
+  return std::min(kFixBits, 63 - slots);
 }
 
 int mass_span(int dtype, int D, int64_t units, int W) {
@@ -574,6 +587,7 @@ extern "C" int lsa_key_mass(const void* q, const void* k, int dtype, int64_t B, 
   a.scores = (float*)scratch;
   a.stats = (float*)((char*)scratch + p.scores);
   a.fixed = p.fixed ? (uint64_t*)((char*)scratch + p.scores + p.stats) : nullptr;
+  a.fix = ldexpf(1.0f, mass_fix_bits(B * Tq / caches, Hq / Hkv, W, lse != nullptr));
   a.whole = p.whole ? 1 : 0;
   a.mass = mass; a.m_sb = caches > 1 ? mass_batch_stride : 0; a.m_sh = mass_head_stride;
   // offsets within a unit's scores are 32 bits of bytes

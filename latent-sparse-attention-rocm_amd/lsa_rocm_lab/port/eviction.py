@@ -45,9 +45,12 @@ def key_mass(
     ``read_lists`` / ``lengths`` as ``lsa_read`` takes them (``[B, Tq, W]`` or ``[B, Tq, Hkv, W]``;
     ids outside the cache are skipped, a key listed twice counts twice). The weights are of the
     softmax over the row's list, or, with ``lse`` [B, Tq, Hq] (``prefix_read(return_lse=True)``'s),
-    of the wider softmax it belongs to. A row whose sum is not a number gives none, as it reads
-    as no keys in ``lsa_read``. Returns [B or 1, Hkv, Tk] fp32: new, or ``mass`` with the weights
-    added in place. The bits do not depend on the order in which rows and workgroups run.
+    of the wider softmax it belongs to (whose weights are at most 1: by an ``lse`` that is too low
+    they are 1). A row whose sum is not a number gives none, as it reads as no keys in
+    ``lsa_read``. Where several query rows share a cache a weight is rounded to a multiple of 2^-44
+    (by a given ``lse`` and lists of n > 2^19 slots times heads, of n 2^-63). Returns
+    [B or 1, Hkv, Tk] fp32: new, or ``mass`` with the weights added in place. The bits do not
+    depend on the order in which rows and workgroups run.
     """
     device = one_device("key_mass", q, k, lse, mass)
     if q.dim() != 4 or k.dim() != 4 or k.shape[0] not in (q.shape[0], 1) or k.shape[3] != q.shape[3]:

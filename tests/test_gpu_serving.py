@@ -34,3 +34,18 @@ def test_words_a_decode_left_in_its_counters():
         assert (words == 1).all()
     finally:
         words.zero_()
+
+
+@pytest.mark.parametrize("Tq,W", [(1, 64), (2, 64), (64, 4096)])
+@pytest.mark.parametrize("pool", [False, True])
+def test_weights_by_an_lse_that_is_too_low(Tq, W, pool):
+    """A weight is at most 1, and no sum of such wraps: a key that fills every list of every row is the heaviest."""
+    q, k, ids, lens = rows_and_lists(torch.bfloat16, 2, Tq, 16, 2, 64, 5, W, pool)
+    k.zero_()
+    ids.fill_(3)
+    ids[:, :, 1::4] = 1
+    lens.fill_(W)
+    got = pipeline.key_mass(q, k, ids, lens, lse=torch.full((2, Tq, 16), -40.0, device=DEV))
+    n = (2 if pool else 1) * Tq * W * 8  # whole numbers, exact in fp32
+    assert got.shape == (1 if pool else 2, 2, 5)
+    assert (got == torch.tensor([0.0, n / 4, 0.0, n * 3 / 4, 0.0], device=DEV)).all()
