@@ -184,7 +184,7 @@ def prefix_read(
             ws, counters, stream = _abi.call_memory(device, "prefix_read", nbytes, B * Tq * Hkv)
             _abi.call_in_order("lsa_prefix_read", q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), dt, B, Tq, P, Tp,
                                k_prefix.shape[1], Hq, Hkv, D, psb, pst, psh, _abi.ptr(prow), _abi.ptr(plen),
-                               _abi.ptr(slots), slots.stride(0) if slots is not None else 0, _abi.ptr(k), _abi.ptr(v),
+                               _abi.ptr(slots), Tp, _abi.ptr(k), _abi.ptr(v),
                                Tk, sb, st, sh, _abi.ptr(ids), _abi.ptr(lens), W, 1 if per_head else 0,
                                float(D ** -0.5 if scale is None else scale), _abi.ptr(counters), _abi.ptr(ws), nbytes,
                                out.data_ptr(), _abi.ptr(lse), stream)

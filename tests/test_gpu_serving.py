@@ -49,3 +49,11 @@ def test_weights_by_an_lse_that_is_too_low(Tq, W, pool):
     n = (2 if pool else 1) * Tq * W * 8  # whole numbers, exact in fp32
     assert got.shape == (1 if pool else 2, 2, 5)
     assert (got == torch.tensor([0.0, n / 4, 0.0, n * 3 / 4, 0.0], device=DEV)).all()
+
+
+def test_a_slot_table_that_is_a_column_turned():
+    q, pool, _, _ = rows_and_lists(torch.bfloat16, T=128, pool=True)
+    v = pool * 2
+    column = torch.randperm(128, device=DEV).to(torch.int32)[:90, None]
+    assert torch.equal(pipeline.prefix_read(q, pool, v, prefix_slots=column.t()),
+                       pipeline.prefix_read(q, pool, v, prefix_slots=column.flatten()[None].clone()))

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from lsa_rocm_lab import _abi
+from lsa_rocm_lab.port import pipeline
 
 GPU = torch.device("cuda", 0)
 
@@ -35,3 +36,34 @@ def test_counters_are_not_the_decodes(host):
     assert _abi.Counters.get(GPU, 64) is decode
     _abi.Counters.reset(GPU)
     assert not decode.any()
+
+
+class OnGpu(torch.Tensor):
+    """A CPU tensor that says it is on the GPU."""
+
+    device = GPU
+
+
+def fake(x):
+    return x.as_subclass(OnGpu)
+
+
+@pytest.fixture
+def calls(host):
+    """What the entry points are called with, in order; nothing is launched."""
+    seen = []
+    host.setattr(_abi, "current_device", lambda: 0)
+    host.setattr(_abi, "call_in_order", lambda name, *args: seen.append((name, args)))
+    host.setattr(_abi, "call", lambda name, *args: seen.append((name, args)))
+    return seen
+
+
+def test_a_slot_table_of_one_row_with_any_stride(calls):
+    """A row axis of one has whatever stride its view left it; the table is dense all the same."""
+    q, pool = fake(torch.zeros(2, 1, 4, 64)), fake(torch.zeros(1, 80, 2, 64))
+    column = torch.arange(64, dtype=torch.int32)[:, None]
+    for slots in (column.t(), column.t().contiguous().as_strided((1, 64), (1, 1))):
+        pipeline.prefix_read(q, pool, pool, prefix_slots=fake(slots))
+        name, args = calls.pop()
+        assert name == "lsa_prefix_read" and args[6:8] == (1, 64)
+        assert args[18] >= 64, "slot rows closer than their length are refused"
