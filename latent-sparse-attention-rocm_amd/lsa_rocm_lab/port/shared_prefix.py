@@ -34,9 +34,12 @@ def one_device(what: str, *tensors: torch.Tensor | None) -> torch.device:
 
 
 def int32_on(t: torch.Tensor, device: torch.device) -> torch.Tensor:
-    """``t`` as a kernel reads it: int32, contiguous, on ``device``."""
+    """``t`` as a kernel reads it: int32, contiguous, on ``device``. A number past 32 bits becomes the
+    nearest that they hold (an id, slot or prefix outside every cache, a length past every row)."""
     if t.dtype is torch.int32 and (t.get_device() == device.index or t.device == device) and t.is_contiguous():
         return t
+    if t.dtype is not torch.int32 and t.dtype.itemsize >= 4:
+        t = t.to(torch.int64).clamp(-(1 << 31), (1 << 31) - 1)
     return t.to(device=device, dtype=torch.int32).contiguous()
 
 

@@ -57,3 +57,24 @@ def test_a_slot_table_that_is_a_column_turned():
     column = torch.randperm(128, device=DEV).to(torch.int32)[:90, None]
     assert torch.equal(pipeline.prefix_read(q, pool, v, prefix_slots=column.t()),
                        pipeline.prefix_read(q, pool, v, prefix_slots=column.flatten()[None].clone()))
+
+
+def test_numbers_past_32_bits():
+    """An id, slot, prefix or length that int32 does not hold: outside everything, as its int64 value is."""
+    q, k, ids, lens = rows_and_lists(torch.bfloat16, T=200, W=40)
+    far = torch.where(torch.arange(40, device=DEV) % 3 == 0, ids.long() + (1 << 32), ids.long())
+    near = torch.where(far < 200, far, -1).to(torch.int32)
+    assert torch.equal(pipeline.key_mass(q, k, far, lens), pipeline.key_mass(q, k, near, lens))
+    rows = torch.tensor([0, 1 << 32, 1], device=DEV)  # the second: none
+    args = (k[:2], k[:2] * 2, k, k)
+    lengths = torch.tensor([(1 << 32) + 7, 90], device=DEV)
+    assert torch.equal(
+        pipeline.prefix_read(q, *args, far, lens.long(), prefix_rows=rows, prefix_lengths=lengths),
+        pipeline.prefix_read(q, *args, near, lens, prefix_rows=rows.clamp(max=9).int(), prefix_lengths=lengths.clamp(max=200).int()))
+    table = torch.arange(200, device=DEV)[None].expand(2, 200).clone()
+    mass = torch.rand(1, 2, 200, device=DEV)
+    none = table.clone()
+    table[:, 5::9] += 1 << 32
+    none[:, 5::9] = -1
+    kept = pipeline.evict_slots(table, mass, 60, lens[:2].flatten().long() + (1 << 32))[2]
+    assert torch.equal(kept, pipeline.evict_slots(none, mass, 60)[2])

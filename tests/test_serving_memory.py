@@ -1,10 +1,10 @@
-"""The memory that prefix_read, key_mass and the evictions hand their kernels: host logic, nothing is launched."""
+"""What prefix_read, key_mass and the evictions hand their kernels: host logic, nothing is launched."""
 
 import pytest
 import torch
 
 from lsa_rocm_lab import _abi
-from lsa_rocm_lab.port import pipeline
+from lsa_rocm_lab.port import pipeline, shared_prefix
 
 GPU = torch.device("cuda", 0)
 
@@ -67,3 +67,17 @@ def test_a_slot_table_of_one_row_with_any_stride(calls):
         name, args = calls.pop()
         assert name == "lsa_prefix_read" and args[6:8] == (1, 64)
         assert args[18] >= 64, "slot rows closer than their length are refused"
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32, torch.int16, torch.uint8])
+def test_numbers_past_32_bits_stay_outside(dtype):
+    """2^32 + 5 is no key, slot or prefix 5: numbers that int32 does not hold become its ends, which name nothing."""
+    small = torch.tensor([[0, 5, 100]], dtype=dtype)
+    assert shared_prefix.int32_on(small, small.device).tolist() == [[0, 5, 100]]
+    if dtype == torch.uint8:
+        assert shared_prefix.int32_on(torch.tensor([2 ** 32 - 1], dtype=torch.uint32), small.device).tolist() == [2 ** 31 - 1]
+    if dtype == torch.int64:
+        far = torch.tensor([2 ** 32 + 5, 2 ** 31, -(2 ** 31) - 1, -(2 ** 32) + 5, 2 ** 63 - 1, 2 ** 31 - 1, -1])
+        got = shared_prefix.int32_on(far, far.device)
+        top = 2 ** 31 - 1
+        assert got.dtype == torch.int32 and got.tolist() == [top, top, -top - 1, -top - 1, top, top, -1]
