@@ -133,6 +133,58 @@ def _extent(t: torch.Tensor) -> tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
+def _axes(t: torch.Tensor) -> list[tuple[int, int]]:
+    """(step in bytes, size) of a tensor's axes, the largest step first; elements that follow each other
+    are one axis, the last, of step 1. Of an ``_apart`` tensor each step holds all of the smaller ones."""
+    size = t.element_size()
+    found = [(1, size)]
+    for step, n in sorted((step * size, n) for step, n in zip(t.stride(), t.shape) if n > 1):
+        found = [*found[:-1], (1, n * step)] if len(found) == 1 and step == found[-1][1] else [*found, (step, n)]
+    return [*found[:0:-1], found[0]]
+
+
+def _meets_twin(k: torch.Tensor, v: torch.Tensor) -> bool:
+    """Whether two ``_apart`` tensors of the same shape and steps share a byte."""
+    axes = _axes(k)
+
+    def hit(rest: int, i: int) -> bool:  # rest: a sum of steps, each taken fewer than its size of times either way?
+        step, n = axes[i]
+        if i == len(axes) - 1:
+            return abs(rest) < n
+        return any(abs(x) < n and hit(rest - x * step, i + 1) for x in (rest // step, rest // step + 1))
+
+    return k.numel() > 0 and hit(v.data_ptr() - k.data_ptr(), 0)
+
+
+def _meets(t: torch.Tensor, lo: int, hi: int) -> bool:
+    """Whether an ``_apart`` tensor has a byte at an address in [lo, hi)."""
+    axes = _axes(t)
+
+    def hit(at: int, i: int) -> bool:
+        step, n = axes[i]
+        reach = sum((m - 1) * s for s, m in axes[i + 1:]) + 1  # bytes from the first to past the last of one index
+        first, last = max(0, (lo - at - reach) // step + 1), min(n - 1, (hi - 1 - at) // step)  # whose bytes' span meets it
+        if first > last or i == len(axes) - 1 or last - first > 1:  # of three in a line it holds the middle one
+            return first <= last
+        return any(hit(at + x * step, i + 1) for x in range(first, last + 1))
+
+    return t.numel() > 0 and lo < hi and hit(t.data_ptr(), 0)
+
+
+def _places_apart(k: torch.Tensor, v: torch.Tensor, mass: torch.Tensor) -> bool:
+    """Whether what is written of ``evict``'s out (K and V at the same steps) has a place of its own."""
+    if not (_apart(k) and _apart(v) and _apart(mass)) or _meets_twin(k, v):
+        return False
+    lo, hi = _extent(mass)
+    if not (_meets(k, lo, hi) or _meets(v, lo, hi)):
+        return True
+    *outer, (_, run) = _axes(mass)
+    starts = [mass.data_ptr()]
+    for step, n in outer:
+        starts = [at + x * step for at in starts for x in range(n)]
+    return not any(_meets(x, at, at + run) for at in starts for x in (k, v))
+
+
 def evict(
     k: torch.Tensor,
     v: torch.Tensor,
@@ -188,7 +240,7 @@ def evict(
             a, b = _extent(new)
             if any(a < hi and lo < b for lo, hi in map(_extent, (k, v, mass))):
                 raise ValueError("evict: out must not overlap the cache it is made from")
-        if not (_apart(k2) and _apart(v2) and _apart(m2)) or (k2.data_ptr() == v2.data_ptr() and k2.numel()):
+        if not _places_apart(k2[:, :budget], v2[:, :budget], m2[..., :budget]):
             raise ValueError("evict: out k, v and mass need a place of their own for every element")
     ob, ot, oh = cache_strides(k2)
     kept = torch.empty((B, budget) if shared else (B, Hkv, budget), dtype=torch.int32, device=device)

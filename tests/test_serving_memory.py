@@ -1,10 +1,11 @@
 """What prefix_read, key_mass and the evictions hand their kernels: host logic, nothing is launched."""
 
+import numpy as np
 import pytest
 import torch
 
 from lsa_rocm_lab import _abi
-from lsa_rocm_lab.port import pipeline, shared_prefix
+from lsa_rocm_lab.port import eviction, pipeline, shared_prefix
 
 GPU = torch.device("cuda", 0)
 
@@ -81,3 +82,86 @@ def test_numbers_past_32_bits_stay_outside(dtype):
         got = shared_prefix.int32_on(far, far.device)
         top = 2 ** 31 - 1
         assert got.dtype == torch.int32 and got.tolist() == [top, top, -top - 1, -top - 1, top, top, -1]
+
+
+def places(t):
+    """The bytes that a tensor's elements lie at."""
+    at = torch.tensor([t.data_ptr()])
+    for n, step in zip(t.shape, t.stride()):
+        at = (at[:, None] + torch.arange(n) * step * t.element_size()).flatten()
+    return set((at[:, None] + torch.arange(t.element_size())).flatten().tolist())
+
+
+def test_buffers_of_an_eviction_that_share_memory(calls):
+    """K, V and mass to be filled: refused where two of them share a place among the rows that are written,
+    taken where they lie between each other."""
+    B, T, Hkv, D, budget = 2, 20, 2, 16, 6
+    k = fake(torch.zeros(B, T, Hkv, D, dtype=torch.bfloat16))
+    seen = fake(torch.zeros(B, Hkv, T))
+    arena = torch.zeros(40000, dtype=torch.bfloat16)
+    floats = arena.view(torch.float32)
+    token, head = Hkv * D, D
+
+    def rows(at, step=(9 * token, token, head), n=budget):
+        return arena.as_strided((B, n, Hkv, D), (*step, 1), at)
+
+    def masses(at, step=(Hkv * budget, budget)):
+        return floats.as_strided((B, Hkv, budget), (*step, 1), at // 2)
+
+    apart = masses(30000)
+    wide = (100 * token, 2 * token, 2 * head)  # K and V of a head side by side
+    byhead = (1000, D, 400)                    # head by head: K, V and masses in turn
+    tried = {True: 0, False: 0}
+    for k2, v2, m2 in [
+        (rows(0), rows(5000), apart),
+        (rows(0), rows(token), apart),                      # V a row behind K
+        (rows(0), rows(5 * token), apart), (rows(0), rows(6 * token), apart), (rows(6 * token), rows(0), apart),
+        (rows(0), rows(16 * token), apart), (rows(0), rows(17 * token), apart),
+        (rows(0), rows(8), apart), (rows(8), rows(0), apart),
+        (rows(0, wide), rows(D, wide), apart), (rows(0, wide), rows(8, wide), apart),
+        (rows(0, wide), rows(token, wide), apart), (rows(0, wide), rows(2 * token, wide), apart),
+        (rows(0, byhead), rows(D * budget, byhead), masses(2 * D * budget, (500, 200))),
+        (rows(0, byhead), rows(D * budget, byhead), masses(2 * D * budget - 2, (500, 200))),
+        (rows(0, byhead), rows(D * budget, byhead), masses(400 - 2 * budget, (500, 200))),
+        (rows(0, byhead), rows(D * budget, byhead), masses(402 - 2 * budget, (500, 200))),
+        (rows(0), rows(5000), masses(0)), (rows(0), rows(5000), masses(5000 + 100)),
+        (rows(0), rows(5000), masses(6 * token)), (rows(0), rows(5000), masses(6 * token - 2)),
+        (rows(0, n=9), rows(6 * token, n=9), masses(5000)),  # rows behind the budget are not written
+    ]:
+        k3, v3 = k2[:, :budget], v2[:, :budget]
+        share = bool(places(k3) & places(v3) or places(k3) & places(m2) or places(v3) & places(m2))
+        tried[share] += 1
+        out = tuple(map(fake, (k2, v2, m2)))
+        if share:
+            with pytest.raises(ValueError, match="place of their own"):
+                eviction.evict(k, k, seen, budget, out=out)
+            assert not calls
+        else:
+            eviction.evict(k, k, seen, budget, out=out)
+            assert [name for name, _ in calls] == ["lsa_evict_keep", "lsa_evict_rows"]
+            calls.clear()
+    assert min(tried.values()) >= 7
+
+
+def test_shared_places_by_enumeration():
+    """Nested views at random: whether they share a byte, against the bytes themselves."""
+    rng = np.random.default_rng(0)
+    arena = torch.zeros(4000, dtype=torch.float32)
+    found = {True: 0, False: 0}
+    for _ in range(1500):
+        shape, steps, reach = [], [], 1
+        for n in rng.integers(1, 5, 3).tolist():
+            step = reach + int(rng.integers(0, 3)) * int(rng.integers(1, 4))
+            shape.append(n), steps.append(step)
+            reach = step * n
+        turn = rng.permutation(3).tolist()
+        view = lambda at: arena.as_strided([shape[i] for i in turn], [steps[i] for i in turn], at)  # noqa: B023, E731
+        k, v = view(500), view(500 + int(rng.integers(-reach, reach)))
+        assert eviction._apart(k)
+        share = bool(places(k) & places(v))
+        found[share] += 1
+        assert eviction._meets_twin(k, v) == share == eviction._meets_twin(v, k)
+        lo = k.data_ptr() + int(rng.integers(-20, 4 * reach))
+        hi = lo + int(rng.integers(0, 40))
+        assert eviction._meets(k, lo, hi) == any(lo <= x < hi for x in places(k))
+    assert min(found.values()) > 300
