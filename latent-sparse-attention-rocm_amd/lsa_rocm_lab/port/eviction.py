@@ -14,8 +14,8 @@ import torch
 from lsa_rocm_lab import _abi
 from lsa_rocm_lab.port.shared_prefix import aligned, cache_pair, cache_strides, int32_on, launch_device, lists_of, one_device
 
-# Query rows go through in slabs: of so many bytes of scores, so many softmaxes a cache (their sums are
-# 64-bit integers) and so many kv-heads of rows (a launch's limit)
+# Batch rows and their query rows go through in slabs: of so many bytes of scratch, so many softmaxes a cache
+# (their sums are 64-bit integers) and so many kv-heads of rows (a launch's limit)
 _SLAB_BYTES, _SLAB_SUMS, _SLAB_UNITS = 256 << 20, 1 << 19, (1 << 24) - 1
 
 
@@ -81,27 +81,35 @@ def key_mass(
     sb, st, sh = cache_strides(k)
     lse = None if lse is None else lse.contiguous()
     scale = float(D ** -0.5 if scale is None else scale)
-    # every query row's scores are held until its sums are known
-    step = Tq
-    if 4 * B * Tq * Hq * W > _SLAB_BYTES or B * Tq * Hq > _SLAB_SUMS:
-        step = max(1, min(Tq, _SLAB_BYTES // (4 * B * Hq * W), _SLAB_SUMS * caches // (B * (Hq // Hkv)),
-                          _SLAB_UNITS // (B * Hkv)))
+    # every query row's scores are held until its sums are known, beside the integers that several rows of a cache
+    # add up in (twice its masses: a pool's, or one cache's, are not cut)
+    many, step = B, Tq
+    scores, cell = 4 * Hq * W, 8 * Hkv * Tk if caches == B and Tq > 1 else 0  # bytes of a query row, of a cache
+    if B * (Tq * scores + cell) > _SLAB_BYTES or B * Tq * Hq > _SLAB_SUMS:
+        group = Hq // Hkv
+        many = max(1, min(B, _SLAB_BYTES // (scores + 2 * cell), _SLAB_SUMS // group if caches < B else B,
+                          _SLAB_UNITS // Hkv))
+        step = max(1, min(Tq, (_SLAB_BYTES - many * cell) // (many * scores),
+                          _SLAB_SUMS // (group if caches == B else many * group), _SLAB_UNITS // (many * Hkv)))
     with launch_device(device):
-        for t in range(0, Tq, step):
-            n = min(step, Tq - t)
-            part, pids, plens, plse = q, ids, lens, lse
-            if n != Tq:  # rows t .. t + n of every batch row
-                part = q[:, t:t + n].contiguous()
-                pids = ids.view(B, Tq, -1)[:, t:t + n].contiguous()
-                plens = lens.view(B, Tq, -1)[:, t:t + n].contiguous()
-                plse = None if lse is None else lse[:, t:t + n].contiguous()
-            nbytes = _abi.shape_size("lsa_key_mass_scratch_bytes", dt, B, n, caches, Tk, Hq, Hkv, D, W)
-            ws, counters, stream = _abi.call_memory(device, "key_mass", nbytes, B * Hkv if n == 1 and caches == B else 0)
-            _abi.call_in_order("lsa_key_mass", part.data_ptr(), k.data_ptr(), dt, B, n, caches, Tk, Hq, Hkv, D, sb, st,
-                               sh, pids.data_ptr(), plens.data_ptr(), W, 1 if per_head else 0, scale, _abi.ptr(plse),
-                               1 if fresh and t == 0 else 0, _abi.ptr(counters), _abi.ptr(ws), nbytes,
-                               mass.data_ptr(), mass.stride(0) if caches > 1 else Hkv * Tk,
-                               mass.stride(1) if Hkv > 1 else Tk, stream)
+        for b in range(0, B, many):
+            m = min(many, B - b)
+            own, kb, mb = (1, k, mass) if caches < B else (m, k[b:b + m], mass[b:b + m])
+            for t in range(0, Tq, step):
+                n = min(step, Tq - t)
+                part, pids, plens, plse = q, ids, lens, lse
+                if (m, n) != (B, Tq):  # rows t .. t + n of batch rows b .. b + m
+                    part = q[b:b + m, t:t + n].contiguous()
+                    pids = ids.view(B, Tq, -1)[b:b + m, t:t + n].contiguous()
+                    plens = lens.view(B, Tq, -1)[b:b + m, t:t + n].contiguous()
+                    plse = None if lse is None else lse[b:b + m, t:t + n].contiguous()
+                nbytes = _abi.shape_size("lsa_key_mass_scratch_bytes", dt, m, n, own, Tk, Hq, Hkv, D, W)
+                ws, counters, stream = _abi.call_memory(device, "key_mass", nbytes, m * Hkv if n == 1 and own == m else 0)
+                first = fresh and t == 0 and (b == 0 or caches == B)
+                _abi.call_in_order("lsa_key_mass", part.data_ptr(), kb.data_ptr(), dt, m, n, own, Tk, Hq, Hkv, D, sb, st,
+                                   sh, pids.data_ptr(), plens.data_ptr(), W, 1 if per_head else 0, scale, _abi.ptr(plse),
+                                   1 if first else 0, _abi.ptr(counters), _abi.ptr(ws), nbytes, mb.data_ptr(),
+                                   mass.stride(0) if own > 1 else Hkv * Tk, mass.stride(1) if Hkv > 1 else Tk, stream)
     return mass
 
 

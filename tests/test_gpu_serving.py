@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from lsa_rocm_lab import _abi
-from lsa_rocm_lab.port import pipeline
+from lsa_rocm_lab.port import eviction, pipeline
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -78,3 +78,23 @@ def test_numbers_past_32_bits():
     none[:, 5::9] = -1
     kept = pipeline.evict_slots(table, mass, 60, lens[:2].flatten().long() + (1 << 32))[2]
     assert torch.equal(kept, pipeline.evict_slots(none, mass, 60)[2])
+
+
+@pytest.mark.parametrize("B,Tq,pool", [(13, 1, False), (13, 1, True), (5, 6, False), (5, 6, True)])
+def test_key_weights_in_slabs_of_the_batch(monkeypatch, B, Tq, pool):
+    """Batch rows that go through a few at a time: the same weights (where rows share a cache, sums in another order:
+    2^-24 a step of an fp32 sum, and 2^-45 a weight)."""
+    q, k, ids, lens = rows_and_lists(torch.bfloat16, B, Tq, pool=pool, seed=3)
+    lse = torch.full((B, Tq, 8), 9.0, device=DEV)
+    for wide in (None, lse):
+        mass = torch.full((1 if pool else B, 2, 900), 0.5, device=DEV)
+        whole = pipeline.key_mass(q, k, ids, lens, lse=wide), pipeline.key_mass(q, k, ids, lens, lse=wide, mass=mass.clone())
+        for rows in (1, 3):
+            monkeypatch.setattr(eviction, "_SLAB_BYTES", rows * (4 * 8 * 300 + (2 * 8 * 2 * 900 if Tq > 1 and not pool else 0)))
+            got = pipeline.key_mass(q, k, ids, lens, lse=wide), pipeline.key_mass(q, k, ids, lens, lse=wide, mass=mass.clone())
+            monkeypatch.undo()
+            for x, y in zip(got, whole):
+                if Tq == 1 and not pool:
+                    assert torch.equal(x, y)
+                else:
+                    assert ((x.double() - y.double()).abs() <= B * Tq * (2.0 ** -23 * y.double() + 8 * 2.0 ** -44)).all()

@@ -165,3 +165,50 @@ def test_shared_places_by_enumeration():
         hi = lo + int(rng.integers(0, 40))
         assert eviction._meets(k, lo, hi) == any(lo <= x < hi for x in places(k))
     assert min(found.values()) > 300
+
+
+@pytest.mark.parametrize("B,Tq,Hq,Hkv,T,W,pool,fresh", [
+    (40, 1, 8, 2, 50, 30, False, True),      # rows of a decode batch, each with its cache
+    (40, 1, 8, 2, 50, 30, True, True),       # over one pool
+    (40, 1, 8, 2, 50, 30, True, False),
+    (5, 7, 8, 2, 50, 30, False, True),
+    (5, 7, 8, 2, 50, 30, True, False),
+    (6, 3, 8, 2, 3000, 4, False, False),     # the integers of several rows' caches are most of it
+    (1, 9, 8, 2, 40, 200, False, True),
+    (3, 2, 8, 2, 40, 2000, False, True),     # one row's scores are more than a slab
+    (2, 2, 8, 2, 10, 5, False, True),
+])
+def test_key_weights_in_slabs_of_memory(calls, B, Tq, Hq, Hkv, T, W, pool, fresh):
+    """Every query row once, each slab of memory within the limit unless one query row's scores are more."""
+    limit = 30000
+    calls_of = eviction._SLAB_BYTES
+    assert calls_of == 256 << 20
+    q, k = fake(torch.zeros(B, Tq, Hq, 64)), fake(torch.zeros(1 if pool else B, T, Hkv, 64))
+    ids, lens = fake(torch.zeros(B, Tq, W, dtype=torch.int32)), fake(torch.zeros(B, Tq, dtype=torch.int32))
+    caches = k.shape[0]
+    mass = None if fresh else fake(torch.zeros(caches, Hkv, T))
+    eviction._SLAB_BYTES = limit
+    try:
+        got = pipeline.key_mass(q, k, ids, lens, mass=mass)
+    finally:
+        eviction._SLAB_BYTES = calls_of
+    rows = []
+    for name, a in calls:
+        b, n, c = a[3], a[4], a[5]
+        assert name == "lsa_key_mass" and a[6:10] == (T, Hq, Hkv, 64) and c == (1 if pool else b)
+        at = (a[1] - k.data_ptr()) // (T * Hkv * 64 * 4)  # the slab's first cache
+        assert (a[23] - got.data_ptr()) == at * Hkv * T * 4
+        nbytes = a[22]
+        whole = 8 * Hkv * T if b * n > 1 and c == 1 else 0  # the integers of one cache, whatever the slab
+        sums = 8 * Hq * b * n * -(-W // 128)                # of spans of fp32 keys of 64
+        assert nbytes - whole - sums <= limit + 64 or b * n == 1
+        rows.append((at, b, n, a[19]))
+    if pool:
+        assert sum(b * n for _, b, n, _ in rows) == B * Tq
+        assert [z for *_, z in rows] == [int(fresh)] + [0] * (len(rows) - 1)
+    else:
+        for cache in range(B):
+            mine = [(n, z) for at, b, n, z in rows if at <= cache < at + b]
+            assert sum(n for n, _ in mine) == Tq
+            assert [z for _, z in mine] == [int(fresh)] + [0] * (len(mine) - 1)
+    assert len(rows) == 1 or 4 * B * Tq * Hq * W + (0 if pool or Tq == 1 else 8 * B * Hkv * T) > limit
