@@ -37,8 +37,11 @@ constexpr int kXcds = 8;
 // stand in one line, and the grid is that line times the (kv-head, piece) units: which prefix a block
 // belongs to follows from how many rows each has, counted here. (A grid of every prefix times the most
 // blocks one may have is nearly all empty where prefixes are many: 512 rows over 128 prefixes of 2048
-// keys took 820 us so, and take 242; 64 rows over 4000 of 256 keys 1922 and 42.) Units come in groups
-// of 8, the blocks of a unit 8 apart, so that those which read the same keys share an XCD and its L2.
+// keys took 820 us so, and take 242; 64 rows over 4000 of 256 keys 1922 and 42.) Into how many pieces a prefix
+// is cut follows from the blocks there are, so rows that all read one prefix of a table of many fill the chip
+// too (32 rows on one of 32 prefixes of 32768 keys: 48 us, and 259 in as many pieces as if they were spread; 39 where
+// the table holds that prefix alone, whose rows then stand in wider blocks). Units come in groups of 8, the blocks of a unit 8 apart, so that those which read the same keys share an XCD
+// and its L2.
 template <int COLS>
 struct PrefixBlock {
   static constexpr int kCount = 1024;  // prefixes counted at once
@@ -53,6 +56,22 @@ struct PrefixBlock {
 
   uint32_t cb;  // the prefix's column block
 
+  // How many rows read each of the kCount prefixes from p0 on. Ends with a barrier.
+  __device__ __forceinline__ void count(const PrefixArgs& a, int p0, int threads, int* rows) const {
+    const int tid = threadIdx.x, np = min(kCount, a.P - p0);
+    for (int i = tid; i < np; i += threads) rows[i] = 0;
+    __syncthreads();
+    for (int64_t b = tid; b < a.B; b += threads) {
+      const int64_t r = (int64_t)a.prefix_rows[b] - p0;
+      if (r >= 0 && r < np) atomicAdd(&rows[r], 1);
+    }
+    __syncthreads();
+  }
+  // The column blocks of the i-th of them (none past the last).
+  __device__ __forceinline__ static int blocks_of(const PrefixArgs& a, int p0, int i, uint32_t per, const int* rows) {
+    return i < min(kCount, a.P - p0) ? (int)(((uint32_t)rows[i] * per + COLS - 1) / COLS) : 0;
+  }
+
   // False: nothing to do (the whole workgroup). Clears the grid's share of the counters. Contains
   // barriers; `rows`: kCount ints of LDS, free again after it.
   __device__ __forceinline__ bool place(const PrefixArgs& a, uint32_t blocks, int threads, int* rows) {
@@ -60,51 +79,57 @@ struct PrefixBlock {
     GQ = a.Hq / a.Hkv;
     const int64_t clear = (int64_t)gridDim.x * threads;
     for (int64_t i = (int64_t)blockIdx.x * threads + tid; i < a.B * a.Tq * a.Hkv; i += clear) a.counters[i] = 0;
-    const uint32_t units = (uint32_t)(a.Hkv * a.splits), together = min(units, (uint32_t)kXcds);
+    const uint32_t per = (uint32_t)a.Tq * (uint32_t)GQ;  // columns of a batch row; all are fewer than 2^31
+    int splits = a.splits, of = 0;  // of: lane c: the blocks of the c-th kCount prefixes (64 times as many at most)
+    if (a.plan) {  // uniform from here on, as every wave finds the same
+      blocks = 0;
+      for (int c = 0; c * kCount < a.P; ++c) {
+        count(a, c * kCount, threads, rows);
+        int own = 0;
+        for (int i0 = 0; i0 < kCount && c * kCount + i0 < a.P; i0 += 64) own += blocks_of(a, c * kCount, i0 + lane, per, rows);
+        own = wave_sum(own);
+        of = lane == c ? own : of;
+        blocks += (uint32_t)own;
+        if (a.P > kCount) __syncthreads();  // before the counts' place is used again
+      }
+      splits = min(splits, prefix_mfma_pieces(blocks, a.Hkv));
+      if (blockIdx.x == 0 && tid == 0) *a.plan = splits;
+      if (blocks == 0) return false;
+    }
+    const uint32_t units = (uint32_t)(a.Hkv * splits), together = min(units, (uint32_t)kXcds);
     const uint32_t x = blockIdx.x, xu = x / together;
     cb = xu % blocks;
     const uint32_t u = xu / blocks * together + x % together;
-    s = (int)(u % (uint32_t)a.splits);
-    g = (int)(u / (uint32_t)a.splits);
+    s = (int)(u % (uint32_t)splits);
+    g = (int)(u / (uint32_t)splits);
     if (g >= a.Hkv) return false;
-    const uint32_t per = (uint32_t)a.Tq * (uint32_t)GQ;  // columns of a batch row; all are fewer than 2^31
     p = 0;
-    if (a.prefix_rows == nullptr) {
-      if (a.P > 1) {
-        const uint32_t each = (per + COLS - 1) / COLS;
-        p = (int)(cb / each);
-        cb %= each;
+    if (a.plan) {
+      int p0 = 0;
+      if (a.P > kCount) {
+        const int to = wave_inclusive_sum(of), c = __builtin_ctzll(__ballot((uint32_t)to > cb));
+        cb -= (uint32_t)__shfl(to - of, c, 64);
+        p0 = c * kCount;
+        count(a, p0, threads, rows);
       }
-    } else if (a.P > 1) {
-      bool found = false;  // uniform, as every wave finds the same
-      uint32_t base = 0;   // blocks of the prefixes before
-      for (int p0 = 0; p0 < a.P && !found; p0 += kCount) {
-        const int np = min(kCount, a.P - p0);
-        for (int i = tid; i < np; i += threads) rows[i] = 0;
-        __syncthreads();
-        for (int64_t b = tid; b < a.B; b += threads) {
-          const int64_t r = (int64_t)a.prefix_rows[b] - p0;
-          if (r >= 0 && r < np) atomicAdd(&rows[r], 1);
+      for (int i0 = 0;; i0 += 64) {  // ends: block cb is one of these
+        const int own = blocks_of(a, p0, i0 + lane, per, rows), to = wave_inclusive_sum(own);
+        const uint64_t after = __ballot((uint32_t)to > cb);
+        if (after != 0ull || i0 >= kCount) {
+          const int l = after != 0ull ? __builtin_ctzll(after) : 0;
+          p = p0 + i0 + l;
+          cb -= (uint32_t)__shfl(to - own, l, 64);
+          break;
         }
-        __syncthreads();
-        for (int i0 = 0; i0 < np && !found; i0 += 64) {
-          const uint32_t n = i0 + lane < np ? (uint32_t)rows[i0 + lane] * per : 0u;
-          const int own = (int)((n + COLS - 1) / COLS), to = wave_inclusive_sum(own);
-          const uint64_t after = __ballot(base + (uint32_t)to > cb);
-          if (after != 0ull) {
-            const int l = __builtin_ctzll(after);
-            found = true;
-            p = p0 + i0 + l;
-            cb -= base + (uint32_t)__shfl(to - own, l, 64);
-          } else {
-            base += (uint32_t)__shfl(to, 63, 64);
-          }
-        }
-        __syncthreads();  // before the counts' place is used again
+        cb -= (uint32_t)__shfl(to, 63, 64);
       }
-      if (!found) return false;
+      __syncthreads();  // the counts are read
+    } else if (a.prefix_rows == nullptr && a.P > 1) {
+      const uint32_t each = (per + COLS - 1) / COLS;
+      p = (int)(cb / each);
+      cb %= each;
     }
-    pc = prefix_pieces(a, p);
+    pc = prefix_pieces(a, p, splits);
     return s < pc.count;
   }
   // The columns; false: none. Contains barriers.
@@ -748,9 +773,17 @@ int64_t column_blocks(const PrefixArgs& a, int64_t wg) {
   return (a.B * per + std::min<int64_t>(a.P, a.B) * (wg - 1)) / wg;
 }
 
+// Workgroups of `blocks` column blocks, a prefix in `splits` pieces (PrefixBlock::place).
+int64_t placed(const PrefixArgs& a, int64_t blocks, int64_t splits) {
+  const int64_t units = (int64_t)a.Hkv * splits, together = std::min<int64_t>(units, kXcds);
+  return (units + together - 1) / together * together * blocks;
+}
 int64_t prefix_grid(const PrefixArgs& a, int64_t wg) {
-  const int64_t units = (int64_t)a.Hkv * a.splits, together = std::min<int64_t>(units, kXcds);
-  return (units + together - 1) / together * together * column_blocks(a, wg);
+  const int64_t blocks = column_blocks(a, wg);
+  if (!a.plan) return placed(a, blocks, a.splits);
+  int64_t most = placed(a, blocks, 1);  // whichever spread of the rows needs most
+  for (int64_t n = 2; n <= a.splits; ++n) most = std::max(most, placed(a, std::min<int64_t>(blocks, 256 / (n * a.Hkv)), n));
+  return most;
 }
 
 template <typename T, int D, int KG, int CG>

@@ -35,7 +35,7 @@ __global__ __launch_bounds__(LSA_BLOCK) void prefix_rows_kernel(PrefixArgs a, in
   if (arrive == kNone && s == 0 && threadIdx.x == 0) a.counters[i] = 0;
   const bool piece = s < a.splits;
   const int p = prefix_of(a, b);
-  const Pieces pc = prefix_pieces(a, p);
+  const Pieces pc = prefix_pieces(a, p, a.plan ? *a.plan : a.splits);
   int n = 0;
   const int32_t* ids = nullptr;  // the keys' rows (a prefix's own order without)
   if (a.W > 0 && !(arrive == kNone && piece)) {
@@ -104,25 +104,24 @@ struct PrefixPlan {
   size_t parts, sums, total;
 };
 
-// Prefixes that rows read, at most, and the query columns of each if the rows are spread evenly.
-int64_t read_prefixes(int64_t B, int64_t P) { return std::max<int64_t>(1, std::min(B, P)); }
+// The query columns of a prefix if the rows are spread evenly over as many as they may read.
 int64_t mean_columns(int64_t B, int64_t Tq, int64_t P, int32_t Hq, int32_t Hkv) {
-  const int64_t n = read_prefixes(B, P);
+  const int64_t n = std::max<int64_t>(1, std::min(B, P));
   return (B * Tq * (Hq / Hkv) + n - 1) / n;
 }
 
-// Pieces and own spans by size. On the matrix cores a workgroup has a CU to itself: as many pieces
-// as make one workgroup a CU, of at least 256 keys. The gather: about 512 workgroups. Own spans of at
-// least 256 slots, as many as make 512 workgroups.
+// Pieces and own spans by size. On the matrix cores room for the pieces, of at least 256 keys, that a prefix is
+// cut into if every row reads the same one (how the rows are spread is known on the device alone). The
+// gather: about 512 workgroups. Own spans of at least 256 slots, as many as make 512 workgroups.
 PrefixPlan prefix_plan(int dtype, int64_t B, int64_t Tq, int64_t P, int64_t Tp, int32_t Hq, int32_t Hkv, int32_t D, int32_t W) {
   PrefixPlan p;
   const int64_t units = B * Tq * Hkv;
   const int64_t tiles = (Tp + kPieceTile - 1) / kPieceTile;
   int64_t most = tiles, want_p = 512 / std::max<int64_t>(units, 1);
   if (prefix_mfma_ok(dtype, D)) {
-    const int64_t cols = mean_columns(B, Tq, P, Hq, Hkv), wg = prefix_mfma_columns(cols);
+    const int64_t wg = prefix_mfma_columns(mean_columns(B, Tq, P, Hq, Hkv));
     most = (tiles + 3) / 4;
-    want_p = 256 / std::max<int64_t>(1, read_prefixes(B, P) * Hkv * ((cols + wg - 1) / wg));
+    want_p = prefix_mfma_pieces((B * Tq * (Hq / Hkv) + wg - 1) / wg, Hkv);
   }
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, kMaxPieces, want_p}));
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kMaxOwn, 512 / std::max<int64_t>(units, 1)));
@@ -132,7 +131,7 @@ PrefixPlan prefix_plan(int dtype, int64_t B, int64_t Tq, int64_t P, int64_t Tp, 
   const int64_t gq = Hq / Hkv;
   p.parts = (size_t)units * (p.splits + p.own_splits) * (size_t)(gq * (D + 2)) * sizeof(float);
   p.sums = (size_t)units * p.splits * gq * sizeof(float);
-  p.total = p.parts + p.sums + (size_t)units * sizeof(int);
+  p.total = p.parts + p.sums + (size_t)(units + 1) * sizeof(int);
   return p;
 }
 
@@ -154,6 +153,7 @@ void launch_prefix_gq(PrefixArgs a, int gq, int64_t units, int* counters, hipStr
   const dim3 all((unsigned)units, (unsigned)(a.splits + a.own_splits));
   const bool mfma = launch_prefix_mfma(a, __is_same(T, float) ? LSA_F32 : (__is_same(T, bf16_t) ? LSA_BF16 : LSA_F16), D,
                                        mean_columns(a.B, a.Tq, a.P, a.Hq, a.Hkv), s);
+  if (!mfma) a.plan = nullptr;
   if (!mfma) a.sums = nullptr;  // row by row the weights are fp32: one sum serves both
   if (!mfma && counters) a.counters = counters;
 #define LSA_PREFIX(GQ)                                                                        \
@@ -246,6 +246,11 @@ extern "C" int lsa_prefix_read(const void* q, const void* k_prefix, const void* 
   hipStream_t s = (hipStream_t)stream;
   const int64_t units = B * Tq * Hkv;
   const int gq = Hq / Hkv;
+  if (P > 1 && prefix_mfma_ok(dtype, D)) {
+    const int64_t per = Tq * gq, wg = prefix_mfma_columns(mean_columns(B, Tq, P, Hq, Hkv));
+    if (prefix_rows) a.plan = a.counters + units;
+    else a.splits = std::min(p.splits, prefix_mfma_pieces(P * ((per + wg - 1) / wg), Hkv));
+  }
   if (dtype == LSA_BF16) launch_prefix<bf16_t>(a, D, gq, units, counters, s);
   else if (dtype == LSA_F16) launch_prefix<_Float16>(a, D, gq, units, counters, s);
   else launch_prefix<float>(a, D, gq, units, counters, s);

@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+import test_gpu_prefix as prefix
 from lsa_rocm_lab import _abi
 from lsa_rocm_lab.port import eviction, pipeline
 
@@ -98,3 +99,45 @@ def test_key_weights_in_slabs_of_the_batch(monkeypatch, B, Tq, pool):
                     assert torch.equal(x, y)
                 else:
                     assert ((x.double() - y.double()).abs() <= B * Tq * (2.0 ** -23 * y.double() + 8 * 2.0 ** -44)).all()
+
+
+SPREADS = {
+    "one": lambda P, B: torch.full((B,), P - 2),
+    "one and none": lambda P, B: torch.where(torch.arange(B) % 3 == 0, -1, P - 2),
+    "two": lambda P, B: torch.where(torch.arange(B) % 5 == 0, 1, P - 1),
+    "few": lambda P, B: (P * torch.linspace(0, 0.99, B) ** 5).long(),
+    "none": lambda P, B: torch.full((B,), P),
+}
+
+
+@pytest.mark.parametrize("dtype,B,Tq,P,Tp,Hq,Hkv,D,paged", [
+    (torch.bfloat16, 8, 1, 8, 2100, 8, 2, 128, 0),
+    (torch.bfloat16, 40, 2, 30, 1500, 4, 1, 64, 16),   # several column blocks of one prefix
+    (torch.float16, 6, 1, 1100, 600, 2, 1, 64, 16),    # past the first thousand
+    (torch.float16, 70, 3, 5, 900, 8, 1, 128, 0),      # wide columns
+    (torch.bfloat16, 5, 1, 2, 33000, 4, 1, 64, 0),     # 128 pieces
+])
+def test_rows_that_crowd_on_few_of_many_prefixes(dtype, B, Tq, P, Tp, Hq, Hkv, D, paged):
+    """However the rows are spread, eagerly and from one graph whose rows change between replays."""
+    c = prefix.make(dtype, B, Tq, P, Tp, Hq, Hkv, D, 20, 5, paged=paged, seed=61)
+    c["plen"][1], c["plen"][P - 2:] = Tp // 3, Tp - 1
+    t = {n: c[n].to(DEV) for n in ("q", "kp", "vp", "k", "v", "ids", "lens", "plen", "prow")}
+    slots = prefix.dev(c["slots"])
+
+    def step():
+        return pipeline.prefix_read(t["q"], t["kp"], t["vp"], t["k"], t["v"], t["ids"], t["lens"], prefix_lengths=t["plen"],
+                                    prefix_rows=t["prow"], prefix_slots=slots, return_lse=True)
+
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for name, spread in SPREADS.items():
+        print("crowd", dtype, B, Tq, P, Tp, name, flush=True)
+        c["prow"] = spread(P, B).int()
+        t["prow"].copy_(c["prow"])
+        exact = prefix.want(c)
+        eager = step()
+        prefix.compare(eager, exact, c)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], eager[0]) and torch.equal(out[1], eager[1])

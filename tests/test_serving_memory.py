@@ -212,3 +212,15 @@ def test_key_weights_in_slabs_of_memory(calls, B, Tq, Hq, Hkv, T, W, pool, fresh
             assert sum(n for n, _ in mine) == Tq
             assert [z for _, z in mine] == [int(fresh)] + [0] * (len(mine) - 1)
     assert len(rows) == 1 or 4 * B * Tq * Hq * W + (0 if pool or Tq == 1 else 8 * B * Hkv * T) > limit
+
+
+@pytest.mark.parametrize("B", [8, 32, 256])
+@pytest.mark.parametrize("P", [8, 32, 2000])
+def test_room_for_a_prefix_that_every_row_reads(B, P):
+    """However many prefixes the table holds: where all rows read one of them it is cut into as many pieces
+    as fill the chip (256 workgroups of 32 or more columns), so there is room for their partials."""
+    need = _abi.size("lsa_prefix_read_scratch_bytes", _abi.LSA_BF16, B, 1, P, 32768, 32, 8, 128, 0)
+    columns = -(-B // min(B, P)) * 4  # a prefix, if the rows are spread
+    blocks = -(-B * 4 // next(n for n in (32, 64, 128, 256) if columns <= n or n == 256))
+    pieces = max(1, 256 // (8 * blocks))
+    assert need >= B * 8 * pieces * 4 * (128 + 2) * 4
