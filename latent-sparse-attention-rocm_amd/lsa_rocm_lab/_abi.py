@@ -304,7 +304,8 @@ class Counters:
     launch and leaves zero, so the buffer is zero-filled only when it is (re)allocated. A fused
     decode that gives up waiting may leave words in its own ("decode", which ``reset`` zeroes);
     purposes whose kernels never wait share none with it.
-    Outgrown buffers are retired, never freed (a captured graph may hold them)."""
+    Outgrown buffers are retired, never freed (a captured graph may hold them), and at least
+    double, as workspaces do."""
 
     _buffers: dict[tuple, torch.Tensor] = {}
     _retired: list[torch.Tensor] = []
@@ -316,6 +317,7 @@ class Counters:
         if buf is None or buf.numel() < n:
             if buf is not None:
                 cls._retired.append(buf)
+                n = max(n, 2 * buf.numel())
             buf = torch.zeros(max(n, 4096), dtype=torch.int32, device=device)
             cls._buffers[key] = buf
         return buf

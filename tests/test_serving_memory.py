@@ -224,3 +224,10 @@ def test_room_for_a_prefix_that_every_row_reads(B, P):
     blocks = -(-B * 4 // next(n for n in (32, 64, 128, 256) if columns <= n or n == 256))
     pieces = max(1, 256 // (8 * blocks))
     assert need >= B * 8 * pieces * 4 * (128 + 2) * 4
+
+
+def test_counters_that_creep_up(host):
+    """Outgrown counters are kept for graphs that hold them: a buffer at least doubles, so they stay few."""
+    for n in range(4000, 40000, 500):
+        assert _abi.call_memory(GPU, "prefix_read", 0, n)[1].numel() >= n
+    assert sum(x.numel() for x in _abi.Counters._retired) < 2 * 40000
