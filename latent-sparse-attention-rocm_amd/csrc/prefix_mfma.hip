@@ -80,18 +80,26 @@ struct PrefixBlock {
     const int64_t clear = (int64_t)gridDim.x * threads;
     for (int64_t i = (int64_t)blockIdx.x * threads + tid; i < a.B * a.Tq * a.Hkv; i += clear) a.counters[i] = 0;
     const uint32_t per = (uint32_t)a.Tq * (uint32_t)GQ;  // columns of a batch row; all are fewer than 2^31
-    int splits = a.splits, of = 0;  // of: lane c: the blocks of the c-th kCount prefixes (64 times as many at most)
-    if (a.plan) {  // uniform from here on, as every wave finds the same
+    int splits = a.splits, own = 0, to = 0;
+    int of = 0;  // lane c: the blocks of the c-th kCount prefixes (64 times as many at most)
+    if (a.plan && a.P <= 64) {  // uniform from here on, as every wave finds the same
+      count(a, 0, threads, rows);
+      own = blocks_of(a, 0, lane, per, rows);
+      to = wave_inclusive_sum(own);
+      blocks = (uint32_t)__builtin_amdgcn_readlane(to, 63);
+    } else if (a.plan) {
       blocks = 0;
       for (int c = 0; c * kCount < a.P; ++c) {
         count(a, c * kCount, threads, rows);
-        int own = 0;
+        own = 0;
         for (int i0 = 0; i0 < kCount && c * kCount + i0 < a.P; i0 += 64) own += blocks_of(a, c * kCount, i0 + lane, per, rows);
         own = wave_sum(own);
         of = lane == c ? own : of;
         blocks += (uint32_t)own;
         if (a.P > kCount) __syncthreads();  // before the counts' place is used again
       }
+    }
+    if (a.plan) {
       splits = min(splits, prefix_mfma_pieces(blocks, a.Hkv));
       if (blockIdx.x == 0 && tid == 0) *a.plan = splits;
       if (blocks == 0) return false;
@@ -107,13 +115,17 @@ struct PrefixBlock {
     if (a.plan) {
       int p0 = 0;
       if (a.P > kCount) {
-        const int to = wave_inclusive_sum(of), c = __builtin_ctzll(__ballot((uint32_t)to > cb));
+        to = wave_inclusive_sum(of);
+        const int c = __builtin_ctzll(__ballot((uint32_t)to > cb));
         cb -= (uint32_t)__shfl(to - of, c, 64);
         p0 = c * kCount;
         count(a, p0, threads, rows);
       }
       for (int i0 = 0;; i0 += 64) {  // ends: block cb is one of these
-        const int own = blocks_of(a, p0, i0 + lane, per, rows), to = wave_inclusive_sum(own);
+        if (a.P > 64) {
+          own = blocks_of(a, p0, i0 + lane, per, rows);
+          to = wave_inclusive_sum(own);
+        }
         const uint64_t after = __ballot((uint32_t)to > cb);
         if (after != 0ull || i0 >= kCount) {
           const int l = after != 0ull ? __builtin_ctzll(after) : 0;

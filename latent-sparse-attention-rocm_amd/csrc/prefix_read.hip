@@ -35,7 +35,7 @@ __global__ __launch_bounds__(LSA_BLOCK) void prefix_rows_kernel(PrefixArgs a, in
   if (arrive == kNone && s == 0 && threadIdx.x == 0) a.counters[i] = 0;
   const bool piece = s < a.splits;
   const int p = prefix_of(a, b);
-  const Pieces pc = prefix_pieces(a, p, a.plan ? *a.plan : a.splits);
+  const int most = a.plan ? *a.plan : a.splits;
   int n = 0;
   const int32_t* ids = nullptr;  // the keys' rows (a prefix's own order without)
   if (a.W > 0 && !(arrive == kNone && piece)) {
@@ -44,10 +44,11 @@ __global__ __launch_bounds__(LSA_BLOCK) void prefix_rows_kernel(PrefixArgs a, in
     n = (n < 0 || a.Tk <= 0) ? 0 : (n > a.W ? a.W : n);
     ids = a.ids + li * a.W;
   }
+  const Pieces pc = prefix_pieces(a, p, most);
   const int n_own = (n + a.own_span - 1) / a.own_span, total = pc.count + n_own;
   const int at = piece ? s : s - a.splits;
   const bool active = at < (piece ? pc.count : n_own);
-  float* parts = a.parts + (i * (a.splits + a.own_splits) + a.splits - pc.count) * (int64_t)PSTRIDE;
+  float* own = a.parts + (i * (a.splits + a.own_splits) + a.splits) * (int64_t)PSTRIDE;
   if (!active) {  // a unit without spans to wait for still joins: its first workgroup
     if (arrive == kNone || blockIdx.y != 0 || (arrive == kAll ? total : n_own) > 0) return;
   } else {
@@ -68,11 +69,12 @@ __global__ __launch_bounds__(LSA_BLOCK) void prefix_rows_kernel(PrefixArgs a, in
                                 },
                                 a.scale_log2, st);
     finish_span<T, D, GQ, kMaxPieces + kMaxOwn, true>(sh, st, false, (T*)nullptr,
-                                                      parts + (int64_t)(piece ? at : pc.count + at) * PSTRIDE, 0);
+                                                      own + (int64_t)(piece ? at - pc.count : at) * PSTRIDE, 0);
     if (arrive == kNone) return;
     // the partials complete before they are read back, by this workgroup or the last one
     if (!arrive_last(&a.counters[i], arrive == kAll ? total : n_own, &sh.flag)) return;
   }
+  const float* parts = own - pc.count * PSTRIDE;
   T* outp = (T*)a.out + (row * a.Hq + (int64_t)g * GQ) * D;
   if (total == 0) {
     for (int j = threadIdx.x; j < GQ * D; j += LSA_BLOCK) store_out<T>(outp + j, 0.0f);
