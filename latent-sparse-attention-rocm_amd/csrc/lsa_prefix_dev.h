@@ -29,7 +29,8 @@ struct PrefixArgs {
   int P, Hq, Hkv;
   float scale_log2;
   int splits;      // pieces of a prefix at most (how many parts a unit has room for)
-  int* plan;       // pieces of a prefix at most for the rows' own spread over prefixes, or nullptr: splits
+  int* plan;       // pieces of a prefix at most for the rows' own spread over prefixes, or nullptr: splits (at
+                   // most 1024 prefixes)
   int own_splits;  // spans of an own list at most
   int own_span;    // list slots of a span
   int* counters;   // [units]: cleared by the prefix kernel, arrivals of the own spans

@@ -82,15 +82,16 @@ struct PrefixBlock {
     const uint32_t per = (uint32_t)a.Tq * (uint32_t)GQ;  // columns of a batch row; all are fewer than 2^31
     int splits = a.splits, own = 0, to = 0;
     int of = 0;  // lane c: the blocks of the c-th kCount prefixes (64 times as many at most)
-    if (a.plan && a.P <= 64) {  // uniform from here on, as every wave finds the same
-      count(a, 0, threads, rows);
+    const bool counted = a.prefix_rows != nullptr && a.P > 1, few = a.P <= 64;
+    if (counted && a.P <= kCount) count(a, 0, threads, rows);
+    if (counted && few) {  // uniform from here on, as every wave finds the same
       own = blocks_of(a, 0, lane, per, rows);
       to = wave_inclusive_sum(own);
-      blocks = (uint32_t)__builtin_amdgcn_readlane(to, 63);
-    } else if (a.plan) {
-      blocks = 0;
-      for (int c = 0; c * kCount < a.P; ++c) {
-        count(a, c * kCount, threads, rows);
+    }
+    if (a.plan) {
+      blocks = few ? (uint32_t)__builtin_amdgcn_readlane(to, 63) : 0u;
+      for (int c = 0; !few && c * kCount < a.P; ++c) {
+        if (a.P > kCount) count(a, c * kCount, threads, rows);
         own = 0;
         for (int i0 = 0; i0 < kCount && c * kCount + i0 < a.P; i0 += 64) own += blocks_of(a, c * kCount, i0 + lane, per, rows);
         own = wave_sum(own);
@@ -98,8 +99,6 @@ struct PrefixBlock {
         blocks += (uint32_t)own;
         if (a.P > kCount) __syncthreads();  // before the counts' place is used again
       }
-    }
-    if (a.plan) {
       splits = min(splits, prefix_mfma_pieces(blocks, a.Hkv));
       if (blockIdx.x == 0 && tid == 0) *a.plan = splits;
       if (blocks == 0) return false;
@@ -112,7 +111,7 @@ struct PrefixBlock {
     g = (int)(u / (uint32_t)splits);
     if (g >= a.Hkv) return false;
     p = 0;
-    if (a.plan) {
+    if (counted) {
       int p0 = 0;
       if (a.P > kCount) {
         to = wave_inclusive_sum(of);
@@ -121,14 +120,15 @@ struct PrefixBlock {
         p0 = c * kCount;
         count(a, p0, threads, rows);
       }
-      for (int i0 = 0;; i0 += 64) {  // ends: block cb is one of these
-        if (a.P > 64) {
+      for (int i0 = 0;; i0 += 64) {
+        if (i0 >= min(kCount, a.P - p0)) return false;  // unplanned: fewer blocks than there may be
+        if (!few) {
           own = blocks_of(a, p0, i0 + lane, per, rows);
           to = wave_inclusive_sum(own);
         }
         const uint64_t after = __ballot((uint32_t)to > cb);
-        if (after != 0ull || i0 >= kCount) {
-          const int l = after != 0ull ? __builtin_ctzll(after) : 0;
+        if (after != 0ull) {
+          const int l = __builtin_ctzll(after);
           p = p0 + i0 + l;
           cb -= (uint32_t)__shfl(to - own, l, 64);
           break;

@@ -249,9 +249,12 @@ extern "C" int lsa_prefix_read(const void* q, const void* k_prefix, const void* 
   const int64_t units = B * Tq * Hkv;
   const int gq = Hq / Hkv;
   if (P > 1 && prefix_mfma_ok(dtype, D)) {
-    const int64_t per = Tq * gq, wg = prefix_mfma_columns(mean_columns(B, Tq, P, Hq, Hkv));
-    if (prefix_rows) a.plan = a.counters + units;
-    else a.splits = std::min(p.splits, prefix_mfma_pieces(P * ((per + wg - 1) / wg), Hkv));
+    const int64_t cols = mean_columns(B, Tq, P, Hq, Hkv), wg = prefix_mfma_columns(cols);
+    const int spread = prefix_mfma_pieces(std::min(B, P) * ((cols + wg - 1) / wg), Hkv);  // rows spread evenly
+    if (!prefix_rows) a.splits = std::min(p.splits, spread);  // a row each
+    // by the rows' own spread, unless it cuts them alike however they are spread (the plan costs 0.9 us: 32 rows on
+    // 8 prefixes of 2048 keys 20.5 us without and 21.4 with it)
+    else if (spread < p.splits || P > 1024) a.plan = a.counters + units;
   }
   if (dtype == LSA_BF16) launch_prefix<bf16_t>(a, D, gq, units, counters, s);
   else if (dtype == LSA_F16) launch_prefix<_Float16>(a, D, gq, units, counters, s);
