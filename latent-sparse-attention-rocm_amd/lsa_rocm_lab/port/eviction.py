@@ -216,7 +216,8 @@ def evict(
     masses [B, Hkv, budget], their positions in the old cache [B, Hkv, budget] int32 (shared:
     [B, budget]; -1 past the row's new length) and the new lengths [B] int32. New tensors hold
     zeros past the new length. ``out`` = (k, v, mass) buffers of ``budget`` rows or more (not the
-    inputs: two caches take turns), whose rows past the new length are left as they were.
+    inputs: two caches take turns; each written element in a place of its own), whose rows past the
+    new length are left as they were.
     """
     device = one_device("evict", k, v, mass)
     if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:

@@ -18,7 +18,7 @@ a HIP kernel in liblsa_rocm.so:
 * ``dense_read`` (:340-370) stays torch SDPA - it is the dense comparator.
 
 Around a decode step, with no counterpart in the reference: ``prefix_read`` (a batch that shares
-a long prefix, read once for all), ``key_mass`` (the attention weight that each listed key
+a long prefix, kept once), ``key_mass`` (the attention weight that each listed key
 received), ``evict`` and ``evict_slots`` (a dense or a paged cache cut down by that weight).
 
 The index grows with the cache: ``extend_buckets`` appends newly closed blocks, and

@@ -1,8 +1,10 @@
 """Attention of a decode batch over a prefix that its rows share.
 
 Requests behind one system prompt hold the same keys at its start. ``prefix_read`` keeps those
-once, reads them once for the whole batch, and joins them in one softmax with what each row
-reads of its own cache (a read list, as ``lsa_read``). No counterpart in the reference.
+once and joins them in one softmax with what each row reads of its own cache (a read list, as
+``lsa_read``). bf16 and fp16 rows of head dim 64 or 128 read them once for the whole batch (up to
+256 query rows times heads a kv-head at a time); fp32, head dims 32 and 256 and a scale that is not
+positive read them once a query row. No counterpart in the reference.
 """
 
 from __future__ import annotations
@@ -103,6 +105,9 @@ def prefix_read(
     (default: the only prefix, or prefix b where there are B; one outside [0, P) means none).
     ``k``, ``v``, ``read_lists``, ``lengths``: the own part, as ``lsa_read`` (lists
     [B, Tq, W] or [B, Tq, Hkv, W]; k/v [B or 1, Tk, Hkv, D]); all four or none.
+    Where the prefix is read once for the batch its softmax weights are rounded to q's type (by half
+    a step at most; the sum that divides them adds the rounded ones); the row forms and ``lsa_read``
+    keep them in fp32.
 
     Returns the output, like q, or with ``return_lse`` also the softmax's logarithm of sums
     [B, Tq, Hq] in fp32 (``key_mass`` takes it). A row with no keys gives zeros and -inf.
