@@ -39,9 +39,9 @@ constexpr int kXcds = 8;
 // blocks one may have is nearly all empty where prefixes are many: 512 rows over 128 prefixes of 2048
 // keys took 820 us so, and take 242; 64 rows over 4000 of 256 keys 1922 and 42.) Into how many pieces a prefix
 // is cut follows from the blocks there are, so rows that all read one prefix of a table of many fill the chip
-// too (32 rows on one of 32 prefixes of 32768 keys: 48 us, and 259 in as many pieces as if they were spread; 39 where
-// the table holds that prefix alone, whose rows then stand in wider blocks). Units come in groups of 8, the blocks of a unit 8 apart, so that those which read the same keys share an XCD
-// and its L2.
+// too (32 rows on one of 32 prefixes of 32768 keys: 48 us, and 259 in as many pieces as if they were spread; 39
+// where the table holds that prefix alone, whose rows then stand in wider blocks). Units come in groups of 8, the
+// blocks of a unit 8 apart, so that those which read the same keys share an XCD and its L2.
 template <int COLS>
 struct PrefixBlock {
   static constexpr int kCount = 1024;  // prefixes counted at once

@@ -118,7 +118,8 @@ SPREADS = {
     (torch.bfloat16, 5, 1, 2, 33000, 4, 1, 64, 0),     # 128 pieces
     (torch.bfloat16, 8, 1, 8, 9000, 8, 8, 64, 0),      # 4 pieces if the rows are spread, 32 if they crowd
     (torch.float16, 40, 2, 100, 2700, 8, 8, 64, 16),   # 1 or 10
-    (torch.bfloat16, 150, 1, 30, 1100, 16, 4, 128, 0), # 2 or 3, of several blocks
+    (torch.bfloat16, 150, 1, 30, 1100, 16, 4, 128, 0),  # 2 or 3, of several blocks
+    (torch.float16, 30, 1, 200, 60, 4, 2, 64, 0),      # one piece at most, past the first 64
 ])
 def test_rows_that_crowd_on_few_of_many_prefixes(dtype, B, Tq, P, Tp, Hq, Hkv, D, paged):
     """However the rows are spread, eagerly and from one graph whose rows change between replays."""
