@@ -513,6 +513,81 @@ int lsa_evict_rows(const void* k, const void* v, const float* mass, int dtype, i
                    int64_t out_head_stride, float* mass_out, int64_t mass_out_batch_stride,
                    int64_t mass_out_head_stride, int zero_tail, void* stream);
 
+/* Norms of head rows and their rotary positions. A row x [D] becomes
+ *   y = x / sqrt(mean(x^2) + eps) * weight           (with a weight; else y = x)
+ *   (y_a, y_b) -> magnitude (y_a cos t - y_b sin t, y_a sin t + y_b cos t),  t = position frequencies[j]
+ * for every pair j < pairs: (2j, 2j + 1) where interleaved, else (j, j + pairs). Dims from 2 * pairs on stay.
+ * Angles are taken in fp64, everything else in fp32, rounded once. */
+typedef struct lsa_turn {
+  const void* frequencies; /* [pairs] fp32, or fp64 (frequencies_f64); NULL with pairs 0: no rotation */
+  const void* q_weight;    /* [D] of the rows' type, or fp32 (weights_f32), 16-byte aligned; NULL: no norm */
+  const void* k_weight;
+  int32_t pairs;
+  int32_t frequencies_f64;
+  int32_t interleaved;
+  int32_t weights_f32;
+  float eps;
+  float magnitude;
+} lsa_turn;
+
+/* q [B, T, Hq, D] and k [B, T, Hkv, D] (element strides, rows of D contiguous elements, 16-byte aligned;
+ * Hkv 0: q alone) to q_out and k_out, dense, of the same dtype, normed and rotated. positions: int32 (or int64)
+ * at b * position_stride + t. D in {32, 64, 128, 256}; at most 2^30 tokens. No counterpart in the reference. */
+int lsa_rotate(const void* q, const void* k, int dtype, int64_t B, int64_t T, int32_t Hq, int32_t Hkv, int32_t D,
+               int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride, int64_t k_batch_stride,
+               int64_t k_token_stride, int64_t k_head_stride, const void* positions, int positions_i64,
+               int64_t position_stride, const lsa_turn* turn, void* q_out, void* k_out, void* stream);
+
+/* A cache of 8-bit codes. Row t of kv-head h of cache c holds code * scale, with K's and V's codes at
+ * c * batch_stride + t * token_stride + h * head_stride (bytes; rows of D contiguous codes, 16-byte aligned) and
+ * their scales at scales[((c * ceil(tokens / block) + t / block) * Hkv + h) * 2 + (0: K, 1: V)]. `caches` is the
+ * call's batch rows, or 1 (a pool for every row). */
+enum lsa_byte_code { LSA_INT8 = 0, LSA_E4M3 = 1 };
+typedef struct lsa_byte_cache {
+  void* k;
+  void* v;
+  float* scales;
+  int32_t code;  /* enum lsa_byte_code */
+  int32_t block; /* tokens of a scale: 1, 2, 4 .. 64 */
+  int64_t caches, tokens;
+  int64_t batch_stride, token_stride, head_stride;
+} lsa_byte_cache;
+
+/* Tokens n < lengths[b] (NULL: T) of row b's k and v [B, T, Hkv, D] (element strides, rows 16-byte aligned) into
+ * the cache at positions starts[b] + n, k normed and rotated (turn's k_weight), and, where q [B, T, Hq, D] is given,
+ * q_out [B, T, Hq, D] (dense), normed and rotated, zeros behind a row's length. Position p is cache row p, or, with
+ * a slot map, that of its block's first position (a multiple of block; slots->rows [B]) plus its offset in the
+ * block. Positions outside the cache, the map or the pool are dropped, and so is a block whose slot is no multiple
+ * of block. A block that is written to gets the scale max(its own where it holds positions before starts[b], its
+ * new tokens' largest magnitude / M, 2^-100), M = 127 or 448; a new token's code is value / scale, rounded to
+ * nearest even, and where the scale grew the block's earlier codes are rescaled and rounded again. What it held
+ * from starts[b] on counts for nothing. A NaN has no part in the scale and is held as e4m3's NaN or int8's 0, an
+ * infinity as the largest code, neither in the scale. No two rows may write to one block. No counterpart in the
+ * reference. */
+int lsa_byte_append(const lsa_byte_cache* cache, const void* k, const void* v, const void* q, int dtype, int64_t B,
+                    int64_t T, int32_t Hq, int32_t Hkv, int32_t D, int64_t k_batch_stride, int64_t k_token_stride,
+                    int64_t k_head_stride, int64_t v_batch_stride, int64_t v_token_stride, int64_t v_head_stride,
+                    int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride, const int32_t* starts,
+                    const int32_t* lengths, const lsa_slot_map* slots, const lsa_turn* turn, void* q_out, void* stream);
+
+/* What the cache holds, as numbers: row w of list r (cache row rows[r * row_stride + w], or w where rows is NULL)
+ * to k_out and v_out [R, W, Hkv, D] (dense), of `dtype`; zeros at w >= lengths[r] (NULL: W) and for rows outside
+ * the cache. cache->caches is R or 1. */
+int lsa_byte_values(const lsa_byte_cache* cache, const int32_t* rows, int64_t row_stride, const int32_t* lengths,
+                    int64_t R, int64_t W, int32_t Hkv, int32_t D, int dtype, void* k_out, void* v_out, void* stream);
+
+/* lsa_read over an 8-bit cache: q [B, Tq, Hq, D] dense, lists as lsa_read's (shared by the heads, or one a
+ * kv-head), out like q; a row with no keys gives zeros. Any Hq that Hkv divides; D in {32, 64, 128, 256}; under
+ * 2^24 rows times kv-heads times blocks of 16 of their query heads (the units). Keys enter exactly, q exactly, a
+ * weight times V's scale with 16 bits of mantissa (fp32 rows: 24). splits 1..64: spans of a list.
+ * counters (or NULL): a unit's int32 that reads zero at launch and is left zero; with them a split read is one
+ * launch instead of two. scratch: lsa_byte_read_scratch_bytes(), 16-byte aligned, no initialisation (0 bytes with
+ * one span). No counterpart in the reference. */
+size_t lsa_byte_read_scratch_bytes(int64_t rows, int32_t Hq, int32_t Hkv, int32_t D, int32_t splits);
+int lsa_byte_read(const void* q, const lsa_byte_cache* cache, int dtype, int64_t B, int64_t Tq, int32_t Hq, int32_t Hkv,
+                  int32_t D, const int32_t* ids, const int32_t* lengths, int32_t W, int ids_per_head, float scale,
+                  int32_t splits, int32_t* counters, void* scratch, size_t scratch_bytes, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -23,7 +23,8 @@ BUILD = HERE / "_build"
 LIB = HERE / "lsa_rocm_lab" / "_lib" / "liblsa_rocm.so"
 SOURCES = ["lsa_abi.cpp", "select.hip", "beam.hip", "read.hip", "read_prefill.hip", "read_rows.hip", "decode.hip", "decode_bf16.hip",
            "decode_f16.hip", "decode_f32.hip", "decode_noalloc.hip", "decode_shared.hip", "decode_tree_shared.hip",
-           "build.hip", "prefix_read.hip", "prefix_mfma.hip", "key_mass.hip", "evict.hip"]
+           "build.hip", "prefix_read.hip", "prefix_mfma.hip", "key_mass.hip", "evict.hip",
+           "rotate.hip", "byte_cache.hip", "byte_read.hip"]
 ARCH = os.environ.get("LSA_OFFLOAD_ARCH", "gfx950")
 
 

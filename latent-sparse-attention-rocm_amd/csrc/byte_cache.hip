@@ -1,0 +1,365 @@
+// A cache of 8-bit codes with a scale for each block of tokens and kv-head: writing to it and reading it back as
+// numbers (gfx950). The rotation is lsa_turn_dev.h's.
+//
+// byte_append_kernel. A workgroup takes a tile of 64 positions (whole blocks) of one batch row and a part of the
+// kv-heads, K and V of a head in turn: its lanes hold the tile's new tokens in registers (fp32, normed and rotated),
+// the largest magnitude of each block meets in LDS (an integer maximum: its order changes nothing), one barrier,
+// and every lane divides, rounds and stores. The block belongs to one workgroup, so its scale and the codes that
+// were there before are read and rewritten with no atomics on memory. The sines of the tile's tokens are taken once
+// for all heads of the workgroup. The rows of q, if any, go through workgroups of the same launch.
+// Memory bounds the large calls (16 bits read, 8 written), the launch and two memory round trips the small ones.
+#include <math.h>
+
+#include <algorithm>
+
+#include "lsa_abi_common.h"
+#include "lsa_turn_dev.h"
+
+using namespace lsa;
+
+namespace {
+
+constexpr int kTile = 64;
+constexpr float kLeast = 7.888609052210118e-31f;  // 2^-100, the smallest scale: its reciprocal is finite
+
+struct CacheArgs {
+  uint8_t* k;
+  uint8_t* v;
+  float* scales;
+  int block;
+  int64_t tokens, sb, st, sh;  // sb 0: one pool
+  int64_t scale_sb;            // scale pairs of a cache, times kv-heads
+};
+
+struct AppendArgs {
+  CacheArgs c;
+  const void* k;
+  const void* v;
+  const void* q;
+  void* q_out;
+  int64_t k_sb, k_st, k_sh, v_sb, v_st, v_sh, q_sb, q_st, q_sh;
+  const int32_t* starts;
+  const int32_t* lengths;
+  SlotMap slots;
+  int Hq, Hkv, T;
+  int B, tiles;      // tiles of a row
+  int parts, heads;  // workgroups of a tile, kv-heads of one
+  int q_tokens;      // tokens of a q workgroup
+  int64_t kv_groups; // workgroups before the first of q's
+  TurnArgs turn;
+};
+
+__device__ __forceinline__ int new_tokens(const AppendArgs& a, int b) {
+  const int n = a.lengths ? a.lengths[b] : a.T;
+  return n < 0 ? 0 : (n > a.T ? a.T : n);
+}
+
+// Rows of q: `q_tokens` tokens from t0 on, flat over the batch; a lane walks the heads of one token.
+template <typename T, int D>
+__device__ __forceinline__ void append_queries(const AppendArgs& a, int64_t group, float* stage, float2* angles) {
+  using L = HeadLanes<D>;
+  const int tid = threadIdx.x, lp = tid % L::LPT, slot = tid / L::LPT;
+  const int nt = a.q_tokens, rows = L::SLOTS / nt;
+  const int64_t t0 = group * nt, all = (int64_t)a.B * a.T;
+  for (int i = tid; i < nt * a.turn.pairs; i += LSA_BLOCK) {
+    const int n = i / a.turn.pairs, j = i - n * a.turn.pairs;
+    const int64_t at = min(t0 + n, all - 1);
+    angles[n * (D / 2) + j] = turn_angle(a.turn, (int64_t)a.starts[at / a.T] + at % a.T, j);
+  }
+  float w[8];
+  load_weights<T>(a.turn.qw, a.turn.w32, lp, w);
+  __syncthreads();
+  const int64_t mine = t0 + slot / rows;
+  if (mine >= all) return;
+  const int b = (int)(mine / a.T), t = (int)(mine % a.T);
+  LaneTurn turn;
+  if (a.turn.pairs > 0) turn.load(a.turn, angles + slot / rows * (D / 2), lp);
+  const bool live = t < new_tokens(a, b);
+  const T* q = (const T*)a.q + b * a.q_sb + t * a.q_st + 8 * lp;
+  T* out = (T*)a.q_out + mine * a.Hq * D + 8 * lp;
+  constexpr int AHEAD = 4;
+  for (int h0 = slot % rows; h0 < a.Hq; h0 += AHEAD * rows) {
+    Raw8<T> raw[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (h0 + i * rows < a.Hq && live) raw[i].load(q + (h0 + i * rows) * a.q_sh);
+      else raw[i].zero();
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int h = h0 + i * rows;
+      if (h >= a.Hq) break;
+      float y[8];
+      raw[i].get(y);
+      if (live) {
+        if (a.turn.qw) norm8<D>(y, w, a.turn.eps);
+        if (a.turn.pairs > 0) turn8(a.turn, y, turn, stage + slot * D, lp);
+      }
+      store8(out + (int64_t)h * D, y);
+    }
+  }
+}
+
+template <typename T, int D, typename C>
+__global__ __launch_bounds__(LSA_BLOCK) void byte_append_kernel(AppendArgs a) {
+  using L = HeadLanes<D>;
+  constexpr int STEPS = kTile / L::SLOTS;  // tokens of a lane
+  __shared__ __attribute__((aligned(16))) float stage[LSA_BLOCK * 8];
+  __shared__ __attribute__((aligned(16))) float2 angles[kTile * (D / 2)];
+  __shared__ uint32_t most[3][kTile];  // of a unit's blocks, as integers; three units take turns
+  __shared__ float before[3];          // the first block's scale, where it holds earlier tokens
+  __shared__ int32_t block_row[kTile];
+  const int tid = threadIdx.x;
+  if ((int64_t)blockIdx.x >= a.kv_groups) {
+    append_queries<T, D>(a, (int64_t)blockIdx.x - a.kv_groups, stage, angles);
+    return;
+  }
+  const int part = blockIdx.x % a.parts, tile = blockIdx.x / a.parts % a.tiles;
+  const int b = blockIdx.x / a.parts / a.tiles;
+  const int64_t start = a.starts[b];
+  const int64_t end = start + new_tokens(a, b);
+  const int64_t p0 = (start >= 0 ? start / kTile : 0) * kTile + (int64_t)tile * kTile;
+  const int64_t from = start > p0 ? start : p0;  // the tile's new positions: [from, to)
+  const int64_t to = end < p0 + kTile ? end : p0 + kTile;
+  if (from >= to) return;
+  const int block = a.c.block, blocks = kTile / block;
+  const int lo = (int)(from - p0), hi = (int)(to - p0);
+  const int begin = lo / block * block;  // the first written block's first token
+  if (tid < blocks) {
+    const int64_t p = p0 + (int64_t)tid * block;
+    int64_t row = p;
+    if (a.slots.table) {
+      const SlotRow map = slot_row_of(a.slots, b);
+      row = p < map.width ? map.row[p] : -1;
+    }
+    if (row < 0 || row >= a.c.tokens || row % block) row = -1;
+    block_row[tid] = (int32_t)row;
+  }
+  for (int i = tid; i < 3 * kTile; i += LSA_BLOCK) (&most[0][0])[i] = 0u;
+  for (int i = tid; i < (hi - lo) * a.turn.pairs; i += LSA_BLOCK) {
+    const int n = i / a.turn.pairs, j = i - n * a.turn.pairs;
+    angles[(lo + n) * (D / 2) + j] = turn_angle(a.turn, from + n, j);
+  }
+  const int lp = tid % L::LPT, slot = tid / L::LPT;
+  const int first = slot * STEPS;  // a lane's tokens are consecutive
+  float wk[8];
+  load_weights<T>(a.turn.kw, a.turn.w32, lp, wk);
+  __syncthreads();
+
+  const int h0 = part * a.heads, h1 = min(h0 + a.heads, a.Hkv);
+  const int64_t cb = b * a.c.sb;
+  float* scales = a.c.scales + (b * a.c.scale_sb) * 2;
+  const bool had = begin < lo && block_row[begin / block] >= 0;
+  const int64_t n0 = p0 - start;  // token of the tile's first position
+  const T* kb = (const T*)a.k + b * a.k_sb + 8 * lp;
+  const T* vb = (const T*)a.v + b * a.v_sb + 8 * lp;
+  Raw8<T> raw[STEPS];
+  auto fetch = [&](int u) {
+    const int h = h0 + (u >> 1);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const int x = first + i;
+      if (h < h1 && x >= lo && x < hi)
+        raw[i].load((u & 1) ? vb + (n0 + x) * a.v_st + h * a.v_sh : kb + (n0 + x) * a.k_st + h * a.k_sh);
+      else raw[i].zero();
+    }
+  };
+  fetch(0);
+  for (int u = 0; u < 2 * (h1 - h0); ++u) {
+    const int h = h0 + (u >> 1), kv = u & 1, turn_no = u % 3;
+    if (tid == 0)
+      before[turn_no] = had ? scales[((int64_t)(block_row[begin / block] / block) * a.Hkv + h) * 2 + kv] : 0.0f;
+    float y[STEPS][8];
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) raw[i].get(y[i]);
+    fetch(u + 1);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const int x = first + i;
+      if (x >= lo && x < hi) {  // uniform over the lanes of a row
+        if (kv == 0) {
+          if (a.turn.kw) norm8<D>(y[i], wk, a.turn.eps);
+          if (a.turn.pairs > 0) {
+            LaneTurn turn;
+            turn.load(a.turn, angles + x * (D / 2), lp);
+            turn8(a.turn, y[i], turn, stage + slot * D, lp);
+          }
+        }
+        float m = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float z = fabsf(y[i][e]);
+          m = z > m && z < INFINITY ? z : m;
+        }
+        m = group_max<L::LPT>(m);
+        if (lp == 0) atomicMax(&most[turn_no][x / block], __float_as_uint(m));
+      }
+    }
+    if (tid < kTile) most[(u + 1) % 3][tid] = 0u;  // unit u - 2's: every thread read it before the last barrier
+    __syncthreads();
+    const float held = before[turn_no];
+    uint8_t* cache = (kv ? a.c.v : a.c.k) + cb + h * a.c.sh + 8 * lp;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const int x = first + i, blk = x / block;
+      const int32_t row0 = block_row[blk];
+      if (x < begin || x >= hi || row0 < 0) continue;
+      const bool old_block = had && blk == begin / block;
+      float scale = fmaxf(__uint_as_float(most[turn_no][blk]) / C::kMost, kLeast);
+      if (old_block) scale = fmaxf(scale, held);
+      const int64_t row = (int64_t)row0 + (x - blk * block);
+      if (row >= a.c.tokens) continue;
+      uint2* at = (uint2*)(cache + row * a.c.st);
+      if (x >= lo) {
+        const float inv = 1.0f / scale;
+        float z[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e] = divided(y[i][e], scale, inv);
+        *at = codes8<C>(z);
+      } else if (scale != held) {  // the block's earlier tokens, where its scale grew
+        const float ratio = held / scale;
+        float z[8];
+        C::get8(*at, z);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e] *= ratio;
+        *at = codes8<C>(z);
+      }
+      if (lp == 0 && x == max(blk * block, lo))  // the block's first new token
+        scales[((int64_t)(row0 / block) * a.Hkv + h) * 2 + kv] = scale;
+    }
+  }
+}
+
+struct ValueArgs {
+  CacheArgs c;
+  const int32_t* rows;
+  int64_t row_stride;
+  const int32_t* lengths;
+  int64_t R, W;
+  int Hkv;
+  void* k_out;
+  void* v_out;
+};
+
+// A workgroup takes consecutive rows of the output, 8 codes of K and of V a lane.
+template <typename T, int D, typename C>
+__global__ __launch_bounds__(LSA_BLOCK) void byte_values_kernel(ValueArgs a) {
+  const int per = a.Hkv * (D / 8);  // lanes of a row
+  const int64_t total = a.R * a.W * per, step = (int64_t)gridDim.x * LSA_BLOCK;
+  for (int64_t i = (int64_t)blockIdx.x * LSA_BLOCK + threadIdx.x; i < total; i += step) {
+    const int64_t rw = i / per;
+    const int x = (int)(i - rw * per), h = x / (D / 8), lp = x % (D / 8);
+    const int64_t r = rw / a.W, w = rw - r * a.W;
+    const int64_t n = a.lengths ? (int64_t)a.lengths[r] : a.W;
+    const int64_t row = a.rows ? (int64_t)a.rows[r * a.row_stride + w] : w;
+    float k[8], v[8];
+    if (w < n && row >= 0 && row < a.c.tokens) {
+      const int64_t at = r * a.c.sb + row * a.c.st + h * a.c.sh + 8 * lp;
+      const float2 s = ((const float2*)a.c.scales)[r * a.c.scale_sb + row / a.c.block * a.Hkv + h];
+      C::get8(*(const uint2*)(a.c.k + at), k);
+      C::get8(*(const uint2*)(a.c.v + at), v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        k[e] *= s.x;
+        v[e] *= s.y;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) k[e] = v[e] = 0.0f;
+    }
+    store8((T*)a.k_out + 8 * i, k);
+    store8((T*)a.v_out + 8 * i, v);
+  }
+}
+
+template <typename T, int D, typename C>
+void launch_append(AppendArgs a, hipStream_t s) {
+  // kv-heads of a tile over several workgroups while those leave CUs idle; q's tokens likewise
+  const int64_t tiles = (int64_t)a.B * a.tiles;
+  a.parts = (int)std::max<int64_t>(1, std::min<int64_t>(a.Hkv, 1024 / std::max<int64_t>(tiles, 1)));
+  a.heads = (a.Hkv + a.parts - 1) / a.parts;
+  a.parts = (a.Hkv + a.heads - 1) / a.heads;
+  a.kv_groups = tiles * a.parts;
+  const int64_t tokens = a.q ? (int64_t)a.B * a.T : 0;
+  a.q_tokens = tokens >= 1024 ? 4 : 1;
+  byte_append_kernel<T, D, C><<<dim3((unsigned)(a.kv_groups + (tokens + a.q_tokens - 1) / a.q_tokens)), LSA_BLOCK, 0, s>>>(a);
+}
+
+template <typename T, int D, typename C>
+void launch_values(const ValueArgs& a, hipStream_t s) {
+  const int64_t total = a.R * a.W * a.Hkv * (D / 8);
+  const int64_t groups = std::min<int64_t>((total + LSA_BLOCK - 1) / LSA_BLOCK, 1 << 20);
+  byte_values_kernel<T, D, C><<<dim3((unsigned)groups), LSA_BLOCK, 0, s>>>(a);
+}
+
+CacheArgs cache_args(const lsa_byte_cache* c, int32_t Hkv) {
+  const int64_t pairs = (c->tokens + c->block - 1) / c->block * Hkv;
+  return CacheArgs{(uint8_t*)c->k, (uint8_t*)c->v, c->scales, c->block, c->tokens, c->caches == 1 ? 0 : c->batch_stride,
+                   c->token_stride, c->head_stride, c->caches == 1 ? 0 : pairs};
+}
+
+}  // namespace
+
+#define LSA_DISPATCH_CODES(D, code, LAUNCH, ...)                                   \
+  switch (D) {                                                                     \
+    case 32: code == LSA_INT8 ? LAUNCH<QT, 32, Int8Code>(__VA_ARGS__) : LAUNCH<QT, 32, E4m3Code>(__VA_ARGS__); break;    \
+    case 64: code == LSA_INT8 ? LAUNCH<QT, 64, Int8Code>(__VA_ARGS__) : LAUNCH<QT, 64, E4m3Code>(__VA_ARGS__); break;    \
+    case 128: code == LSA_INT8 ? LAUNCH<QT, 128, Int8Code>(__VA_ARGS__) : LAUNCH<QT, 128, E4m3Code>(__VA_ARGS__); break; \
+    default: code == LSA_INT8 ? LAUNCH<QT, 256, Int8Code>(__VA_ARGS__) : LAUNCH<QT, 256, E4m3Code>(__VA_ARGS__); break;  \
+  }
+
+extern "C" int lsa_byte_append(const lsa_byte_cache* cache, const void* k, const void* v, const void* q, int dtype,
+                               int64_t B, int64_t T, int32_t Hq, int32_t Hkv, int32_t D, int64_t k_batch_stride,
+                               int64_t k_token_stride, int64_t k_head_stride, int64_t v_batch_stride,
+                               int64_t v_token_stride, int64_t v_head_stride, int64_t q_batch_stride,
+                               int64_t q_token_stride, int64_t q_head_stride, const int32_t* starts,
+                               const int32_t* lengths, const lsa_slot_map* slots, const lsa_turn* turn, void* q_out,
+                               void* stream) {
+  LSA_REQUIRE(k && v && starts && turn && (!q || q_out), LSA_ERR_NULL, "lsa_byte_append: NULL pointer");
+  LSA_TRY(check_dtype(dtype));
+  LSA_REQUIRE(B >= 0 && T >= 0 && (!q || (Hq >= 1 && Hq <= 65536)) && (B == 0 || T <= 0x3FFFFFFF / B), LSA_ERR_SHAPE,
+              "lsa_byte_append: B %lld T %lld Hq %d (at most 2^30 tokens)", (long long)B, (long long)T, Hq);
+  LSA_TRY(check_byte_cache("lsa_byte_append", cache, B, Hkv, D));
+  TurnArgs t;
+  LSA_TRY(check_turn("lsa_byte_append", turn, D, &t));
+  AppendArgs a = {};
+  LSA_TRY(check_slots("lsa_byte_append", slots, &a.slots));
+  LSA_REQUIRE(slots || cache->caches == B, LSA_ERR_SHAPE, "lsa_byte_append: a pool for %lld rows needs a slot map", (long long)B);
+  const int64_t e = dtype == LSA_F32 ? 4 : 2;
+  LSA_REQUIRE((((uintptr_t)k | (uintptr_t)v | (q ? (uintptr_t)q | (uintptr_t)q_out : 0)) & 15) == 0 &&
+                  ((k_batch_stride | k_token_stride | k_head_stride | v_batch_stride | v_token_stride | v_head_stride |
+                    (q ? q_batch_stride | q_token_stride | q_head_stride : 0)) * e) % 16 == 0,
+              LSA_ERR_ALIGN, "lsa_byte_append: rows of q, k and v must be 16-byte aligned");
+  if (B * T == 0) return LSA_OK;
+  a.c = cache_args(cache, Hkv);
+  a.k = k; a.v = v; a.q = q; a.q_out = q_out;
+  a.k_sb = k_batch_stride; a.k_st = k_token_stride; a.k_sh = k_head_stride;
+  a.v_sb = v_batch_stride; a.v_st = v_token_stride; a.v_sh = v_head_stride;
+  a.q_sb = q_batch_stride; a.q_st = q_token_stride; a.q_sh = q_head_stride;
+  a.starts = starts; a.lengths = lengths; a.Hq = Hq; a.Hkv = Hkv; a.T = (int)T; a.B = (int)B;
+  a.tiles = (int)((T + kTile - 2) / kTile + 1);  // from any start
+  a.turn = t;
+  hipStream_t s = (hipStream_t)stream;
+  const int code = cache->code;
+  LSA_DISPATCH_QT(dtype, { LSA_DISPATCH_CODES(D, code, launch_append, a, s) });
+  LSA_LAUNCHED("lsa_byte_append");
+  return LSA_OK;
+}
+
+extern "C" int lsa_byte_values(const lsa_byte_cache* cache, const int32_t* rows, int64_t row_stride,
+                               const int32_t* lengths, int64_t R, int64_t W, int32_t Hkv, int32_t D, int dtype,
+                               void* k_out, void* v_out, void* stream) {
+  LSA_REQUIRE(k_out && v_out, LSA_ERR_NULL, "lsa_byte_values: NULL pointer");
+  LSA_TRY(check_dtype(dtype));
+  LSA_REQUIRE(R >= 0 && W >= 0 && R <= 0x7FFFFFFF && W <= 0x7FFFFFFF && (!rows || row_stride >= 0), LSA_ERR_SHAPE,
+              "lsa_byte_values: R %lld W %lld", (long long)R, (long long)W);
+  LSA_TRY(check_byte_cache("lsa_byte_values", cache, R, Hkv, D));
+  LSA_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, LSA_ERR_ALIGN, "lsa_byte_values: outputs must be 16-byte aligned");
+  if (R * W == 0) return LSA_OK;
+  ValueArgs a = {cache_args(cache, Hkv), rows, row_stride, lengths, R, W, Hkv, k_out, v_out};
+  hipStream_t s = (hipStream_t)stream;
+  const int code = cache->code;
+  LSA_DISPATCH_QT(dtype, { LSA_DISPATCH_CODES(D, code, launch_values, a, s) });
+  LSA_LAUNCHED("lsa_byte_values");
+  return LSA_OK;
+}

@@ -90,6 +90,38 @@ inline int check_slots(const char* who, const lsa_slot_map* m, SlotMapT* out) {
   return LSA_OK;
 }
 
+// Checks a rotation and copies it into the kernels' by-value form `out` (the device TurnArgs).
+template <typename TurnT>
+inline int check_turn(const char* who, const lsa_turn* m, int32_t D, TurnT* out) {
+  LSA_REQUIRE(D == 32 || D == 64 || D == 128 || D == 256, LSA_ERR_SHAPE, "%s: head dim %d not in {32,64,128,256}", who, D);
+  LSA_REQUIRE(m->pairs >= 0 && m->pairs <= D / 2, LSA_ERR_SHAPE, "%s: %d pairs in heads of %d", who, m->pairs, D);
+  LSA_REQUIRE(m->pairs == 0 || m->frequencies, LSA_ERR_NULL, "%s: NULL frequencies", who);
+  LSA_REQUIRE((((uintptr_t)m->q_weight | (uintptr_t)m->k_weight) & 15) == 0, LSA_ERR_ALIGN,
+              "%s: weights must be 16-byte aligned", who);
+  LSA_REQUIRE(m->eps >= 0.0f, LSA_ERR_SHAPE, "%s: eps %g", who, (double)m->eps);
+  *out = TurnT{m->frequencies, m->q_weight, m->k_weight, m->pairs, m->frequencies_f64 ? 1 : 0, m->interleaved ? 1 : 0,
+               m->weights_f32 ? 1 : 0, m->eps, m->magnitude};
+  return LSA_OK;
+}
+
+// Checks an 8-bit cache for rows of Hkv heads of D.
+inline int check_byte_cache(const char* who, const lsa_byte_cache* c, int64_t B, int32_t Hkv, int32_t D) {
+  LSA_REQUIRE(c && (c->tokens == 0 || (c->k && c->v && c->scales)), LSA_ERR_NULL, "%s: NULL cache", who);
+  LSA_REQUIRE(c->code == LSA_INT8 || c->code == LSA_E4M3, LSA_ERR_DTYPE, "%s: code %d", who, c->code);
+  LSA_REQUIRE(is_pow2(c->block) && c->block <= 64, LSA_ERR_POW2, "%s: blocks of %d tokens (1, 2, 4 .. 64)", who, c->block);
+  LSA_REQUIRE(D == 32 || D == 64 || D == 128 || D == 256, LSA_ERR_SHAPE, "%s: head dim %d not in {32,64,128,256}", who, D);
+  LSA_REQUIRE(Hkv >= 1 && Hkv <= 65535 && c->tokens >= 0 && c->tokens <= 0x7FFFFFFF && (c->caches == B || c->caches == 1),
+              LSA_ERR_SHAPE, "%s: %lld caches of %lld tokens, %d kv-heads, for %lld rows", who, (long long)c->caches,
+              (long long)c->tokens, Hkv, (long long)B);
+  LSA_REQUIRE(c->batch_stride >= 0 && c->token_stride >= D && c->head_stride >= D && c->token_stride <= 0x7FFFFFFF,
+              LSA_ERR_SHAPE, "%s: cache strides (%lld, %lld, %lld) must leave rows of %d codes apart", who,
+              (long long)c->batch_stride, (long long)c->token_stride, (long long)c->head_stride, D);
+  LSA_REQUIRE((((uintptr_t)c->k | (uintptr_t)c->v | (uint64_t)(c->batch_stride | c->token_stride | c->head_stride)) & 15) == 0 &&
+                  ((uintptr_t)c->scales & 7) == 0,
+              LSA_ERR_ALIGN, "%s: rows of codes must be 16-byte aligned, scales 8-byte", who);
+  return LSA_OK;
+}
+
 }  // namespace lsa
 
 #define LSA_LAUNCHED(what)                                                                    \

@@ -1,0 +1,223 @@
+// Norms and rotary positions of head rows, and 8-bit codes: what rotate.hip and byte_cache.hip share.
+//
+// A head row of D elements is held by D / 8 lanes, 8 elements a lane, as fp32:
+//   y = x / sqrt(mean(x^2) + eps) * w,
+//   (y_a, y_b) -> m (y_a cos t - y_b sin t, y_a sin t + y_b cos t),  t = position * frequency_j
+// for pair j = (2j, 2j + 1) or (j, j + pairs); dims past 2 * pairs stay. Written for one element i with
+// its pair's other one as y' = c y + s y_other, c and s hold the cosine and the signed sine.
+// The angle is taken in fp64 as turns (position * frequency / 2 pi less its nearest integer), so that far
+// positions lose nothing, and its sine and cosine in fp32.
+#pragma once
+
+#include "lsa_read_dev.h"
+
+namespace lsa {
+
+struct TurnArgs {
+  const void* freq;
+  const void* qw;
+  const void* kw;
+  int pairs;
+  int freq64, interleaved, w32;
+  float eps, magnitude;
+};
+
+template <int D>
+struct HeadLanes {
+  static constexpr int LPT = D / 8;             // lanes of a row
+  static constexpr int RPW = LSA_WAVE / LPT;    // rows of a wave
+  static constexpr int SLOTS = LSA_WAVES * RPW; // rows of a workgroup
+};
+
+// Maximum over each group of N consecutive lanes, in every lane of the group (as group_sum).
+template <int N>
+__device__ __forceinline__ float group_max(float x) {
+  if constexpr (N >= 2) x = fmaxf(x, dpp_mov<0xB1>(x));
+  if constexpr (N >= 4) x = fmaxf(x, dpp_mov<0x4E>(x));
+  if constexpr (N >= 8) x = fmaxf(x, dpp_mov<0x141>(x));
+  if constexpr (N >= 16) x = fmaxf(x, dpp_mov<0x140>(x));
+  if constexpr (N >= 32) x = fmaxf(x, lane_xor(x, 16));
+  return x;
+}
+
+// 8 elements, raw.
+template <typename T> struct Raw8 {
+  uint4 u;
+  __device__ __forceinline__ void load(const T* p) { u = *(const uint4*)p; }
+  __device__ __forceinline__ void zero() { u = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ __forceinline__ void get(float* f) const { Row16<T>::cvt(u, f); }
+};
+template <> struct Raw8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) { a = ((const float4*)p)[0]; b = ((const float4*)p)[1]; }
+  __device__ __forceinline__ void zero() { a = b = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
+  __device__ __forceinline__ void get(float* f) const {
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  }
+};
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {  // v_cvt_pk_bf16_f32 (RNE)
+  typedef __bf16 v2_t __attribute__((ext_vector_type(2)));
+  typedef float f2_t __attribute__((ext_vector_type(2)));
+  const f2_t f = {lo, hi};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, v2_t));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  typedef _Float16 v2_t __attribute__((ext_vector_type(2)));
+  const v2_t h = {(_Float16)lo, (_Float16)hi};
+  return __builtin_bit_cast(uint32_t, h);
+}
+__device__ __forceinline__ void store8(float* p, const float* f) {
+  ((float4*)p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+  ((float4*)p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+}
+__device__ __forceinline__ void store8(bf16_t* p, const float* f) {
+  *(uint4*)p = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+}
+__device__ __forceinline__ void store8(_Float16* p, const float* f) {
+  *(uint4*)p = make_uint4(pack_f16(f[0], f[1]), pack_f16(f[2], f[3]), pack_f16(f[4], f[5]), pack_f16(f[6], f[7]));
+}
+
+// (cos, sin) * magnitude of pair j at a position.
+__device__ __forceinline__ float2 turn_angle(const TurnArgs& a, int64_t pos, int j) {
+  const double f = a.freq64 ? ((const double*)a.freq)[j] : (double)((const float*)a.freq)[j];
+  const double turns = (double)pos * f * 0.15915494309189533577;  // 1 / (2 pi)
+  const float x = (float)(turns - rint(turns));
+  float s, c;
+  sincospif(2.0f * x, &s, &c);
+  return make_float2(c * a.magnitude, s * a.magnitude);
+}
+
+// This lane's dims 8 lp .. + 8 of the row's rotation.
+struct LaneTurn {
+  float c[8], s[8];
+  // angles: the token's (cos, sin) of every pair
+  __device__ __forceinline__ void load(const TurnArgs& a, const float2* angles, int lp) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int i = 8 * lp + e;
+      const bool in = i < 2 * a.pairs;
+      const bool low = a.interleaved ? (i & 1) == 0 : i < a.pairs;
+      const int j = a.interleaved ? i >> 1 : (low ? i : i - a.pairs);
+      const float2 cs = angles[in ? j : 0];
+      c[e] = cs.x;
+      s[e] = low ? -cs.y : cs.y;
+    }
+  }
+};
+
+// The norm's factors of this lane's dims (ones without weights).
+template <typename T>
+__device__ __forceinline__ void load_weights(const void* w, int w32, int lp, float* f) {
+  if (w == nullptr) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = 1.0f;
+  } else if (w32) {
+    Raw8<float> r;
+    r.load((const float*)w + 8 * lp);
+    r.get(f);
+  } else {
+    Raw8<T> r;
+    r.load((const T*)w + 8 * lp);
+    r.get(f);
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void norm8(float* y, const float* w, float eps) {
+  float ss = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
+  ss = group_sum<HeadLanes<D>::LPT>(ss);
+  const float r = 1.0f / sqrtf(ss * (1.0f / D) + eps);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = y[e] * r * w[e];
+}
+
+// Rotates the row whose dims 8 lp .. + 8 this lane holds. stage: LDS of the row's D floats, where the lanes
+// of a row (of one wave) show each other their elements.
+__device__ __forceinline__ void turn8(const TurnArgs& a, float* y, const LaneTurn& t, float* stage, int lp) {
+  if (a.interleaved) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (e & 1) continue;
+      const float y0 = y[e], y1 = y[e + 1];
+      if (8 * lp + e < 2 * a.pairs) {
+        y[e] = t.c[e] * y0 + t.s[e] * y1;
+        y[e + 1] = t.c[e + 1] * y1 + t.s[e + 1] * y0;
+      }
+    }
+    return;
+  }
+  ((float4*)(stage + 8 * lp))[0] = make_float4(y[0], y[1], y[2], y[3]);
+  ((float4*)(stage + 8 * lp))[1] = make_float4(y[4], y[5], y[6], y[7]);
+  __builtin_amdgcn_wave_barrier();
+  float other[8];
+  if ((a.pairs & 7) == 0) {  // the lane's other elements are eight in a row
+    const int at = 8 * lp < a.pairs ? 8 * lp + a.pairs : (8 * lp < 2 * a.pairs ? 8 * lp - a.pairs : 8 * lp);
+    const float4 u = ((const float4*)(stage + at))[0], v = ((const float4*)(stage + at))[1];
+    other[0] = u.x; other[1] = u.y; other[2] = u.z; other[3] = u.w;
+    other[4] = v.x; other[5] = v.y; other[6] = v.z; other[7] = v.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int i = 8 * lp + e;
+      other[e] = stage[i < a.pairs ? i + a.pairs : (i < 2 * a.pairs ? i - a.pairs : i)];
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (8 * lp + e < 2 * a.pairs) y[e] = t.c[e] * y[e] + t.s[e] * other[e];
+  }
+}
+
+// ---------------------------------------------------------------- 8-bit codes
+
+struct Int8Code {
+  static constexpr float kMost = 127.0f;
+  static __device__ __forceinline__ void get8(const uint2& u, float* f) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[e] = (float)(int8_t)(u.x >> (8 * e));
+      f[4 + e] = (float)(int8_t)(u.y >> (8 * e));
+    }
+  }
+  static __device__ __forceinline__ uint32_t put4(const float* f) {
+    uint32_t r = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r |= ((uint32_t)(int)rintf(f[e]) & 0xFFu) << (8 * e);  // NaN is 0
+    return r;
+  }
+};
+struct E4m3Code {
+  static constexpr float kMost = 448.0f;
+  static __device__ __forceinline__ void get8(const uint2& u, float* f) {
+    typedef float f2_t __attribute__((ext_vector_type(2)));
+    const f2_t a = __builtin_amdgcn_cvt_pk_f32_fp8(u.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(u.x, true);
+    const f2_t c = __builtin_amdgcn_cvt_pk_f32_fp8(u.y, false), d = __builtin_amdgcn_cvt_pk_f32_fp8(u.y, true);
+    f[0] = a[0]; f[1] = a[1]; f[2] = b[0]; f[3] = b[1]; f[4] = c[0]; f[5] = c[1]; f[6] = d[0]; f[7] = d[1];
+  }
+  static __device__ __forceinline__ uint32_t put4(const float* f) {
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], r, true);
+  }
+};
+
+// x / scale (inv = 1 / scale), rounded as a division rounds it: one residual step behind the product.
+__device__ __forceinline__ float divided(float x, float scale, float inv) {
+  const float y = x * inv;
+  const float z = fmaf(fmaf(-y, scale, x), inv, y);
+  return fabsf(y) < 3.0e38f ? z : y;  // an infinity has no residual
+}
+
+// The codes of 8 numbers already divided by their scale; past the range: its ends; NaN: e4m3's own, int8's 0.
+template <typename C>
+__device__ __forceinline__ uint2 codes8(const float* y) {
+  float f[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = y[e] != y[e] ? y[e] : fminf(fmaxf(y[e], -C::kMost), C::kMost);
+  return make_uint2(C::put4(f), C::put4(f + 4));
+}
+
+}  // namespace lsa

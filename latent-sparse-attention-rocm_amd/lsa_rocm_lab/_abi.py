@@ -117,6 +117,14 @@ SIGNATURES = {
                               _p, _p, _i64, _p]),
     "lsa_evict_rows": (_int, [_p, _p, _p, _int, _i64, _i64, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _p, _int, _i32,
                               _p, _p, _i64, _i64, _i64, _p, _i64, _i64, _int, _p]),
+    "lsa_rotate": (_int, [_p, _p, _int, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _p, _int, _i64,
+                          _p, _p, _p, _p]),
+    "lsa_byte_append": (_int, [_p, _p, _p, _p, _int, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                               _i64, _i64, _p, _p, _p, _p, _p, _p]),
+    "lsa_byte_values": (_int, [_p, _p, _i64, _p, _i64, _i64, _i32, _i32, _int, _p, _p, _p]),
+    "lsa_byte_read_scratch_bytes": (_sz, [_i64, _i32, _i32, _i32, _i32]),
+    "lsa_byte_read": (_int, [_p, _p, _int, _i64, _i64, _i32, _i32, _i32, _p, _p, _i32, _int, _f32, _i32, _p, _p, _sz, _p,
+                             _p]),
 }
 
 

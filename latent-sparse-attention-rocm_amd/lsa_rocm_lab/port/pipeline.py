@@ -55,6 +55,8 @@ import torch.nn.functional as F
 from lsa_rocm_lab import _abi
 from lsa_rocm_lab.port import keys as keys_mod
 from lsa_rocm_lab.port.eviction import evict, evict_slots, key_mass  # noqa: F401
+from lsa_rocm_lab.port.byte_cache import ByteCache, byte_append, byte_cache, byte_read, byte_values  # noqa: F401
+from lsa_rocm_lab.port.rotary import rotary_frequencies, rotate  # noqa: F401
 from lsa_rocm_lab.port.shared_prefix import prefix_read  # noqa: F401
 
 
