@@ -532,7 +532,7 @@ typedef struct lsa_turn {
 
 /* q [B, T, Hq, D] and k [B, T, Hkv, D] (element strides, rows of D contiguous elements, 16-byte aligned;
  * Hkv 0: q alone) to q_out and k_out, dense, of the same dtype, normed and rotated. positions: int32 (or int64)
- * at b * position_stride + t. D in {32, 64, 128, 256}; at most 2^30 tokens. No counterpart in the reference. */
+ * at b * position_stride + t. D in {32, 64, 128, 256}; under 2^26 tokens. No counterpart in the reference. */
 int lsa_rotate(const void* q, const void* k, int dtype, int64_t B, int64_t T, int32_t Hq, int32_t Hkv, int32_t D,
                int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride, int64_t k_batch_stride,
                int64_t k_token_stride, int64_t k_head_stride, const void* positions, int positions_i64,
@@ -562,7 +562,7 @@ typedef struct lsa_byte_cache {
  * new tokens' largest magnitude / M, 2^-100), M = 127 or 448; a new token's code is value / scale, rounded to
  * nearest even, and where the scale grew the block's earlier codes are rescaled and rounded again. What it held
  * from starts[b] on counts for nothing. A NaN has no part in the scale and is held as e4m3's NaN or int8's 0, an
- * infinity as the largest code, neither in the scale. No two rows may write to one block. No counterpart in the
+ * infinity as the largest code, neither in the scale. No two rows may write to one block. Under 2^24 tokens. No counterpart in the
  * reference. */
 int lsa_byte_append(const lsa_byte_cache* cache, const void* k, const void* v, const void* q, int dtype, int64_t B,
                     int64_t T, int32_t Hq, int32_t Hkv, int32_t D, int64_t k_batch_stride, int64_t k_token_stride,
@@ -579,14 +579,16 @@ int lsa_byte_values(const lsa_byte_cache* cache, const int32_t* rows, int64_t ro
 /* lsa_read over an 8-bit cache: q [B, Tq, Hq, D] dense, lists as lsa_read's (shared by the heads, or one a
  * kv-head), out like q; a row with no keys gives zeros. Any Hq that Hkv divides; D in {32, 64, 128, 256}; under
  * 2^24 rows times kv-heads times blocks of 16 of their query heads (the units). Keys enter exactly, q exactly, a
- * weight times V's scale with 16 bits of mantissa (fp32 rows: 24). splits 1..64: spans of a list.
+ * weight times V's scale with 16 bits of mantissa (fp32 rows: 24). splits 1..64: spans of a list (splits times units
+ * under 2^24).
  * counters (or NULL): a unit's int32 that reads zero at launch and is left zero; with them a split read is one
  * launch instead of two. scratch: lsa_byte_read_scratch_bytes(), 16-byte aligned, no initialisation (0 bytes with
  * one span). No counterpart in the reference. */
 size_t lsa_byte_read_scratch_bytes(int64_t rows, int32_t Hq, int32_t Hkv, int32_t D, int32_t splits);
 int lsa_byte_read(const void* q, const lsa_byte_cache* cache, int dtype, int64_t B, int64_t Tq, int32_t Hq, int32_t Hkv,
                   int32_t D, const int32_t* ids, const int32_t* lengths, int32_t W, int ids_per_head, float scale,
-                  int32_t splits, int32_t* counters, void* scratch, size_t scratch_bytes, void* out, void* stream);
+                  int32_t splits, int32_t* counters, void* scratch, size_t scratch_bytes, void* out,
+                  void* stream);
 
 #ifdef __cplusplus
 }

@@ -20,6 +20,8 @@ using namespace lsa;
 namespace {
 
 constexpr int kTile = 64;
+constexpr int kValueLanes = 512;  // 8-element lanes of a workgroup that reads back, about
+constexpr int kPartHeads = 64;  // kv-heads of a workgroup at most
 constexpr float kLeast = 7.888609052210118e-31f;  // 2^-100, the smallest scale: its reciprocal is finite
 
 struct CacheArgs {
@@ -35,18 +37,17 @@ struct AppendArgs {
   CacheArgs c;
   const void* k;
   const void* v;
-  const void* q;
-  void* q_out;
-  int64_t k_sb, k_st, k_sh, v_sb, v_st, v_sh, q_sb, q_st, q_sh;
+  int64_t k_sb, k_st, k_sh, v_sb, v_st, v_sh;
   const int32_t* starts;
   const int32_t* lengths;
   SlotMap slots;
-  int Hq, Hkv, T;
+  int Hkv, T;
   int B, tiles;      // tiles of a row
   int parts, heads;  // workgroups of a tile, kv-heads of one
-  int q_tokens;      // tokens of a q workgroup
   int64_t kv_groups; // workgroups before the first of q's
   TurnArgs turn;
+  RotateArgs q;      // few tokens' rows of q, in workgroups behind the others:
+  uint32_t q_parts;  // so many a token
 };
 
 __device__ __forceinline__ int new_tokens(const AppendArgs& a, int b) {
@@ -54,68 +55,38 @@ __device__ __forceinline__ int new_tokens(const AppendArgs& a, int b) {
   return n < 0 ? 0 : (n > a.T ? a.T : n);
 }
 
-// Rows of q: `q_tokens` tokens from t0 on, flat over the batch; a lane walks the heads of one token.
-template <typename T, int D>
-__device__ __forceinline__ void append_queries(const AppendArgs& a, int64_t group, float* stage, float2* angles) {
-  using L = HeadLanes<D>;
-  const int tid = threadIdx.x, lp = tid % L::LPT, slot = tid / L::LPT;
-  const int nt = a.q_tokens, rows = L::SLOTS / nt;
-  const int64_t t0 = group * nt, all = (int64_t)a.B * a.T;
-  for (int i = tid; i < nt * a.turn.pairs; i += LSA_BLOCK) {
-    const int n = i / a.turn.pairs, j = i - n * a.turn.pairs;
-    const int64_t at = min(t0 + n, all - 1);
-    angles[n * (D / 2) + j] = turn_angle(a.turn, (int64_t)a.starts[at / a.T] + at % a.T, j);
-  }
-  float w[8];
-  load_weights<T>(a.turn.qw, a.turn.w32, lp, w);
-  __syncthreads();
-  const int64_t mine = t0 + slot / rows;
-  if (mine >= all) return;
-  const int b = (int)(mine / a.T), t = (int)(mine % a.T);
-  LaneTurn turn;
-  if (a.turn.pairs > 0) turn.load(a.turn, angles + slot / rows * (D / 2), lp);
-  const bool live = t < new_tokens(a, b);
-  const T* q = (const T*)a.q + b * a.q_sb + t * a.q_st + 8 * lp;
-  T* out = (T*)a.q_out + mine * a.Hq * D + 8 * lp;
-  constexpr int AHEAD = 4;
-  for (int h0 = slot % rows; h0 < a.Hq; h0 += AHEAD * rows) {
-    Raw8<T> raw[AHEAD];
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      if (h0 + i * rows < a.Hq && live) raw[i].load(q + (h0 + i * rows) * a.q_sh);
-      else raw[i].zero();
-    }
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      const int h = h0 + i * rows;
-      if (h >= a.Hq) break;
-      float y[8];
-      raw[i].get(y);
-      if (live) {
-        if (a.turn.qw) norm8<D>(y, w, a.turn.eps);
-        if (a.turn.pairs > 0) turn8(a.turn, y, turn, stage + slot * D, lp);
-      }
-      store8(out + (int64_t)h * D, y);
-    }
-  }
-}
+template <int D>
+struct alignas(16) AppendLds {
+  float stage[LSA_BLOCK * 8 + 8];
+  float2 angles[kTile * (D / 2)];
+  uint32_t most[3][kTile];       // of a unit's blocks, as integers; three units take turns
+  float before[2 * kPartHeads];  // the first block's scales, where it holds earlier tokens
+  int32_t block_row[kTile];
+};
 
 template <typename T, int D, typename C>
 __global__ __launch_bounds__(LSA_BLOCK) void byte_append_kernel(AppendArgs a) {
   using L = HeadLanes<D>;
   constexpr int STEPS = kTile / L::SLOTS;  // tokens of a lane
-  __shared__ __attribute__((aligned(16))) float stage[LSA_BLOCK * 8];
-  __shared__ __attribute__((aligned(16))) float2 angles[kTile * (D / 2)];
-  __shared__ uint32_t most[3][kTile];  // of a unit's blocks, as integers; three units take turns
-  __shared__ float before[3];          // the first block's scale, where it holds earlier tokens
-  __shared__ int32_t block_row[kTile];
-  const int tid = threadIdx.x;
+  __shared__ union {
+    AppendLds<D> kv;
+    RotateLds<D, 1> q;
+  } sh;
   if ((int64_t)blockIdx.x >= a.kv_groups) {
-    append_queries<T, D>(a, (int64_t)blockIdx.x - a.kv_groups, stage, angles);
+    const uint32_t g = (uint32_t)(blockIdx.x - a.kv_groups), token = g / a.q_parts;
+    rotate_rows<T, D, 1, false>(a.q, token, g - token * a.q_parts, sh.q);
     return;
   }
+  const int tid = threadIdx.x;
+  auto& most = sh.kv.most;
+  auto& block_row = sh.kv.block_row;
+  float* before = sh.kv.before;
+  float* stage = sh.kv.stage;
+  float2* angles = sh.kv.angles;
+  if (tid < 8) stage[LSA_BLOCK * 8 + tid] = 0.0f;
   const int part = blockIdx.x % a.parts, tile = blockIdx.x / a.parts % a.tiles;
   const int b = blockIdx.x / a.parts / a.tiles;
+  const SlotRow map = slot_row_of(a.slots, b);  // beside the start's load
   const int64_t start = a.starts[b];
   const int64_t end = start + new_tokens(a, b);
   const int64_t p0 = (start >= 0 ? start / kTile : 0) * kTile + (int64_t)tile * kTile;
@@ -125,50 +96,50 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_append_kernel(AppendArgs a) {
   const int block = a.c.block, blocks = kTile / block;
   const int lo = (int)(from - p0), hi = (int)(to - p0);
   const int begin = lo / block * block;  // the first written block's first token
-  if (tid < blocks) {
-    const int64_t p = p0 + (int64_t)tid * block;
-    int64_t row = p;
-    if (a.slots.table) {
-      const SlotRow map = slot_row_of(a.slots, b);
-      row = p < map.width ? map.row[p] : -1;
+  const int h0 = part * a.heads, h1 = min(h0 + a.heads, a.Hkv), units = 2 * (h1 - h0);
+  const int lp = tid % L::LPT, slot = tid / L::LPT;
+  const int first = slot * STEPS;  // a lane's tokens are consecutive
+  const int64_t n0 = p0 - start;   // token of the tile's first position
+  const T* kb = (const T*)a.k + b * a.k_sb + 8 * lp;
+  const T* vb = (const T*)a.v + b * a.v_sb + 8 * lp;
+  Raw8<T> raw[STEPS];
+  auto fetch = [&](int u) {  // unit u: K (even) or V of a head
+    const int h = h0 + (u >> 1);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const int x = first + i;
+      if (u < units && x >= lo && x < hi)
+        raw[i].load((u & 1) ? vb + (n0 + x) * a.v_st + h * a.v_sh : kb + (n0 + x) * a.k_st + h * a.k_sh);
+      else raw[i].zero();
     }
-    if (row < 0 || row >= a.c.tokens || row % block) row = -1;
-    block_row[tid] = (int32_t)row;
+  };
+  fetch(0);
+  float* scales = a.c.scales + (b * a.c.scale_sb) * 2;
+  auto row_of = [&](int blk) {  // the cache row of the tile's block blk, or -1
+    const int64_t p = p0 + (int64_t)blk * block;
+    int64_t row = p;
+    if (map.row) row = p < map.width ? map.row[p] : -1;
+    return row < 0 || row >= a.c.tokens || (row & (block - 1)) ? -1 : (int32_t)row;
+  };
+  if (tid < blocks) block_row[tid] = row_of(tid);
+  if (tid >= kTile && tid < kTile + units) {
+    const int u = tid - kTile;
+    const int32_t row = begin < lo ? row_of(begin / block) : -1;
+    before[u] = row < 0 ? 0.0f : scales[((int64_t)(row / block) * a.Hkv + h0 + (u >> 1)) * 2 + (u & 1)];
   }
   for (int i = tid; i < 3 * kTile; i += LSA_BLOCK) (&most[0][0])[i] = 0u;
   for (int i = tid; i < (hi - lo) * a.turn.pairs; i += LSA_BLOCK) {
     const int n = i / a.turn.pairs, j = i - n * a.turn.pairs;
     angles[(lo + n) * (D / 2) + j] = turn_angle(a.turn, from + n, j);
   }
-  const int lp = tid % L::LPT, slot = tid / L::LPT;
-  const int first = slot * STEPS;  // a lane's tokens are consecutive
   float wk[8];
   load_weights<T>(a.turn.kw, a.turn.w32, lp, wk);
   __syncthreads();
 
-  const int h0 = part * a.heads, h1 = min(h0 + a.heads, a.Hkv);
   const int64_t cb = b * a.c.sb;
-  float* scales = a.c.scales + (b * a.c.scale_sb) * 2;
-  const bool had = begin < lo && block_row[begin / block] >= 0;
-  const int64_t n0 = p0 - start;  // token of the tile's first position
-  const T* kb = (const T*)a.k + b * a.k_sb + 8 * lp;
-  const T* vb = (const T*)a.v + b * a.v_sb + 8 * lp;
-  Raw8<T> raw[STEPS];
-  auto fetch = [&](int u) {
-    const int h = h0 + (u >> 1);
-#pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-      const int x = first + i;
-      if (h < h1 && x >= lo && x < hi)
-        raw[i].load((u & 1) ? vb + (n0 + x) * a.v_st + h * a.v_sh : kb + (n0 + x) * a.k_st + h * a.k_sh);
-      else raw[i].zero();
-    }
-  };
-  fetch(0);
-  for (int u = 0; u < 2 * (h1 - h0); ++u) {
+  const bool had = begin < lo;  // the first block holds earlier tokens
+  for (int u = 0; u < units; ++u) {
     const int h = h0 + (u >> 1), kv = u & 1, turn_no = u % 3;
-    if (tid == 0)
-      before[turn_no] = had ? scales[((int64_t)(block_row[begin / block] / block) * a.Hkv + h) * 2 + kv] : 0.0f;
     float y[STEPS][8];
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) raw[i].get(y[i]);
@@ -182,7 +153,7 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_append_kernel(AppendArgs a) {
           if (a.turn.pairs > 0) {
             LaneTurn turn;
             turn.load(a.turn, angles + x * (D / 2), lp);
-            turn8(a.turn, y[i], turn, stage + slot * D, lp);
+            turn8(a.turn, y[i], turn, stage + slot * D, stage + LSA_BLOCK * 8, lp);
           }
         }
         float m = 0.0f;
@@ -197,7 +168,7 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_append_kernel(AppendArgs a) {
     }
     if (tid < kTile) most[(u + 1) % 3][tid] = 0u;  // unit u - 2's: every thread read it before the last barrier
     __syncthreads();
-    const float held = before[turn_no];
+    const float held = before[u];
     uint8_t* cache = (kv ? a.c.v : a.c.k) + cb + h * a.c.sh + 8 * lp;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
@@ -239,23 +210,27 @@ struct ValueArgs {
   int Hkv;
   void* k_out;
   void* v_out;
+  int block_shift;
+  uint32_t many, chunks;  // rows of a workgroup, workgroups of a list
 };
 
-// A workgroup takes consecutive rows of the output, 8 codes of K and of V a lane.
+// A workgroup takes `many` consecutive rows of a list, 8 codes of K and of V a lane.
 template <typename T, int D, typename C>
 __global__ __launch_bounds__(LSA_BLOCK) void byte_values_kernel(ValueArgs a) {
-  const int per = a.Hkv * (D / 8);  // lanes of a row
-  const int64_t total = a.R * a.W * per, step = (int64_t)gridDim.x * LSA_BLOCK;
-  for (int64_t i = (int64_t)blockIdx.x * LSA_BLOCK + threadIdx.x; i < total; i += step) {
-    const int64_t rw = i / per;
-    const int x = (int)(i - rw * per), h = x / (D / 8), lp = x % (D / 8);
-    const int64_t r = rw / a.W, w = rw - r * a.W;
-    const int64_t n = a.lengths ? (int64_t)a.lengths[r] : a.W;
+  const uint32_t per = (uint32_t)a.Hkv * (D / 8);  // lanes of a row
+  const uint32_t r = blockIdx.x / a.chunks;
+  const int64_t w0 = (int64_t)(blockIdx.x - r * a.chunks) * a.many;
+  const int64_t n = a.lengths ? (int64_t)a.lengths[r] : a.W;
+  const uint32_t lanes = (uint32_t)min((int64_t)a.many, a.W - w0) * per;
+  const int64_t out = ((int64_t)r * a.W + w0) * per;
+  for (uint32_t i = threadIdx.x; i < lanes; i += LSA_BLOCK) {
+    const uint32_t dw = i / per, x = i - dw * per, h = x / (D / 8), lp = x % (D / 8);
+    const int64_t w = w0 + dw;
     const int64_t row = a.rows ? (int64_t)a.rows[r * a.row_stride + w] : w;
     float k[8], v[8];
     if (w < n && row >= 0 && row < a.c.tokens) {
       const int64_t at = r * a.c.sb + row * a.c.st + h * a.c.sh + 8 * lp;
-      const float2 s = ((const float2*)a.c.scales)[r * a.c.scale_sb + row / a.c.block * a.Hkv + h];
+      const float2 s = ((const float2*)a.c.scales)[r * a.c.scale_sb + (row >> a.block_shift) * a.Hkv + h];
       C::get8(*(const uint2*)(a.c.k + at), k);
       C::get8(*(const uint2*)(a.c.v + at), v);
 #pragma unroll
@@ -267,29 +242,19 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_values_kernel(ValueArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) k[e] = v[e] = 0.0f;
     }
-    store8((T*)a.k_out + 8 * i, k);
-    store8((T*)a.v_out + 8 * i, v);
+    store8((T*)a.k_out + 8 * (out + i), k);
+    store8((T*)a.v_out + 8 * (out + i), v);
   }
 }
 
 template <typename T, int D, typename C>
-void launch_append(AppendArgs a, hipStream_t s) {
-  // kv-heads of a tile over several workgroups while those leave CUs idle; q's tokens likewise
-  const int64_t tiles = (int64_t)a.B * a.tiles;
-  a.parts = (int)std::max<int64_t>(1, std::min<int64_t>(a.Hkv, 1024 / std::max<int64_t>(tiles, 1)));
-  a.heads = (a.Hkv + a.parts - 1) / a.parts;
-  a.parts = (a.Hkv + a.heads - 1) / a.heads;
-  a.kv_groups = tiles * a.parts;
-  const int64_t tokens = a.q ? (int64_t)a.B * a.T : 0;
-  a.q_tokens = tokens >= 1024 ? 4 : 1;
-  byte_append_kernel<T, D, C><<<dim3((unsigned)(a.kv_groups + (tokens + a.q_tokens - 1) / a.q_tokens)), LSA_BLOCK, 0, s>>>(a);
+void launch_append(const AppendArgs& a, int64_t groups, hipStream_t s) {
+  byte_append_kernel<T, D, C><<<dim3((unsigned)groups), LSA_BLOCK, 0, s>>>(a);
 }
 
 template <typename T, int D, typename C>
 void launch_values(const ValueArgs& a, hipStream_t s) {
-  const int64_t total = a.R * a.W * a.Hkv * (D / 8);
-  const int64_t groups = std::min<int64_t>((total + LSA_BLOCK - 1) / LSA_BLOCK, 1 << 20);
-  byte_values_kernel<T, D, C><<<dim3((unsigned)groups), LSA_BLOCK, 0, s>>>(a);
+  byte_values_kernel<T, D, C><<<dim3((unsigned)(a.R * a.chunks)), LSA_BLOCK, 0, s>>>(a);
 }
 
 CacheArgs cache_args(const lsa_byte_cache* c, int32_t Hkv) {
@@ -317,8 +282,8 @@ extern "C" int lsa_byte_append(const lsa_byte_cache* cache, const void* k, const
                                void* stream) {
   LSA_REQUIRE(k && v && starts && turn && (!q || q_out), LSA_ERR_NULL, "lsa_byte_append: NULL pointer");
   LSA_TRY(check_dtype(dtype));
-  LSA_REQUIRE(B >= 0 && T >= 0 && (!q || (Hq >= 1 && Hq <= 65536)) && (B == 0 || T <= 0x3FFFFFFF / B), LSA_ERR_SHAPE,
-              "lsa_byte_append: B %lld T %lld Hq %d (at most 2^30 tokens)", (long long)B, (long long)T, Hq);
+  LSA_REQUIRE(B >= 0 && T >= 0 && (!q || (Hq >= 1 && Hq <= 65536)) && (B == 0 || T <= kMaxGroups / B), LSA_ERR_SHAPE,
+              "lsa_byte_append: B %lld T %lld Hq %d (under 2^24 tokens)", (long long)B, (long long)T, Hq);
   LSA_TRY(check_byte_cache("lsa_byte_append", cache, B, Hkv, D));
   TurnArgs t;
   LSA_TRY(check_turn("lsa_byte_append", turn, D, &t));
@@ -332,16 +297,35 @@ extern "C" int lsa_byte_append(const lsa_byte_cache* cache, const void* k, const
               LSA_ERR_ALIGN, "lsa_byte_append: rows of q, k and v must be 16-byte aligned");
   if (B * T == 0) return LSA_OK;
   a.c = cache_args(cache, Hkv);
-  a.k = k; a.v = v; a.q = q; a.q_out = q_out;
+  a.k = k; a.v = v;
   a.k_sb = k_batch_stride; a.k_st = k_token_stride; a.k_sh = k_head_stride;
   a.v_sb = v_batch_stride; a.v_st = v_token_stride; a.v_sh = v_head_stride;
-  a.q_sb = q_batch_stride; a.q_st = q_token_stride; a.q_sh = q_head_stride;
-  a.starts = starts; a.lengths = lengths; a.Hq = Hq; a.Hkv = Hkv; a.T = (int)T; a.B = (int)B;
+  a.starts = starts; a.lengths = lengths; a.Hkv = Hkv; a.T = (int)T; a.B = (int)B;
   a.tiles = (int)((T + kTile - 2) / kTile + 1);  // from any start
   a.turn = t;
+  // kv-heads of a tile over several workgroups while those leave CUs idle; q's tokens likewise
+  const int64_t tiles = B * a.tiles;
+  a.parts = (int)std::max<int64_t>((Hkv + kPartHeads - 1) / kPartHeads, std::min<int64_t>(Hkv, 1024 / tiles));
+  a.heads = (Hkv + a.parts - 1) / a.parts;
+  a.parts = (Hkv + a.heads - 1) / a.heads;
+  a.kv_groups = tiles * a.parts;
+  RotateArgs& r = a.q;
+  r.q = r.k = q; r.q_out = r.k_out = q_out; r.starts = starts; r.lengths = lengths;
+  r.q_sb = q_batch_stride; r.q_st = q_token_stride; r.q_sh = q_head_stride;
+  r.Hq = Hq; r.T = (int)T; r.tokens = (int)(B * T); r.turn = t;
+  // q of few tokens in the same launch (a part of its heads a workgroup while there are fewer than 512), of more in
+  // one of its own, whose workgroups need a quarter of the LDS and fewer registers (32768 tokens: 198 us together)
+  const bool same = q && B * T < 1024;
+  const int rows = 256 / (D / 8);
+  r.heads = B * T * ((Hq + rows - 1) / rows) <= 512 ? rows : Hq;
+  a.q_parts = (uint32_t)((Hq + r.heads - 1) / std::max(r.heads, 1));
+  const int64_t groups = a.kv_groups + (same ? B * T * a.q_parts : 0);
+  LSA_REQUIRE(groups <= kMaxGroups, LSA_ERR_SHAPE, "lsa_byte_append: %lld tokens of %d kv-heads (2^24 workgroups)",
+              (long long)(B * T), Hkv);
   hipStream_t s = (hipStream_t)stream;
   const int code = cache->code;
-  LSA_DISPATCH_QT(dtype, { LSA_DISPATCH_CODES(D, code, launch_append, a, s) });
+  LSA_DISPATCH_QT(dtype, { LSA_DISPATCH_CODES(D, code, launch_append, a, groups, s) });
+  if (q && !same) launch_rotate(r, dtype, D, s);
   LSA_LAUNCHED("lsa_byte_append");
   return LSA_OK;
 }
@@ -357,6 +341,11 @@ extern "C" int lsa_byte_values(const lsa_byte_cache* cache, const int32_t* rows,
   LSA_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, LSA_ERR_ALIGN, "lsa_byte_values: outputs must be 16-byte aligned");
   if (R * W == 0) return LSA_OK;
   ValueArgs a = {cache_args(cache, Hkv), rows, row_stride, lengths, R, W, Hkv, k_out, v_out};
+  a.block_shift = __builtin_ctz((unsigned)cache->block);
+  a.many = (uint32_t)std::max(1, kValueLanes / (Hkv * (D / 8)));
+  const int64_t chunks = (W + a.many - 1) / a.many;
+  LSA_REQUIRE(chunks <= kMaxGroups / R, LSA_ERR_SHAPE, "lsa_byte_values: %lld rows", (long long)(R * W));
+  a.chunks = (uint32_t)chunks;
   hipStream_t s = (hipStream_t)stream;
   const int code = cache->code;
   LSA_DISPATCH_QT(dtype, { LSA_DISPATCH_CODES(D, code, launch_values, a, s) });

@@ -27,9 +27,10 @@ using namespace lsa;
 
 namespace {
 
-constexpr int kKeys = 32;                   // of a wave's tile
-constexpr int kStep = kKeys * LSA_WAVES;    // of a workgroup's
+constexpr int kKeys = 32;                 // of a wave's tile
+constexpr int kStep = kKeys * LSA_WAVES;  // of a workgroup's
 constexpr int kByteSplits = 64;
+constexpr int kXcds = 8;
 constexpr int kHeads = 16;                  // query heads of a workgroup
 
 __device__ const uint4 g_zeros[16] = {};  // a row of codes, or a pair of scales, of nothing
@@ -45,7 +46,7 @@ struct ByteReadArgs {
   const int32_t* ids;
   const int32_t* lengths;
   int W, per_head;
-  int64_t Tq;
+  uint32_t Tq, rows;
   int Hq, Hkv, group, blocks;  // query heads a kv-head, in blocks of 16
   float scale_log2;
   int span, splits;
@@ -59,17 +60,19 @@ __host__ __device__ constexpr int part_floats(int heads, int D) { return heads *
 // A workgroup's unit: query row, kv-head, its query heads, and its list.
 struct Unit {
   int64_t row, list;
-  int g, h0, heads, n;
-  __device__ __forceinline__ Unit(const ByteReadArgs& a, int64_t i) {
-    const int cb = (int)(i % a.blocks);
-    const int64_t rg = i / a.blocks;
-    row = rg / a.Hkv;
-    g = (int)(rg % a.Hkv);
+  int g, h0, heads;
+  __device__ __forceinline__ Unit(const ByteReadArgs& a, uint32_t i) {  // units are fewer than 2^24
+    const uint32_t rg = i / (uint32_t)a.blocks, r = rg / (uint32_t)a.Hkv;
+    const int cb = (int)(i - rg * (uint32_t)a.blocks);
+    row = r;
+    g = (int)(rg - r * (uint32_t)a.Hkv);
     h0 = g * a.group + cb * kHeads;
     heads = min(kHeads, a.group - cb * kHeads);
     list = a.per_head ? rg : row;
-    const int len = a.lengths[list];
-    n = len < 0 ? 0 : (len > a.W ? a.W : len);
+  }
+  __device__ __forceinline__ int keys(const ByteReadArgs& a) const {
+    const int n = a.lengths[list];
+    return n < 0 ? 0 : (n > a.W ? a.W : n);
   }
 };
 
@@ -103,10 +106,11 @@ template <int D> __device__ __forceinline__ int swizzle(int r) {
 
 template <int D>
 struct WaveLds {
-  uint8_t k[2][kKeys * D];
-  uint8_t v[2][kKeys * D];
+  uint8_t k[kKeys * D];
+  uint8_t v[kKeys * D];
   float scales[2][64];  // K's 32, V's 32
   int32_t ids[2][64];   // 32 and their copies
+  uint64_t rows[kKeys][2];  // where the codes of the tile that is being fetched lie, K's and V's
 };
 template <int D>
 struct ByteLds {
@@ -118,6 +122,10 @@ struct ByteLds {
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x2_t __attribute__((ext_vector_type(2)));
+typedef uint64_t u64x2_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) u64x2_t lds_u64x2;
+typedef __attribute__((address_space(3))) uint64_t lds_u64;
+typedef __attribute__((address_space(3))) f32x4_t lds_f4;
 typedef __attribute__((address_space(3))) u32x2_t lds_u2;
 typedef __attribute__((address_space(3))) u32x4_t lds_u4;
 typedef __attribute__((address_space(3))) i32x2_t lds_i2;
@@ -129,6 +137,22 @@ __device__ __forceinline__ void dma16_far(uint32_t lds, const void* p) {  // a l
 }
 __device__ __forceinline__ void dma4_far(uint32_t lds, const void* p) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
+}
+
+// What the weighted sum is divided by: no keys give zeros.
+__device__ __forceinline__ float inverse(float l) { return l > 0.0f || l != l ? 1.0f / l : 0.0f; }
+template <typename T> __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d);
+template <> __device__ __forceinline__ void store4<float>(float* p, float a, float b, float c, float d) { *(float4*)p = make_float4(a, b, c, d); }
+template <> __device__ __forceinline__ void store4<bf16_t>(bf16_t* p, float a, float b, float c, float d) { *(uint2*)p = make_uint2(pack_bf16(a, b), pack_bf16(c, d)); }
+template <> __device__ __forceinline__ void store4<_Float16>(_Float16* p, float a, float b, float c, float d) { *(uint2*)p = make_uint2(pack_f16(a, b), pack_f16(c, d)); }
+
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// v_max3_f32 as it is: fmaxf quiets its operands first.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
 }
 
 // x and y as N bf16 parts each that add up to them (to 8 N bits).
@@ -157,129 +181,134 @@ __device__ __forceinline__ void split_any(float x, float y, uint32_t* out) {
   }
 }
 
+// Waves a SIMD holds: as many as LDS does (a wave takes 1.5 KB and 64 D bytes of a CU's 160 KB), or fewer for the registers of
+// fp32 rows' parts.
+template <typename T, int D> constexpr int waves_per_simd() { return D == 256 ? (sizeof(T) == 4 ? 1 : 2) : (sizeof(T) == 4 && D == 128 ? 2 : 4); }
+
 template <typename T> struct Parts;
 template <> struct Parts<bf16_t> { static constexpr int Q = 1, P = 2; };
 template <> struct Parts<_Float16> { static constexpr int Q = 2, P = 2; };
 template <> struct Parts<float> { static constexpr int Q = 3, P = 3; };
 
-// The partials of a unit's n_act spans into its output rows. Every thread calls it.
+// The partials of n_act spans into `heads` output rows that follow each other. Every thread calls it. w: [64][16]
+// floats, ltot: [16].
 template <typename T, int D>
-__device__ __forceinline__ void join(const ByteReadArgs& a, const Unit& u, const float* parts, int n_act, float* w, float* ltot) {
-  const int tid = threadIdx.x, heads = u.heads, stride = part_floats(heads, D);
+__device__ __forceinline__ void join(T* out, int heads, const float* parts, int n_act, float* w, float* ltot) {
+  constexpr int BATCH = 8;
+  const int tid = threadIdx.x, lane = tid & 63, stride = part_floats(heads, D), columns = heads * D / 4;
   const CoherentRows rows(parts);  // under 2 GiB
+  float4 x[BATCH];
+  auto fetch = [&](int c, int s0) {
+#pragma unroll
+    for (int s = 0; s < BATCH; ++s) x[s] = rows.load4(4 * (min(s0 + s, n_act - 1) * stride + 4 * c));
+  };
+  if (tid < columns) fetch(tid, 0);  // beside the weights' loads
   __syncthreads();
-  for (int t = tid; t < n_act * heads; t += LSA_BLOCK) {
-    const int s = t / heads, h = t % heads;
-    w[t] = coherent_load(parts + (int64_t)s * stride + heads * D + h);
-    w[kByteSplits * kHeads + t] = coherent_load(parts + (int64_t)s * stride + heads * D + heads + h);
+  for (int h = tid / 64; h < heads; h += LSA_WAVES) {  // a head a wave, a span a lane
+    const float* p = parts + (int64_t)min(lane, n_act - 1) * stride + heads * D + h;
+    const float m = coherent_load(p), l = coherent_load(p + heads);
+    const float f = lane < n_act ? fast_exp2(m - wave_max(m)) : 0.0f;
+    const float ll = wave_sum(f * l);
+    if (lane < n_act) w[lane * kHeads + h] = f;
+    if (lane == 0) ltot[h] = ll;
   }
   __syncthreads();
-  if (tid < heads) {
-    float m = kNegBig, l = 0.0f;
-    for (int s = 0; s < n_act; ++s) m = fmaxf(m, w[s * heads + tid]);
-    for (int s = 0; s < n_act; ++s) {
-      const float f = fast_exp2(w[s * heads + tid] - m);
-      l += f * w[kByteSplits * kHeads + s * heads + tid];
-      w[s * heads + tid] = f;
-    }
-    ltot[tid] = l;
-  }
-  __syncthreads();
-  T* out = (T*)a.out + (u.row * a.Hq + u.h0) * D;
-  for (int c = tid; c < heads * D / 4; c += LSA_BLOCK) {
+  for (int c = tid; c < columns; c += LSA_BLOCK) {
     const int h = 4 * c / D;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int s0 = 0; s0 < n_act; s0 += 8) {
-      float4 x[8];
+    for (int s0 = 0; s0 < n_act; s0 += BATCH) {
+      if (c != tid || s0 > 0) fetch(c, s0);
 #pragma unroll
-      for (int s = 0; s < 8; ++s) x[s] = rows.load4(4 * (min(s0 + s, n_act - 1) * stride + 4 * c));
-#pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        const float f = s0 + s < n_act ? w[(s0 + s) * heads + h] : 0.0f;
+      for (int s = 0; s < BATCH; ++s) {
+        const float f = s0 + s < n_act ? w[(s0 + s) * kHeads + h] : 0.0f;
         acc.x += f * x[s].x; acc.y += f * x[s].y; acc.z += f * x[s].z; acc.w += f * x[s].w;
       }
     }
-    const float l = ltot[h], inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    const float r[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) store_out<T>(out + 4 * c + e, r[e]);
+    const float inv = inverse(ltot[h]);
+    store4<T>(out + 4 * c, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
   }
 }
 
 template <typename T, int D, typename C>
-__global__ __launch_bounds__(LSA_BLOCK) void byte_read_kernel(ByteReadArgs a) {
+__global__ __launch_bounds__(LSA_BLOCK) __attribute__((amdgpu_waves_per_eu(waves_per_simd<T, D>(), waves_per_simd<T, D>())))
+void byte_read_kernel(ByteReadArgs a) {
   constexpr int SEGS = D / 16, NI = D / 32;     // 16-byte segments of a row; DMAs of a tile, K and V each
   constexpr int KS = D / 32, DB = D / 16;       // matrix steps over the dims; 16-dim blocks of the output
   constexpr int RPI = 64 / SEGS;                // rows of a DMA
-  constexpr int NV = 2 * NI + 1;                // memory operations of a tile
   constexpr int QP = Parts<T>::Q, PP = Parts<T>::P;
   __shared__ __attribute__((aligned(1024))) ByteLds<D> sh;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid / 64);
   const int row = lane >> 4, col = lane & 15;
-  const Unit u(a, blockIdx.x);
-  const int s = blockIdx.y, n_act = (u.n + a.span - 1) / a.span;
-  if (s >= max(n_act, 1)) return;
-  T* out = (T*)a.out + (u.row * a.Hq + u.h0) * D;
-  if (u.n == 0) {
-    for (int j = tid; j < u.heads * D; j += LSA_BLOCK) store_out<T>(out + j, 0.0f);
-    return;
-  }
-  const int lo = s * a.span + kKeys * w, hi = min((s + 1) * a.span, u.n);
-  const int n_tiles = hi > lo ? (hi - lo + kStep - 1) / kStep : 0;
+  // Workgroup x is on XCD x % 8. The heads of a span follow each other on one XCD: their rows are neighbours in
+  // memory, so that the lines of a page are asked for together. The spans of a row are dealt over the XCDs (its
+  // place moves by one from span to span), so that rows of many lengths keep all of them busy.
+  const uint32_t units = (uint32_t)(a.Hkv * a.blocks), x8 = blockIdx.x / kXcds;  // workgroups of a query row's span
+  const uint32_t pair = x8 / units * kXcds + blockIdx.x % kXcds;  // of a span and a query row, span by span
+  const uint32_t s0 = pair / a.rows, at = pair - s0 * a.rows + s0 % a.rows;
+  const int s = (int)s0;
+  if (s >= a.splits) return;
+  const uint32_t unit = (at < a.rows ? at : at - a.rows) * units + x8 % units;
+  const Unit u(a, unit);
   const int32_t* ids = a.ids + u.list * a.W;
-  const int64_t b = u.row / a.Tq;
+  const int lo = s * a.span + kKeys * w, end = min((s + 1) * a.span, a.W);  // of the list's slots
+  const int64_t b = (uint32_t)u.row / a.Tq;
   const uint8_t* kb = a.k + b * a.sb + u.g * a.sh;
   const uint8_t* vb = a.v + b * a.sb + u.g * a.sh;
   const float* scales = a.scales + (b * a.scale_sb + u.g) * 2;
   WaveLds<D>& mem = sh.wave[w];
-  const lds_char* base = (const lds_char*)&mem;
+  lds_char* base = (lds_char*)&mem;
   const uint32_t lds = (uint32_t)(uintptr_t)base;
-  constexpr uint32_t V_AT = 2 * kKeys * D, S_AT = 4 * kKeys * D, I_AT = S_AT + 512;
+  constexpr uint32_t V_AT = kKeys * D, S_AT = 2 * kKeys * D, I_AT = S_AT + 512, R_AT = I_AT + 512;
 
   auto load_ids = [&](int i) {
     const int j = lo + kStep * i + (lane & 31);
-    dma4_far(lds + I_AT + (uint32_t)(i & 1) * 256u, ids + min(j, hi - 1));
+    dma4_far(lds + I_AT + (uint32_t)(i & 1) * 256u, ids + min(j, end - 1));
   };
-  uint32_t live[2] = {0u, 0u};  // which keys of the two buffers' tiles count
-  auto load = [&](int i) {
-    const uint32_t buf = (uint32_t)(i & 1);
-    const lds_int* at = (const lds_int*)(base + I_AT + buf * 256u);
-    const int left = hi - (lo + kStep * i);  // keys from the tile's first on
-    auto good = [&](int id, int x) { return x < left && id >= 0 && id < a.tokens; };
-    {
-      const int x = lane & 31, id = at[x];
-      const bool ok = good(id, x);
-      live[i & 1] = (uint32_t)__ballot(ok);
-      const float* p = scales + ((int64_t)((uint32_t)id >> a.block_shift) * a.Hkv) * 2 + (lane >> 5);
-      dma4_far(lds + S_AT + buf * 256u, ok ? (const void*)p : (const void*)g_zeros);
-    }
+  int hi = 0;                   // past the list's last key here
+  uint32_t live[2] = {0u, 0u};  // which keys of tiles of even and odd number count
+  uint64_t seg[NI];  // the lane's 16 bytes of a row, by DMA
 #pragma unroll
-    for (int y = 0; y < NI; ++y) {
-      const int r = y * RPI + lane / SEGS, id = at[r];
-      const int sg = (lane % SEGS) ^ swizzle<D>(r);
-      const bool ok = good(id, r);
-      const uint64_t off = (uint64_t)(uint32_t)id * (uint32_t)a.st + 16 * sg;
-      dma16_far(lds + buf * (kKeys * D) + 1024u * y, ok ? (const void*)(kb + off) : (const void*)g_zeros);
-      dma16_far(lds + V_AT + buf * (kKeys * D) + 1024u * y, ok ? (const void*)(vb + off) : (const void*)g_zeros);
-    }
+  for (int y = 0; y < NI; ++y) seg[y] = 16u * (uint32_t)((lane % SEGS) ^ swizzle<D>(y * RPI + lane / SEGS));
+  auto load_k = [&](int i) {  // and the tile's scales
+    const uint32_t buf = (uint32_t)(i & 1);
+    const int x = lane & 31, id = ((const lds_int*)(base + I_AT + buf * 256u))[x];
+    const bool ok = x < hi - (lo + kStep * i) && id >= 0 && id < a.tokens;
+    live[i & 1] = (uint32_t)__ballot(ok);
+    const float* p = scales + ((int64_t)((uint32_t)id >> a.block_shift) * a.Hkv) * 2 + (lane >> 5);
+    const uint64_t zeros = (uint64_t)(uintptr_t)g_zeros;
+    const uint64_t off = (uint64_t)(uint32_t)id * (uint32_t)a.st;
+    const uint64_t kr = ok ? (uint64_t)(uintptr_t)kb + off : zeros, vr = ok ? (uint64_t)(uintptr_t)vb + off : zeros;
+    *(lds_u64x2*)(base + R_AT + 16 * x) = u64x2_t{kr, vr};
+    wait_lds();  // the reads of K's buffer, too
+    dma4_far(lds + S_AT + buf * 256u, ok ? (const void*)p : (const void*)g_zeros);
+#pragma unroll
+    for (int y = 0; y < NI; ++y)
+      dma16_far(lds + 1024u * y, (const void*)(uintptr_t)(*(const lds_u64*)(base + R_AT + 16 * (y * RPI + lane / SEGS)) + seg[y]));
+  };
+  auto load_v = [&]() {  // of the tile whose K was loaded last
+    wait_lds();  // the reads of V's buffer
+#pragma unroll
+    for (int y = 0; y < NI; ++y)
+      dma16_far(lds + V_AT + 1024u * y,
+                (const void*)(uintptr_t)(*(const lds_u64*)(base + R_AT + 8 + 16 * (y * RPI + lane / SEGS)) + seg[y]));
   };
 
+  // The list's first entries and q come in beside its length.
+  if (lo < end) {  // wave-uniform
+    load_ids(0);
+    load_ids(1);
+  }
   // this lane's part of Q^T: head col, dims 16 (row + 4 j) .. + 16 for steps 2 j, 2 j + 1 (D = 32: 8 row .. + 8)
   uint4 q[KS][QP];
-  float m = kNegBig, l = 0.0f;
-  f32x4_t o[DB];
-#pragma unroll
-  for (int d = 0; d < DB; ++d) o[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  if (n_tiles > 0) {  // wave-uniform
-    load_ids(0);
-    if (n_tiles > 1) load_ids(1);
+  {
     const T* qr = (const T*)a.q + (u.row * a.Hq + u.h0 + (col < u.heads ? col : 0)) * D;
+    Raw8<T> raw[KS];
+#pragma unroll
+    for (int j = 0; j < KS; ++j) raw[j].load(qr + (D == 32 ? 8 * row : 16 * (row + 4 * (j >> 1)) + 8 * (j & 1)));
 #pragma unroll
     for (int j = 0; j < KS; ++j) {
-      Raw8<T> raw;
-      raw.load(qr + (D == 32 ? 8 * row : 16 * (row + 4 * (j >> 1)) + 8 * (j & 1)));
       float f[8];
-      raw.get(f);
+      raw[j].get(f);
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[e] = col < u.heads ? f[e] : 0.0f;
       uint32_t p[4][QP];
@@ -291,28 +320,33 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_read_kernel(ByteReadArgs a) {
         asm volatile("" : "+v"(q[j][x].x), "+v"(q[j][x].y), "+v"(q[j][x].z), "+v"(q[j][x].w));  // here, before the DMAs
       }
     }
-    wait_vm<0>();
-    load(0);
   }
+  wait_vm<0>();  // also where there is nothing to do: no DMA outlives its workgroup
+  const int n = u.keys(a), n_act = (n + a.span - 1) / a.span;
+  if (s >= max(n_act, 1)) return;
+  T* out = (T*)a.out + (u.row * a.Hq + u.h0) * D;
+  if (n == 0) {
+    for (int j = tid; j < u.heads * D; j += LSA_BLOCK) store_out<T>(out + j, 0.0f);
+    return;
+  }
+  hi = min(end, n);
+  const int n_tiles = hi > lo ? (hi - lo + kStep - 1) / kStep : 0;
+  float m = kNegBig, l = 0.0f;
+  f32x4_t o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) o[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  if (n_tiles > 0) {  // wave-uniform
+    load_k(0);
+    load_v();
+  }
+  // Memory operations retire in order. V of tile i is the newest at the loop's head; the list of tile i + 1 came before it.
   for (int i = 0; i < n_tiles; ++i) {
-    if (i + 1 < n_tiles) {
-      wait_vm<NV>();  // the list of tile i + 1
-      if (i + 2 < n_tiles) {
-        load_ids(i + 2);
-        load(i + 1);
-        wait_vm<NV + 1>();  // tile i
-      } else {
-        load(i + 1);
-        wait_vm<NV>();
-      }
-    } else {
-      wait_vm<0>();
-    }
     const uint32_t buf = (uint32_t)(i & 1);
-    const uint32_t mine = (i & 1 ? live[1] : live[0]) >> (8 * row);
+    const uint32_t mine = i & 1 ? live[1] : live[0];
+    wait_vm<NI>();  // K and scales of tile i, the list of tile i + 1
     // S^T: rows 4 a + u of the first product are keys 8 a + u, of the second 8 a + 4 + u
     f32x4_t c[2];
-    const lds_char* kt = base + buf * (kKeys * D);
+    const lds_char* kt = base;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       c[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
@@ -335,13 +369,28 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_read_kernel(ByteReadArgs a) {
         }
       }
     }
-    const lds_float* sc = (const lds_float*)(base + S_AT + buf * 256u) + 8 * row;
-    float x[8], top = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = (mine >> e & 1u) ? c[e >> 2][e & 3] * (sc[e] * a.scale_log2) : -INFINITY;
-      top = fmaxf(top, x[e]);
+    const bool more = i + 1 < n_tiles;
+    if (more) {
+      load_k(i + 1);
+      load_ids(i + 2);
+      wait_vm<NI + 2>();  // V of tile i
+    } else {
+      wait_vm<0>();
     }
+    f32x4_t ks[2], vs[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      ks[h] = ((const lds_f4*)(base + S_AT + buf * 256u + 32 * row))[h];
+      vs[h] = ((const lds_f4*)(base + S_AT + buf * 256u + 128 + 32 * row))[h];
+    }
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = c[e >> 2][e & 3] * (ks[e >> 2][e & 3] * a.scale_log2);
+    if (mine != ~0u) {  // wave-uniform
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = mine >> (8 * row + e) & 1u ? x[e] : -INFINITY;
+    }
+    float top = max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), fmaxf(x[6], x[7]));
     top = fmaxf(top, lane_xor(top, 16));
     top = fmaxf(top, lane_xor(top, 32));
     if (__ballot(top > m + 8.0f) != 0) {  // the reference moves where a head's maximum passes it by 2^8
@@ -356,9 +405,9 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_read_kernel(ByteReadArgs a) {
     for (int e = 0; e < 4; ++e) {
       const float p0 = fast_exp2(x[2 * e] - m), p1 = fast_exp2(x[2 * e + 1] - m);
       l += p0 + p1;
-      split_pair<PP>(p0 * sc[32 + 2 * e], p1 * sc[32 + 2 * e + 1], pr[e]);
+      split_pair<PP>(p0 * vs[e >> 1][2 * (e & 1)], p1 * vs[e >> 1][2 * (e & 1) + 1], pr[e]);
     }
-    const lds_char* vt = base + V_AT + buf * (kKeys * D);
+    const lds_char* vt = base + V_AT;
     const int vr = 8 * row + (col >> 1);
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
@@ -368,11 +417,16 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_read_kernel(ByteReadArgs a) {
       for (int p = 0; p < PP; ++p)
         o[d] = Mfma16<bf16_t>::run(vc, make_uint4(pr[0][p], pr[1][p], pr[2][p], pr[3][p]), o[d]);
     }
+    if (more) load_v();
   }
 
-  // the waves' states meet in LDS, each in its wave's own buffers: [16][D]
   l += lane_xor(l, 16);
   l += lane_xor(l, 32);
+  const int stride = part_floats(u.heads, D);
+  float* parts = a.parts + (int64_t)unit * a.splits * (int64_t)part_floats(min(kHeads, a.group), D);
+  float* part = parts + (int64_t)s * stride;
+  const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(part, 0, 4 * stride, 0x00020000);
+  // the waves' states meet in LDS, each in its wave's own buffers: [16][D]
   float* mo = (float*)&mem;
   if (lane < kHeads) {
     sh.m[w][lane] = m;
@@ -381,10 +435,6 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_read_kernel(ByteReadArgs a) {
 #pragma unroll
   for (int d = 0; d < DB; ++d) *(float4*)(mo + col * D + 16 * d + 4 * row) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
   __syncthreads();
-  const int64_t unit = blockIdx.x;
-  const int stride = part_floats(u.heads, D);
-  float* parts = a.parts + unit * a.splits * (int64_t)part_floats(min(kHeads, a.group), D);
-  float* part = parts + (int64_t)s * stride;
   for (int t = tid; t < u.heads * D / 4; t += LSA_BLOCK) {
     const int h = 4 * t / D, d = 4 * t % D;
     float top = kNegBig;
@@ -399,12 +449,11 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_read_kernel(ByteReadArgs a) {
       r[0] += f * z.x; r[1] += f * z.y; r[2] += f * z.z; r[3] += f * z.w;
     }
     if (n_act == 1) {
-      const float inv = ll > 0.0f || ll != ll ? 1.0f / ll : 0.0f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) store_out<T>(out + 4 * t + e, r[e] * inv);
+      const float inv = inverse(ll);
+      store4<T>(out + 4 * t, r[0] * inv, r[1] * inv, r[2] * inv, r[3] * inv);
     } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) coherent_store(part + 4 * t + e, r[e]);
+      const f32x4_t z = {r[0], r[1], r[2], r[3]};  // past the XCD's cache (sc1), as CoherentRows reads it
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, z), rsrc, 16 * t, 0, 16);
       if (d == 0) {
         coherent_store(part + u.heads * D + h, top);
         coherent_store(part + u.heads * D + u.heads + h, ll);
@@ -413,23 +462,25 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_read_kernel(ByteReadArgs a) {
   }
   if (n_act == 1 || a.counters == nullptr) return;
   if (!arrive_last(&a.counters[unit], n_act, &sh.flag)) return;
-  join<T, D>(a, u, parts, n_act, (float*)&sh.wave[0], &sh.m[0][0]);
+  join<T, D>(out, u.heads, parts, n_act, (float*)&sh.wave[0], &sh.m[0][0]);
 }
 
 // The join as a launch of its own, where there are no counters.
 template <typename T, int D>
 __global__ __launch_bounds__(LSA_BLOCK) void byte_join_kernel(ByteReadArgs a) {
-  __shared__ float w[2 * kByteSplits * kHeads];
+  __shared__ float w[kByteSplits * kHeads];
   __shared__ float ltot[kHeads];
   const Unit u(a, blockIdx.x);
-  const int n_act = (u.n + a.span - 1) / a.span;
+  const int n_act = (u.keys(a) + a.span - 1) / a.span;
   if (n_act <= 1) return;
-  join<T, D>(a, u, a.parts + (int64_t)blockIdx.x * a.splits * part_floats(min(kHeads, a.group), D), n_act, w, ltot);
+  join<T, D>((T*)a.out + (u.row * a.Hq + u.h0) * D, u.heads,
+             a.parts + (int64_t)blockIdx.x * a.splits * part_floats(min(kHeads, a.group), D), n_act, w, ltot);
 }
 
 template <typename T, int D>
 void launch_byte_read(const ByteReadArgs& a, int code, int64_t units, hipStream_t s) {
-  const dim3 grid((unsigned)units, (unsigned)a.splits);
+  const int64_t pairs = ((int64_t)a.rows * a.splits + kXcds - 1) / kXcds * kXcds;
+  const dim3 grid((unsigned)(pairs * a.Hkv * a.blocks));
   if (code == LSA_INT8) byte_read_kernel<T, D, Int8Code><<<grid, LSA_BLOCK, 0, s>>>(a);
   else byte_read_kernel<T, D, E4m3Code><<<grid, LSA_BLOCK, 0, s>>>(a);
   if (a.splits > 1 && a.counters == nullptr) byte_join_kernel<T, D><<<dim3((unsigned)units), LSA_BLOCK, 0, s>>>(a);
@@ -446,8 +497,8 @@ extern "C" size_t lsa_byte_read_scratch_bytes(int64_t rows, int32_t Hq, int32_t 
 
 extern "C" int lsa_byte_read(const void* q, const lsa_byte_cache* cache, int dtype, int64_t B, int64_t Tq, int32_t Hq,
                              int32_t Hkv, int32_t D, const int32_t* ids, const int32_t* lengths, int32_t W,
-                             int ids_per_head, float scale, int32_t splits, int32_t* counters, void* scratch,
-                             size_t scratch_bytes, void* out, void* stream) {
+                             int ids_per_head, float scale, int32_t splits, int32_t* counters,
+                             void* scratch, size_t scratch_bytes, void* out, void* stream) {
   LSA_REQUIRE(q && out && (ids || W == 0) && lengths, LSA_ERR_NULL, "lsa_byte_read: NULL pointer");
   LSA_TRY(check_dtype(dtype));
   LSA_REQUIRE(B >= 0 && Tq >= 0 && W >= 0, LSA_ERR_SHAPE, "lsa_byte_read: negative size");
@@ -462,16 +513,17 @@ extern "C" int lsa_byte_read(const void* q, const lsa_byte_cache* cache, int dty
   const size_t need = lsa_byte_read_scratch_bytes(B * Tq, Hq, Hkv, D, splits);
   LSA_REQUIRE(need == 0 || (scratch && scratch_bytes >= need && ((uintptr_t)scratch & 15) == 0), LSA_ERR_WORKSPACE,
               "lsa_byte_read: scratch missing, not 16-byte aligned or %zu < %zu bytes", scratch_bytes, need);
+  LSA_REQUIRE((B * Tq * splits + kXcds) * Hkv * blocks <= kMaxGroups, LSA_ERR_SHAPE,
+              "lsa_byte_read: %d spans of %lld rows x kv-heads (2^24 workgroups)", splits, (long long)units);
   if (units == 0) return LSA_OK;
   ByteReadArgs a = {};
   a.q = q; a.k = (const uint8_t*)cache->k; a.v = (const uint8_t*)cache->v; a.scales = cache->scales;
   a.sb = cache->caches == 1 ? 0 : cache->batch_stride; a.st = cache->token_stride; a.sh = cache->head_stride;
   a.scale_sb = cache->caches == 1 ? 0 : (cache->tokens + cache->block - 1) / cache->block * Hkv;
   a.tokens = cache->tokens; a.block_shift = __builtin_ctz((unsigned)cache->block);
-  a.ids = ids; a.lengths = lengths; a.W = W; a.per_head = ids_per_head ? 1 : 0; a.Tq = Tq;
+  a.ids = ids; a.lengths = lengths; a.W = W; a.per_head = ids_per_head ? 1 : 0; a.Tq = (uint32_t)Tq; a.rows = (uint32_t)(B * Tq);
   a.Hq = Hq; a.Hkv = Hkv; a.group = Hq / Hkv; a.blocks = (int)blocks; a.scale_log2 = scale * kLog2e;
-  a.span = (int)(((int64_t)(W + splits - 1) / splits + kStep - 1) / kStep * kStep);
-  a.span = std::max(a.span, kStep);
+  a.span = std::max((int)(((int64_t)W + splits - 1) / splits + kStep - 1) / kStep * kStep, kStep);
   a.splits = splits; a.counters = counters; a.parts = (float*)scratch; a.out = out;
   hipStream_t s = (hipStream_t)stream;
   const int code = cache->code;

@@ -23,6 +23,8 @@ struct DecodeDebug {
 };
 const DecodeDebug& decode_debug();
 
+constexpr int64_t kMaxGroups = (1 << 24) - 1;  // of 256 threads in a launch: HIP counts threads in 32 bits
+
 inline bool is_pow2(int64_t x) { return x > 0 && (x & (x - 1)) == 0; }
 inline int next_pow2(int x) {
   int p = 1;

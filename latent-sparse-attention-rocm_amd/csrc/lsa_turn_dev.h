@@ -67,15 +67,23 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const v2_t h = {(_Float16)lo, (_Float16)hi};
   return __builtin_bit_cast(uint32_t, h);
 }
-__device__ __forceinline__ void store8(float* p, const float* f) {
-  ((float4*)p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-  ((float4*)p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+// 8 numbers to memory. STREAM: past the caches, for outputs that they could not hold.
+typedef uint32_t words4_t __attribute__((ext_vector_type(4)));
+template <bool STREAM> __device__ __forceinline__ void store_words(void* p, words4_t x) {
+  if constexpr (STREAM) __builtin_nontemporal_store(x, (words4_t*)p);
+  else *(words4_t*)p = x;
 }
-__device__ __forceinline__ void store8(bf16_t* p, const float* f) {
-  *(uint4*)p = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+template <bool STREAM = false> __device__ __forceinline__ void store8(float* p, const float* f) {
+  const words4_t lo = {__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+  const words4_t hi = {__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7])};
+  store_words<STREAM>(p, lo);
+  store_words<STREAM>(p + 4, hi);
 }
-__device__ __forceinline__ void store8(_Float16* p, const float* f) {
-  *(uint4*)p = make_uint4(pack_f16(f[0], f[1]), pack_f16(f[2], f[3]), pack_f16(f[4], f[5]), pack_f16(f[6], f[7]));
+template <bool STREAM = false> __device__ __forceinline__ void store8(bf16_t* p, const float* f) {
+  store_words<STREAM>(p, words4_t{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])});
+}
+template <bool STREAM = false> __device__ __forceinline__ void store8(_Float16* p, const float* f) {
+  store_words<STREAM>(p, words4_t{pack_f16(f[0], f[1]), pack_f16(f[2], f[3]), pack_f16(f[4], f[5]), pack_f16(f[6], f[7])});
 }
 
 // (cos, sin) * magnitude of pair j at a position.
@@ -100,8 +108,8 @@ struct LaneTurn {
       const bool low = a.interleaved ? (i & 1) == 0 : i < a.pairs;
       const int j = a.interleaved ? i >> 1 : (low ? i : i - a.pairs);
       const float2 cs = angles[in ? j : 0];
-      c[e] = cs.x;
-      s[e] = low ? -cs.y : cs.y;
+      c[e] = in ? cs.x : 1.0f;
+      s[e] = in ? (low ? -cs.y : cs.y) : 0.0f;
     }
   }
 };
@@ -129,18 +137,17 @@ __device__ __forceinline__ void norm8(float* y, const float* w, float eps) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
   ss = group_sum<HeadLanes<D>::LPT>(ss);
-  const float r = 1.0f / sqrtf(ss * (1.0f / D) + eps);
+  const float r = rsqrtf(ss * (1.0f / D) + eps);
 #pragma unroll
   for (int e = 0; e < 8; ++e) y[e] = y[e] * r * w[e];
 }
 
 // Rotates the row whose dims 8 lp .. + 8 this lane holds. stage: LDS of the row's D floats, where the lanes
-// of a row (of one wave) show each other their elements.
-__device__ __forceinline__ void turn8(const TurnArgs& a, float* y, const LaneTurn& t, float* stage, int lp) {
+// of a row (of one wave) show each other their elements; none: eight zeros, the others of a dim that stays.
+__device__ __forceinline__ void turn8(const TurnArgs& a, float* y, const LaneTurn& t, float* stage, const float* none, int lp) {
   if (a.interleaved) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (e & 1) continue;
+    for (int e = 0; e < 8; e += 2) {
       const float y0 = y[e], y1 = y[e + 1];
       if (8 * lp + e < 2 * a.pairs) {
         y[e] = t.c[e] * y0 + t.s[e] * y1;
@@ -154,23 +161,119 @@ __device__ __forceinline__ void turn8(const TurnArgs& a, float* y, const LaneTur
   __builtin_amdgcn_wave_barrier();
   float other[8];
   if ((a.pairs & 7) == 0) {  // the lane's other elements are eight in a row
-    const int at = 8 * lp < a.pairs ? 8 * lp + a.pairs : (8 * lp < 2 * a.pairs ? 8 * lp - a.pairs : 8 * lp);
-    const float4 u = ((const float4*)(stage + at))[0], v = ((const float4*)(stage + at))[1];
+    const float* at = 8 * lp < a.pairs ? stage + 8 * lp + a.pairs : (8 * lp < 2 * a.pairs ? stage + 8 * lp - a.pairs : none);
+    const float4 u = ((const float4*)at)[0], v = ((const float4*)at)[1];
     other[0] = u.x; other[1] = u.y; other[2] = u.z; other[3] = u.w;
     other[4] = v.x; other[5] = v.y; other[6] = v.z; other[7] = v.w;
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int i = 8 * lp + e;
-      other[e] = stage[i < a.pairs ? i + a.pairs : (i < 2 * a.pairs ? i - a.pairs : i)];
+      other[e] = *(i < a.pairs ? stage + i + a.pairs : (i < 2 * a.pairs ? stage + i - a.pairs : none));
     }
   }
   __builtin_amdgcn_wave_barrier();
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    if (8 * lp + e < 2 * a.pairs) y[e] = t.c[e] * y[e] + t.s[e] * other[e];
+  for (int e = 0; e < 8; ++e) y[e] = t.c[e] * y[e] + t.s[e] * other[e];
+}
+
+// ---------------------------------------------------------------- rows of q and k
+
+struct RotateArgs {
+  const void* q;
+  const void* k;
+  void* q_out;  // [B, T, Hq, D]
+  void* k_out;
+  const void* pos;  // positions, int32 or int64 at b pos_sb + t, or, without, those from starts[b] on
+  int pos64;
+  int64_t pos_sb;
+  const int32_t* starts;
+  const int32_t* lengths;  // or nullptr: T. Zeros are written behind a row's length
+  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh;
+  int Hq, Hkv;
+  int T, tokens;   // tokens = B T
+  int heads;       // of a workgroup
+  TurnArgs turn;
+};
+
+template <int D, int TOKENS>
+struct alignas(16) RotateLds {
+  float stage[LSA_BLOCK * 8 + 8];
+  float weights[2][D];
+  float2 angles[TOKENS][D / 2];
+};
+
+// The heads [part, part + 1) * heads of TOKENS tokens from TOKENS * group on: a workgroup's work. Its threads take the
+// sines of the tokens' pairs first, once for all heads, through LDS; a lane keeps those of its 8 dims in registers
+// and walks the heads of its token, so that a wave reads and writes consecutive heads of one token.
+template <typename T, int D, int TOKENS, bool STREAM>
+__device__ __forceinline__ void rotate_rows(const RotateArgs& a, uint32_t group, uint32_t part, RotateLds<D, TOKENS>& sh) {
+  using L = HeadLanes<D>;
+  constexpr int ROWS = L::SLOTS / TOKENS;  // heads at a time
+  constexpr int AHEAD = 4;                 // rows a lane loads before it works on them
+  const int tid = threadIdx.x, lp = tid % L::LPT, slot = tid / L::LPT;
+  const int t0 = group * TOKENS;
+  const int mine = t0 + slot / ROWS;
+  const int token = mine < a.tokens ? mine : a.tokens - 1;
+  const int b = token / a.T, t = token - b * a.T;
+  const T* q = (const T*)a.q + b * a.q_sb + t * a.q_st + 8 * lp;
+  const T* k = (const T*)a.k + b * a.k_sb + t * a.k_st + 8 * lp;
+  T* qo = (T*)a.q_out + (int64_t)token * a.Hq * D + 8 * lp;
+  T* ko = (T*)a.k_out + (int64_t)token * a.Hkv * D + 8 * lp;
+  const int first = part * a.heads + slot % ROWS;
+  const int end = mine < a.tokens ? min(a.Hq + a.Hkv, (int)(part + 1) * a.heads) : 0;
+  const bool live = a.lengths == nullptr || t < a.lengths[b];
+
+  Raw8<T> raw[AHEAD];
+  auto fetch = [&](int h, Raw8<T>& r) {
+    if (h >= end) return;
+    if (live) r.load(h < a.Hq ? q + h * a.q_sh : k + (h - a.Hq) * a.k_sh);
+    else r.zero();
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) fetch(first + i * ROWS, raw[i]);
+  for (int i = tid; i < TOKENS * a.turn.pairs; i += LSA_BLOCK) {
+    const int n = i / a.turn.pairs, j = i - n * a.turn.pairs;
+    const int at = min(t0 + n, a.tokens - 1), row = at / a.T, x = at - row * a.T;
+    const int64_t p = row * a.pos_sb + x;
+    const int64_t pos = a.pos == nullptr ? (int64_t)a.starts[row] + x
+                                         : (a.pos64 ? ((const int64_t*)a.pos)[p] : (int64_t)((const int32_t*)a.pos)[p]);
+    sh.angles[n][j] = turn_angle(a.turn, pos, j);
+  }
+  if (tid < 8) sh.stage[LSA_BLOCK * 8 + tid] = 0.0f;
+  if (tid < 2 * L::LPT) {  // the norms' weights, q's and k's: in LDS they leave the registers to a fifth wave a SIMD
+    float w[8];
+    load_weights<T>(tid < L::LPT ? a.turn.qw : a.turn.kw, a.turn.w32, lp, w);
+    store8(&sh.weights[tid / L::LPT][8 * lp], w);
+  }
+  __syncthreads();
+  LaneTurn turn;
+  if (a.turn.pairs > 0) turn.load(a.turn, sh.angles[slot / ROWS], lp);
+  for (int h0 = first; h0 < end; h0 += AHEAD * ROWS) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int h = h0 + i * ROWS;
+      if (h >= end) break;
+      float y[8];
+      raw[i].get(y);
+      fetch(h + AHEAD * ROWS, raw[i]);
+      const bool is_q = h < a.Hq;
+      if (live) {
+        if (is_q ? a.turn.qw != nullptr : a.turn.kw != nullptr) {
+          Raw8<float> r;
+          float w[8];
+          r.load(&sh.weights[is_q ? 0 : 1][8 * lp]);
+          r.get(w);
+          norm8<D>(y, w, a.turn.eps);
+        }
+        if (a.turn.pairs > 0) turn8(a.turn, y, turn, sh.stage + slot * D, sh.stage + LSA_BLOCK * 8, lp);
+      }
+      store8<STREAM>(is_q ? qo + (int64_t)h * D : ko + (int64_t)(h - a.Hq) * D, y);
+    }
   }
 }
+
+void launch_rotate(const RotateArgs& a, int dtype, int D, hipStream_t s);  // rotate.hip
 
 // ---------------------------------------------------------------- 8-bit codes
 

@@ -9,6 +9,7 @@ costs in 16 bits, in memory and in a read. No counterpart in the reference.
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -130,11 +131,15 @@ def byte_append(
     lens = None if lengths is None else int32_on(lengths, device)
     if starts.numel() != B or (lens is not None and lens.numel() != B):
         raise ValueError(f"byte_append: starts and lengths [{B}]")
+    if slot_table is not None:  # numbers past 32 bits are rows of no cache
+        if slot_table.dtype is not torch.int32:
+            slot_table = int32_on(slot_table, device)
+        slot_rows = None if slot_rows is None else int32_on(slot_rows, device)
     turn, _keep = turn_of("byte_append", device, D, k.dtype, frequencies, q_weight, k_weight, eps, interleaved, magnitude)
     slots, _slots = _slot_args(slot_table, slot_rows, B, device)
     out, Hq, qsb, qst, qsh = None, 0, 0, 0, 0
     if q is not None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         Hq = q.shape[2]
     if k.numel() == 0:
         return out
@@ -170,7 +175,8 @@ def byte_values(cache: ByteCache, rows: torch.Tensor | None = None, lengths: tor
     lens = None if lengths is None else int32_on(lengths, device)
     if lens is not None and lens.numel() != R:
         raise ValueError(f"byte_values: {lens.numel()} lengths for {R} rows")
-    k, v = (torch.empty(R, W, Hkv, D, dtype=dtype, device=device) for _ in range(2))
+    k = torch.empty((R, W, Hkv, D), dtype=dtype, device=device)
+    v = torch.empty_like(k)
     if R * W * Hkv:
         with launch_device(device):
             _abi.call("lsa_byte_values", ctypes.addressof(held), _abi.ptr(rows), W, _abi.ptr(lens), R, W, Hkv, D, dt,
@@ -178,8 +184,18 @@ def byte_values(cache: ByteCache, rows: torch.Tensor | None = None, lengths: tor
     return k, v
 
 
-# Workgroups that a read is split into at least while its lists are long enough (one of four waves takes 128 keys at a time)
-_READ_GROUPS, _READ_KEYS, _READ_SPLITS = 512, 128, 64
+_READ_SPLITS = 64
+
+
+@functools.lru_cache(maxsize=4096)
+def _read_splits(units: int, width: int) -> int:
+    """Spans of a list, a workgroup each. 256 units (a CU each) and more read theirs whole, fewer are cut until
+    there are about 512 workgroups, lists of any number past 1500 slots, so that lengths that differ even out;
+    a span has 192 slots or more, below which its start costs more than it saves. Measured, us, by spans: 8
+    units of 2816 slots 4: 12.6, 8: 9.4, 14: 9.0, 22: 9.3; 256 of them 1: 30.8, 2: 35.2, 8: 36.4; 160 of 6336
+    2: 56, 4: 41.4, 8: 46; 128 of 32768 4: 196, 16: 173, 32: 168."""
+    few = -(-512 // units) if units < 256 else 1
+    return max(1, min(_READ_SPLITS, width // 192, max(few, width // 1500), (1 << 23) // units))
 
 
 def byte_read(q: torch.Tensor, cache: ByteCache, read_lists: torch.Tensor, lengths: torch.Tensor,
@@ -203,12 +219,12 @@ def byte_read(q: torch.Tensor, cache: ByteCache, read_lists: torch.Tensor, lengt
     if held.caches not in (B, 1):
         raise ValueError(f"byte_read: a cache of {B} rows or a pool of one, got {held.caches}")
     ids, lens, W, per_head = lists_of(read_lists, lengths, B * Tq, Hkv, device)
-    out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.numel() == 0:
         return out
     q = aligned(q)
     units = B * Tq * Hkv * -(-Hq // Hkv // 16)
-    splits = max(1, min(-(-W // _READ_KEYS), -(-_READ_GROUPS // units), _READ_SPLITS))
+    splits = _read_splits(units, W)
     nbytes = _abi.shape_size("lsa_byte_read_scratch_bytes", B * Tq, Hq, Hkv, D, splits)
     with launch_device(device):
         ws, counters, stream = _abi.call_memory(device, "byte_read", nbytes, units if nbytes else 0)

@@ -73,7 +73,6 @@ def turn_of(what: str, device: torch.device, D: int, dtype: torch.dtype, frequen
     if D not in (32, 64, 128, 256):
         raise ValueError(f"{what}: head dim {D} not in 32, 64, 128, 256")
     if frequencies is not None:
-        one_device(what, frequencies)
         if frequencies.dim() != 1 or frequencies.device != device:
             raise ValueError(f"{what}: frequencies [pairs] on {device}, got {tuple(frequencies.shape)} on {frequencies.device}")
         pairs = frequencies.shape[0]
@@ -81,22 +80,35 @@ def turn_of(what: str, device: torch.device, D: int, dtype: torch.dtype, frequen
             raise ValueError(f"{what}: {pairs} pairs in heads of {D}")
         if frequencies.dtype not in (torch.float32, torch.float64):
             raise ValueError(f"{what}: frequencies in fp32 or fp64, got {frequencies.dtype}")
-        frequencies = frequencies.contiguous()
+        if pairs > 1 and frequencies.stride(0) != 1:
+            frequencies = frequencies.contiguous()
         f64 = 1 if frequencies.dtype is torch.float64 else 0
     if not eps >= 0.0:
         raise ValueError(f"{what}: eps {eps}")
-    weights = (q_weight, k_weight)
-    for w in weights:
-        if w is not None and (tuple(w.shape) != (D,) or w.device != device or w.dtype not in (dtype, torch.float32)):
-            raise ValueError(f"{what}: norm weights [{D}] in {dtype} or fp32 on {device}, got {w.dtype} {tuple(w.shape)} "
-                             f"on {w.device}")
-    f32 = any(w is not None and w.dtype is torch.float32 for w in weights)
-    if f32:  # one type for both
-        weights = tuple(None if w is None else w.float() for w in weights)
-    qw, kw = (None if w is None else aligned(w) for w in weights)
-    turn = _Turn(_abi.ptr(frequencies) if pairs else None, _abi.ptr(qw), _abi.ptr(kw), pairs, f64, 1 if interleaved else 0,
-                 1 if f32 else 0, eps, magnitude)
+    f32 = 0
+    qw = kw = None
+    if q_weight is not None or k_weight is not None:
+        for w in (q_weight, k_weight):
+            if w is None:
+                continue
+            if w.shape != (D,) or w.device != device or (w.dtype is not dtype and w.dtype is not torch.float32):
+                raise ValueError(f"{what}: norm weights [{D}] in {dtype} or fp32 on {device}, got {w.dtype} "
+                                 f"{tuple(w.shape)} on {w.device}")
+            if w.dtype is torch.float32:
+                f32 = 1
+        qw, kw = _weight(q_weight, f32), _weight(k_weight, f32)
+    turn = _Turn(frequencies.data_ptr() if pairs else None, None if qw is None else qw.data_ptr(),
+                 None if kw is None else kw.data_ptr(), pairs, f64, 1 if interleaved else 0, f32, eps, magnitude)
     return turn, (frequencies, qw, kw)
+
+
+def _weight(w: torch.Tensor | None, f32: int) -> torch.Tensor | None:
+    """A norm's weight as the kernels read it: dense, 16-byte aligned, in fp32 where one of the two is."""
+    if w is None:
+        return None
+    if f32 and w.dtype is not torch.float32:
+        w = w.float()
+    return w if w.stride(0) == 1 and not w.data_ptr() & 15 else aligned(w)
 
 
 def head_rows(x: torch.Tensor):
@@ -105,7 +117,7 @@ def head_rows(x: torch.Tensor):
     sb, st, sh, sd = x.stride()
     B, T, H, _ = x.shape
     sb, st, sh = sb if B > 1 else 0, st if T > 1 else 0, sh if H > 1 else 0
-    if sd != 1 or x.data_ptr() % 16 or ((sb | st | sh) * x.element_size()) % 16:
+    if sd != 1 or x.data_ptr() & 15 or (sb | st | sh) & (3 if x.dtype is torch.float32 else 7):
         x = aligned(x)
         sb, st, sh, _ = x.stride()
     return x, sb, st, sh
@@ -142,7 +154,7 @@ def rotate(
     turn, _keep = turn_of("rotate", device, D, q.dtype, frequencies, q_weight, k_weight, eps, interleaved, magnitude)
     i64 = stride = 0
     if turn.pairs:
-        if positions is None or tuple(positions.shape) not in ((B, T), (T,)) or positions.device != device:
+        if positions is None or positions.shape not in ((B, T), (T,)) or positions.device != device:
             raise ValueError(f"rotate: positions [{B}, {T}] or [{T}] on {device}, got "
                              f"{None if positions is None else (tuple(positions.shape), positions.device)}")
         if positions.dtype not in (torch.int32, torch.int64):
@@ -151,8 +163,8 @@ def rotate(
         if T > 1 and positions.stride(-1) != 1:
             positions = positions.contiguous()
         stride = positions.stride(0) if positions.dim() == 2 and B > 1 else 0
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=device)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     if q.numel() == 0:
         return q_out, k_out
     q, qsb, qst, qsh = head_rows(q)

@@ -44,7 +44,7 @@ def call_rotate(t=None, **over):
 @pytest.mark.parametrize("over,match", [
     (dict(q=None), "NULL"), (dict(ko=None), "NULL"), (dict(turn=None), "NULL"), (dict(pos=None), "NULL positions"),
     (dict(dt=4), "dtype"), (dict(D=96), "head dim"), (dict(Hq=0), "LSA_ERR_SHAPE"), (dict(Hkv=-1), "LSA_ERR_SHAPE"),
-    (dict(T=1 << 30), "2\\^30"), (dict(q=P + 8), "aligned"), (dict(kst=258), "aligned"), (dict(ps=-1), "position stride"),
+    (dict(T=1 << 25), "2\\^26"), (dict(q=P + 8), "aligned"), (dict(kst=258), "aligned"), (dict(ps=-1), "position stride"),
 ])
 def test_rotate_abi(over, match):
     with pytest.raises(ValueError, match=match):
@@ -71,7 +71,7 @@ def append(c=None, t=None, **over):
 @pytest.mark.parametrize("over,match", [
     (dict(k=None), "NULL"), (dict(starts=None), "NULL"), (dict(out=None), "NULL"), (dict(cache=None), "NULL cache"),
     (dict(dt=3), "dtype"), (dict(D=48), "head dim"), (dict(Hq=0), "LSA_ERR_SHAPE"), (dict(T=-1), "LSA_ERR_SHAPE"),
-    (dict(T=1 << 30), "2\\^30"), (dict(B=3), "2 caches"), (dict(v=P + 2), "aligned"), (dict(vsh=100), "aligned"),
+    (dict(T=1 << 24), "2\\^24"), (dict(B=3), "2 caches"), (dict(v=P + 2), "aligned"), (dict(vsh=100), "aligned"),
 ])
 def test_append_abi(over, match):
     with pytest.raises(ValueError, match=match):
@@ -114,7 +114,7 @@ def read(c=None, **over):
 @pytest.mark.parametrize("over,match", [
     (dict(q=None), "NULL"), (dict(ids=None), "NULL"), (dict(lens=None), "NULL"), (dict(dt=3), "dtype"), (dict(D=100), "head dim"),
     (dict(Hq=7), "must group"), (dict(Hq=1), "must group"), (dict(splits=0), "splits"), (dict(splits=65), "splits"),
-    (dict(W=-1), "negative"), (dict(B=4), "2 caches"), (dict(Tq=1 << 23), "under 2\\^24"), (dict(Tq=1 << 40), "too many"),
+    (dict(W=-1), "negative"), (dict(B=4), "2 caches"), (dict(Tq=1 << 23), "under 2\\^24"), (dict(Tq=1 << 40), "too many"), (dict(Tq=1 << 21, ws=P), "2\\^24 workgroups"),
     (dict(out=P + 8), "aligned"),
 ])
 def test_read_abi(over, match):
@@ -159,7 +159,7 @@ def test_rotate_arguments():
         ((q, k, pos, fake(33, dtype=f32)), {}, "33 pairs"),
         ((q, k, pos, fake(32, 1, dtype=f32)), {}, "frequencies \\[pairs\\]"),
         ((q, k, pos, fake(32)), {}, "fp32 or fp64"),
-        ((q, k, pos, torch.zeros(32)), {}, "ROCm kernel"),
+        ((q, k, pos, torch.zeros(32)), {}, "on cuda:0"),
         ((q, k, pos, freq), dict(q_weight=fake(32)), "norm weights"),
         ((q, k, pos, freq), dict(k_weight=fake(64, dtype=torch.float16)), "norm weights"),
         ((q, k, pos, freq), dict(eps=-1e-6), "eps"),
@@ -188,7 +188,7 @@ def test_append_arguments():
         ((c, k, k, n), dict(q=fake(3, 4, 8, 64)), "q \\[3, 5, Hq, 64\\]"),
         ((pool, k, k, n), {}, "or a pool of one with a slot_table"),
         ((c, k, k, n), dict(slot_table=table), "or a pool of one with a slot_table"),
-        ((pool, k, k, n), dict(slot_table=table[:2]), "slot_rows is needed"),
+        ((c, k, k, n), dict(slot_rows=n), "slot_rows without"),
         ((c, k, k, n[:2]), {}, "starts and lengths"),
         ((c, k, k, n), dict(lengths=n[:1]), "starts and lengths"),
         ((shared, k, k, n), {}, "place of their own"),
