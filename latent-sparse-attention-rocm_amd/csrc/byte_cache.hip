@@ -28,10 +28,12 @@ struct CacheArgs {
   uint8_t* k;
   uint8_t* v;
   float* scales;
-  int block;
+  int block_shift;
   int64_t tokens, sb, st, sh;  // sb 0: one pool
   int64_t scale_sb;            // scale pairs of a cache, times kv-heads
 };
+
+enum QueryMode { kFew, kMany, kStream };
 
 struct AppendArgs {
   CacheArgs c;
@@ -46,8 +48,9 @@ struct AppendArgs {
   int parts, heads;  // workgroups of a tile, kv-heads of one
   int64_t kv_groups; // workgroups before the first of q's
   TurnArgs turn;
-  RotateArgs q;      // few tokens' rows of q, in workgroups behind the others:
-  uint32_t q_parts;  // so many a token
+  RotateArgs q;      // rows of q, in workgroups behind the others:
+  int q_mode;        // of a token (and a part of its heads), or of 4
+  uint32_t q_parts;  // workgroups of a token
 };
 
 __device__ __forceinline__ int new_tokens(const AppendArgs& a, int b) {
@@ -58,7 +61,7 @@ __device__ __forceinline__ int new_tokens(const AppendArgs& a, int b) {
 template <int D>
 struct alignas(16) AppendLds {
   float stage[LSA_BLOCK * 8 + 8];
-  float2 angles[kTile * (D / 2)];
+  Angles<D> angles[kTile];
   uint32_t most[3][kTile];       // of a unit's blocks, as integers; three units take turns
   float before[2 * kPartHeads];  // the first block's scales, where it holds earlier tokens
   int32_t block_row[kTile];
@@ -71,10 +74,13 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_append_kernel(AppendArgs a) {
   __shared__ union {
     AppendLds<D> kv;
     RotateLds<D, 1> q;
+    RotateLds<D, 4> q4;
   } sh;
   if ((int64_t)blockIdx.x >= a.kv_groups) {
     const uint32_t g = (uint32_t)(blockIdx.x - a.kv_groups), token = g / a.q_parts;
-    rotate_rows<T, D, 1, false>(a.q, token, g - token * a.q_parts, sh.q);
+    if (a.q_mode == kStream) rotate_rows<T, D, 4, true>(a.q, g, 0, sh.q4);
+    else if (a.q_mode == kMany) rotate_rows<T, D, 4, false>(a.q, g, 0, sh.q4);
+    else rotate_rows<T, D, 1, false>(a.q, token, g - token * a.q_parts, sh.q);
     return;
   }
   const int tid = threadIdx.x;
@@ -82,7 +88,7 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_append_kernel(AppendArgs a) {
   auto& block_row = sh.kv.block_row;
   float* before = sh.kv.before;
   float* stage = sh.kv.stage;
-  float2* angles = sh.kv.angles;
+  auto& angles = sh.kv.angles;
   if (tid < 8) stage[LSA_BLOCK * 8 + tid] = 0.0f;
   const int part = blockIdx.x % a.parts, tile = blockIdx.x / a.parts % a.tiles;
   const int b = blockIdx.x / a.parts / a.tiles;
@@ -93,30 +99,36 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_append_kernel(AppendArgs a) {
   const int64_t from = start > p0 ? start : p0;  // the tile's new positions: [from, to)
   const int64_t to = end < p0 + kTile ? end : p0 + kTile;
   if (from >= to) return;
-  const int block = a.c.block, blocks = kTile / block;
+  const int shift = a.c.block_shift, block = 1 << shift, blocks = kTile >> shift;
   const int lo = (int)(from - p0), hi = (int)(to - p0);
-  const int begin = lo / block * block;  // the first written block's first token
+  const int begin = lo >> shift << shift;  // the first written block's first token
   const int h0 = part * a.heads, h1 = min(h0 + a.heads, a.Hkv), units = 2 * (h1 - h0);
   const int lp = tid % L::LPT, slot = tid / L::LPT;
   const int first = slot * STEPS;  // a lane's tokens are consecutive
   const int64_t n0 = p0 - start;   // token of the tile's first position
-  const T* kb = (const T*)a.k + b * a.k_sb + 8 * lp;
-  const T* vb = (const T*)a.v + b * a.v_sb + 8 * lp;
+  const T* k_row[STEPS];  // where a lane's tokens lie
+  const T* v_row[STEPS];
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int x = first + i;
+    const int64_t n = x >= lo && x < hi ? n0 + x : 0;
+    k_row[i] = (const T*)a.k + b * a.k_sb + n * a.k_st + 8 * lp;
+    v_row[i] = (const T*)a.v + b * a.v_sb + n * a.v_st + 8 * lp;
+  }
   Raw8<T> raw[STEPS];
   auto fetch = [&](int u) {  // unit u: K (even) or V of a head
-    const int h = h0 + (u >> 1);
+    const int64_t off = (h0 + (u >> 1)) * ((u & 1) ? a.v_sh : a.k_sh);
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
       const int x = first + i;
-      if (u < units && x >= lo && x < hi)
-        raw[i].load((u & 1) ? vb + (n0 + x) * a.v_st + h * a.v_sh : kb + (n0 + x) * a.k_st + h * a.k_sh);
+      if (u < units && x >= lo && x < hi) raw[i].load(((u & 1) ? v_row[i] : k_row[i]) + off);
       else raw[i].zero();
     }
   };
   fetch(0);
   float* scales = a.c.scales + (b * a.c.scale_sb) * 2;
   auto row_of = [&](int blk) {  // the cache row of the tile's block blk, or -1
-    const int64_t p = p0 + (int64_t)blk * block;
+    const int64_t p = p0 + (blk << shift);
     int64_t row = p;
     if (map.row) row = p < map.width ? map.row[p] : -1;
     return row < 0 || row >= a.c.tokens || (row & (block - 1)) ? -1 : (int32_t)row;
@@ -124,79 +136,121 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_append_kernel(AppendArgs a) {
   if (tid < blocks) block_row[tid] = row_of(tid);
   if (tid >= kTile && tid < kTile + units) {
     const int u = tid - kTile;
-    const int32_t row = begin < lo ? row_of(begin / block) : -1;
-    before[u] = row < 0 ? 0.0f : scales[((int64_t)(row / block) * a.Hkv + h0 + (u >> 1)) * 2 + (u & 1)];
+    const int32_t row = begin < lo ? row_of(begin >> shift) : -1;
+    before[u] = row < 0 ? 0.0f : scales[((int64_t)(row >> shift) * a.Hkv + h0 + (u >> 1)) * 2 + (u & 1)];
   }
   for (int i = tid; i < 3 * kTile; i += LSA_BLOCK) (&most[0][0])[i] = 0u;
-  for (int i = tid; i < (hi - lo) * a.turn.pairs; i += LSA_BLOCK) {
-    const int n = i / a.turn.pairs, j = i - n * a.turn.pairs;
-    angles[(lo + n) * (D / 2) + j] = turn_angle(a.turn, from + n, j);
+  // the sines of the tile's tokens: a pair a thread (64 or 128 threads a token), the tile's first angle and a
+  // multiple of the pair's frequency, in fp64 turns
+  {
+    const int wide = a.turn.pairs > 64 ? 7 : 6, j = tid & ((1 << wide) - 1);
+    if (j < a.turn.pairs) {
+      const double f = turn_frequency(a.turn, j), each = f * kPerTurn;
+      double base = (double)p0 * f * kPerTurn;
+      base -= rint(base);
+#pragma unroll 4
+      for (int x = lo + (tid >> wide); x < hi; x += LSA_BLOCK >> wide) angles[x].put(j, turn_angle(a.turn, fma((double)x, each, base)));
+    }
   }
   float wk[8];
   load_weights<T>(a.turn.kw, a.turn.w32, lp, wk);
   __syncthreads();
 
-  const int64_t cb = b * a.c.sb;
   const bool had = begin < lo;  // the first block holds earlier tokens
+  int64_t to_row[STEPS];  // where their codes go, or -1: nowhere; earlier tokens of the first block among them
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int x = first + i;
+    const int64_t row0 = block_row[x >> shift], row = row0 + (x & (block - 1));
+    to_row[i] = x < begin || x >= hi || row0 < 0 || row >= a.c.tokens ? -1 : b * a.c.sb + row * a.c.st + 8 * lp;
+  }
   for (int u = 0; u < units; ++u) {
     const int h = h0 + (u >> 1), kv = u & 1, turn_no = u % 3;
     float y[STEPS][8];
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) raw[i].get(y[i]);
     fetch(u + 1);
+    uint32_t tops[STEPS];  // a token's largest magnitude, as an integer: infinities and NaN are the largest of all
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
       const int x = first + i;
-      if (x >= lo && x < hi) {  // uniform over the lanes of a row
-        if (kv == 0) {
-          if (a.turn.kw) norm8<D>(y[i], wk, a.turn.eps);
-          if (a.turn.pairs > 0) {
-            LaneTurn turn;
-            turn.load(a.turn, angles + x * (D / 2), lp);
-            turn8(a.turn, y[i], turn, stage + slot * D, stage + LSA_BLOCK * 8, lp);
-          }
+      if (kv == 0 && x >= lo && x < hi) {  // uniform over the lanes of a row
+        if (a.turn.kw) norm8<D>(y[i], wk, a.turn.eps);
+        if (a.turn.pairs > 0) {
+          LaneTurn turn;
+          turn.load(a.turn, angles[x], lp);
+          turn8(a.turn, y[i], turn, stage + slot * D, stage + LSA_BLOCK * 8, lp);
         }
-        float m = 0.0f;
+      }
+      uint32_t m = 0u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(y[i][e]) & 0x7FFFFFFFu);
+      tops[i] = m;
+    }
+    bool strange = false;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) strange |= tops[i] >= 0x7F800000u;
+    const bool odd = __ballot(strange) != 0ull;  // wave-uniform, and rare
+    if (odd) {  // the finite ones' maximum
+      asm volatile("; kept a branch");
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        tops[i] = 0u;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float z = fabsf(y[i][e]);
-          m = z > m && z < INFINITY ? z : m;
+          const uint32_t z = __float_as_uint(y[i][e]) & 0x7FFFFFFFu;
+          tops[i] = z < 0x7F800000u && z > tops[i] ? z : tops[i];
         }
-        m = group_max<L::LPT>(m);
-        if (lp == 0) atomicMax(&most[turn_no][x / block], __float_as_uint(m));
+      }
+    }
+    // tokens that are not new are zeros, here and in their blocks' maxima
+    if (block >= STEPS) {  // a lane's tokens are of one block
+      uint32_t m = 0u;
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) m = max(m, tops[i]);
+      const float top = group_max<L::LPT>(__uint_as_float(m));
+      if (lp == 0) atomicMax(&most[turn_no][first >> shift], __float_as_uint(top));
+    } else {
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const float top = group_max<L::LPT>(__uint_as_float(tops[i]));
+        if (lp == 0) atomicMax(&most[turn_no][(first + i) >> shift], __float_as_uint(top));
       }
     }
     if (tid < kTile) most[(u + 1) % 3][tid] = 0u;  // unit u - 2's: every thread read it before the last barrier
     __syncthreads();
     const float held = before[u];
-    uint8_t* cache = (kv ? a.c.v : a.c.k) + cb + h * a.c.sh + 8 * lp;
+    uint8_t* cache = (kv ? a.c.v : a.c.k) + h * a.c.sh;
+    float scale = 0.0f, inv = 0.0f;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
-      const int x = first + i, blk = x / block;
-      const int32_t row0 = block_row[blk];
-      if (x < begin || x >= hi || row0 < 0) continue;
-      const bool old_block = had && blk == begin / block;
-      float scale = fmaxf(__uint_as_float(most[turn_no][blk]) / C::kMost, kLeast);
-      if (old_block) scale = fmaxf(scale, held);
-      const int64_t row = (int64_t)row0 + (x - blk * block);
-      if (row >= a.c.tokens) continue;
-      uint2* at = (uint2*)(cache + row * a.c.st);
+      const int x = first + i, blk = x >> shift;
+      if (i == 0 || block < STEPS) {  // else the lane's tokens are of one block
+        scale = fmaxf(__uint_as_float(most[turn_no][blk]) / C::kMost, kLeast);
+        if (had && blk == begin >> shift) scale = fmaxf(scale, held);
+        inv = 1.0f / scale;
+      }
+      if (to_row[i] < 0) continue;
+      uint2* at = (uint2*)(cache + to_row[i]);
       if (x >= lo) {
-        const float inv = 1.0f / scale;
-        float z[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[e] = divided(y[i][e], scale, inv);
-        *at = codes8<C>(z);
+        uint2 codes;
+        if (odd) {
+          asm volatile("; kept a branch");
+          codes = put8<C>(y[i], scale, inv, true);
+        } else {
+          codes = put8<C>(y[i], scale, inv, false);
+        }
+        *at = codes;
       } else if (scale != held) {  // the block's earlier tokens, where its scale grew
         const float ratio = held / scale;
         float z[8];
         C::get8(*at, z);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) z[e] *= ratio;
-        *at = codes8<C>(z);
+        for (int e = 0; e < 8; ++e) z[e] = C::odd(z[e] * ratio);
+        *at = make_uint2(C::put4(z), C::put4(z + 4));
       }
-      if (lp == 0 && x == max(blk * block, lo))  // the block's first new token
-        scales[((int64_t)(row0 / block) * a.Hkv + h) * 2 + kv] = scale;
+      if (lp == 0 && x == max(blk << shift, lo))  // the block's first new token
+        scales[((int64_t)(block_row[blk] >> shift) * a.Hkv + h) * 2 + kv] = scale;
     }
   }
 }
@@ -210,7 +264,6 @@ struct ValueArgs {
   int Hkv;
   void* k_out;
   void* v_out;
-  int block_shift;
   uint32_t many, chunks;  // rows of a workgroup, workgroups of a list
 };
 
@@ -230,7 +283,7 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_values_kernel(ValueArgs a) {
     float k[8], v[8];
     if (w < n && row >= 0 && row < a.c.tokens) {
       const int64_t at = r * a.c.sb + row * a.c.st + h * a.c.sh + 8 * lp;
-      const float2 s = ((const float2*)a.c.scales)[r * a.c.scale_sb + (row >> a.block_shift) * a.Hkv + h];
+      const float2 s = ((const float2*)a.c.scales)[r * a.c.scale_sb + (row >> a.c.block_shift) * a.Hkv + h];
       C::get8(*(const uint2*)(a.c.k + at), k);
       C::get8(*(const uint2*)(a.c.v + at), v);
 #pragma unroll
@@ -259,7 +312,7 @@ void launch_values(const ValueArgs& a, hipStream_t s) {
 
 CacheArgs cache_args(const lsa_byte_cache* c, int32_t Hkv) {
   const int64_t pairs = (c->tokens + c->block - 1) / c->block * Hkv;
-  return CacheArgs{(uint8_t*)c->k, (uint8_t*)c->v, c->scales, c->block, c->tokens, c->caches == 1 ? 0 : c->batch_stride,
+  return CacheArgs{(uint8_t*)c->k, (uint8_t*)c->v, c->scales, __builtin_ctz((unsigned)c->block), c->tokens, c->caches == 1 ? 0 : c->batch_stride,
                    c->token_stride, c->head_stride, c->caches == 1 ? 0 : pairs};
 }
 
@@ -313,19 +366,18 @@ extern "C" int lsa_byte_append(const lsa_byte_cache* cache, const void* k, const
   r.q = r.k = q; r.q_out = r.k_out = q_out; r.starts = starts; r.lengths = lengths;
   r.q_sb = q_batch_stride; r.q_st = q_token_stride; r.q_sh = q_head_stride;
   r.Hq = Hq; r.T = (int)T; r.tokens = (int)(B * T); r.turn = t;
-  // q of few tokens in the same launch (a part of its heads a workgroup while there are fewer than 512), of more in
-  // one of its own, whose workgroups need a quarter of the LDS and fewer registers (32768 tokens: 198 us together)
-  const bool same = q && B * T < 1024;
+  // q in the same launch: its workgroups wait for memory while those of K and V wait for barriers and each other
+  // (32768 tokens: 107 us for q and 73 for K and V, one after the other). Its outputs go past the caches as rotate's.
+  a.q_mode = B * T < 1024 ? kFew : (B * T * Hq * D * e > (64 << 20) ? kStream : kMany);
   const int rows = 256 / (D / 8);
-  r.heads = B * T * ((Hq + rows - 1) / rows) <= 512 ? rows : Hq;
-  a.q_parts = (uint32_t)((Hq + r.heads - 1) / std::max(r.heads, 1));
-  const int64_t groups = a.kv_groups + (same ? B * T * a.q_parts : 0);
+  r.heads = a.q_mode == kFew && B * T * ((Hq + rows - 1) / rows) <= 512 ? rows : std::max(Hq, 1);
+  a.q_parts = (uint32_t)((Hq + r.heads - 1) / r.heads);
+  const int64_t groups = a.kv_groups + (!q ? 0 : (a.q_mode == kFew ? B * T * a.q_parts : (B * T + 3) / 4));
   LSA_REQUIRE(groups <= kMaxGroups, LSA_ERR_SHAPE, "lsa_byte_append: %lld tokens of %d kv-heads (2^24 workgroups)",
               (long long)(B * T), Hkv);
   hipStream_t s = (hipStream_t)stream;
   const int code = cache->code;
   LSA_DISPATCH_QT(dtype, { LSA_DISPATCH_CODES(D, code, launch_append, a, groups, s) });
-  if (q && !same) launch_rotate(r, dtype, D, s);
   LSA_LAUNCHED("lsa_byte_append");
   return LSA_OK;
 }
@@ -341,7 +393,6 @@ extern "C" int lsa_byte_values(const lsa_byte_cache* cache, const int32_t* rows,
   LSA_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, LSA_ERR_ALIGN, "lsa_byte_values: outputs must be 16-byte aligned");
   if (R * W == 0) return LSA_OK;
   ValueArgs a = {cache_args(cache, Hkv), rows, row_stride, lengths, R, W, Hkv, k_out, v_out};
-  a.block_shift = __builtin_ctz((unsigned)cache->block);
   a.many = (uint32_t)std::max(1, kValueLanes / (Hkv * (D / 8)));
   const int64_t chunks = (W + a.many - 1) / a.many;
   LSA_REQUIRE(chunks <= kMaxGroups / R, LSA_ERR_SHAPE, "lsa_byte_values: %lld rows", (long long)(R * W));

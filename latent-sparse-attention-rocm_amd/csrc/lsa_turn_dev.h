@@ -86,30 +86,57 @@ template <bool STREAM = false> __device__ __forceinline__ void store8(_Float16* 
   store_words<STREAM>(p, words4_t{pack_f16(f[0], f[1]), pack_f16(f[2], f[3]), pack_f16(f[4], f[5]), pack_f16(f[6], f[7])});
 }
 
-// (cos, sin) * magnitude of pair j at a position.
-__device__ __forceinline__ float2 turn_angle(const TurnArgs& a, int64_t pos, int j) {
-  const double f = a.freq64 ? ((const double*)a.freq)[j] : (double)((const float*)a.freq)[j];
-  const double turns = (double)pos * f * 0.15915494309189533577;  // 1 / (2 pi)
+constexpr double kPerTurn = 0.15915494309189533577;  // 1 / (2 pi)
+
+__device__ __forceinline__ double turn_frequency(const TurnArgs& a, int j) {
+  return a.freq64 ? ((const double*)a.freq)[j] : (double)((const float*)a.freq)[j];
+}
+// (cos, sin) * magnitude of an angle in turns.
+__device__ __forceinline__ float2 turn_angle(const TurnArgs& a, double turns) {
   const float x = (float)(turns - rint(turns));
   float s, c;
   sincospif(2.0f * x, &s, &c);
   return make_float2(c * a.magnitude, s * a.magnitude);
 }
 
-// This lane's dims 8 lp .. + 8 of the row's rotation.
+// A token's angles in LDS: the cosines of its pairs, then their sines.
+template <int D>
+struct alignas(16) Angles {
+  float c[D / 2], s[D / 2];
+  __device__ __forceinline__ void put(int j, float2 cs) {
+    c[j] = cs.x;
+    s[j] = cs.y;
+  }
+};
+
+// This lane's dims 8 lp .. + 8 of the row's rotation; those that stay: cosine 1, sine 0.
 struct LaneTurn {
   float c[8], s[8];
-  // angles: the token's (cos, sin) of every pair
-  __device__ __forceinline__ void load(const TurnArgs& a, const float2* angles, int lp) {
+  template <int D>
+  __device__ __forceinline__ void load(const TurnArgs& a, const Angles<D>& angles, int lp) {
+    if (!a.interleaved && (a.pairs & 7) == 0) {  // eight angles in a row, one side of their pairs
+      const bool in = 8 * lp < 2 * a.pairs, low = 8 * lp < a.pairs;
+      const int j = in ? (low ? 8 * lp : 8 * lp - a.pairs) : 0;
+      const float4 c0 = *(const float4*)&angles.c[j], c1 = *(const float4*)&angles.c[j + 4];
+      const float4 s0 = *(const float4*)&angles.s[j], s1 = *(const float4*)&angles.s[j + 4];
+      const float cc[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+      const float ss[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+      const uint32_t sign = low ? 0x80000000u : 0u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        c[e] = in ? cc[e] : 1.0f;
+        s[e] = in ? __uint_as_float(__float_as_uint(ss[e]) ^ sign) : 0.0f;
+      }
+      return;
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int i = 8 * lp + e;
       const bool in = i < 2 * a.pairs;
       const bool low = a.interleaved ? (i & 1) == 0 : i < a.pairs;
-      const int j = a.interleaved ? i >> 1 : (low ? i : i - a.pairs);
-      const float2 cs = angles[in ? j : 0];
-      c[e] = in ? cs.x : 1.0f;
-      s[e] = in ? (low ? -cs.y : cs.y) : 0.0f;
+      const int j = in ? (a.interleaved ? i >> 1 : (low ? i : i - a.pairs)) : 0;
+      c[e] = in ? angles.c[j] : 1.0f;
+      s[e] = in ? (low ? -angles.s[j] : angles.s[j]) : 0.0f;
     }
   }
 };
@@ -200,7 +227,7 @@ template <int D, int TOKENS>
 struct alignas(16) RotateLds {
   float stage[LSA_BLOCK * 8 + 8];
   float weights[2][D];
-  float2 angles[TOKENS][D / 2];
+  Angles<D> angles[TOKENS];
 };
 
 // The heads [part, part + 1) * heads of TOKENS tokens from TOKENS * group on: a workgroup's work. Its threads take the
@@ -238,7 +265,7 @@ __device__ __forceinline__ void rotate_rows(const RotateArgs& a, uint32_t group,
     const int64_t p = row * a.pos_sb + x;
     const int64_t pos = a.pos == nullptr ? (int64_t)a.starts[row] + x
                                          : (a.pos64 ? ((const int64_t*)a.pos)[p] : (int64_t)((const int32_t*)a.pos)[p]);
-    sh.angles[n][j] = turn_angle(a.turn, pos, j);
+    sh.angles[n].put(j, turn_angle(a.turn, (double)pos * turn_frequency(a.turn, j) * kPerTurn));
   }
   if (tid < 8) sh.stage[LSA_BLOCK * 8 + tid] = 0.0f;
   if (tid < 2 * L::LPT) {  // the norms' weights, q's and k's: in LDS they leave the registers to a fifth wave a SIMD
@@ -273,10 +300,10 @@ __device__ __forceinline__ void rotate_rows(const RotateArgs& a, uint32_t group,
   }
 }
 
-void launch_rotate(const RotateArgs& a, int dtype, int D, hipStream_t s);  // rotate.hip
-
 // ---------------------------------------------------------------- 8-bit codes
 
+// put8: the codes of 8 numbers x / scale, inv = 1 / scale. The quotient is rounded as a division rounds it (one
+// residual step behind the product), then to the nearest code, ties to even. Finite numbers of at most kMost scales.
 struct Int8Code {
   static constexpr float kMost = 127.0f;
   static __device__ __forceinline__ void get8(const uint2& u, float* f) {
@@ -286,12 +313,14 @@ struct Int8Code {
       f[4 + e] = (float)(int8_t)(u.y >> (8 * e));
     }
   }
-  static __device__ __forceinline__ uint32_t put4(const float* f) {
-    uint32_t r = 0;
+  static __device__ __forceinline__ uint32_t put4(const float* z) {
+    uint32_t b[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) r |= ((uint32_t)(int)rintf(f[e]) & 0xFFu) << (8 * e);  // NaN is 0
-    return r;
+    for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(z[e] + 12582912.0f);  // 1.5 2^23: a whole number's low byte is its code
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0C0C0400u), __builtin_amdgcn_perm(b[1], b[0], 0x0C0C0400u),
+                                 0x05040100u);
   }
+  static __device__ __forceinline__ float odd(float z) { return z != z ? 0.0f : fminf(fmaxf(z, -kMost), kMost); }
 };
 struct E4m3Code {
   static constexpr float kMost = 448.0f;
@@ -301,26 +330,24 @@ struct E4m3Code {
     const f2_t c = __builtin_amdgcn_cvt_pk_f32_fp8(u.y, false), d = __builtin_amdgcn_cvt_pk_f32_fp8(u.y, true);
     f[0] = a[0]; f[1] = a[1]; f[2] = b[0]; f[3] = b[1]; f[4] = c[0]; f[5] = c[1]; f[6] = d[0]; f[7] = d[1];
   }
-  static __device__ __forceinline__ uint32_t put4(const float* f) {
-    int r = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], r, true);
+  static __device__ __forceinline__ uint32_t put4(const float* z) {
+    const int r = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], r, true);
   }
+  static __device__ __forceinline__ float odd(float z) { return z != z ? z : fminf(fmaxf(z, -kMost), kMost); }
 };
 
-// x / scale (inv = 1 / scale), rounded as a division rounds it: one residual step behind the product.
-__device__ __forceinline__ float divided(float x, float scale, float inv) {
-  const float y = x * inv;
-  const float z = fmaf(fmaf(-y, scale, x), inv, y);
-  return fabsf(y) < 3.0e38f ? z : y;  // an infinity has no residual
-}
-
-// The codes of 8 numbers already divided by their scale; past the range: its ends; NaN: e4m3's own, int8's 0.
+// strange: some of the numbers may be infinite (the largest code) or NaN (e4m3's own, int8's 0).
 template <typename C>
-__device__ __forceinline__ uint2 codes8(const float* y) {
-  float f[8];
+__device__ __forceinline__ uint2 put8(const float* x, float scale, float inv, bool strange) {
+  float z[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = y[e] != y[e] ? y[e] : fminf(fmaxf(y[e], -C::kMost), C::kMost);
-  return make_uint2(C::put4(f), C::put4(f + 4));
+  for (int e = 0; e < 8; ++e) {
+    const float y = x[e] * inv;
+    z[e] = fmaf(fmaf(-y, scale, x[e]), inv, y);
+    if (strange) z[e] = C::odd(fabsf(y) < 3.0e38f ? z[e] : y);  // an infinity has no residual
+  }
+  return make_uint2(C::put4(z), C::put4(z + 4));
 }
 
 }  // namespace lsa

@@ -41,9 +41,7 @@ void launch_rotate_of(RotateArgs a, hipStream_t s) {
   rotate_kernel<T, D, 1, false><<<dim3(a.tokens, (heads + a.heads - 1) / a.heads), LSA_BLOCK, 0, s>>>(a);
 }
 
-}  // namespace
-
-void lsa::launch_rotate(const RotateArgs& a, int dtype, int D, hipStream_t s) {
+void launch_rotate(const RotateArgs& a, int dtype, int D, hipStream_t s) {
   LSA_DISPATCH_QT(dtype, {
     switch (D) {
       case 32: launch_rotate_of<QT, 32>(a, s); break;
@@ -53,6 +51,8 @@ void lsa::launch_rotate(const RotateArgs& a, int dtype, int D, hipStream_t s) {
     }
   });
 }
+
+}  // namespace
 
 extern "C" int lsa_rotate(const void* q, const void* k, int dtype, int64_t B, int64_t T, int32_t Hq, int32_t Hkv,
                           int32_t D, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
