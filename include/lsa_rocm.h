@@ -562,7 +562,7 @@ typedef struct lsa_byte_cache {
  * new tokens' largest magnitude / M, 2^-100), M = 127 or 448; a new token's code is value / scale, rounded to
  * nearest even, and where the scale grew the block's earlier codes are rescaled and rounded again. What it held
  * from starts[b] on counts for nothing. A NaN has no part in the scale and is held as e4m3's NaN or int8's 0, an
- * infinity as the largest code, neither in the scale. No two rows may write to one block. Under 2^24 tokens. No counterpart in the
+ * infinity as the largest code, neither in the scale. No block may be written to twice in a call. Under 2^24 tokens. No counterpart in the
  * reference. */
 int lsa_byte_append(const lsa_byte_cache* cache, const void* k, const void* v, const void* q, int dtype, int64_t B,
                     int64_t T, int32_t Hq, int32_t Hkv, int32_t D, int64_t k_batch_stride, int64_t k_token_stride,

@@ -94,7 +94,7 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_append_kernel(AppendArgs a) {
   const int b = blockIdx.x / a.parts / a.tiles;
   const SlotRow map = slot_row_of(a.slots, b);  // beside the start's load
   const int64_t start = a.starts[b];
-  const int64_t end = start + new_tokens(a, b);
+  const int64_t end = min(start + new_tokens(a, b), a.slots.table ? (int64_t)map.width : a.c.tokens);  // what is past it is dropped
   const int64_t p0 = (start >= 0 ? start / kTile : 0) * kTile + (int64_t)tile * kTile;
   const int64_t from = start > p0 ? start : p0;  // the tile's new positions: [from, to)
   const int64_t to = end < p0 + kTile ? end : p0 + kTile;
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_append_kernel(AppendArgs a) {
       uint32_t m = 0u;
 #pragma unroll
       for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(y[i][e]) & 0x7FFFFFFFu);
-      tops[i] = m;
+      tops[i] = to_row[i] < 0 ? 0u : m;  // a dropped one has no part in the scale
     }
     bool strange = false;
 #pragma unroll
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_append_kernel(AppendArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const uint32_t z = __float_as_uint(y[i][e]) & 0x7FFFFFFFu;
-          tops[i] = z < 0x7F800000u && z > tops[i] ? z : tops[i];
+          tops[i] = z < 0x7F800000u && z > tops[i] && to_row[i] >= 0 ? z : tops[i];
         }
       }
     }

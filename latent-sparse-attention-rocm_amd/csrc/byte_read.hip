@@ -501,7 +501,7 @@ extern "C" int lsa_byte_read(const void* q, const lsa_byte_cache* cache, int dty
                              void* scratch, size_t scratch_bytes, void* out, void* stream) {
   LSA_REQUIRE(q && out && (ids || W == 0) && lengths, LSA_ERR_NULL, "lsa_byte_read: NULL pointer");
   LSA_TRY(check_dtype(dtype));
-  LSA_REQUIRE(B >= 0 && Tq >= 0 && W >= 0, LSA_ERR_SHAPE, "lsa_byte_read: negative size");
+  LSA_REQUIRE(B >= 0 && Tq >= 0 && W >= 0 && W <= 1 << 30, LSA_ERR_SHAPE, "lsa_byte_read: negative size, or a list of more than 2^30");
   LSA_TRY(check_byte_cache("lsa_byte_read", cache, B, Hkv, D));
   LSA_REQUIRE(Hq >= Hkv && Hq % Hkv == 0 && Hq <= 65536, LSA_ERR_SHAPE, "lsa_byte_read: Hq %d must group onto Hkv %d", Hq, Hkv);
   LSA_REQUIRE(splits >= 1 && splits <= kByteSplits, LSA_ERR_SHAPE, "lsa_byte_read: splits in [1, %d], got %d", kByteSplits, splits);

@@ -98,8 +98,8 @@ def byte_append(
     ``frequencies``) first, as ``rotate`` does, and so is q [B, T, Hq, D] (zeros behind a row's
     length). ``cache`` has B rows, or is a pool [1, rows, Hkv, D] that ``slot_table`` [n, width] and
     ``slot_rows`` [B] (as in the selects) map positions to, whole blocks at a time. Positions outside
-    are dropped, and so is a block whose slot is not a multiple of ``cache.block``. No two rows may
-    write to one block.
+    are dropped, and so is a block whose slot is not a multiple of ``cache.block``; dropped tokens have no
+    part in a scale. No block may be written to twice in a call (by two rows, or two entries of a table).
 
     A block's scale is its largest magnitude over 127 (int8) or 448 (e4m3), at least 2^-100, and
     codes are rounded to nearest. Tokens before ``starts[b]`` in the first block stay: where its scale

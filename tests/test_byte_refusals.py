@@ -114,7 +114,7 @@ def read(c=None, **over):
 @pytest.mark.parametrize("over,match", [
     (dict(q=None), "NULL"), (dict(ids=None), "NULL"), (dict(lens=None), "NULL"), (dict(dt=3), "dtype"), (dict(D=100), "head dim"),
     (dict(Hq=7), "must group"), (dict(Hq=1), "must group"), (dict(splits=0), "splits"), (dict(splits=65), "splits"),
-    (dict(W=-1), "negative"), (dict(B=4), "2 caches"), (dict(Tq=1 << 23), "under 2\\^24"), (dict(Tq=1 << 40), "too many"), (dict(Tq=1 << 21, ws=P), "2\\^24 workgroups"),
+    (dict(W=-1), "negative"), (dict(W=(1 << 30) + 1), "2\\^30"), (dict(B=4), "2 caches"), (dict(Tq=1 << 23), "under 2\\^24"), (dict(Tq=1 << 40), "too many"), (dict(Tq=1 << 21, ws=P), "2\\^24 workgroups"),
     (dict(out=P + 8), "aligned"),
 ])
 def test_read_abi(over, match):

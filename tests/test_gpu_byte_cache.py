@@ -170,6 +170,49 @@ def test_append_drops_what_is_outside_and_takes_a_row_back():
     assert torch.equal(again[0, 30:32], got[0, 30:32]) and torch.equal(again[1], got[1])
 
 
+def test_dropped_tokens_have_no_part_in_a_scale():
+    """Past a dense cache's end, past a table's width, past a pool's end: inside a block that is written to."""
+    k = torch.ones(1, 16, 1, 64, device=DEV)
+    k[:, 4:] = 100.0
+    zero = torch.zeros(1, dtype=torch.int32, device=DEV)
+    dense = pipeline.byte_cache(1, 20, 1, 64, 16, torch.int8, DEV)
+    pipeline.byte_append(dense, k, k, zero + 16)
+    pool = pipeline.byte_cache(1, 20, 1, 64, 16, torch.int8, DEV)
+    pipeline.byte_append(pool, k, k, zero, slot_table=torch.arange(16, 32, dtype=torch.int32, device=DEV)[None])
+    table = pipeline.byte_cache(1, 32, 1, 64, 16, torch.int8, DEV)
+    pipeline.byte_append(table, k, k, zero + 16, slot_table=torch.arange(20, dtype=torch.int32, device=DEV)[None])
+    for cache in (dense, pool, table):
+        got = pipeline.byte_values(cache, dtype=torch.float32)[0][0, :, 0]
+        assert (got[16:20] == 1).all() and (got[:16] == 0).all() and (got[20:] == 0).all()
+        assert abs(float(cache.scales[0, 1, 0, 0]) - 1 / 127) <= 2.0 ** -20 / 127
+
+
+def test_threads_on_one_stream():
+    """Reads of two threads on one stream, of sizes that grow its scratch."""
+    import threading
+
+    held = cached(torch.float8_e4m3fn, 16, 1, 5000, 2, 64)
+    g = torch.Generator().manual_seed(13)
+    calls = []
+    for n in range(2):
+        q = torch.randn(1, 3 + n, 8, 64, generator=g).to(torch.bfloat16).to(DEV)
+        ids = torch.randint(0, 5000, (1, 3 + n, 4000), generator=g).to(torch.int32).to(DEV)
+        lens = torch.full((1, 3 + n), 4000 - n, dtype=torch.int32, device=DEV)
+        calls.append((q, ids, lens, pipeline.byte_read(q, held, ids, lens)))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(q, ids, lens, want):
+        for _ in range(50):
+            if not torch.equal(pipeline.byte_read(q, held, ids, lens), want):
+                bad.append(1)
+
+    threads = [threading.Thread(target=work, args=c) for c in calls]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad
+
+
 def test_append_with_bad_slots():
     """Blocks whose slot is missing, past the pool, negative or no multiple of the block are dropped; so are
     rows of a slot table that does not have them."""
