@@ -7,7 +7,11 @@
 // and every lane divides, rounds and stores. The block belongs to one workgroup, so its scale and the codes that
 // were there before are read and rewritten with no atomics on memory. The sines of the tile's tokens are taken once
 // for all heads of the workgroup. The rows of q, if any, go through workgroups of the same launch.
-// Memory bounds the large calls (16 bits read, 8 written), the launch and two memory round trips the small ones.
+// 32768 bf16 tokens of 32 + 8 + 8 heads of 128 (738 MB): 163 us, 4.5 TB/s; K and V alone (201 MB) take 73, bound by
+// the vector unit and each head's barrier. 32 decode tokens: 8 us, the launch and four round trips to memory (start,
+// slot, the block's old scale, K and V beside them).
+//
+// byte_values_kernel copies: codes in, numbers out, 8 a lane. A whole cache of 32768 tokens (201 MB): 34 us, 5.9 TB/s.
 #include <math.h>
 
 #include <algorithm>
