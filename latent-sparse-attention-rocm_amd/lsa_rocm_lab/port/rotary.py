@@ -164,6 +164,8 @@ def rotate(
             positions = positions.contiguous()
         stride = positions.stride(0) if positions.dim() == 2 and B > 1 else 0
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if Hq == 0 and k is not None and k.numel():  # the keys alone
+        return q_out, rotate(k, None, positions, frequencies, k_weight, None, eps, interleaved, magnitude)[0]
     k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     if q.numel() == 0:
         return q_out, k_out

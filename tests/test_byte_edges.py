@@ -1,0 +1,22 @@
+"""Calls of rotate, byte_append and byte_read that are all edge, as far as the host goes: nothing is launched."""
+
+import pytest
+import torch
+
+from lsa_rocm_lab.port import pipeline
+from test_serving_memory import calls, fake, host  # noqa: F401 (fixtures)
+
+
+def test_rotate_of_keys_alone(calls):
+    """No query heads: the keys are normed and rotated all the same."""
+    q, k = fake(torch.ones(2, 3, 0, 64)), fake(torch.ones(2, 3, 2, 64))
+    pos, freq, w = fake(torch.arange(3)), fake(torch.ones(32)), fake(torch.ones(64))
+    got = pipeline.rotate(q, k, pos, freq, k_weight=w)
+    assert got[0].shape == q.shape and got[1].shape == k.shape
+    (name, args), = calls
+    assert name == "lsa_rotate" and args[0] == k.data_ptr() and args[5:8] == (2, 0, 64) and args[-3] == got[1].data_ptr()
+    for empty in ((q, None), (q, fake(torch.ones(2, 3, 0, 64))), (fake(torch.ones(0, 3, 4, 64)), fake(torch.ones(0, 3, 2, 64)))):
+        pipeline.rotate(*empty, pos, freq)
+    assert len(calls) == 1
+    with pytest.raises(ValueError, match="norm weights"):
+        pipeline.rotate(q, k, pos, freq, q_weight=fake(torch.ones(32)))
