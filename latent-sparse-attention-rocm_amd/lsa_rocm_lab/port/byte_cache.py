@@ -123,6 +123,8 @@ def byte_append(
             not (_apart(k8) and _apart(v8)) or _meets_twin(k8, v8)):
         raise ValueError("byte_append: the cache's codes must each have a place of their own")
     B, T, Hkv, D = k.shape
+    if Hkv < 1:
+        raise ValueError(f"byte_append: k and v of a kv-head or more, got {tuple(k.shape)}")
     if q is not None and (q.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != D):
         raise ValueError(f"byte_append: q [{B}, {T}, Hq, {D}], got {tuple(q.shape)}")
     if held.caches != (B if slot_table is None else 1):

@@ -20,3 +20,13 @@ def test_rotate_of_keys_alone(calls):
     assert len(calls) == 1
     with pytest.raises(ValueError, match="norm weights"):
         pipeline.rotate(q, k, pos, freq, q_weight=fake(torch.ones(32)))
+
+
+def test_append_without_kv_heads_is_refused(calls):
+    """A cache of no kv-heads takes nothing, and q is not handed back unwritten."""
+    held = pipeline.ByteCache(*(fake(torch.zeros(2, 32, 0, 64, dtype=torch.int8)) for _ in range(2)),
+                              fake(torch.zeros(2, 2, 0, 2)), 16)
+    kv, starts = fake(torch.ones(2, 3, 0, 64)), fake(torch.zeros(2, dtype=torch.int32))
+    with pytest.raises(ValueError, match="kv-head"):
+        pipeline.byte_append(held, kv, kv, starts, q=fake(torch.ones(2, 3, 4, 64)))
+    assert not calls
