@@ -557,13 +557,14 @@ typedef struct lsa_byte_cache {
  * the cache at positions starts[b] + n, k normed and rotated (turn's k_weight), and, where q [B, T, Hq, D] is given,
  * q_out [B, T, Hq, D] (dense), normed and rotated, zeros behind a row's length. Position p is cache row p, or, with
  * a slot map, that of its block's first position (a multiple of block; slots->rows [B]) plus its offset in the
- * block. Positions outside the cache, the map or the pool are dropped, and so is a block whose slot is no multiple
- * of block. A block that is written to gets the scale max(its own where it holds positions before starts[b], its
- * new tokens' largest magnitude / M, 2^-100), M = 127 or 448; a new token's code is value / scale, rounded to
- * nearest even, and where the scale grew the block's earlier codes are rescaled and rounded again. What it held
- * from starts[b] on counts for nothing. A NaN has no part in the scale and is held as e4m3's NaN or int8's 0, an
- * infinity as the largest code, neither in the scale. No block may be written to twice in a call. Under 2^24 tokens. No counterpart in the
- * reference. */
+ * block. Positions outside the cache, the map or the pool are dropped, and so is a block of positions whose slots (as
+ * far as the map goes) are not `block` rows in order from a multiple of block on; those behind its new tokens may also
+ * name no row of the pool. A block that is written to gets the scale max(its own where it holds positions before
+ * starts[b], its new tokens' largest magnitude / M, 2^-100), M = 127 or 448; a new token's code is value / scale,
+ * rounded to nearest even, and where the scale grew the block's earlier codes are rescaled and rounded again. What it
+ * held from starts[b] on counts for nothing. NaN and infinities have no part in the scale: a NaN is held as e4m3's NaN
+ * or int8's 0, an infinity as the largest code. No block may be written to twice in a call. Under 2^24 tokens. No
+ * counterpart in the reference. */
 int lsa_byte_append(const lsa_byte_cache* cache, const void* k, const void* v, const void* q, int dtype, int64_t B,
                     int64_t T, int32_t Hq, int32_t Hkv, int32_t D, int64_t k_batch_stride, int64_t k_token_stride,
                     int64_t k_head_stride, int64_t v_batch_stride, int64_t v_token_stride, int64_t v_head_stride,

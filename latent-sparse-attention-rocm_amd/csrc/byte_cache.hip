@@ -103,7 +103,7 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_append_kernel(AppendArgs a) {
   const int64_t from = start > p0 ? start : p0;  // the tile's new positions: [from, to)
   const int64_t to = end < p0 + kTile ? end : p0 + kTile;
   if (from >= to) return;
-  const int shift = a.c.block_shift, block = 1 << shift, blocks = kTile >> shift;
+  const int shift = a.c.block_shift, block = 1 << shift;
   const int lo = (int)(from - p0), hi = (int)(to - p0);
   const int begin = lo >> shift << shift;  // the first written block's first token
   const int h0 = part * a.heads, h1 = min(h0 + a.heads, a.Hkv), units = 2 * (h1 - h0);
@@ -131,16 +131,29 @@ __global__ __launch_bounds__(LSA_BLOCK) void byte_append_kernel(AppendArgs a) {
   };
   fetch(0);
   float* scales = a.c.scales + (b * a.c.scale_sb) * 2;
-  auto row_of = [&](int blk) {  // the cache row of the tile's block blk, or -1
-    const int64_t p = p0 + (blk << shift);
-    int64_t row = p;
-    if (map.row) row = p < map.width ? map.row[p] : -1;
+  auto usable = [&](int64_t row) {  // a block's first slot, or -1
     return row < 0 || row >= a.c.tokens || (row & (block - 1)) ? -1 : (int32_t)row;
   };
-  if (tid < blocks) block_row[tid] = row_of(tid);
+  // a wave, a position a lane: a block is written to where its slots are a whole block of the pool (those behind the
+  // new tokens may name no row yet)
+  if (tid < kTile) {
+    const int off = tid & (block - 1);
+    const int64_t p = p0 + tid;
+    int64_t row = p;
+    bool whole = true;
+    if (map.row) {
+      const int32_t slot = p < map.width ? map.row[p] : -1;
+      const int64_t first_slot = __shfl(slot, tid - off);
+      row = slot;
+      whole = p >= map.width || row == first_slot + off || (tid >= hi && (row < 0 || row >= a.c.tokens));
+    }
+    const uint64_t bad = __ballot(!whole) >> (tid - off) << (kTile - block);  // of this lane's block
+    if (off == 0) block_row[tid >> shift] = bad ? -1 : usable(row);
+  }
   if (tid >= kTile && tid < kTile + units) {
     const int u = tid - kTile;
-    const int32_t row = begin < lo ? row_of(begin >> shift) : -1;
+    const int64_t p = p0 + begin;
+    const int32_t row = begin < lo ? usable(!map.row ? p : (p < map.width ? map.row[p] : -1)) : -1;
     before[u] = row < 0 ? 0.0f : scales[((int64_t)(row >> shift) * a.Hkv + h0 + (u >> 1)) * 2 + (u & 1)];
   }
   for (int i = tid; i < 3 * kTile; i += LSA_BLOCK) (&most[0][0])[i] = 0u;

@@ -26,7 +26,8 @@ _CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 class ByteCache:
     """Keys and values in 8 bits: row t of kv-head h stands for ``code * scale``, with the scale of
     the ``block`` tokens that t is among. A pool that is read through slot tables is one batch row;
-    its pages are multiples of ``block`` (with ``block`` 1 any slot table serves)."""
+    any table serves to read it. To be written through one its pages are multiples of ``block``: a table
+    that ``evict_slots`` has made, whose slots move one by one, is appended to with ``block`` 1."""
 
     k: torch.Tensor  # [B or 1, T, Hkv, D] int8 or float8_e4m3fn
     v: torch.Tensor
@@ -96,10 +97,13 @@ def byte_append(
     k, v [B, T, Hkv, D] (fp32, bf16 or fp16): the first ``lengths[b]`` (default T) tokens of row b go to
     positions ``starts[b]``, ``starts[b] + 1``, ..; k is normed (with ``k_weight``) and rotated (with
     ``frequencies``) first, as ``rotate`` does, and so is q [B, T, Hq, D] (zeros behind a row's
-    length). ``cache`` has B rows, or is a pool [1, rows, Hkv, D] that ``slot_table`` [n, width] and
+    length); where a token's position is not its place in the cache (after an eviction, say), ``rotate``
+    first and give no ``frequencies``. ``cache`` has B rows, or is a pool [1, rows, Hkv, D] that ``slot_table`` [n, width] and
     ``slot_rows`` [B] (as in the selects) map positions to, whole blocks at a time. Positions outside
-    are dropped, and so is a block whose slot is not a multiple of ``cache.block``; dropped tokens have no
-    part in a scale. No block may be written to twice in a call (by two rows, or two entries of a table).
+    are dropped, and so are new tokens of a block of positions whose slots are not a block of the pool:
+    ``block`` rows in order from a multiple of it on (slots behind the new tokens may also name no row
+    of the pool). Dropped tokens change no row and have no part in a scale. No block may be written to
+    twice in a call (by two rows, or two entries of a table).
 
     A block's scale is its largest magnitude over 127 (int8) or 448 (e4m3), at least 2^-100, and
     codes are rounded to nearest. Tokens before ``starts[b]`` in the first block stay: where its scale

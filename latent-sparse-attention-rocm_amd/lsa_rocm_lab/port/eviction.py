@@ -287,7 +287,8 @@ def evict_slots(
     order, then the ones it gave up, in theirs (the sequence's next tokens may take them, or an
     allocator), then what was behind its length; the new lengths [R] and the kept positions
     [R, budget] (-1 past the new length), int32. The masses stay with their cache rows: clear
-    those that are given to a new token.
+    those that are given to a new token. (An 8-bit cache shares a scale among the rows of a block, so
+    ``byte_append`` writes through such a table row by row only with ``block`` 1.)
     """
     device = one_device("evict_slots", slot_table, mass)
     if slot_table.dim() != 2 or slot_table.shape[1] < 1:

@@ -19,3 +19,95 @@ def test_rotate_of_keys_alone(interleaved):
     want = pipeline.rotate(q, k, *rest, interleaved=interleaved)[1]
     none, got = pipeline.rotate(q[:, :, :0], k, *rest, interleaved=interleaved)
     assert none.shape == (2, 5, 0, 64) and torch.equal(got, want)
+
+
+CODES = [torch.int8, torch.float8_e4m3fn]
+
+
+def held(code, block, rows, seed=0, batch=1):
+    """A cache whose rows hold numbers of N(0, 1), and those numbers as it holds them."""
+    g = torch.Generator().manual_seed(seed)
+    cache = pipeline.byte_cache(batch, rows, 2, 64, block, code, DEV)
+    kv = torch.randn(2, batch, rows, 2, 64, generator=g).to(DEV)
+    pipeline.byte_append(cache, kv[0], kv[1], torch.zeros(batch, dtype=torch.int32, device=DEV),
+                         slot_table=None if batch > 1 else torch.arange(rows, dtype=torch.int32, device=DEV)[None])
+    return cache, pipeline.byte_values(cache, dtype=torch.float32)
+
+
+def slots(*pieces):
+    return torch.cat([torch.arange(a, b) if b >= a else torch.arange(a, b, -1) for a, b in pieces]).to(torch.int32)
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("block,table,start,n", [
+    # the block's first slots are whole, its own first position's is not where the new token goes
+    (16, slots((32, 40), (64, 96)), 8, 3),
+    # aligned where the block begins, another row's in the middle: a new token there, one before it, one behind it
+    (16, slots((16, 24), (90, 98)), 10, 2),
+    (16, slots((16, 20), (90, 94), (24, 32)), 9, 5),
+    (16, slots((16, 24), (90, 98)), 2, 3),
+    # given-up rows at the end of an evicted table: half a block, the other half of it is kept elsewhere
+    (32, slots((0, 32), (64, 80), (96, 112)), 32, 1),
+    (64, slots((64, 128), (0, 32), (33, 65)), 64, 20),
+    # whole slots, in the wrong order
+    (8, slots((23, 15),), 0, 8),
+    (2, slots((1, 3), (5, 3)), 0, 4),
+])
+def test_append_leaves_blocks_that_a_table_does_not_map_whole(code, block, table, start, n):
+    """Slots permuted token by token, as an evicted table's are: where a block of positions is no block of the pool
+    nothing is written, so no other key changes."""
+    cache, before = held(code, block, 128, seed=block)
+    k = 100.0 * torch.randn(1, n, 2, 64, generator=torch.Generator().manual_seed(2)).to(DEV)
+    raw = [x.clone() for x in (cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.scales)]
+    pipeline.byte_append(cache, k, k, torch.tensor([start], dtype=torch.int32, device=DEV), slot_table=table[None].to(DEV))
+    for x, y in zip((cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.scales), raw):
+        assert torch.equal(x, y)
+
+
+def test_append_writes_the_whole_blocks_of_such_a_table():
+    """The blocks beside them are written, and a table that ends inside a block."""
+    cache, before = held(torch.int8, 16, 96)
+    table = slots((80, 96), (3, 19), (32, 48), (64, 70))  # whole, not, whole, whole as far as it goes
+    k = torch.randn(1, 54, 2, 64, generator=torch.Generator().manual_seed(2)).to(DEV)
+    pipeline.byte_append(cache, k, -k, torch.zeros(1, dtype=torch.int32, device=DEV), slot_table=table[None].to(DEV))
+    got = pipeline.byte_values(cache, dtype=torch.float32)
+    lim = (0.5 + 2.0 ** -9) * cache.scales.repeat_interleave(16, 1)
+    rest = torch.ones(96, dtype=torch.bool, device=DEV)
+    for at, row, m in ((0, 80, 16), (32, 32, 16), (48, 64, 6)):
+        rest[row:row + 16] = False
+        for i, x in enumerate((k, -k)):
+            assert ((got[i][0, row:row + m] - x[0, at:at + m]).abs() <= lim[0, row:row + m, :, i, None]).all()
+    assert all(torch.equal(x[0, rest], y[0, rest]) for x, y in zip(got, before))
+
+
+def test_append_through_a_table_that_is_filled_token_by_token():
+    """Entries behind the new tokens that name no row yet (negative, past the pool) are no matter."""
+    got = []
+    for rest in (None, -1, 64, (1 << 31) - 1, -(1 << 31)):
+        cache = held(torch.int8, 16, 64)[0]
+        table = slots((48, 64), (16, 32))
+        k = torch.randn(1, 9, 2, 64, generator=torch.Generator().manual_seed(2)).to(DEV)
+        for t in range(9):
+            now = table.clone()
+            if rest is not None:
+                now[13 + t + 1:] = rest
+            pipeline.byte_append(cache, k[:, t:t + 1], -k[:, t:t + 1], torch.tensor([13 + t], dtype=torch.int32, device=DEV),
+                                 slot_table=now[None].to(DEV))
+        got.append((cache.k, cache.v, cache.scales))
+    values = pipeline.byte_values(cache, table[None].to(DEV), dtype=torch.float32)[0]
+    assert ((values[0, 21] - k[0, 8]).abs() <= (0.5 + 2.0 ** -9) * cache.scales[0, 1, :, 0, None]).all()  # the last one
+    assert all(torch.equal(x, y) for other in got[1:] for x, y in zip(other, got[0]))
+
+
+def test_append_through_an_evicted_table_of_single_rows():
+    """With a block a row any table serves: the new tokens land in the rows given up, the kept ones stay."""
+    cache, before = held(torch.int8, 1, 64)
+    mass = torch.rand(1, 2, 64, generator=torch.Generator().manual_seed(5)).to(DEV)
+    table, lens, kept = pipeline.evict_slots(torch.arange(64, dtype=torch.int32, device=DEV)[None], mass, 40, window=4)
+    k = 100.0 * torch.randn(1, 5, 2, 64, generator=torch.Generator().manual_seed(2)).to(DEV)
+    pipeline.byte_append(cache, k, k, lens, slot_table=table)
+    got = pipeline.byte_values(cache, table, lens + 5, dtype=torch.float32)
+    at = kept[0].long()
+    for i in range(2):
+        assert torch.equal(got[i][0, :40], before[i][0, at])
+        assert ((got[i][0, 40:45] - k[0]).abs() <= (0.5 + 2.0 ** -9) * cache.scales[0, table[0, 40:45].long(), :, i, None]).all()
