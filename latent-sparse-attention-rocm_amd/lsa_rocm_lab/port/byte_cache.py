@@ -191,6 +191,7 @@ def byte_values(cache: ByteCache, rows: torch.Tensor | None = None, lengths: tor
 
 
 _READ_SPLITS = 64
+_SLAB_BYTES = 256 << 20  # partials held at once (more query rows go through in slabs)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -202,6 +203,11 @@ def _read_splits(units: int, width: int) -> int:
     2: 56, 4: 41.4, 8: 46; 128 of 32768 4: 196, 16: 173, 32: 168."""
     few = -(-512 // units) if units < 256 else 1
     return max(1, min(_READ_SPLITS, width // 192, max(few, width // 1500), (1 << 23) // units))
+
+
+def _even(n: int, most: int) -> int:
+    """The size of even pieces of n, of at most ``most``."""
+    return -(-n // -(-n // most))
 
 
 def byte_read(q: torch.Tensor, cache: ByteCache, read_lists: torch.Tensor, lengths: torch.Tensor,
@@ -229,12 +235,33 @@ def byte_read(q: torch.Tensor, cache: ByteCache, read_lists: torch.Tensor, lengt
     if out.numel() == 0:
         return out
     q = aligned(q)
-    units = B * Tq * Hkv * -(-Hq // Hkv // 16)
+    rows = B * Tq
+    units = rows * Hkv * -(-Hq // Hkv // 16)
     splits = _read_splits(units, W)
-    nbytes = _abi.shape_size("lsa_byte_read_scratch_bytes", B * Tq, Hq, Hkv, D, splits)
+    nbytes = _abi.shape_size("lsa_byte_read_scratch_bytes", rows, Hq, Hkv, D, splits)
+    many, step = B, Tq  # batch rows at once, query rows of each
+    if nbytes > _SLAB_BYTES and rows > 1:
+        if held.caches == 1:  # all of the rows are of one cache
+            B, Tq, many = 1, rows, 1
+        most = max(1, _SLAB_BYTES // (nbytes // rows))
+        many, step = (_even(B, most // Tq), Tq) if Tq <= most else (1, _even(Tq, most))
+        nbytes = nbytes // rows * many * step
+    lists = Hkv if per_head else 1
+    scale = float(D ** -0.5 if scale is None else scale)
     with launch_device(device):
-        ws, counters, stream = _abi.call_memory(device, "byte_read", nbytes, units if nbytes else 0)
-        _abi.call_in_order("lsa_byte_read", q.data_ptr(), ctypes.addressof(held), dt, B, Tq, Hq, Hkv, D, ids.data_ptr(),
-                           lens.data_ptr(), W, 1 if per_head else 0, float(D ** -0.5 if scale is None else scale), splits,
-                           _abi.ptr(counters), _abi.ptr(ws), nbytes, out.data_ptr(), stream)
+        ws, counters, stream = _abi.call_memory(device, "byte_read", nbytes,
+                                                many * step * units // rows if nbytes else 0)
+        for b in range(0, B, many):
+            m = min(many, B - b)
+            part = held
+            if m < B:  # caches b .. b + m
+                k, v, scales = (x[b:b + m].data_ptr() for x in (cache.k, cache.v, cache.scales))
+                part = _Cache(k, v, scales, held.code, held.block, m, held.tokens, held.batch_stride, held.token_stride,
+                              held.head_stride)
+            for t in range(0, Tq, step):
+                at, n = b * Tq + t, min(step, Tq - t)
+                _abi.call_in_order("lsa_byte_read", q.data_ptr() + at * Hq * D * q.element_size(), ctypes.addressof(part), dt,
+                                   m, n, Hq, Hkv, D, ids.data_ptr() + 4 * at * lists * W, lens.data_ptr() + 4 * at * lists,
+                                   W, 1 if per_head else 0, scale, splits, _abi.ptr(counters), _abi.ptr(ws), nbytes,
+                                   out.data_ptr() + at * Hq * D * q.element_size(), stream)
     return out

@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from lsa_rocm_lab.port import byte_cache as module
 from lsa_rocm_lab.port import pipeline
 
 pytestmark = pytest.mark.gpu
@@ -111,3 +112,38 @@ def test_append_through_an_evicted_table_of_single_rows():
     for i in range(2):
         assert torch.equal(got[i][0, :40], before[i][0, at])
         assert ((got[i][0, 40:45] - k[0]).abs() <= (0.5 + 2.0 ** -9) * cache.scales[0, table[0, 40:45].long(), :, i, None]).all()
+
+
+@pytest.mark.parametrize("B,Tq,per_head,pool,dtype", [
+    (1, 50, False, True, torch.bfloat16), (3, 7, True, True, torch.float16), (5, 4, False, False, torch.bfloat16),
+    (3, 20, True, False, torch.float32), (37, 1, True, False, torch.bfloat16),
+])
+def test_read_in_slabs(monkeypatch, B, Tq, per_head, pool, dtype):
+    """Query rows that go through in slabs: the bits of one piece, eagerly and in a graph."""
+    g = torch.Generator().manual_seed(B)
+    rows, W = 3000, 1300
+    cache, _ = held(torch.int8, 16, rows, batch=1 if pool else B)
+    q = torch.randn(B, Tq, 6, 64, generator=g).to(dtype).to(DEV)
+    lead = (B, Tq, 2) if per_head else (B, Tq)
+    ids = torch.randint(-1, rows, (*lead, W), generator=g).to(torch.int32).to(DEV)
+    lens = torch.randint(0, W + 1, lead, generator=g).to(torch.int32).to(DEV)
+    want = pipeline.byte_read(q, cache, ids, lens)
+    one = module._abi.size("lsa_byte_read_scratch_bytes", 1, 6, 2, 64, module._read_splits(B * Tq * 2, W))
+    assert one > 0
+    for slab in (1, 3 * one, 11 * one + 5, (B * Tq - 1) * one):
+        monkeypatch.setattr(module, "_SLAB_BYTES", slab)
+        assert torch.equal(pipeline.byte_read(q, cache, ids, lens), want)
+    monkeypatch.setattr(module, "_SLAB_BYTES", 3 * one)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream), torch.cuda.graph(graph, stream=stream):
+        out = pipeline.byte_read(q, cache, ids, lens)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        q.mul_(-1.0)
+        graph.replay()
+        monkeypatch.setattr(module, "_SLAB_BYTES", 1 << 28)
+        eager = pipeline.byte_read(q, cache, ids, lens)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
