@@ -197,12 +197,15 @@ _SLAB_BYTES = 256 << 20  # partials held at once (more query rows go through in 
 @functools.lru_cache(maxsize=4096)
 def _read_splits(units: int, width: int) -> int:
     """Spans of a list, a workgroup each. 256 units (a CU each) and more read theirs whole, fewer are cut until
-    there are about 512 workgroups, lists of any number past 1500 slots, so that lengths that differ even out;
-    a span has 192 slots or more, below which its start costs more than it saves. Measured, us, by spans: 8
-    units of 2816 slots 4: 12.6, 8: 9.4, 14: 9.0, 22: 9.3; 256 of them 1: 30.8, 2: 35.2, 8: 36.4; 160 of 6336
-    2: 56, 4: 41.4, 8: 46; 128 of 32768 4: 196, 16: 173, 32: 168."""
+    there are about 512 workgroups, lists of any number past 1500 slots, so that lengths that differ even out and rows
+    that walk the same keys meet in the caches; a span has 192 slots or more, below which its start costs more
+    than it saves, in whole steps of 128. Measured, us, by spans: 8 units of 2816 slots 4: 12.6, 8: 9.4, 11: 9.0,
+    22: 9.3; 256 of them 1: 30.8, 2: 35.2, 8: 36.4; 160 of 6336 2: 56, 4: 41.4, 8: 46; 128 of 32768 4: 196, 16: 173,
+    32: 168; 16384 of 4608 1: 2492, 3: 2417, 8: 2463; 32768 of 32768 1: 33100, 4: 26800, 16: 22800, 20: 23400."""
     few = -(-512 // units) if units < 256 else 1
-    return max(1, min(_READ_SPLITS, width // 192, max(few, width // 1500), (1 << 23) // units))
+    splits = max(1, min(_READ_SPLITS, width // 192, max(few, width // 1500), (1 << 23) // units))
+    span = -(-(-(-width // splits)) // 128) * 128
+    return max(1, -(-width // max(span, 1)))
 
 
 def _even(n: int, most: int) -> int:

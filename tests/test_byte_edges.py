@@ -85,3 +85,13 @@ def test_small_reads_are_one_call(calls):
     read_call(32, 1, 32, 8, 128, 4612, True, False)
     read_call(16, 1, 32, 8, 128, 32768, False, True)
     assert [args[3:5] for _, args in calls] == [(32, 1), (16, 1)]
+
+
+def test_every_span_of_a_read_has_slots():
+    """Spans are whole steps of 128 slots; as many are asked for as that leaves."""
+    for units in (1, 8, 31, 160, 255, 256, 1000, 40000, 1 << 22):
+        for width in (0, 1, 191, 192, 384, 577, 1300, 2816, 4612, 6336, 9001, 32768, 131072, 1 << 30):
+            splits = module._read_splits(units, width)
+            span = max(-(-(-(-width // splits)) // 128) * 128, 128)  # as the kernel cuts
+            assert 1 <= splits <= 64 and (splits - 1) * span < max(width, 1)
+    assert module._read_splits(8, 2816) == 11 and module._read_splits(128, 32768) == 20
