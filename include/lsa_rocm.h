@@ -561,7 +561,8 @@ typedef struct lsa_byte_cache {
  * far as the map goes) are not `block` rows in order from a multiple of block on; those behind its new tokens may also
  * name no row of the pool. A block that is written to gets the scale max(its own where it holds positions before
  * starts[b], its new tokens' largest magnitude / M, 2^-100), M = 127 or 448; a new token's code is value / scale,
- * rounded to nearest even, and where the scale grew the block's earlier codes are rescaled and rounded again. What it
+ * rounded to nearest even, and where the scale grew the block's earlier codes are rescaled and rounded again (half a
+ * step at most, each time: a token is off by up to g + 1 half steps where the scale grew g times behind it). What it
  * held from starts[b] on counts for nothing. NaN and infinities have no part in the scale: a NaN is held as e4m3's NaN
  * or int8's 0, an infinity as the largest code. No block may be written to twice in a call. Under 2^24 tokens. No
  * counterpart in the reference. */

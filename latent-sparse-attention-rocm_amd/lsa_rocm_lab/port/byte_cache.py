@@ -107,10 +107,14 @@ def byte_append(
 
     A block's scale is its largest magnitude over 127 (int8) or 448 (e4m3), at least 2^-100, and
     codes are rounded to nearest. Tokens before ``starts[b]`` in the first block stay: where its scale
-    grows, their codes are rescaled and rounded again (by at most half a step of the new scale). What
-    the block held from ``starts[b]`` on is given up, so a row may be taken back by appending at an
-    earlier position. NaN and infinities stay out of the scale; a NaN is held as e4m3's NaN or as 0,
-    an infinity as the largest code.
+    grows, their codes are rescaled and rounded again, by at most half a step. That adds up: a token of a
+    block that is filled token by token is off by up to g + 1 half steps where the scale grew g times
+    behind it. Rows of N(0, 1) grow it 3 to 6 times in 64 tokens, for 1.2 to 1.6 times the error of one
+    append in rms (e4m3 2.0); magnitudes that rise by 3% with every token, less than a code's step, 11
+    times (e4m3 40: the codes stay and their values rise with the scale). With ``block`` 1 a token is
+    rounded once. What the block held from ``starts[b]`` on is given up, so a row may be taken back by
+    appending at an earlier position. NaN and infinities stay out of the scale; a NaN is held as e4m3's
+    NaN or as 0, an infinity as the largest code.
     """
     from lsa_rocm_lab.port.pipeline import _slot_args
 

@@ -147,3 +147,49 @@ def test_read_in_slabs(monkeypatch, B, Tq, per_head, pool, dtype):
         eager = pipeline.byte_read(q, cache, ids, lens)
         torch.cuda.synchronize()
         assert torch.equal(out, eager)
+
+
+@pytest.mark.parametrize("code", CODES)
+def test_block_that_is_filled_token_by_token(code):
+    """Each time its scale grows a block's codes are rounded again. int8: a token written before g growths is off by
+    (g + 1) / 2 steps of the last scale, 2^-9 of a step more each time for the quotient. e4m3: by half a step of the
+    code each time, which is 2^-3 of its power of two (at least 2^-9) and grows with what it is off by already."""
+    B, T, D = 6, 64, 64
+    g = torch.Generator().manual_seed(4)
+    k = torch.randn(B, T, 2, D, generator=g)
+    k[3:] *= 1.03 ** torch.arange(T).view(T, 1, 1)  # many tokens grow the scale
+    k[5] = k[5].abs().clamp(max=1.0) * 1.03 ** torch.arange(T).view(T, 1, 1)  # every token does
+    cache = pipeline.byte_cache(B, T, 2, D, 64, code, DEV)
+    kd = k.to(DEV)
+    scales = []
+    for t in range(T):
+        pipeline.byte_append(cache, kd[:, t:t + 1], kd[:, t:t + 1], torch.full((B,), t, dtype=torch.int32, device=DEV))
+        scales.append(cache.scales[:, 0, :, 0].clone())
+    scales = torch.stack(scales, 1).double().cpu()  # [B, T, 2] after each token
+    assert (scales[:, 1:] >= scales[:, :-1]).all()
+    x, half = k.double(), 0.5 + 2.0 ** -9
+    lim = torch.zeros_like(x)
+    for t in range(T):  # what tokens 0 .. t are off by at most after append t
+        s = scales[:, t, None, :, None]
+        again = torch.ones(B, t + 1, 2, 1, dtype=torch.bool)  # rounded by this append
+        if t:
+            again[:, :t] = (scales[:, t] > scales[:, t - 1])[:, None, :, None]
+        step = s
+        if code == torch.float8_e4m3fn:
+            _, e = torch.frexp((x[:, :t + 1].abs() + lim[:, :t + 1]) / s)
+            step = torch.exp2((e - 4).clamp(-9, 5).double()) * s
+        lim[:, :t + 1] += torch.where(again, half * step, 0.0)
+    grown = (scales[:, 1:] > scales[:, :-1]).sum(1)
+    top = k.abs().amax(-1).cummax(1).values
+    assert torch.equal(grown, (top[:, 1:] > top[:, :-1]).sum(1)) and (grown[5] == T - 1).all()
+    got = pipeline.byte_values(cache, dtype=torch.float32)[0].double().cpu()
+    off = (got - x).abs()
+    assert (off <= lim).all(), f"off by {(off / lim).max():.2f} of the bound"
+    last = scales[:, -1, None, :, None]
+    print(f"{code}: grown {grown.tolist()}, off by {(off / last).amax((1, 2, 3)).tolist()} of the last scale, "
+          f"rms {((off / last).square().mean((1, 2, 3)).sqrt() / (1 / 12) ** 0.5).tolist()} of one rounding's")
+    bulk = pipeline.byte_cache(B, T, 2, D, 64, code, DEV)
+    pipeline.byte_append(bulk, kd, kd, torch.zeros(B, dtype=torch.int32, device=DEV))
+    assert torch.equal(bulk.scales, cache.scales)
+    print("in one append: rms", [float(((pipeline.byte_values(bulk, dtype=torch.float32)[0].double().cpu() - x) / last)[b]
+                                       .square().mean().sqrt() / (1 / 12) ** 0.5) for b in range(B)])
