@@ -1,5 +1,7 @@
 """Calls of rotate and of the 8-bit cache that are all edge, vs 64 bits or the ordinary call."""
 
+import math
+
 import pytest
 import torch
 
@@ -193,3 +195,93 @@ def test_block_that_is_filled_token_by_token(code):
     assert torch.equal(bulk.scales, cache.scales)
     print("in one append: rms", [float(((pipeline.byte_values(bulk, dtype=torch.float32)[0].double().cpu() - x) / last)[b]
                                        .square().mean().sqrt() / (1 / 12) ** 0.5) for b in range(B)])
+
+
+@pytest.mark.parametrize("code", CODES)
+def test_a_weight_times_a_scale_keeps_24_bits_for_fp32_rows(code):
+    """One key weighs 1, so the output is its code times V's scale: exact in three parts of 8 bits, whose products
+    add up in two roundings of 2^-24. Two parts would be off by up to 2^-17."""
+    cache, _ = held(code, 1, 500)
+    cache.scales.copy_(0.5 + torch.rand(cache.scales.shape, generator=torch.Generator().manual_seed(8)))
+    q = torch.randn(1, 500, 4, 64, generator=torch.Generator().manual_seed(9)).to(DEV)
+    ids = torch.arange(500, dtype=torch.int32, device=DEV).view(1, 500, 1)
+    got = pipeline.byte_read(q, cache, ids, torch.ones(1, 500, dtype=torch.int32, device=DEV))
+    want = (cache.v.float().double() * cache.scales[..., 1:].double()).repeat_interleave(2, 2)
+    assert ((got.double() - want).abs() <= 2.0 ** -22 * want.abs()).all()
+
+
+@pytest.mark.parametrize("dtype,low", [(torch.float32, 2.0 ** -18), (torch.float16, 2.0 ** -9)])
+def test_q_enters_exactly(dtype, low):
+    """q's elements differ in their last part of 8 bits alone: 1 + 2^-9 + 2^-18 and -(1 + 2^-9 - 2^-18) in fp32, 1 + 2^-9
+    and -(1 - 2^-9) in fp16. Against keys of 64 and of -64 every product and every sum of them is a multiple of 2^-12
+    under 2^13: exact. The score is 64 low of a product that is 0 without that part; its exponential, the weights'
+    sum, the products with V (1 and -1) and the division take eight roundings or so of 2^-24."""
+    D = 128
+    a = 1.0 + (2.0 ** -9 if dtype == torch.float32 else 0.0)
+    row = torch.tensor([a + low, -(a - low)], dtype=torch.float64).repeat(D // 2)
+    q = row.to(dtype).view(1, 1, 1, D)
+    assert torch.equal(q.double().view(-1), row)
+    signs = torch.tensor([64, -64], dtype=torch.int8).view(1, 2, 1, 1).expand(1, 2, 1, D).contiguous().to(DEV)
+    scales = torch.tensor([1.0, 2.0 ** -6]).expand(1, 2, 1, 2).contiguous().to(DEV)
+    cache = pipeline.ByteCache(signs, signs.clone(), scales, 1)
+    ids = torch.tensor([0, 1], dtype=torch.int32, device=DEV).view(1, 1, 2)
+    got = pipeline.byte_read(q.to(DEV), cache, ids, torch.tensor([[2]], device=DEV), scale=2.0 ** -7).double().cpu()
+    want = math.tanh(64 * low)
+    assert ((got - want).abs() <= torch.finfo(dtype).eps / 2 * want + 2.0 ** -20).all() and want > 2.0 ** -12.1
+
+
+def test_read_of_scores_in_the_thousands():
+    """By the scores' own error: a matrix instruction adds 32 exact products (and what came before) with four roundings
+    of 2^-24 of their magnitudes or fewer, D / 32 of them follow each other, and the scale takes two more. A weight is
+    then off by e^(2 d), the output by 2 d of the largest value; 2^-15 of it are the weights' parts and the sums."""
+    D, n = 64, 80
+    cache, _ = held(torch.int8, 16, 100, seed=3)
+    g = torch.Generator().manual_seed(6)
+    q = torch.randn(1, 9, 4, D, generator=g).to(torch.bfloat16)
+    ids = torch.randint(0, 100, (1, 9, n), generator=g).to(torch.int32)
+    k, v = (c.float().double().cpu() * cache.scales[..., i, None].double().cpu().repeat_interleave(16, 1)[:, :100]
+            for i, c in enumerate((cache.k, cache.v)))
+    got = pipeline.byte_read(q.to(DEV), cache, ids.to(DEV), torch.full((1, 9), n, device=DEV), scale=100.0).double().cpu()
+    for t in range(9):
+        for h in range(4):
+            x, kk, vv = q[0, t, h].double(), k[0, ids[0, t].long(), h // 2], v[0, ids[0, t].long(), h // 2]
+            s = 100.0 * kk @ x
+            assert s.abs().max() > 1000
+            d = (D / 32 * 2.0 ** -22 + 2.0 ** -23) * 100.0 * (kk.abs() @ x.abs()).max()
+            want = torch.softmax(s, 0) @ vv
+            lim = 2.0 ** -8 * want.abs() + (torch.expm1(2 * d) + 2.0 ** -15) * vv.abs().max()
+            assert ((got[0, t, h] - want).abs() <= lim).all()
+
+
+def test_threads_whose_reads_grow_the_scratch():
+    """Four threads on one stream that has none yet, each with reads of growing size: the results of another stream."""
+    import threading
+
+    cache, _ = held(torch.float8_e4m3fn, 16, 5000)
+    g = torch.Generator().manual_seed(13)
+    calls = []
+    for n in range(4):
+        for rows in (1, 3, 17, 60, 150):
+            q = torch.randn(1, rows + n, 8, 64, generator=g).to(torch.bfloat16).to(DEV)
+            ids = torch.randint(0, 5000, (1, rows + n, 4000), generator=g).to(torch.int32).to(DEV)
+            lens = torch.full((1, rows + n), 4000 - n, dtype=torch.int32, device=DEV)
+            calls.append((n, q, ids, lens, pipeline.byte_read(q, cache, ids, lens)))
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    for kind in (module._abi.Workspace, module._abi.Counters):
+        kind._buffers.pop((q.device.index, stream.cuda_stream, "byte_read"), None)
+    bad, start = [], threading.Barrier(4)
+
+    def work(me):
+        start.wait()
+        with torch.cuda.stream(stream):
+            for n, q, ids, lens, want in calls:
+                if n == me and not torch.equal(pipeline.byte_read(q, cache, ids, lens), want):
+                    bad.append(me)
+
+    before = len(module._abi.Workspace._retired)
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    torch.cuda.synchronize()
+    assert not bad and len(module._abi.Workspace._retired) > before
