@@ -7,9 +7,11 @@
 // and every lane divides, rounds and stores. The block belongs to one workgroup, so its scale and the codes that
 // were there before are read and rewritten with no atomics on memory. The sines of the tile's tokens are taken once
 // for all heads of the workgroup. The rows of q, if any, go through workgroups of the same launch.
-// 32768 bf16 tokens of 32 + 8 + 8 heads of 128 (738 MB): 163 us, 4.5 TB/s; K and V alone (201 MB) take 73, bound by
-// the vector unit and each head's barrier. 32 decode tokens: 8 us, the launch and four round trips to memory (start,
-// slot, the block's old scale, K and V beside them).
+// 32768 bf16 tokens of 32 + 8 + 8 heads of 128 (738 MB): 151 us a call among others, 4.9 TB/s; K and V alone (201 MB)
+// take 69: 513 workgroups, two a CU, each with 16 units (K or V of a head) one after the other and a barrier a unit.
+// Five pieces of 300 tokens: 16 us (13 without q): a head a workgroup there, so that a tile's sines are taken eight
+// times over, in front of two units. 32 decode tokens: 8 us, the launch and four round trips to memory (start, slot,
+// the block's old scale, K and V beside them).
 //
 // byte_values_kernel copies: codes in, numbers out, 8 a lane. A whole cache of 32768 tokens (201 MB): 34 us, 5.9 TB/s.
 #include <math.h>
@@ -384,7 +386,7 @@ extern "C" int lsa_byte_append(const lsa_byte_cache* cache, const void* k, const
   r.q_sb = q_batch_stride; r.q_st = q_token_stride; r.q_sh = q_head_stride;
   r.Hq = Hq; r.T = (int)T; r.tokens = (int)(B * T); r.turn = t;
   // q in the same launch: its workgroups wait for memory while those of K and V wait for barriers and each other
-  // (32768 tokens: 107 us for q and 73 for K and V, one after the other). Its outputs go past the caches as rotate's.
+  // (32768 tokens: 151 us, and 96 for q and 69 for K and V one after the other). Its outputs go past the caches as rotate's.
   a.q_mode = B * T < 1024 ? kFew : (B * T * Hq * D * e > (64 << 20) ? kStream : kMany);
   const int rows = 256 / (D / 8);
   r.heads = a.q_mode == kFew && B * T * ((Hq + rows - 1) / rows) <= 512 ? rows : std::max(Hq, 1);

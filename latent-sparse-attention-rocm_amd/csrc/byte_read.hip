@@ -7,17 +7,18 @@
 // from memory straight to LDS, so that what is in flight takes no registers. A wave has one buffer each of K and V
 // and fills it again as soon as its product is through: K of the next tile loads while the softmax and V's product
 // run, V while it waits for K (8 KB a wave in flight at head dim 128, four waves a SIMD). Both products are matrix
-// instructions in bf16, whose 8 bits of mantissa hold every code exactly: S^T = K Q^T, and O^T += V^T P^T with V's columns by the transposing LDS
-// read. q enters exactly too: bf16 as it is, fp16 in two parts, fp32 in three. A weight times V's scale goes in as
+// instructions in bf16, whose 8 bits of mantissa hold every code exactly: S^T = K Q^T, and O^T += V^T P^T with V's
+// columns by the transposing LDS read. q enters exactly too: bf16 as it is, fp16 in two parts, fp32 in three. A weight times V's scale goes in as
 // two parts (16 bits), for fp32 rows as three, so that rounding it costs nothing beside the output's own rounding.
 // The keys of a tile are dealt to the rows of S^T so that a lane's 8 scores are those of the 8 keys whose V codes
 // it holds (keys 8 row .. + 8): weights go from one product to the other in their registers.
 //
 // What bounds it: memory. Measured at bf16, head dim 128, 32 query heads on 8: 32 lists of about 2048 keys a kv-head
 // (134 MB, spans of 64 keys at 128 bytes a key) 29 us, where the loads alone take 28; sixteen whole caches of about
-// 24600 keys (805 MB) 168 us, 4.8 TB/s, and no less with the products left out (a plain read of as much in one piece
-// reaches 6.2); one list of 2048, 9.2 us: the launch, five round trips to memory and the join. With two buffers and
-// two waves a SIMD these took 32, 163 and 9.0 us.
+// 24600 keys (805 MB) 170 us a call among others, 4.7 TB/s, and no less with the products left out (a plain read of as
+// much in one piece reaches 6.2); one list of 2048, 9.3 us: the launch, five round trips to memory and the join. One
+// buffer and four waves a SIMD against two and two, measured together: 29 for 32, 168 for 163, 9.2 for 9.0. What a
+// decode batch reads, many short spans, gains a tenth, the others lose 3%: one form for all of them.
 //
 // An id outside the cache reads zeros in place of codes and scales and weighs nothing, so what the cache holds
 // elsewhere never enters. Spans of a list leave fp32 partials (m, l, o) that the last of them to finish joins, in
