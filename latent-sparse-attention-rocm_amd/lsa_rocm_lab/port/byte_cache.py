@@ -246,18 +246,27 @@ def byte_read(q: torch.Tensor, cache: ByteCache, read_lists: torch.Tensor, lengt
     units = rows * Hkv * -(-Hq // Hkv // 16)
     splits = _read_splits(units, W)
     nbytes = _abi.shape_size("lsa_byte_read_scratch_bytes", rows, Hq, Hkv, D, splits)
-    many, step = B, Tq  # batch rows at once, query rows of each
-    if nbytes > _SLAB_BYTES and rows > 1:
+    slabs = nbytes > _SLAB_BYTES and rows > 1
+    if slabs:
         if held.caches == 1:  # all of the rows are of one cache
-            B, Tq, many = 1, rows, 1
+            B, Tq = 1, rows
         most = max(1, _SLAB_BYTES // (nbytes // rows))
-        many, step = (_even(B, most // Tq), Tq) if Tq <= most else (1, _even(Tq, most))
-        nbytes = nbytes // rows * many * step
-    lists = Hkv if per_head else 1
+        many, step = (_even(B, most // Tq), Tq) if Tq <= most else (1, _even(Tq, most))  # batch rows, query rows of each
+        nbytes, units = nbytes // rows * many * step, units // rows * many * step
     scale = float(D ** -0.5 if scale is None else scale)
+    q_at, out_at, ids_at, lens_at = q.data_ptr(), out.data_ptr(), ids.data_ptr(), lens.data_ptr()
     with launch_device(device):
-        ws, counters, stream = _abi.call_memory(device, "byte_read", nbytes,
-                                                many * step * units // rows if nbytes else 0)
+        ws, counters, stream = _abi.call_memory(device, "byte_read", nbytes, units if nbytes else 0)
+
+        def launch(part, m, n, at):  # n query rows of m batch rows, the first of them row `at`
+            first, row = at * Hq * D * q.element_size(), 4 * at * (Hkv if per_head else 1)
+            _abi.call_in_order("lsa_byte_read", q_at + first, ctypes.addressof(part), dt, m, n, Hq, Hkv, D,
+                               ids_at + row * W, lens_at + row, W, 1 if per_head else 0, scale, splits,
+                               _abi.ptr(counters), _abi.ptr(ws), nbytes, out_at + first, stream)
+
+        if not slabs:
+            launch(held, B, Tq, 0)
+            return out
         for b in range(0, B, many):
             m = min(many, B - b)
             part = held
@@ -266,9 +275,5 @@ def byte_read(q: torch.Tensor, cache: ByteCache, read_lists: torch.Tensor, lengt
                 part = _Cache(k, v, scales, held.code, held.block, m, held.tokens, held.batch_stride, held.token_stride,
                               held.head_stride)
             for t in range(0, Tq, step):
-                at, n = b * Tq + t, min(step, Tq - t)
-                _abi.call_in_order("lsa_byte_read", q.data_ptr() + at * Hq * D * q.element_size(), ctypes.addressof(part), dt,
-                                   m, n, Hq, Hkv, D, ids.data_ptr() + 4 * at * lists * W, lens.data_ptr() + 4 * at * lists,
-                                   W, 1 if per_head else 0, scale, splits, _abi.ptr(counters), _abi.ptr(ws), nbytes,
-                                   out.data_ptr() + at * Hq * D * q.element_size(), stream)
+                launch(part, m, min(step, Tq - t), b * Tq + t)
     return out
