@@ -8,8 +8,9 @@
 // and fills it again as soon as its product is through: K of the next tile loads while the softmax and V's product
 // run, V while it waits for K (8 KB a wave in flight at head dim 128, four waves a SIMD). Both products are matrix
 // instructions in bf16, whose 8 bits of mantissa hold every code exactly: S^T = K Q^T, and O^T += V^T P^T with V's
-// columns by the transposing LDS read. q enters exactly too: bf16 as it is, fp16 in two parts, fp32 in three. A weight times V's scale goes in as
-// two parts (16 bits), for fp32 rows as three, so that rounding it costs nothing beside the output's own rounding.
+// columns by the transposing LDS read. q enters exactly too: bf16 as it is, fp16 in two parts, fp32 in three. A weight
+// times V's scale goes in as two parts (16 bits), for fp32 rows as three, so that rounding it costs nothing beside the
+// output's own rounding.
 // The keys of a tile are dealt to the rows of S^T so that a lane's 8 scores are those of the 8 keys whose V codes
 // it holds (keys 8 row .. + 8): weights go from one product to the other in their registers.
 //
